@@ -468,6 +468,85 @@ int starkv_few_linear(void *stream, const void *x, int64_t x_s0, const void *w, 
                       int64_t r_s0, void *out, int64_t o_s0);
 
 /*
+ * starkv_norm_rope_qkv: starkv_rope_qkv with an RMS norm of each q and k row in front of its rotation, in
+ * the same launch: x / sqrt(mean(x^2) + eps) * weight over the row's 128 dimensions, q_weight / k_weight
+ * [128] (bf16, fp16 or fp32, 16-byte aligned; k_weight where k is given). fp32 arithmetic, one rounding
+ * behind the rotation. v is not normed. Slots of one call are distinct (or outside the cache).
+ */
+int starkv_norm_rope_qkv(void *stream, const void *q, int64_t q_s0, int64_t q_s1, const void *k, int64_t k_s0,
+                         int64_t k_s1, const void *v, int64_t v_s0, int64_t v_s1, int dtype, int num_tokens,
+                         int num_heads, int num_kv_heads, const void *q_weight, const void *k_weight, int w_dtype,
+                         float eps, const void *positions, int pos_bits, const void *cos_sin, int64_t cs_s0,
+                         int cs_dtype, int64_t cs_rows, void *q_out, void *k_out, void *k_cache, void *v_cache,
+                         int64_t c_s0, int64_t c_s1, int64_t c_s2, int block_size, int64_t num_blocks,
+                         const void *slot_mapping, int slot_bits, void *k_half, void *v_half);
+
+/*
+ * The operators over an uncompressed layer's paged caches [num_blocks, block_size, num_kv_heads, 128] (bf16 or
+ * fp16, element strides c_s0, c_s1, c_s2 shared by K and V, rows 16-byte aligned, block_size 16 * 2^s). Common
+ * to them: block_table [n, bt_width] int32; seq_lens [n] int32, clamped to the table's row; num_heads a
+ * multiple of num_kv_heads; query and out of the cache's dtype. A block id outside [0, num_blocks) stands for
+ * no tokens. n is at most 65535, workspaces are 16-byte aligned.
+ *
+ * starkv_key_bounds: bounds [num_blocks, num_kv_heads, 2, 128] (element strides b_s0, b_s1, b_s2; the cache's
+ * dtype) of every block that holds one of a request's last max_new tokens: the elementwise least and largest
+ * of the block's keys up to the request's length (NaN stays NaN). max_new 1 after a decode step, the longest
+ * prompt after a prefill.
+ *
+ * starkv_select_blocks: for each request and KV head the `keep` logical blocks (indices into the request's
+ * block-table row) that its query token reads, ascending, to selected [n, num_kv_heads, keep] (contiguous
+ * int32, -1 behind the last): the first `sink`, the last `recent` and between them those of the largest
+ * sum over the KV head's query heads and dimensions of max(q lo, q hi), which bounds q . k from above. The sum
+ * is in 64 bits, rounded once to fp32; equal scores go to the lower index, NaN counts as the largest. Lengths
+ * are clamped to max_seq_len. A request of at most `keep` blocks gets all of them.
+ *
+ * starkv_sparse_decode: out[b, h] = softmax(scale q . k) v over the tokens of the blocks selected [n,
+ * num_kv_heads, keep] (strides sel_s0, sel_s1; ids outside the request's blocks, such as -1, hold no tokens;
+ * each block at most once). At most 16 query heads a KV head. A row without tokens gives zeros.
+ *
+ * starkv_weighted_decode: the decode over all of a request's tokens (lengths clamped to max_seq_len), and
+ * weights [n, num_kv_heads, weights_len >= max_seq_len] (fp32, strides w_s0, w_s1) += the softmax weight of each
+ * token, summed over the KV head's query heads; the newest token's entry is set, entries behind it stay. A
+ * request without tokens gives zeros and leaves its weights. At most 16 query heads a KV head.
+ *
+ * starkv_evict: cuts each request to `keep` tokens per KV head: the first `sink`, the last `recent` and those
+ * of the largest weights between (equal ones: the lower index; NaN counts as the largest). Kept rows of both
+ * caches move to the front in place, in their order; new_weights [n, num_kv_heads, weights_len] (contiguous)
+ * takes their weights, zeros behind; new_lens [n] = min(length, keep). Requests of at most `keep` tokens keep
+ * their rows. Lengths are clamped to weights_len; the blocks of a request that is cut are its own, no other's.
+ */
+int starkv_key_bounds(void *stream, const void *k_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype,
+                      int block_size, int64_t num_blocks, void *bounds, int64_t b_s0, int64_t b_s1, int64_t b_s2,
+                      const int32_t *block_table, int64_t bt_s0, int64_t bt_s1, int bt_width, const int32_t *seq_lens,
+                      int n, int num_kv_heads, int max_new);
+size_t starkv_select_blocks_workspace_bytes(int n, int num_kv_heads, int bt_width, int block_size, int max_seq_len);
+int starkv_select_blocks(void *stream, const void *query, int64_t q_s0, int64_t q_s1, const void *bounds, int64_t b_s0,
+                         int64_t b_s1, int64_t b_s2, int dtype, int block_size, int64_t num_blocks,
+                         const int32_t *block_table, int64_t bt_s0, int64_t bt_s1, int bt_width,
+                         const int32_t *seq_lens, int n, int num_heads, int num_kv_heads, int max_seq_len, int keep,
+                         int sink, int recent, int32_t *selected, void *workspace, size_t workspace_bytes);
+size_t starkv_sparse_decode_workspace_bytes(int n, int num_heads, int num_kv_heads, int block_size, int keep);
+int starkv_sparse_decode(void *stream, const void *query, int64_t q_s0, int64_t q_s1, const void *k_cache,
+                         const void *v_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype, int block_size,
+                         int64_t num_blocks, const int32_t *block_table, int64_t bt_s0, int64_t bt_s1, int bt_width,
+                         const int32_t *seq_lens, int n, int num_heads, int num_kv_heads, const int32_t *selected,
+                         int64_t sel_s0, int64_t sel_s1, int keep, float scale, void *out, int64_t o_s0, int64_t o_s1,
+                         void *workspace, size_t workspace_bytes);
+size_t starkv_weighted_decode_workspace_bytes(int n, int num_heads, int num_kv_heads, int max_seq_len);
+int starkv_weighted_decode(void *stream, const void *query, int64_t q_s0, int64_t q_s1, const void *k_cache,
+                           const void *v_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype, int block_size,
+                           int64_t num_blocks, const int32_t *block_table, int64_t bt_s0, int64_t bt_s1, int bt_width,
+                           const int32_t *seq_lens, int n, int num_heads, int num_kv_heads, int max_seq_len,
+                           float scale, float *weights, int64_t w_s0, int64_t w_s1, int weights_len, void *out,
+                           int64_t o_s0, int64_t o_s1, void *workspace, size_t workspace_bytes);
+size_t starkv_evict_workspace_bytes(int n, int num_kv_heads, int keep);
+int starkv_evict(void *stream, void *k_cache, void *v_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype,
+                 int block_size, int64_t num_blocks, const int32_t *block_table, int64_t bt_s0, int64_t bt_s1,
+                 int bt_width, const int32_t *seq_lens, int n, int num_kv_heads, const float *weights, int64_t w_s0,
+                 int64_t w_s1, int weights_len, int keep, int sink, int recent, int32_t *new_lens, float *new_weights,
+                 void *workspace, size_t workspace_bytes);
+
+/*
  * Timing for benchmarks (no counterpart in the reference, whose benchmark reads profiler
  * traces instead, bench_serving.py:71-115). starkv_profile_begin arms up to max_calls
  * event pairs; each following decode call records one pair on its stream, around its

@@ -1,0 +1,264 @@
+// Eviction by accumulated attention weight, for uncompressed caches.
+//
+// starkv_weighted_decode is a paged decode over a request's whole cache that also sums up what each
+// cached token weighs: weights[b, h, t] += sum_g softmax_g(t) over the G query heads of KV head h (the
+// newest token's entry starts there: it is set). attend_kernel<.., false> (paged_attend.hpp) leaves every
+// score behind (4 bytes a query head and token beside 512 bytes of keys and values), weigh_kernel turns
+// them into weights once the splits' references and sums are known, and joins the splits' outputs. A
+// token's entry belongs to one thread, which sums the heads in order: no atomics, the same bits every run.
+//
+// starkv_evict cuts each request and KV head to `keep` tokens: the first `sink`, the last `recent` and
+// those of the largest weights between (topk_select.hpp). The order of tokens stays, so `recent` means the
+// same at the next eviction, and kept[j] >= j ascends: compact_kernel moves row kept[j] to row j in place,
+// reading rows of a chunk before any of them is written; a later chunk's sources lie behind every
+// earlier chunk's targets. Columns are independent of each other, so K and V and their halves of 128
+// bytes go to workgroups of their own.
+#include <algorithm>
+
+#include "common.hpp"
+#include "paged_attend.hpp"
+#include "topk_select.hpp"
+
+namespace starkv {
+
+namespace {
+
+struct WeighParams {
+    AttendParams a;
+    float* w; int64_t w_s0, w_s1;  // weights [n][Hkv][>= span], last dimension contiguous
+    int chunks;                    // workgroups of WG_TOKENS tokens a (request, KV head)
+};
+
+constexpr int WG_TOKENS = 1024;
+
+// blockIdx.x < chunks: weights of WG_TOKENS tokens of a (request, KV head); behind them, where there are
+// splits, two query heads' outputs a workgroup.
+template <int DT>
+__global__ __launch_bounds__(256) void weigh_kernel(const WeighParams wp) {
+    const AttendParams& p = wp.a;
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, H = p.Hkv * p.G;
+    if ((int)blockIdx.x >= wp.chunks) {
+        const int g = 2 * (blockIdx.x - wp.chunks) + (tid >> 7);
+        if (g < p.G) attend_merge_head<DT>(p, b, h * p.G + g, tid & 127);
+        return;
+    }
+    const int L = attend_length(p, b), t0 = blockIdx.x * WG_TOKENS;
+    if (t0 >= L) return;
+    // Each head's log2 of its sum of weights, 16 lanes a head.
+    __shared__ float s_lse[AT_MAX_GROUP];
+    const int g16 = tid >> 4;
+    if (g16 < p.G) {
+        const float* pp = p.part + ((int64_t)b * H + h * p.G + g16) * p.splits * AT_PART;
+        float M = -INFINITY, l = 0.f;
+        for (int s = tid & 15; s < p.splits; s += 16) M = fmaxf(M, pp[s * AT_PART]);
+        M = row16_max(M);
+        for (int s = tid & 15; s < p.splits; s += 16) {
+            const float m = pp[s * AT_PART];
+            l = fmaf(pp[s * AT_PART + 2], m == -INFINITY ? 1.f : exp2f(m - M), l);
+        }
+        l = row16_sum(l);
+        if ((tid & 15) == 0) s_lse[g16] = l == 0.f ? 0.f : M + log2f(l);  // no block of the cache: weights of 0
+    }
+    __syncthreads();
+    const float* lg = p.lg + ((int64_t)b * H + h * p.G) * p.lg_row;
+    float* w = wp.w + b * wp.w_s0 + h * wp.w_s1;
+#pragma unroll
+    for (int u = 0; u < WG_TOKENS / 256; ++u) {
+        const int t = t0 + 256 * u + tid;
+        if (t >= L) return;
+        float sum = 0.f;
+        for (int g = 0; g < p.G; ++g) sum += exp2f(lg[g * p.lg_row + t] - s_lse[g]);
+        w[t] = t == L - 1 ? sum : w[t] + sum;
+    }
+}
+
+struct EvictParams {
+    uint16_t* kc; uint16_t* vc; int64_t c_s0, c_s1, c_s2; int block_shift; int64_t num_blocks;
+    const int32_t* bt; int64_t bt_s0, bt_s1;
+    const int32_t* seq_lens; int span;
+    const float* w; int64_t w_s0, w_s1;
+    int Hkv, cap, keep, sink, recent;
+    int32_t* new_lens; float* new_w;  // [n], [n][Hkv][cap]
+    int32_t* kept;                    // [n][Hkv][keep]
+};
+
+__device__ __forceinline__ int evict_length(const EvictParams& p, int b) { return min(max(p.seq_lens[b], 0), p.span); }
+
+constexpr int EV_THR = 1024;
+constexpr int EV_LDS = 12288;  // keys of a row kept in LDS
+
+template <bool IN_LDS>
+__global__ __launch_bounds__(EV_THR) void evict_select_kernel(const EvictParams p) {
+    __shared__ TopkShared<EV_THR> sh;
+    __shared__ uint32_t s_key[IN_LDS ? EV_LDS : 1];
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const int L = evict_length(p, b), left = min(L, p.keep);
+    const float* w = p.w + b * p.w_s0 + h * p.w_s1;
+    float* nw = p.new_w + ((int64_t)b * p.Hkv + h) * p.cap;
+    if (h == 0 && tid == 0) p.new_lens[b] = left;
+    for (int i = left + tid; i < p.cap; i += EV_THR) nw[i] = 0.f;
+    if (L <= p.keep) {
+        for (int i = tid; i < L; i += EV_THR) nw[i] = w[i];
+        return;
+    }
+    int32_t* kept = p.kept + ((int64_t)b * p.Hkv + h) * p.keep;
+    const int middle = L - p.sink - p.recent, k = p.keep - p.sink - p.recent;
+    for (int i = tid; i < p.sink + p.recent; i += EV_THR) {
+        const int from = i < p.sink ? i : middle + i, to = i < p.sink ? i : k + i;
+        kept[to] = from;
+        nw[to] = w[from];
+    }
+    if (k == 0) return;
+    w += p.sink;
+    if constexpr (IN_LDS) {
+        for (int i = tid; i < middle; i += EV_THR) s_key[i] = order_key(w[i]);
+        __syncthreads();
+    }
+    topk_ascending<EV_THR>(
+        sh, middle, k, [&](int i) { return IN_LDS ? s_key[i] : order_key(w[i]); },
+        [&](int pos, int i) {
+            kept[p.sink + pos] = p.sink + i;
+            nw[p.sink + pos] = w[i];
+        });
+}
+
+constexpr int CP_THR = 1024, CP_U = 4;  // 128 rows of 128 bytes a round, four rounds a chunk
+
+__global__ __launch_bounds__(CP_THR) void compact_kernel(const EvictParams p) {
+    const int h = blockIdx.y, b = blockIdx.z;
+    if (evict_length(p, b) <= p.keep) return;
+    uint16_t* c = (blockIdx.x & 1 ? p.vc : p.kc) + h * p.c_s2 + (blockIdx.x >> 1) * 64 + 8 * (threadIdx.x & 7);
+    const int row = threadIdx.x >> 3, mask = (1 << p.block_shift) - 1;
+    const int32_t* kept = p.kept + ((int64_t)b * p.Hkv + h) * p.keep;
+    const int32_t* bt = p.bt + b * p.bt_s0;
+    for (int j0 = 0; j0 < p.keep; j0 += CP_U * CP_THR / 8) {
+        uint4 v[CP_U];
+        uint16_t* to[CP_U];
+#pragma unroll
+        for (int u = 0; u < CP_U; ++u) {
+            const int j = j0 + u * (CP_THR / 8) + row;
+            const int from = j < p.keep ? kept[j] : j;
+            to[u] = nullptr;
+            if (from == j) continue;
+            const int sb = bt[(from >> p.block_shift) * p.bt_s1], db = bt[(j >> p.block_shift) * p.bt_s1];
+            if (sb < 0 || sb >= p.num_blocks || db < 0 || db >= p.num_blocks) continue;
+            v[u] = *(const uint4*)(c + sb * p.c_s0 + (from & mask) * p.c_s1);
+            to[u] = c + db * p.c_s0 + (j & mask) * p.c_s1;
+        }
+        __syncthreads();  // every row of the chunk is read
+#pragma unroll
+        for (int u = 0; u < CP_U; ++u)
+            if (to[u]) *(uint4*)to[u] = v[u];
+    }
+}
+
+}  // namespace
+
+}  // namespace starkv
+
+using namespace starkv;
+
+extern "C" {
+
+static size_t weighted_logits_bytes(int n, int num_heads, int max_seq_len) {
+    return (size_t)n * num_heads * (((size_t)max_seq_len + 15) / 16 * 16) * 4;
+}
+
+static int weighted_splits(int n, int num_kv_heads, int max_seq_len) {
+    return attend_splits((int64_t)n * num_kv_heads, (int)(((int64_t)max_seq_len + 15) / 16));
+}
+
+size_t starkv_weighted_decode_workspace_bytes(int n, int num_heads, int num_kv_heads, int max_seq_len) {
+    if (n < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || max_seq_len < 1) return 256;
+    return weighted_logits_bytes(n, num_heads, max_seq_len) +
+           (size_t)n * num_heads * weighted_splits(n, num_kv_heads, max_seq_len) * AT_PART * 4;
+}
+
+int starkv_weighted_decode(void* stream, const void* query, int64_t q_s0, int64_t q_s1, const void* k_cache,
+                           const void* v_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype, int block_size,
+                           int64_t num_blocks, const int32_t* block_table, int64_t bt_s0, int64_t bt_s1, int bt_width,
+                           const int32_t* seq_lens, int n, int num_heads, int num_kv_heads, int max_seq_len,
+                           float scale, float* weights, int64_t w_s0, int64_t w_s1, int weights_len, void* out,
+                           int64_t o_s0, int64_t o_s1, void* workspace, size_t workspace_bytes) {
+    clear_error();
+    SKV_CHECK(n >= 0 && n <= 65535 && max_seq_len >= 1 && max_seq_len <= 1 << 30,
+              "weighted_decode: n=%d (up to 65535) max_seq_len=%d", n, max_seq_len);
+    if (n == 0) return STARKV_OK;
+    WeighParams wp = {};
+    AttendParams& p = wp.a;
+    const int rc = attend_setup(p, "weighted_decode", query, q_s0, q_s1, k_cache, v_cache, c_s0, c_s1, c_s2, dtype,
+                                block_size, num_blocks, block_table, bt_s0, bt_s1, bt_width, seq_lens, n, num_heads,
+                                num_kv_heads, scale, out, o_s0, o_s1, workspace);
+    if (rc != STARKV_OK) return rc;
+    SKV_CHECK(num_kv_heads <= 65535, "weighted_decode: %d KV heads", num_kv_heads);
+    SKV_CHECK(weights && weights_len >= max_seq_len, "weighted_decode: weights of %d tokens for max_seq_len=%d",
+              weights_len, max_seq_len);
+    const size_t need = starkv_weighted_decode_workspace_bytes(n, num_heads, num_kv_heads, max_seq_len);
+    SKV_CHECK(workspace_bytes >= need, "weighted_decode: workspace %zu bytes < %zu", workspace_bytes, need);
+    p.span = std::min(p.span, max_seq_len);
+    const int pages = (p.span + 15) / 16;
+    p.splits = weighted_splits(n, num_kv_heads, max_seq_len);
+    p.pps = (pages + p.splits - 1) / p.splits;
+    p.lg = (float*)workspace;
+    p.lg_row = ((int64_t)max_seq_len + 15) / 16 * 16;
+    p.part = (float*)((char*)workspace + weighted_logits_bytes(n, num_heads, max_seq_len));
+    wp.w = weights; wp.w_s0 = w_s0; wp.w_s1 = w_s1;
+    wp.chunks = (p.span + WG_TOKENS - 1) / WG_TOKENS;
+    const int err = attend_launch<false>(stream, dtype, p);
+    if (err != STARKV_OK) return err;
+    const dim3 grid(wp.chunks + (p.splits > 1 ? (p.G + 1) / 2 : 0), num_kv_heads, n);
+    if (dtype == STARKV_BF16)
+        hipLaunchKernelGGL(weigh_kernel<STARKV_BF16>, grid, dim3(256), 0, (hipStream_t)stream, wp);
+    else
+        hipLaunchKernelGGL(weigh_kernel<STARKV_F16>, grid, dim3(256), 0, (hipStream_t)stream, wp);
+    SKV_HIP(hipGetLastError());
+    return STARKV_OK;
+}
+
+size_t starkv_evict_workspace_bytes(int n, int num_kv_heads, int keep) {
+    if (n < 1 || num_kv_heads < 1 || keep < 1) return 256;
+    return std::max<size_t>(256, (size_t)n * num_kv_heads * keep * 4);
+}
+
+int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype,
+                 int block_size, int64_t num_blocks, const int32_t* block_table, int64_t bt_s0, int64_t bt_s1,
+                 int bt_width, const int32_t* seq_lens, int n, int num_kv_heads, const float* weights, int64_t w_s0,
+                 int64_t w_s1, int weights_len, int keep, int sink, int recent, int32_t* new_lens, float* new_weights,
+                 void* workspace, size_t workspace_bytes) {
+    clear_error();
+    SKV_CHECK(n >= 0 && n <= 65535 && num_kv_heads >= 1 && num_kv_heads <= 65535,
+              "evict: n=%d (up to 65535) num_kv_heads=%d", n, num_kv_heads);
+    SKV_CHECK(sink >= 0 && recent >= 0 && keep >= 1 && sink <= keep && recent <= keep - sink,
+              "evict: keep %d tokens, %d first and %d last ones among them", keep, sink, recent);
+    if (n == 0) return STARKV_OK;
+    SKV_CHECK(k_cache && v_cache && block_table && seq_lens && weights && new_lens && new_weights && workspace,
+              "evict: null pointer");
+    SKV_CHECK(dtype == STARKV_BF16 || dtype == STARKV_F16, "evict: bf16 or fp16");
+    SKV_CHECK(block_shift(block_size) >= 0, "evict: block_size must be 16 times a power of two");
+    SKV_CHECK(num_blocks >= 1 && num_blocks <= 0x7fffffff && bt_width >= 1 && weights_len >= 1,
+              "evict: empty cache, block table or weights");
+    SKV_CHECK(((uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 && (c_s0 | c_s1 | c_s2) % 8 == 0,
+              "evict: cache rows must be 16-byte aligned");
+    const size_t need = starkv_evict_workspace_bytes(n, num_kv_heads, keep);
+    SKV_CHECK(workspace_bytes >= need, "evict: workspace %zu bytes < %zu", workspace_bytes, need);
+    EvictParams p = {};
+    p.kc = (uint16_t*)k_cache; p.vc = (uint16_t*)v_cache; p.c_s0 = c_s0; p.c_s1 = c_s1; p.c_s2 = c_s2;
+    p.block_shift = block_shift(block_size) + 4; p.num_blocks = num_blocks;
+    p.bt = block_table; p.bt_s0 = bt_s0; p.bt_s1 = bt_s1;
+    p.seq_lens = seq_lens; p.span = (int)std::min<int64_t>((int64_t)bt_width * block_size, weights_len);
+    p.w = weights; p.w_s0 = w_s0; p.w_s1 = w_s1;
+    p.Hkv = num_kv_heads; p.cap = weights_len; p.keep = keep; p.sink = sink; p.recent = recent;
+    p.new_lens = new_lens; p.new_w = new_weights; p.kept = (int32_t*)workspace;
+    if (p.span <= EV_LDS)
+        hipLaunchKernelGGL(evict_select_kernel<true>, dim3(num_kv_heads, n), dim3(EV_THR), 0, (hipStream_t)stream, p);
+    else
+        hipLaunchKernelGGL(evict_select_kernel<false>, dim3(num_kv_heads, n), dim3(EV_THR), 0, (hipStream_t)stream, p);
+    SKV_HIP(hipGetLastError());
+    if (p.span > keep) {
+        hipLaunchKernelGGL(compact_kernel, dim3(4, num_kv_heads, n), dim3(CP_THR), 0, (hipStream_t)stream, p);
+        SKV_HIP(hipGetLastError());
+    }
+    return STARKV_OK;
+}
+
+}  // extern "C"

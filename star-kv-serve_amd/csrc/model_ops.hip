@@ -11,6 +11,11 @@
 // decode step. 2048 tokens of 32 + 64 rows with cache and fp16 rows 26 us (134 MB), where 22
 // elementwise launches, the write and two conversions took 330.
 //
+// With NORM the same launch first norms each q and k row over its 128 dimensions (the norm of
+// queries and keys for each head): x / sqrt(mean(x^2) + eps) * weight, the squares summed in fp32
+// over the row's 8 lanes, the normed row kept in fp32 into the rotation and rounded once behind it.
+// A step's norms cost no launch and no pass over q and k of their own.
+//
 // silu_mul_kernel: silu(gate) * up, the gate rounded to the model dtype before the product as the
 // two elementwise kernels did. 2048 tokens of 2 x 11008: 31 us (135 MB) against 56.
 //
@@ -51,6 +56,7 @@ struct RopeParams {
     int64_t block_size, num_blocks;
     const void* slots; int slot64;
     uint16_t* k16; uint16_t* v16;       // contiguous fp16 [T][Hkv][128], or null
+    const void* qw; const void* kw; int w_dt; float eps;  // NORM: the norms' weights [128]
 };
 
 __device__ __forceinline__ void store8(void* p, int64_t i, int dt, const float* f) {
@@ -78,6 +84,7 @@ __device__ __forceinline__ float2 rotate(float x1, float x2, float c, float s) {
     return make_float2(x1 * c - x2 * s, x2 * c + x1 * s);
 }
 
+template <bool NORM>
 __global__ __launch_bounds__(256) void rope_qkv_kernel(const RopeParams p) {
     const int rows = p.H + (p.k ? p.Hkv : 0) + (p.v ? p.Hkv : 0);
     const int t = blockIdx.x, it = blockIdx.y * 256 + threadIdx.x;
@@ -96,6 +103,23 @@ __global__ __launch_bounds__(256) void rope_qkv_kernel(const RopeParams p) {
         float c[8], s[8];
         load8_f(p.cs, pos * p.cs_s0 + d, p.cs_dt, c);
         load8_f(p.cs, pos * p.cs_s0 + 64 + d, p.cs_dt, s);
+        if constexpr (NORM) {
+            const void* w = isq ? p.qw : p.kw;
+            float wa[8], wb[8], ss = 0.f;
+            load8_f(w, d, p.w_dt, wa);
+            load8_f(w, 64 + d, p.w_dt, wb);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
+            ss += dpp_f<0xB1>(ss);   // the row's 8 lanes: quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror
+            ss += dpp_f<0x4E>(ss);
+            ss += dpp_f<0x141>(ss);
+            const float inv = 1.f / sqrtf(ss * (1.f / 128.f) + p.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                a[e] *= inv * wa[e];
+                b[e] *= inv * wb[e];
+            }
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float2 r = rotate(a[e], b[e], c[e], s[e]);
@@ -392,20 +416,13 @@ const void* few_pick(int dt, int mode, bool norm, bool wide) {
                              : (const void*)&few_linear_kernel<STARKV_F16, FEW_PLAIN, false, 1>;
 }
 
-}  // namespace
-
-}  // namespace starkv
-
-using namespace starkv;
-
-extern "C" {
-
-int starkv_rope_qkv(void* stream, const void* q, int64_t q_s0, int64_t q_s1, const void* k, int64_t k_s0, int64_t k_s1,
+// starkv_rope_qkv, and with q_weight starkv_norm_rope_qkv.
+int rope_call(void* stream, const void* q, int64_t q_s0, int64_t q_s1, const void* k, int64_t k_s0, int64_t k_s1,
                     const void* v, int64_t v_s0, int64_t v_s1, int dtype, int num_tokens, int num_heads,
                     int num_kv_heads, const void* positions, int pos_bits, const void* cos_sin, int64_t cs_s0,
                     int cs_dtype, int64_t cs_rows, void* q_out, void* k_out, void* k_cache, void* v_cache, int64_t c_s0,
                     int64_t c_s1, int64_t c_s2, int block_size, int64_t num_blocks, const void* slot_mapping,
-                    int slot_bits, void* k_half, void* v_half) {
+                    int slot_bits, void* k_half, void* v_half, const void* q_weight, const void* k_weight, int w_dtype, float eps) {
     clear_error();
     SKV_CHECK(num_tokens >= 0 && num_heads > 0 && num_kv_heads >= 0, "rope_qkv: bad sizes");
     SKV_CHECK(dtype >= STARKV_F32 && dtype <= STARKV_BF16 && cs_dtype >= STARKV_F32 && cs_dtype <= STARKV_BF16,
@@ -422,7 +439,7 @@ int starkv_rope_qkv(void* stream, const void* q, int64_t q_s0, int64_t q_s1, con
                (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)k_half | (uintptr_t)v_half) % 16 == 0 &&
                   (q_s0 | q_s1 | k_s0 | k_s1 | v_s0 | v_s1 | c_s0 | c_s1 | c_s2) % al == 0 && cs_s0 % cal == 0,
               "rope_qkv: rows must be 16-byte aligned");
-    RopeParams p;
+    RopeParams p = {};
     p.q = q; p.q_s0 = q_s0; p.q_s1 = q_s1;
     p.k = k; p.k_s0 = k_s0; p.k_s1 = k_s1;
     p.v = v; p.v_s0 = v_s0; p.v_s1 = v_s1;
@@ -434,10 +451,54 @@ int starkv_rope_qkv(void* stream, const void* q, int64_t q_s0, int64_t q_s1, con
     p.block_size = block_size; p.num_blocks = num_blocks;
     p.slots = slot_mapping; p.slot64 = slot_bits == 64;
     p.k16 = (uint16_t*)k_half; p.v16 = (uint16_t*)v_half;
+    p.qw = q_weight; p.kw = k_weight; p.w_dt = w_dtype; p.eps = eps;
     const int rows = num_heads + (k ? num_kv_heads : 0) + (v ? num_kv_heads : 0);
-    hipLaunchKernelGGL(rope_qkv_kernel, dim3(num_tokens, (8 * rows + 255) / 256), dim3(256), 0, (hipStream_t)stream, p);
+    const dim3 grid(num_tokens, (8 * rows + 255) / 256);
+    if (q_weight)
+        hipLaunchKernelGGL(rope_qkv_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    else
+        hipLaunchKernelGGL(rope_qkv_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, p);
     SKV_HIP(hipGetLastError());
     return STARKV_OK;
+}
+
+}  // namespace
+
+}  // namespace starkv
+
+using namespace starkv;
+
+extern "C" {
+
+int starkv_rope_qkv(void* stream, const void* q, int64_t q_s0, int64_t q_s1, const void* k, int64_t k_s0, int64_t k_s1,
+                    const void* v, int64_t v_s0, int64_t v_s1, int dtype, int num_tokens, int num_heads,
+                    int num_kv_heads, const void* positions, int pos_bits, const void* cos_sin, int64_t cs_s0,
+                    int cs_dtype, int64_t cs_rows, void* q_out, void* k_out, void* k_cache, void* v_cache, int64_t c_s0,
+                    int64_t c_s1, int64_t c_s2, int block_size, int64_t num_blocks, const void* slot_mapping,
+                    int slot_bits, void* k_half, void* v_half) {
+    return rope_call(stream, q, q_s0, q_s1, k, k_s0, k_s1, v, v_s0, v_s1, dtype, num_tokens, num_heads, num_kv_heads,
+                     positions, pos_bits, cos_sin, cs_s0, cs_dtype, cs_rows, q_out, k_out, k_cache, v_cache, c_s0, c_s1,
+                     c_s2, block_size, num_blocks, slot_mapping, slot_bits, k_half, v_half, nullptr, nullptr, STARKV_F32,
+                     0.f);
+}
+
+int starkv_norm_rope_qkv(void* stream, const void* q, int64_t q_s0, int64_t q_s1, const void* k, int64_t k_s0,
+                         int64_t k_s1, const void* v, int64_t v_s0, int64_t v_s1, int dtype, int num_tokens,
+                         int num_heads, int num_kv_heads, const void* q_weight, const void* k_weight, int w_dtype,
+                         float eps, const void* positions, int pos_bits, const void* cos_sin, int64_t cs_s0,
+                         int cs_dtype, int64_t cs_rows, void* q_out, void* k_out, void* k_cache, void* v_cache,
+                         int64_t c_s0, int64_t c_s1, int64_t c_s2, int block_size, int64_t num_blocks,
+                         const void* slot_mapping, int slot_bits, void* k_half, void* v_half) {
+    clear_error();
+    SKV_CHECK(q_weight && (!k || k_weight), "norm_rope_qkv: a weight for each of q and k");
+    SKV_CHECK(w_dtype >= STARKV_F32 && w_dtype <= STARKV_BF16 &&
+                  ((uintptr_t)q_weight | (uintptr_t)k_weight) % 16 == 0,
+              "norm_rope_qkv: weights must be bf16, fp16 or fp32 and 16-byte aligned");
+    SKV_CHECK(eps >= 0.f, "norm_rope_qkv: eps is not negative");
+    return rope_call(stream, q, q_s0, q_s1, k, k_s0, k_s1, v, v_s0, v_s1, dtype, num_tokens, num_heads, num_kv_heads,
+                     positions, pos_bits, cos_sin, cs_s0, cs_dtype, cs_rows, q_out, k_out, k_cache, v_cache, c_s0, c_s1,
+                     c_s2, block_size, num_blocks, slot_mapping, slot_bits, k_half, v_half, q_weight, k_weight, w_dtype,
+                     eps);
 }
 
 int starkv_decode_slots(void* stream, const void* block_table, int64_t bt_s0, int64_t bt_s1, int bt_bits, int width,

@@ -242,7 +242,7 @@ using namespace starkv;
 
 extern "C" {
 
-int starkv_abi_version(void) { return 7; }
+int starkv_abi_version(void) { return 8; }
 
 const char* starkv_last_error(void) { return g_err; }
 

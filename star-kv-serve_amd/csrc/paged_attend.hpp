@@ -1,0 +1,329 @@
+// One token's attention over pages of an uncompressed paged cache, on matrix instructions: the body
+// that the decode over selected blocks (sparse_decode.hip) and the decode that weighs its tokens
+// (evict.hip) share.
+//
+// For a request b, a KV head h and its G <= 16 query heads: s_g(t) = scale log2(e) q_g . k_t over the
+// tokens t of the unit's pages, p = 2^(s - m), out_g = sum p v / sum p. A page is 16 tokens of one
+// block. A workgroup of 4 waves takes a range of the unit's pages (a split); a wave takes two pages,
+// 32 tokens, at a time and keeps its own running reference m and sums; the waves meet in LDS at the
+// end, the splits in attend_merge_kernel.
+//
+// Both products run on v_mfma_f32_16x16x32 with nothing but registers between memory and the matrix
+// unit: S^T = K q^T takes 16 tokens as rows, so a lane holds row l % 16 of the page's keys as they lie
+// in memory (64 bytes of each of 16 rows a load) and the 16 columns are the query heads, zeros past
+// the G-th. The result gives lane l the scores of head l % 16 at tokens 4 (l / 16) .. + 3 of either
+// page, which is the B operand of out^T = V^T P^T with the product's 32 terms in the order (l / 16,
+// page, token): P goes from one product into the other in place. V^T's rows are the head's dimensions
+// in the order 8 (l % 16) + i for the i-th of 8 products, so the A operand is dimension i of the 16
+// bytes that lane l loaded of each of its 8 tokens (4 rows of 256 bytes a load), gathered with 4 byte
+// permutes. A lane ends with 32 consecutive dimensions of one head. Any G costs the same instructions,
+// far below memory's time.
+//
+// Rounding: scores, references and sums are fp32. The weights are rounded to the cache's type for the
+// second product (2^-8 relative for bf16, 2^-11 for fp16, as the output is in the end), and the
+// sum that divides takes the rounded weights, so that they sum to one. The reference lies 2^7 below
+// the largest score seen when it was set and moves when a score passes it by 2^15 (fp16 weights stay
+// finite, and small ones keep 22 bits of range above its subnormals).
+#pragma once
+
+#include <algorithm>
+
+#include "common.hpp"
+
+namespace starkv {
+
+constexpr int AT_THR = 256;
+constexpr int AT_CHUNK = 512;      // pages whose places are looked up at a time
+constexpr int AT_PART = 132;       // floats of a partial: reference, sum of rounded weights, sum of weights, 0, out[128]
+constexpr int AT_MAX_SPLITS = 128;
+constexpr int AT_MAX_GROUP = 16;   // query heads per KV head: the columns of a matrix product
+constexpr float AT_LOG2E = 1.4426950408889634f;
+
+struct AttendParams {
+    const uint16_t* q; int64_t q_s0, q_s1;                               // elements, as all strides here
+    const uint16_t* kc; const uint16_t* vc; int64_t c_s0, c_s1, c_s2;
+    int bs_shift; int64_t num_blocks;                                    // block_size = 16 << bs_shift
+    const int32_t* bt; int64_t bt_s0, bt_s1;
+    const int32_t* seq_lens; int span;                                   // lengths are clamped to span
+    int n, Hkv, G, splits, pps;                                          // pps: pages per split
+    float sc;                                                            // scale * log2(e)
+    const int32_t* sel; int64_t sel_s0, sel_s1; int keep;                // SPARSE: logical blocks [n][Hkv][keep]
+    float* lg; int64_t lg_row;                                           // else: scores [n][H][lg_row]
+    float* part;                                                         // [n][H][splits][AT_PART]
+    uint16_t* out; int64_t o_s0, o_s1;
+};
+
+__device__ __forceinline__ int attend_length(const AttendParams& p, int b) {
+    return min(max(p.seq_lens[b], 0), p.span);
+}
+
+template <int DT>
+__device__ __forceinline__ f32x4_t attend_mfma(uint4 a, uint4 b, f32x4_t c) {
+    if constexpr (DT == STARKV_BF16)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                       c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c,
+                                                      0, 0, 0);
+}
+
+// Two values rounded to DT, packed, and their sum as rounded.
+template <int DT>
+__device__ __forceinline__ uint32_t attend_pack(float a, float b, float& sum) {
+    if constexpr (DT == STARKV_BF16) {
+        const uint32_t lo = f32_to_bf16_rne(a), hi = f32_to_bf16_rne(b);
+        sum += bf16_bits_to_f32(lo) + bf16_bits_to_f32(hi);
+        return lo | (hi << 16);
+    } else {
+        const _Float16 lo = (_Float16)a, hi = (_Float16)b;
+        sum += (float)lo + (float)hi;
+        return (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
+    }
+}
+
+// Component i of a 16-byte register row.
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// The workgroup's unit: (request, KV head, split) from the block index.
+template <int DT, bool SPARSE>
+__global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p) {
+    __shared__ int2 s_page[AT_CHUNK];           // a page's block, and its tokens | its place in the block << 8
+    extern __shared__ float s_dyn[];            // [4 waves][G][AT_PART] for the merge
+    const int id = blockIdx.x, s = id % p.splits, u = id / p.splits, h = u % p.Hkv, b = u / p.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    const int H = p.Hkv * p.G;
+    const int L = attend_length(p, b);
+    const int pages = SPARSE ? p.keep << p.bs_shift : (L + 15) >> 4;
+    const int k0 = min(s * p.pps, pages), k1 = min(k0 + p.pps, pages);
+    const int mask = (1 << p.bs_shift) - 1, blocks = (((L + 15) >> 4) + mask) >> p.bs_shift;
+
+    uint4 qf[4];
+#pragma unroll
+    for (int st = 0; st < 4; ++st)
+        qf[st] = col < p.G ? *(const uint4*)(p.q + b * p.q_s0 + (int64_t)(h * p.G + col) * p.q_s1 + 32 * st + 8 * quad)
+                           : make_uint4(0, 0, 0, 0);
+    float m = -INFINITY, l = 0.f, lx = 0.f;
+    f32x4_t acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const uint16_t* kh = p.kc + (int64_t)h * p.c_s2 + 8 * quad;
+    const uint16_t* vh = p.vc + (int64_t)h * p.c_s2 + 8 * col;
+
+    for (int c0 = k0; c0 < k1; c0 += AT_CHUNK) {
+        const int count = min(AT_CHUNK, k1 - c0);
+        if (c0 != k0) __syncthreads();
+        for (int i = tid; i < count; i += AT_THR) {
+            const int pg = c0 + i;
+            const int lb = SPARSE ? p.sel[b * p.sel_s0 + h * p.sel_s1 + (pg >> p.bs_shift)] : pg >> p.bs_shift;
+            int blk = 0, tokens = 0;
+            if (lb >= 0 && lb < blocks) {
+                tokens = min(max(L - 16 * ((lb << p.bs_shift) + (pg & mask)), 0), 16);
+                blk = p.bt[b * p.bt_s0 + lb * p.bt_s1];
+                if (blk < 0 || blk >= p.num_blocks) tokens = 0;  // no block of the cache: no tokens
+            }
+            s_page[i] = make_int2(blk, tokens | (pg & mask) << 8);
+        }
+        __syncthreads();
+        for (int i = 2 * wave; i < count; i += 8) {
+            int2 e[2];
+            int nt[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int2 v = s_page[min(i + x, count - 1)];
+                e[x].x = __builtin_amdgcn_readfirstlane(v.x);
+                e[x].y = __builtin_amdgcn_readfirstlane(v.y);
+                nt[x] = i + x < count ? e[x].y & 255 : 0;
+            }
+            float* lg = p.lg + ((int64_t)b * H + h * p.G + col) * p.lg_row + 16 * (c0 + i) + 4 * quad;
+            if (nt[0] + nt[1] == 0) {
+                if (!SPARSE && col < p.G)
+                    for (int x = 0; x < 2 && i + x < count; ++x)
+                        *(float4*)(lg + 16 * x) = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                continue;
+            }
+            uint4 kr[2][4], vr[2][4];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                // A page without tokens reads the other one's rows, one with fewer than 16 its last row
+                // again: every address lies in the request's tokens, and nothing of them is used.
+                const int2 at = nt[x] ? e[x] : e[x ^ 1];
+                const int last = (nt[x] ? nt[x] : nt[x ^ 1]) - 1;
+                const int64_t base = at.x * p.c_s0 + (int64_t)((at.y >> 8) << 4) * p.c_s1;
+#pragma unroll
+                for (int st = 0; st < 4; ++st)
+                    kr[x][st] = *(const uint4*)(kh + base + min(col, last) * p.c_s1 + 32 * st);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    vr[x][j] = *(const uint4*)(vh + base + min(4 * quad + j, last) * p.c_s1);
+            }
+            float sv[2][4];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int st = 0; st < 4; ++st) d = attend_mfma<DT>(kr[x][st], qf[st], d);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) sv[x][r] = d[r] * p.sc;
+                if (nt[x] < 16) {  // tokens past the end: no score, and no value that a weight of 0 could turn into NaN
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const bool ok = 4 * quad + r < nt[x];
+                        sv[x][r] = ok ? sv[x][r] : -INFINITY;
+                        vr[x][r] = ok ? vr[x][r] : make_uint4(0, 0, 0, 0);
+                    }
+                }
+                if (!SPARSE && col < p.G && i + x < count)
+                    *(float4*)(lg + 16 * x) = make_float4(sv[x][0], sv[x][1], sv[x][2], sv[x][3]);
+            }
+            float mx = sv[0][0];
+#pragma unroll
+            for (int r = 1; r < 8; ++r) mx = fmaxf(mx, sv[r >> 2][r & 3]);
+            mx = max_rows(mx);
+            if (__builtin_amdgcn_ballot_w64(mx > m + 15.f) != 0) {
+                const float mn = mx > m + 15.f ? mx - 7.f : m;
+                const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
+                m = mn;
+                l *= alpha;
+                lx *= alpha;
+#pragma unroll
+                for (int i8 = 0; i8 < 8; ++i8) acc[i8] *= alpha;
+            }
+            float pe[2][4];
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    pe[x][r] = 4 * quad + r < nt[x] ? exp2f(sv[x][r] - m) : 0.f;
+                    if (!SPARSE) lx += pe[x][r];
+                }
+            const uint4 pf = make_uint4(attend_pack<DT>(pe[0][0], pe[0][1], l), attend_pack<DT>(pe[0][2], pe[0][3], l),
+                                        attend_pack<DT>(pe[1][0], pe[1][1], l), attend_pack<DT>(pe[1][2], pe[1][3], l));
+#pragma unroll
+            for (int i8 = 0; i8 < 8; ++i8) {
+                const uint32_t pick = i8 & 1 ? 0x07060302u : 0x05040100u;  // both high halves, or both low ones
+                uint4 vt;
+                vt.x = __builtin_amdgcn_perm(word_of(vr[0][1], i8 >> 1), word_of(vr[0][0], i8 >> 1), pick);
+                vt.y = __builtin_amdgcn_perm(word_of(vr[0][3], i8 >> 1), word_of(vr[0][2], i8 >> 1), pick);
+                vt.z = __builtin_amdgcn_perm(word_of(vr[1][1], i8 >> 1), word_of(vr[1][0], i8 >> 1), pick);
+                vt.w = __builtin_amdgcn_perm(word_of(vr[1][3], i8 >> 1), word_of(vr[1][2], i8 >> 1), pick);
+                acc[i8] = attend_mfma<DT>(vt, pf, acc[i8]);
+            }
+        }
+    }
+    l = sum_rows(l);
+    lx = sum_rows(lx);
+    if (col < p.G) {
+        float* w = s_dyn + (wave * p.G + col) * AT_PART;
+        if (quad == 0) {
+            w[0] = m;
+            w[1] = l;
+            w[2] = lx;
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {  // dimensions 32 quad + 8 x + i
+            *(float4*)(w + 4 + 32 * quad + 8 * x) = make_float4(acc[0][x], acc[1][x], acc[2][x], acc[3][x]);
+            *(float4*)(w + 8 + 32 * quad + 8 * x) = make_float4(acc[4][x], acc[5][x], acc[6][x], acc[7][x]);
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < p.G * 128; i += AT_THR) {
+        const int g = i >> 7, d = i & 127;
+        const float* w = s_dyn + g * AT_PART;
+        float M = -INFINITY, lt = 0.f, lxt = 0.f, a = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) M = fmaxf(M, w[k * p.G * AT_PART]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float* r = w + k * p.G * AT_PART;
+            // A wave without tokens has reference -inf and sums 0; NaN scores leave sums of NaN.
+            const float f = r[0] == -INFINITY ? 1.f : exp2f(r[0] - M);
+            lt = fmaf(r[1], f, lt);
+            lxt = fmaf(r[2], f, lxt);
+            a = fmaf(r[4 + d], f, a);
+        }
+        const int hq = h * p.G + g;
+        if (p.splits == 1) store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, DT, lt == 0.f ? 0.f : a / lt);
+        if (p.splits > 1 || !SPARSE) {
+            float* pp = p.part + (((int64_t)b * H + hq) * p.splits + s) * AT_PART;
+            if (d == 0) *(float4*)pp = make_float4(M, lt, lxt, 0.f);
+            pp[4 + d] = a;
+        }
+    }
+}
+
+// A head's splits joined: thread d sums dimension d, every thread the references and sums.
+template <int DT>
+__device__ __forceinline__ void attend_merge_head(const AttendParams& p, int b, int hq, int d) {
+    const float* pp = p.part + ((int64_t)b * p.Hkv * p.G + hq) * p.splits * AT_PART;
+    float M = -INFINITY;
+    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, pp[s * AT_PART]);
+    float lt = 0.f, a = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+        const float m = pp[s * AT_PART], f = m == -INFINITY ? 1.f : exp2f(m - M);
+        lt = fmaf(pp[s * AT_PART + 1], f, lt);
+        a = fmaf(pp[s * AT_PART + 4 + d], f, a);
+    }
+    store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, DT, lt == 0.f ? 0.f : a / lt);
+}
+
+// Splits per unit (request and KV head) of at most `pages` pages: workgroups for two a CU, 8 pages a
+// split at least.
+inline int attend_splits(int64_t units, int pages) {
+    int dev = 0, cus = 256, c = 0;
+    if (hipGetDevice(&dev) == hipSuccess &&
+        hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && c > 0)
+        cus = c;
+    const int64_t s = std::min<int64_t>((2 * (int64_t)cus + units - 1) / units, (pages + 7) / 8);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(s, AT_MAX_SPLITS));
+}
+
+inline int block_shift(int block_size) {
+    for (int s = 0; s < 16; ++s)
+        if (block_size == (16 << s)) return s;
+    return -1;
+}
+
+// The checks and fields that both decodes share; STARKV_OK or the error's code.
+inline int attend_setup(AttendParams& p, const char* what, const void* query, int64_t q_s0, int64_t q_s1,
+                        const void* k_cache, const void* v_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype,
+                        int block_size, int64_t num_blocks, const int32_t* block_table, int64_t bt_s0, int64_t bt_s1,
+                        int bt_width, const int32_t* seq_lens, int n, int num_heads, int num_kv_heads, float scale,
+                        void* out, int64_t o_s0, int64_t o_s1, const void* workspace) {
+    SKV_CHECK(query && k_cache && v_cache && block_table && seq_lens && out && workspace, "%s: null pointer", what);
+    SKV_CHECK(num_kv_heads >= 1 && num_heads >= num_kv_heads && num_heads % num_kv_heads == 0 &&
+                  num_heads / num_kv_heads <= AT_MAX_GROUP,
+              "%s: %d query heads over %d KV heads (1 to 16 each)", what, num_heads, num_kv_heads);
+    SKV_CHECK(dtype == STARKV_BF16 || dtype == STARKV_F16, "%s: bf16 or fp16", what);
+    SKV_CHECK(block_shift(block_size) >= 0, "%s: block_size must be 16 times a power of two", what);
+    SKV_CHECK(num_blocks >= 1 && num_blocks <= 0x7fffffff && bt_width >= 1, "%s: empty cache or block table", what);
+    SKV_CHECK(((uintptr_t)query | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 &&
+                  (q_s0 | q_s1 | c_s0 | c_s1 | c_s2) % 8 == 0 && (uintptr_t)workspace % 16 == 0,
+              "%s: rows must be 16-byte aligned", what);
+    p.q = (const uint16_t*)query; p.q_s0 = q_s0; p.q_s1 = q_s1;
+    p.kc = (const uint16_t*)k_cache; p.vc = (const uint16_t*)v_cache;
+    p.c_s0 = c_s0; p.c_s1 = c_s1; p.c_s2 = c_s2;
+    p.bs_shift = block_shift(block_size); p.num_blocks = num_blocks;
+    p.bt = block_table; p.bt_s0 = bt_s0; p.bt_s1 = bt_s1;
+    p.seq_lens = seq_lens;
+    p.span = (int)std::min<int64_t>((int64_t)bt_width * block_size, 0x7ffffff0);
+    p.n = n; p.Hkv = num_kv_heads; p.G = num_heads / num_kv_heads;
+    p.sc = scale * AT_LOG2E;
+    p.out = (uint16_t*)out; p.o_s0 = o_s0; p.o_s1 = o_s1;
+    return STARKV_OK;
+}
+
+template <bool SPARSE>
+inline int attend_launch(void* stream, int dtype, const AttendParams& p) {
+    SKV_CHECK((int64_t)p.n * p.Hkv * p.splits < 1 << 23, "%d requests of %d KV heads in one call", p.n, p.Hkv);
+    const dim3 grid((unsigned)((int64_t)p.n * p.Hkv * p.splits));
+    const size_t lds = (size_t)4 * p.G * AT_PART * 4;
+    if (dtype == STARKV_BF16)
+        hipLaunchKernelGGL((attend_kernel<STARKV_BF16, SPARSE>), grid, dim3(AT_THR), lds, (hipStream_t)stream, p);
+    else
+        hipLaunchKernelGGL((attend_kernel<STARKV_F16, SPARSE>), grid, dim3(AT_THR), lds, (hipStream_t)stream, p);
+    SKV_HIP(hipGetLastError());
+    return STARKV_OK;
+}
+
+}  // namespace starkv

@@ -283,12 +283,13 @@ void prefill_lift(const at::Tensor& k_codes, const at::Tensor& v_codes, const at
 const void* data_of(const std::optional<at::Tensor>& t) { return t ? t->data_ptr() : nullptr; }
 
 // RoPE of q (and k), with the cache write and the fp16 rows of an uncompressed layer; q, k, v
-// [T, heads, 128].
-void rope_qkv(const at::Tensor& q, const std::optional<at::Tensor>& k, const std::optional<at::Tensor>& v,
+// [T, heads, 128]. With q_weight: behind the norms of q's and k's rows.
+void rope_call(const at::Tensor& q, const std::optional<at::Tensor>& k, const std::optional<at::Tensor>& v,
               const at::Tensor& positions, const at::Tensor& cos_sin, const at::Tensor& q_out,
               const std::optional<at::Tensor>& k_out, const std::optional<at::Tensor>& k_cache,
               const std::optional<at::Tensor>& v_cache, const std::optional<at::Tensor>& slots,
-              const std::optional<at::Tensor>& k_half, const std::optional<at::Tensor>& v_half) {
+              const std::optional<at::Tensor>& k_half, const std::optional<at::Tensor>& v_half,
+              const at::Tensor* q_weight, const at::Tensor* k_weight, double eps) {
     const c10::DeviceGuard guard(q.device());
     const int64_t T = q.size(0), H = q.size(1), Hkv = k ? k->size(1) : 0;
     const auto rows = [&](const at::Tensor& t, int64_t heads) {
@@ -313,16 +314,205 @@ void rope_qkv(const at::Tensor& q, const std::optional<at::Tensor>& k, const std
                         k_cache->stride(3) == 1 && k_cache->scalar_type() == q.scalar_type() &&
                         v_cache->scalar_type() == q.scalar_type(),
                     "starkv.rope_qkv: caches");
-    check(starkv_rope_qkv(stream_of(q), q.data_ptr(), q.stride(0), q.stride(1), data_of(k), k ? k->stride(0) : 0,
-                          k ? k->stride(1) : 0, data_of(v), v ? v->stride(0) : 0, v ? v->stride(1) : 0, dtype_code(q),
-                          (int)T, (int)H, (int)Hkv, positions.data_ptr(),
-                          positions.scalar_type() == at::kLong ? 64 : 32, cos_sin.data_ptr(), cos_sin.stride(0),
-                          dtype_code(cos_sin), cos_sin.size(0), q_out.data_ptr(), (void*)data_of(k_out),
-                          (void*)data_of(k_cache), (void*)data_of(v_cache), k_cache ? k_cache->stride(0) : 0,
-                          k_cache ? k_cache->stride(1) : 0, k_cache ? k_cache->stride(2) : 0,
-                          k_cache ? (int)k_cache->size(1) : 0, k_cache ? k_cache->size(0) : 0, data_of(slots),
-                          slots ? slot_bits(*slots) : 64, (void*)data_of(k_half), (void*)data_of(v_half)),
+    const int64_t s0 = k ? k->stride(0) : 0, s1 = k ? k->stride(1) : 0, v0 = v ? v->stride(0) : 0, v1 = v ? v->stride(1) : 0;
+    const int64_t c0 = k_cache ? k_cache->stride(0) : 0, c1 = k_cache ? k_cache->stride(1) : 0,
+                  c2 = k_cache ? k_cache->stride(2) : 0;
+    const int pos_bits = positions.scalar_type() == at::kLong ? 64 : 32, bits = slots ? slot_bits(*slots) : 64;
+    const int block_size = k_cache ? (int)k_cache->size(1) : 0;
+    const int64_t blocks = k_cache ? k_cache->size(0) : 0;
+    if (q_weight) {
+        for (const auto* w : {q_weight, k_weight})
+            TORCH_CHECK(!w || (w->is_contiguous() && w->numel() == 128 && w->scalar_type() == q_weight->scalar_type()),
+                        "starkv.norm_rope_qkv: weights [128] of one dtype");
+        check(starkv_norm_rope_qkv(stream_of(q), q.data_ptr(), q.stride(0), q.stride(1), data_of(k), s0, s1, data_of(v),
+                                   v0, v1, dtype_code(q), (int)T, (int)H, (int)Hkv, q_weight->data_ptr(),
+                                   k_weight ? k_weight->data_ptr() : nullptr, dtype_code(*q_weight), (float)eps,
+                                   positions.data_ptr(), pos_bits, cos_sin.data_ptr(), cos_sin.stride(0),
+                                   dtype_code(cos_sin), cos_sin.size(0), q_out.data_ptr(), (void*)data_of(k_out),
+                                   (void*)data_of(k_cache), (void*)data_of(v_cache), c0, c1, c2, block_size, blocks,
+                                   data_of(slots), bits, (void*)data_of(k_half), (void*)data_of(v_half)),
+              "norm_rope_qkv");
+        return;
+    }
+    check(starkv_rope_qkv(stream_of(q), q.data_ptr(), q.stride(0), q.stride(1), data_of(k), s0, s1, data_of(v), v0, v1,
+                          dtype_code(q), (int)T, (int)H, (int)Hkv, positions.data_ptr(), pos_bits, cos_sin.data_ptr(),
+                          cos_sin.stride(0), dtype_code(cos_sin), cos_sin.size(0), q_out.data_ptr(),
+                          (void*)data_of(k_out), (void*)data_of(k_cache), (void*)data_of(v_cache), c0, c1, c2,
+                          block_size, blocks, data_of(slots), bits, (void*)data_of(k_half), (void*)data_of(v_half)),
           "rope_qkv");
+}
+
+void rope_qkv(const at::Tensor& q, const std::optional<at::Tensor>& k, const std::optional<at::Tensor>& v,
+              const at::Tensor& positions, const at::Tensor& cos_sin, const at::Tensor& q_out,
+              const std::optional<at::Tensor>& k_out, const std::optional<at::Tensor>& k_cache,
+              const std::optional<at::Tensor>& v_cache, const std::optional<at::Tensor>& slots,
+              const std::optional<at::Tensor>& k_half, const std::optional<at::Tensor>& v_half) {
+    rope_call(q, k, v, positions, cos_sin, q_out, k_out, k_cache, v_cache, slots, k_half, v_half, nullptr, nullptr, 0.0);
+}
+
+void norm_rope_qkv(const at::Tensor& q, const std::optional<at::Tensor>& k, const std::optional<at::Tensor>& v,
+                   const at::Tensor& q_weight, const std::optional<at::Tensor>& k_weight, double eps,
+                   const at::Tensor& positions, const at::Tensor& cos_sin, const at::Tensor& q_out,
+                   const std::optional<at::Tensor>& k_out, const std::optional<at::Tensor>& k_cache,
+                   const std::optional<at::Tensor>& v_cache, const std::optional<at::Tensor>& slots,
+                   const std::optional<at::Tensor>& k_half, const std::optional<at::Tensor>& v_half) {
+    rope_call(q, k, v, positions, cos_sin, q_out, k_out, k_cache, v_cache, slots, k_half, v_half, &q_weight,
+              k_weight ? &*k_weight : nullptr, eps);
+}
+
+// The paged caches [num_blocks, block_size, heads, 128] that an operator reads, of one dtype and layout.
+void check_caches(const at::Tensor& k_cache, const at::Tensor& v_cache, const char* what) {
+    TORCH_CHECK(k_cache.dim() == 4 && k_cache.size(3) == 128 && k_cache.stride(3) == 1 &&
+                    k_cache.sizes() == v_cache.sizes() && k_cache.strides() == v_cache.strides() &&
+                    k_cache.scalar_type() == v_cache.scalar_type(),
+                "starkv.", what, ": caches [blocks, block_size, heads, 128] of one dtype and layout");
+}
+
+// block_table [n, width] and seq_lens [n].
+void check_table(const at::Tensor& block_table, const at::Tensor& seq_lens, int64_t n, const char* what) {
+    TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == n && block_table.size(1) >= 1 && seq_lens.dim() == 1 &&
+                    seq_lens.size(0) == n,
+                "starkv.", what, ": block_table [n, blocks] and seq_lens [n]");
+}
+
+void check_query(const at::Tensor& query, const at::Tensor& like, int64_t heads, const char* what) {
+    TORCH_CHECK(query.dim() == 3 && query.size(2) == 128 && query.stride(2) == 1 && query.size(1) % heads == 0 &&
+                    query.scalar_type() == like.scalar_type(),
+                "starkv.", what, ": query [n, heads, 128] of the cache's dtype");
+}
+
+int as_int(int64_t v, const char* name) {
+    TORCH_CHECK(v >= INT32_MIN && v <= INT32_MAX, "starkv: ", name, " = ", v);
+    return (int)v;
+}
+
+// The least and largest key of the blocks that hold a request's last max_new tokens.
+void key_bounds(const at::Tensor& k_cache, const at::Tensor& bounds, const at::Tensor& block_table,
+                const at::Tensor& seq_lens, int64_t max_new) {
+    const c10::DeviceGuard guard(k_cache.device());
+    check_caches(k_cache, k_cache, "key_bounds");
+    check_table(block_table, seq_lens, block_table.size(0), "key_bounds");
+    TORCH_CHECK(bounds.dim() == 4 && bounds.size(0) == k_cache.size(0) && bounds.size(1) == k_cache.size(2) &&
+                    bounds.size(2) == 2 && bounds.size(3) == 128 && bounds.stride(3) == 1 &&
+                    bounds.scalar_type() == k_cache.scalar_type(),
+                "starkv.key_bounds: bounds [blocks, heads, 2, 128] of the cache's dtype");
+    check(starkv_key_bounds(stream_of(k_cache), k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
+                            k_cache.stride(2), dtype_code(k_cache), (int)k_cache.size(1), k_cache.size(0),
+                            bounds.data_ptr(), bounds.stride(0), bounds.stride(1), bounds.stride(2),
+                            i32(block_table, "block_table"), block_table.stride(0), block_table.stride(1),
+                            (int)block_table.size(1), i32(seq_lens, "seq_lens"), (int)block_table.size(0),
+                            (int)k_cache.size(2), as_int(max_new, "max_new")),
+          "key_bounds");
+}
+
+// The blocks that each request and KV head reads, by the bounds' scores.
+void select_blocks(const at::Tensor& query, const at::Tensor& bounds, const at::Tensor& block_table,
+                   const at::Tensor& seq_lens, int64_t max_seq_len, int64_t block_size, int64_t sink, int64_t recent,
+                   const at::Tensor& selected) {
+    const c10::DeviceGuard guard(query.device());
+    const int64_t n = query.size(0);
+    TORCH_CHECK(bounds.dim() == 4 && bounds.size(2) == 2 && bounds.size(3) == 128 && bounds.stride(3) == 1,
+                "starkv.select_blocks: bounds [blocks, heads, 2, 128]");
+    const int Hkv = (int)bounds.size(1);
+    check_query(query, bounds, Hkv, "select_blocks");
+    check_table(block_table, seq_lens, n, "select_blocks");
+    TORCH_CHECK(selected.dim() == 3 && selected.size(0) == n && selected.size(1) == Hkv,
+                "starkv.select_blocks: selected [n, heads, keep]");
+    const int span = as_int(max_seq_len, "max_seq_len"), bs = as_int(block_size, "block_size");
+    const at::Tensor ws = workspace(
+        query, starkv_select_blocks_workspace_bytes((int)n, Hkv, (int)block_table.size(1), bs, span));
+    check(starkv_select_blocks(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), bounds.data_ptr(),
+                               bounds.stride(0), bounds.stride(1), bounds.stride(2), dtype_code(bounds), bs,
+                               bounds.size(0), i32(block_table, "block_table"), block_table.stride(0),
+                               block_table.stride(1), (int)block_table.size(1), i32(seq_lens, "seq_lens"), (int)n,
+                               (int)query.size(1), Hkv, span, as_int(selected.size(2), "keep"), as_int(sink, "sink"),
+                               as_int(recent, "recent"), (int32_t*)i32(selected, "selected"), ws.data_ptr(),
+                               (size_t)ws.numel()),
+          "select_blocks");
+}
+
+// One token's attention over the selected blocks.
+void sparse_decode(const at::Tensor& query, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                   const at::Tensor& block_table, const at::Tensor& seq_lens, const at::Tensor& selected, double scale,
+                   const at::Tensor& out) {
+    const c10::DeviceGuard guard(query.device());
+    const int64_t n = query.size(0);
+    check_caches(k_cache, v_cache, "sparse_decode");
+    const int H = (int)query.size(1), Hkv = (int)k_cache.size(2), bs = (int)k_cache.size(1);
+    check_query(query, k_cache, Hkv, "sparse_decode");
+    check_query(out, k_cache, Hkv, "sparse_decode");
+    check_table(block_table, seq_lens, n, "sparse_decode");
+    TORCH_CHECK(out.sizes() == query.sizes(), "starkv.sparse_decode: out as query");
+    TORCH_CHECK(selected.dim() == 3 && selected.size(0) == n && selected.size(1) == Hkv && selected.size(2) >= 1 &&
+                    selected.stride(2) == 1 && selected.scalar_type() == at::kInt,
+                "starkv.sparse_decode: selected [n, heads, keep] int32");
+    const int keep = as_int(selected.size(2), "keep");
+    const at::Tensor ws = workspace(query, starkv_sparse_decode_workspace_bytes((int)n, H, Hkv, bs, keep));
+    check(starkv_sparse_decode(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), k_cache.data_ptr(),
+                               v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+                               dtype_code(k_cache), bs, k_cache.size(0), i32(block_table, "block_table"),
+                               block_table.stride(0), block_table.stride(1), (int)block_table.size(1),
+                               i32(seq_lens, "seq_lens"), (int)n, H, Hkv, selected.data_ptr<int32_t>(),
+                               selected.stride(0), selected.stride(1), keep, (float)scale, out.data_ptr(),
+                               out.stride(0), out.stride(1), ws.data_ptr(), (size_t)ws.numel()),
+          "sparse_decode");
+}
+
+void check_weights(const at::Tensor& weights, int64_t n, int64_t heads, const char* what) {
+    TORCH_CHECK(weights.dim() == 3 && weights.size(0) == n && weights.size(1) == heads && weights.size(2) >= 1 &&
+                    weights.stride(2) == 1 && weights.scalar_type() == at::kFloat,
+                "starkv.", what, ": weights [n, heads, tokens] fp32");
+}
+
+// A decode over the whole cache that adds each token's weight to `weights`.
+void weighted_decode(const at::Tensor& query, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                     const at::Tensor& block_table, const at::Tensor& seq_lens, int64_t max_seq_len, double scale,
+                     const at::Tensor& weights, const at::Tensor& out) {
+    const c10::DeviceGuard guard(query.device());
+    const int64_t n = query.size(0);
+    check_caches(k_cache, v_cache, "weighted_decode");
+    const int H = (int)query.size(1), Hkv = (int)k_cache.size(2);
+    check_query(query, k_cache, Hkv, "weighted_decode");
+    check_query(out, k_cache, Hkv, "weighted_decode");
+    check_table(block_table, seq_lens, n, "weighted_decode");
+    check_weights(weights, n, Hkv, "weighted_decode");
+    TORCH_CHECK(out.sizes() == query.sizes(), "starkv.weighted_decode: out as query");
+    const int span = as_int(max_seq_len, "max_seq_len");
+    const at::Tensor ws = workspace(query, starkv_weighted_decode_workspace_bytes((int)n, H, Hkv, span));
+    check(starkv_weighted_decode(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1),
+                                 k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
+                                 k_cache.stride(2), dtype_code(k_cache), (int)k_cache.size(1), k_cache.size(0),
+                                 i32(block_table, "block_table"), block_table.stride(0), block_table.stride(1),
+                                 (int)block_table.size(1), i32(seq_lens, "seq_lens"), (int)n, H, Hkv, span,
+                                 (float)scale, weights.data_ptr<float>(), weights.stride(0), weights.stride(1),
+                                 as_int(weights.size(2), "weights"), out.data_ptr(), out.stride(0), out.stride(1),
+                                 ws.data_ptr(), (size_t)ws.numel()),
+          "weighted_decode");
+}
+
+// Caches cut to `keep` tokens a request and KV head, in place.
+void evict(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& block_table,
+           const at::Tensor& seq_lens, const at::Tensor& weights, int64_t keep, int64_t sink, int64_t recent,
+           const at::Tensor& new_lens, const at::Tensor& new_weights) {
+    const c10::DeviceGuard guard(k_cache.device());
+    const int64_t n = block_table.size(0);
+    check_caches(k_cache, v_cache, "evict");
+    check_table(block_table, seq_lens, n, "evict");
+    check_weights(weights, n, k_cache.size(2), "evict");
+    TORCH_CHECK(new_lens.sizes() == seq_lens.sizes() && new_weights.sizes() == weights.sizes() &&
+                    new_weights.is_contiguous() && new_weights.scalar_type() == at::kFloat,
+                "starkv.evict: new_lens and new_weights as seq_lens and weights");
+    const int k = as_int(keep, "keep");
+    const at::Tensor ws = workspace(k_cache, starkv_evict_workspace_bytes((int)n, (int)k_cache.size(2), k));
+    check(starkv_evict(stream_of(k_cache), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
+                       k_cache.stride(2), dtype_code(k_cache), (int)k_cache.size(1), k_cache.size(0),
+                       i32(block_table, "block_table"), block_table.stride(0), block_table.stride(1),
+                       (int)block_table.size(1), i32(seq_lens, "seq_lens"), (int)n, (int)k_cache.size(2),
+                       weights.data_ptr<float>(), weights.stride(0), weights.stride(1),
+                       as_int(weights.size(2), "weights"), k, as_int(sink, "sink"), as_int(recent, "recent"),
+                       (int32_t*)i32(new_lens, "new_lens"), new_weights.data_ptr<float>(), ws.data_ptr(),
+                       (size_t)ws.numel()),
+          "evict");
 }
 
 // A decode step's slots (int64) and lengths (int32) from its positions (int64).
@@ -416,6 +606,18 @@ TORCH_LIBRARY(starkv, m) {
     m.def("rope_qkv(Tensor q, Tensor? k, Tensor? v, Tensor positions, Tensor cos_sin, Tensor(a!) q_out, "
           "Tensor(b!)? k_out, Tensor(c!)? k_cache, Tensor(d!)? v_cache, Tensor? slots, Tensor(e!)? k_half, "
           "Tensor(f!)? v_half) -> ()");
+    m.def("norm_rope_qkv(Tensor q, Tensor? k, Tensor? v, Tensor q_weight, Tensor? k_weight, float eps, "
+          "Tensor positions, Tensor cos_sin, Tensor(a!) q_out, Tensor(b!)? k_out, Tensor(c!)? k_cache, "
+          "Tensor(d!)? v_cache, Tensor? slots, Tensor(e!)? k_half, Tensor(f!)? v_half) -> ()");
+    m.def("key_bounds(Tensor k_cache, Tensor(a!) bounds, Tensor block_table, Tensor seq_lens, int max_new) -> ()");
+    m.def("select_blocks(Tensor query, Tensor bounds, Tensor block_table, Tensor seq_lens, int max_seq_len, "
+          "int block_size, int sink, int recent, Tensor(a!) selected) -> ()");
+    m.def("sparse_decode(Tensor query, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, "
+          "Tensor selected, float scale, Tensor(a!) out) -> ()");
+    m.def("weighted_decode(Tensor query, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, "
+          "int max_seq_len, float scale, Tensor(a!) weights, Tensor(b!) out) -> ()");
+    m.def("evict(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor seq_lens, Tensor weights, "
+          "int keep, int sink, int recent, Tensor(c!) new_lens, Tensor(d!) new_weights) -> ()");
     m.def("decode_slots(Tensor block_table, Tensor positions, int block_size, Tensor(a!) slots, "
           "Tensor(b!) seq_lens) -> ()");
     m.def("greedy_step(Tensor logits, Tensor(a!) tokens, Tensor(b!) positions) -> ()");
@@ -438,6 +640,12 @@ TORCH_LIBRARY_IMPL(starkv, CUDA, m) {
     m.impl("stock_write", &stock_write);
     m.impl("prefill", &prefill);
     m.impl("rope_qkv", &rope_qkv);
+    m.impl("norm_rope_qkv", &norm_rope_qkv);
+    m.impl("key_bounds", &key_bounds);
+    m.impl("select_blocks", &select_blocks);
+    m.impl("sparse_decode", &sparse_decode);
+    m.impl("weighted_decode", &weighted_decode);
+    m.impl("evict", &evict);
     m.impl("decode_slots", &decode_slots);
     m.impl("greedy_step", &greedy_step);
     m.impl("silu_mul", &silu_mul);

@@ -19,7 +19,7 @@ import torch
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libstarkv_hip.so")
 OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libstarkv_torch.so")
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 F32, F16, BF16 = 0, 1, 2
 CACHE_Q3_2 = 16  # cache kind of the 3.2-bit QuantRow cache
@@ -65,6 +65,23 @@ SIGNATURES = {
     "starkv_prefill_to_half": (_I, [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _I, _I]),
     "starkv_prefill_lift": (_I, [_P, _P, _I64, _P, _I64, _I, _I, _P, _I, _P, _I64, _P, _P, _I, _P, _I64, _I, _P,
                                  _P, _I]),
+    "starkv_norm_rope_qkv": (_I, [_P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I, _I, _I, _I, _P, _P, _I, _F,
+                                  _P, _I, _P, _I64, _I, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I, _I64, _P, _I, _P,
+                                  _P]),
+    "starkv_key_bounds": (_I, [_P, _P, _I64, _I64, _I64, _I, _I, _I64, _P, _I64, _I64, _I64, _P, _I64, _I64, _I, _P, _I,
+                               _I, _I]),
+    "starkv_select_blocks_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "starkv_select_blocks": (_I, [_P, _P, _I64, _I64, _P, _I64, _I64, _I64, _I, _I, _I64, _P, _I64, _I64, _I, _P, _I,
+                                  _I, _I, _I, _I, _I, _I, _P, _P, _SZ]),
+    "starkv_sparse_decode_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "starkv_sparse_decode": (_I, [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _I64, _P, _I64, _I64, _I, _P,
+                                  _I, _I, _I, _P, _I64, _I64, _I, _F, _P, _I64, _I64, _P, _SZ]),
+    "starkv_weighted_decode_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
+    "starkv_weighted_decode": (_I, [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _I64, _P, _I64, _I64, _I, _P,
+                                    _I, _I, _I, _I, _F, _P, _I64, _I64, _I, _P, _I64, _I64, _P, _SZ]),
+    "starkv_evict_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "starkv_evict": (_I, [_P, _P, _P, _I64, _I64, _I64, _I, _I, _I64, _P, _I64, _I64, _I, _P, _I, _I, _P, _I64, _I64,
+                          _I, _I, _I, _I, _P, _P, _P, _SZ]),
     "starkv_profile_begin": (_I, [_I, _I]),
     "starkv_profile_end": (_I, [ctypes.POINTER(ctypes.c_double), ctypes.POINTER(_I)]),
     "starkv_profile_times": (_I, [ctypes.POINTER(ctypes.c_double), _I]),
@@ -225,3 +242,9 @@ def require_cuda(*ts: torch.Tensor) -> None:
                                f"{t.device}")
         if t.device != dev:
             raise RuntimeError(f"tensors on different devices: {dev} vs {t.device}")
+
+
+def refuse_grad(what: str, *ts: torch.Tensor) -> None:
+    """Serving operators without a backward: a result that looks differentiable and is not would be silent."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise NotImplementedError(f"{what} has no gradient; call it under torch.no_grad()")
