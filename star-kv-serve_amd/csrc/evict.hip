@@ -32,14 +32,14 @@ struct WeighParams {
 constexpr int WG_TOKENS = 1024;
 
 // blockIdx.x < chunks: weights of WG_TOKENS tokens of a (request, KV head); behind them, where there are
-// splits, two query heads' outputs a workgroup.
+// splits, four query heads' outputs a workgroup.
 template <int DT>
 __global__ __launch_bounds__(256) void weigh_kernel(const WeighParams wp) {
     const AttendParams& p = wp.a;
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, H = p.Hkv * p.G;
     if ((int)blockIdx.x >= wp.chunks) {
-        const int g = 2 * (blockIdx.x - wp.chunks) + (tid >> 7);
-        if (g < p.G) attend_merge_head<DT>(p, b, h * p.G + g, tid & 127);
+        const int g = 4 * (blockIdx.x - wp.chunks) + (tid >> 6);
+        if (g < p.G) attend_merge_head<DT>(p, b, h * p.G + g);
         return;
     }
     const int L = attend_length(p, b), t0 = blockIdx.x * WG_TOKENS;
@@ -49,26 +49,44 @@ __global__ __launch_bounds__(256) void weigh_kernel(const WeighParams wp) {
     const int g16 = tid >> 4;
     if (g16 < p.G) {
         const float* pp = p.part + ((int64_t)b * H + h * p.G + g16) * p.splits * AT_PART;
-        float M = -INFINITY, l = 0.f;
-        for (int s = tid & 15; s < p.splits; s += 16) M = fmaxf(M, pp[s * AT_PART]);
-        M = row16_max(M);
-        for (int s = tid & 15; s < p.splits; s += 16) {
-            const float m = pp[s * AT_PART];
-            l = fmaf(pp[s * AT_PART + 2], m == -INFINITY ? 1.f : exp2f(m - M), l);
+        float m[AT_MAX_SPLITS / 16], l[AT_MAX_SPLITS / 16], M = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int x = 0; x < AT_MAX_SPLITS / 16; ++x) {
+            const int s = (tid & 15) + 16 * x;
+            m[x] = s < p.splits ? pp[s * AT_PART] : -INFINITY;
+            l[x] = s < p.splits ? pp[s * AT_PART + 1] : 0.f;
+            M = fmaxf(M, m[x]);
         }
-        l = row16_sum(l);
-        if ((tid & 15) == 0) s_lse[g16] = l == 0.f ? 0.f : M + log2f(l);  // no block of the cache: weights of 0
+        M = row16_max(M);
+#pragma unroll
+        for (int x = 0; x < AT_MAX_SPLITS / 16; ++x) sum = fmaf(l[x], m[x] == -INFINITY ? 1.f : exp2f(m[x] - M), sum);
+        sum = row16_sum(sum);
+        if ((tid & 15) == 0) s_lse[g16] = sum == 0.f ? 0.f : M + log2f(sum);  // no block of the cache: weights of 0
     }
     __syncthreads();
-    const float* lg = p.lg + ((int64_t)b * H + h * p.G) * p.lg_row;
+    const float* lg = p.lg + ((int64_t)b * p.Hkv + h) * p.lg_row;
     float* w = wp.w + b * wp.w_s0 + h * wp.w_s1;
+    constexpr int U = WG_TOKENS / 256;
+    float old[U], sum[U];
+    const float* at[U];
 #pragma unroll
-    for (int u = 0; u < WG_TOKENS / 256; ++u) {
+    for (int u = 0; u < U; ++u) {
+        const int t = min(t0 + 256 * u + tid, L - 1);
+        at[u] = lg + (int64_t)(t >> 4) * p.G * 16 + (t & 15);
+        old[u] = w[t];
+        sum[u] = 0.f;
+    }
+    for (int g = 0; g < p.G; ++g) {
+        float s[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) s[u] = at[u][16 * g];
+#pragma unroll
+        for (int u = 0; u < U; ++u) sum[u] += exp2f(s[u] - s_lse[g]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
         const int t = t0 + 256 * u + tid;
-        if (t >= L) return;
-        float sum = 0.f;
-        for (int g = 0; g < p.G; ++g) sum += exp2f(lg[g * p.lg_row + t] - s_lse[g]);
-        w[t] = t == L - 1 ? sum : w[t] + sum;
+        if (t < L) w[t] = t == L - 1 ? sum[u] : old[u] + sum[u];
     }
 }
 
@@ -79,76 +97,104 @@ struct EvictParams {
     const float* w; int64_t w_s0, w_s1;
     int Hkv, cap, keep, sink, recent;
     int32_t* new_lens; float* new_w;  // [n], [n][Hkv][cap]
-    int32_t* kept;                    // [n][Hkv][keep]
+    int32_t* kept;                    // [n][Hkv][keep]: the kept tokens' rows of the cache, -1 for none
 };
 
 __device__ __forceinline__ int evict_length(const EvictParams& p, int b) { return min(max(p.seq_lens[b], 0), p.span); }
 
-constexpr int EV_THR = 1024;
-constexpr int EV_LDS = 12288;  // keys of a row kept in LDS
+// Token t's row in a cache of rows, -1 where its block is none of the cache's.
+__device__ __forceinline__ int evict_row(const EvictParams& p, const int32_t* bt, int t) {
+    const int blk = bt[(t >> p.block_shift) * p.bt_s1];
+    return blk < 0 || blk >= p.num_blocks ? -1 : (blk << p.block_shift) + (t & ((1 << p.block_shift) - 1));
+}
 
-template <bool IN_LDS>
-__global__ __launch_bounds__(EV_THR) void evict_select_kernel(const EvictParams p) {
-    __shared__ TopkShared<EV_THR> sh;
-    __shared__ uint32_t s_key[IN_LDS ? EV_LDS : 1];
+template <bool KEPT>
+__global__ __launch_bounds__(TK_THR) void evict_select_kernel(const EvictParams p) {
+    __shared__ TopkShared sh;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     const int L = evict_length(p, b), left = min(L, p.keep);
     const float* w = p.w + b * p.w_s0 + h * p.w_s1;
     float* nw = p.new_w + ((int64_t)b * p.Hkv + h) * p.cap;
     if (h == 0 && tid == 0) p.new_lens[b] = left;
-    for (int i = left + tid; i < p.cap; i += EV_THR) nw[i] = 0.f;
+    for (int i = left + tid; i < p.cap; i += TK_THR) nw[i] = 0.f;
     if (L <= p.keep) {
-        for (int i = tid; i < L; i += EV_THR) nw[i] = w[i];
+        for (int i = tid; i < L; i += TK_THR) nw[i] = w[i];
         return;
     }
     int32_t* kept = p.kept + ((int64_t)b * p.Hkv + h) * p.keep;
+    const int32_t* bt = p.bt + b * p.bt_s0;
     const int middle = L - p.sink - p.recent, k = p.keep - p.sink - p.recent;
-    for (int i = tid; i < p.sink + p.recent; i += EV_THR) {
+    for (int i = tid; i < p.sink + p.recent; i += TK_THR) {
         const int from = i < p.sink ? i : middle + i, to = i < p.sink ? i : k + i;
-        kept[to] = from;
+        kept[to] = evict_row(p, bt, from);
         nw[to] = w[from];
     }
     if (k == 0) return;
     w += p.sink;
-    if constexpr (IN_LDS) {
-        for (int i = tid; i < middle; i += EV_THR) s_key[i] = order_key(w[i]);
-        __syncthreads();
-    }
-    topk_ascending<EV_THR>(
-        sh, middle, k, [&](int i) { return IN_LDS ? s_key[i] : order_key(w[i]); },
-        [&](int pos, int i) {
-            kept[p.sink + pos] = p.sink + i;
-            nw[p.sink + pos] = w[i];
-        });
+    topk_ascending<KEPT>(sh, middle, k, [&](int i) { return w[i]; },
+                         [&](int pos, int i, float x) {
+                             kept[p.sink + pos] = evict_row(p, bt, p.sink + i);
+                             nw[p.sink + pos] = x;
+                         });
 }
 
-constexpr int CP_THR = 1024, CP_U = 4;  // 128 rows of 128 bytes a round, four rounds a chunk
+constexpr int CP_THR = 1024, CP_U = 4;
 
-__global__ __launch_bounds__(CP_THR) void compact_kernel(const EvictParams p) {
+// A round: CP_U rows' slices of a lane, on their way or read.
+struct Round {
+    uint4 v[CP_U];
+    int64_t to[CP_U];  // element offset of the target, -1: stays
+};
+
+// 2^lanes lanes a row's slice of 16 << lanes bytes, CP_U slices a lane and chunk. Two chunks are on their way
+// at a time: a chunk is written behind a barrier that waits for its own rows only.
+__global__ __launch_bounds__(CP_THR) void compact_kernel(const EvictParams p, int lanes) {
     const int h = blockIdx.y, b = blockIdx.z;
     if (evict_length(p, b) <= p.keep) return;
-    uint16_t* c = (blockIdx.x & 1 ? p.vc : p.kc) + h * p.c_s2 + (blockIdx.x >> 1) * 64 + 8 * (threadIdx.x & 7);
-    const int row = threadIdx.x >> 3, mask = (1 << p.block_shift) - 1;
+    const int slice = threadIdx.x & ((1 << lanes) - 1), row = threadIdx.x >> lanes, step = CP_THR >> lanes;
+    uint16_t* c = (blockIdx.x & 1 ? p.vc : p.kc) + h * p.c_s2 + ((blockIdx.x >> 1) << lanes) * 8 + 8 * slice;
+    const int mask = (1 << p.block_shift) - 1, chunk = CP_U * step;
     const int32_t* kept = p.kept + ((int64_t)b * p.Hkv + h) * p.keep;
     const int32_t* bt = p.bt + b * p.bt_s0;
-    for (int j0 = 0; j0 < p.keep; j0 += CP_U * CP_THR / 8) {
-        uint4 v[CP_U];
-        uint16_t* to[CP_U];
+    int from[CP_U], to[CP_U];  // the rows of the chunk after those on their way
+    const auto places = [&](int j0) {
 #pragma unroll
         for (int u = 0; u < CP_U; ++u) {
-            const int j = j0 + u * (CP_THR / 8) + row;
-            const int from = j < p.keep ? kept[j] : j;
-            to[u] = nullptr;
-            if (from == j) continue;
-            const int sb = bt[(from >> p.block_shift) * p.bt_s1], db = bt[(j >> p.block_shift) * p.bt_s1];
-            if (sb < 0 || sb >= p.num_blocks || db < 0 || db >= p.num_blocks) continue;
-            v[u] = *(const uint4*)(c + sb * p.c_s0 + (from & mask) * p.c_s1);
-            to[u] = c + db * p.c_s0 + (j & mask) * p.c_s1;
+            const int j = min(j0 + u * step + row, p.keep - 1);
+            from[u] = kept[j];
+            to[u] = evict_row(p, bt, j);
+            if (j0 + u * step + row >= p.keep) from[u] = -1;
         }
-        __syncthreads();  // every row of the chunk is read
+    };
+    const auto offset = [&](int r) { return (r >> p.block_shift) * p.c_s0 + (r & mask) * p.c_s1; };
+    const auto read = [&](Round& r) {
+#pragma unroll
+        for (int u = 0; u < CP_U; ++u) {
+            const bool moves = from[u] >= 0 && to[u] >= 0 && from[u] != to[u];
+            r.to[u] = moves ? offset(to[u]) : -1;
+            r.v[u] = make_uint4(0, 0, 0, 0);
+            if (moves) r.v[u] = *(const uint4*)(c + offset(from[u]));
+        }
+    };
+    const auto write = [&](Round& r) {
+#pragma unroll
+        for (int u = 0; u < CP_U; ++u) asm volatile("" : "+v"(r.v[u].x), "+v"(r.v[u].y), "+v"(r.v[u].z), "+v"(r.v[u].w));
+        lds_barrier();  // every lane has its rows of this chunk
 #pragma unroll
         for (int u = 0; u < CP_U; ++u)
-            if (to[u]) *(uint4*)to[u] = v[u];
+            if (r.to[u] >= 0) *(uint4*)(c + r.to[u]) = r.v[u];
+    };
+    Round x, y;
+    places(0);
+    read(x);
+    places(chunk);
+    for (int j0 = 0; j0 < p.keep; j0 += 2 * chunk) {
+        read(y);
+        places(j0 + 2 * chunk);
+        write(x);
+        read(x);
+        places(j0 + 3 * chunk);
+        write(y);
     }
 }
 
@@ -164,8 +210,10 @@ static size_t weighted_logits_bytes(int n, int num_heads, int max_seq_len) {
     return (size_t)n * num_heads * (((size_t)max_seq_len + 15) / 16 * 16) * 4;
 }
 
+// Requests of one call differ in length: many workgroups, of which the short requests' end at once. 24 requests of
+// 1000 to 8191 tokens over 8 KV heads 141 us with workgroups for 2 a CU, 120 for 4, 110 for 8, 108 for 16.
 static int weighted_splits(int n, int num_kv_heads, int max_seq_len) {
-    return attend_splits((int64_t)n * num_kv_heads, (int)(((int64_t)max_seq_len + 15) / 16));
+    return attend_splits((int64_t)n * num_kv_heads, (int)(((int64_t)max_seq_len + 15) / 16), 16, 16);
 }
 
 size_t starkv_weighted_decode_workspace_bytes(int n, int num_heads, int num_kv_heads, int max_seq_len) {
@@ -200,13 +248,13 @@ int starkv_weighted_decode(void* stream, const void* query, int64_t q_s0, int64_
     p.splits = weighted_splits(n, num_kv_heads, max_seq_len);
     p.pps = (pages + p.splits - 1) / p.splits;
     p.lg = (float*)workspace;
-    p.lg_row = ((int64_t)max_seq_len + 15) / 16 * 16;
+    p.lg_row = ((int64_t)max_seq_len + 15) / 16 * 16 * p.G;
     p.part = (float*)((char*)workspace + weighted_logits_bytes(n, num_heads, max_seq_len));
     wp.w = weights; wp.w_s0 = w_s0; wp.w_s1 = w_s1;
     wp.chunks = (p.span + WG_TOKENS - 1) / WG_TOKENS;
     const int err = attend_launch<false>(stream, dtype, p);
     if (err != STARKV_OK) return err;
-    const dim3 grid(wp.chunks + (p.splits > 1 ? (p.G + 1) / 2 : 0), num_kv_heads, n);
+    const dim3 grid(wp.chunks + (p.splits > 1 ? (p.G + 3) / 4 : 0), num_kv_heads, n);
     if (dtype == STARKV_BF16)
         hipLaunchKernelGGL(weigh_kernel<STARKV_BF16>, grid, dim3(256), 0, (hipStream_t)stream, wp);
     else
@@ -235,8 +283,8 @@ int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64
               "evict: null pointer");
     SKV_CHECK(dtype == STARKV_BF16 || dtype == STARKV_F16, "evict: bf16 or fp16");
     SKV_CHECK(block_shift(block_size) >= 0, "evict: block_size must be 16 times a power of two");
-    SKV_CHECK(num_blocks >= 1 && num_blocks <= 0x7fffffff && bt_width >= 1 && weights_len >= 1,
-              "evict: empty cache, block table or weights");
+    SKV_CHECK(num_blocks >= 1 && num_blocks * block_size <= 0x7fffffff && bt_width >= 1 && weights_len >= 1,
+              "evict: empty cache, block table or weights, or a cache of more than 2^31 rows");
     SKV_CHECK(((uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 && (c_s0 | c_s1 | c_s2) % 8 == 0,
               "evict: cache rows must be 16-byte aligned");
     const size_t need = starkv_evict_workspace_bytes(n, num_kv_heads, keep);
@@ -249,13 +297,18 @@ int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64
     p.w = weights; p.w_s0 = w_s0; p.w_s1 = w_s1;
     p.Hkv = num_kv_heads; p.cap = weights_len; p.keep = keep; p.sink = sink; p.recent = recent;
     p.new_lens = new_lens; p.new_w = new_weights; p.kept = (int32_t*)workspace;
-    if (p.span <= EV_LDS)
-        hipLaunchKernelGGL(evict_select_kernel<true>, dim3(num_kv_heads, n), dim3(EV_THR), 0, (hipStream_t)stream, p);
+    if (p.span <= TK_KEPT)
+        hipLaunchKernelGGL(evict_select_kernel<true>, dim3(num_kv_heads, n), dim3(TK_THR), 0, (hipStream_t)stream, p);
     else
-        hipLaunchKernelGGL(evict_select_kernel<false>, dim3(num_kv_heads, n), dim3(EV_THR), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL(evict_select_kernel<false>, dim3(num_kv_heads, n), dim3(TK_THR), 0, (hipStream_t)stream, p);
     SKV_HIP(hipGetLastError());
     if (p.span > keep) {
-        hipLaunchKernelGGL(compact_kernel, dim3(4, num_kv_heads, n), dim3(CP_THR), 0, (hipStream_t)stream, p);
+        // Whole rows a workgroup where those fill 256 CUs, else their halves: 8192 -> 2048 tokens of 16 requests of
+        // 8 KV heads 81 us whole, 85 in halves; 4096 -> 2048 of 64 requests 255, 265, of 8 53, 42; one of
+        // 32 heads 2176 -> 2048 34, 25 (in quarters 29).
+        const int lanes = (int64_t)n * num_kv_heads >= 128 ? 4 : 3;
+        hipLaunchKernelGGL(compact_kernel, dim3(32 >> lanes, num_kv_heads, n), dim3(CP_THR), 0, (hipStream_t)stream, p,
+                           lanes);
         SKV_HIP(hipGetLastError());
     }
     return STARKV_OK;

@@ -11,10 +11,13 @@
 // decode step. 2048 tokens of 32 + 64 rows with cache and fp16 rows 26 us (134 MB), where 22
 // elementwise launches, the write and two conversions took 330.
 //
-// With NORM the same launch first norms each q and k row over its 128 dimensions (the norm of
-// queries and keys for each head): x / sqrt(mean(x^2) + eps) * weight, the squares summed in fp32
-// over the row's 8 lanes, the normed row kept in fp32 into the rotation and rounded once behind it.
-// A step's norms cost no launch and no pass over q and k of their own.
+// norm_rope_kernel: the same behind an RMS norm of each q and k row (queries' and keys' norms for each
+// head): x / sqrt(mean(x^2) + eps) * weight, the squares summed in fp32 over the row's 8 lanes, the
+// normed row kept in fp32 into the rotation and rounded once behind it. A lane issues its loads (row,
+// position, angles, weights) before any is made numbers: one after the other they took 123 us for 8191
+// tokens of 32 + 64 rows with cache and fp16 rows, together 104 (537 MB, 5.2 TB/s, a large copy's rate
+// is 4.95); a workgroup that kept angles and weights over a token's rows 145 (fewer waves fit). 16
+// tokens of 32 + 16 rows: 5 us, latency.
 //
 // silu_mul_kernel: silu(gate) * up, the gate rounded to the model dtype before the product as the
 // two elementwise kernels did. 2048 tokens of 2 x 11008: 31 us (135 MB) against 56.
@@ -56,7 +59,7 @@ struct RopeParams {
     int64_t block_size, num_blocks;
     const void* slots; int slot64;
     uint16_t* k16; uint16_t* v16;       // contiguous fp16 [T][Hkv][128], or null
-    const void* qw; const void* kw; int w_dt; float eps;  // NORM: the norms' weights [128]
+    const void* qw; const void* kw; int w_dt; float eps;  // the norms' weights [128]
 };
 
 __device__ __forceinline__ void store8(void* p, int64_t i, int dt, const float* f) {
@@ -84,7 +87,13 @@ __device__ __forceinline__ float2 rotate(float x1, float x2, float c, float s) {
     return make_float2(x1 * c - x2 * s, x2 * c + x1 * s);
 }
 
-template <bool NORM>
+// Token t's row of the rotary table.
+__device__ __forceinline__ int64_t table_row(const RopeParams& p, int64_t t) {
+    int64_t pos = p.pos64 ? ((const int64_t*)p.pos)[t] : (int64_t)((const int32_t*)p.pos)[t];
+    if (!wrap_index(pos, p.cs_rows)) __builtin_trap();
+    return pos;
+}
+
 __global__ __launch_bounds__(256) void rope_qkv_kernel(const RopeParams p) {
     const int rows = p.H + (p.k ? p.Hkv : 0) + (p.v ? p.Hkv : 0);
     const int t = blockIdx.x, it = blockIdx.y * 256 + threadIdx.x;
@@ -98,28 +107,10 @@ __global__ __launch_bounds__(256) void rope_qkv_kernel(const RopeParams p) {
     load8_f(src, at + d, p.dt, a);
     load8_f(src, at + 64 + d, p.dt, b);
     if (!isv) {
-        int64_t pos = p.pos64 ? ((const int64_t*)p.pos)[t] : (int64_t)((const int32_t*)p.pos)[t];
-        if (!wrap_index(pos, p.cs_rows)) __builtin_trap();
+        const int64_t pos = table_row(p, t);
         float c[8], s[8];
         load8_f(p.cs, pos * p.cs_s0 + d, p.cs_dt, c);
         load8_f(p.cs, pos * p.cs_s0 + 64 + d, p.cs_dt, s);
-        if constexpr (NORM) {
-            const void* w = isq ? p.qw : p.kw;
-            float wa[8], wb[8], ss = 0.f;
-            load8_f(w, d, p.w_dt, wa);
-            load8_f(w, 64 + d, p.w_dt, wb);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
-            ss += dpp_f<0xB1>(ss);   // the row's 8 lanes: quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror
-            ss += dpp_f<0x4E>(ss);
-            ss += dpp_f<0x141>(ss);
-            const float inv = 1.f / sqrtf(ss * (1.f / 128.f) + p.eps);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                a[e] *= inv * wa[e];
-                b[e] *= inv * wb[e];
-            }
-        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float2 r = rotate(a[e], b[e], c[e], s[e]);
@@ -148,6 +139,98 @@ __global__ __launch_bounds__(256) void rope_qkv_kernel(const RopeParams p) {
         const int64_t c = (slot / p.block_size) * p.c_s0 + (slot % p.block_size) * p.c_s1 + h * p.c_s2 + d;
         store8(isv ? p.vc : p.kc, c, p.dt, a);
         store8(isv ? p.vc : p.kc, c + 64, p.dt, b);
+    }
+}
+
+// Eight elements as they lie in memory: loaded at once, made numbers where they are used, so that a lane's
+// loads are on their way together whatever their types.
+struct Raw8 {
+    uint4 a, b;
+};
+
+__device__ __forceinline__ Raw8 raw8(const void* p, int64_t i, int dt) {
+    if (dt == STARKV_F32) return {((const uint4*)((const float*)p + i))[0], ((const uint4*)((const float*)p + i))[1]};
+    return {*(const uint4*)((const uint16_t*)p + i), make_uint4(0, 0, 0, 0)};
+}
+
+__device__ __forceinline__ void numbers(const Raw8& r, int dt, float* o) {
+    if (dt == STARKV_F32) {
+        const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = __uint_as_float(w[e]);
+        return;
+    }
+    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (dt == STARKV_BF16) {
+            o[2 * e] = __uint_as_float(w[e] << 16);
+            o[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        } else {
+            o[2 * e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] & 0xffffu));
+            o[2 * e + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e] >> 16));
+        }
+    }
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void norm_rope_kernel(const RopeParams p) {
+    const int rows = p.H + (p.k ? p.Hkv : 0) + (p.v ? p.Hkv : 0);
+    const int64_t t = blockIdx.x;
+    const int d = 8 * (threadIdx.x & 7), r = blockIdx.y * 32 + (threadIdx.x >> 3);
+    if (r >= rows) return;
+    const bool isq = r < p.H, isv = r >= p.H + p.Hkv;
+    const int h = isq ? r : isv ? r - p.H - p.Hkv : r - p.H;
+    const void* src = isq ? p.q : isv ? p.v : p.k;
+    const int64_t at = isq ? t * p.q_s0 + h * p.q_s1 : isv ? t * p.v_s0 + h * p.v_s1 : t * p.k_s0 + h * p.k_s1;
+    int64_t slot = -1;
+    if (p.kc) slot = p.slot64 ? ((const int64_t*)p.slots)[t] : (int64_t)((const int32_t*)p.slots)[t];
+    const Raw8 ra = raw8(src, at + d, DT), rb = raw8(src, at + 64 + d, DT);
+    const void* w = isq ? p.qw : p.kw;
+    float a[8], b[8];
+    if (!isv) {
+        const Raw8 rwa = raw8(w, d, p.w_dt), rwb = raw8(w, 64 + d, p.w_dt);
+        const int64_t pos = table_row(p, t);
+        const Raw8 rc = raw8(p.cs, pos * p.cs_s0 + d, p.cs_dt), rs = raw8(p.cs, pos * p.cs_s0 + 64 + d, p.cs_dt);
+        float wa[8], wb[8], c[8], s[8], ss = 0.f;
+        numbers(ra, DT, a);
+        numbers(rb, DT, b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fmaf(a[e], a[e], fmaf(b[e], b[e], ss));
+        ss += dpp_f<0xB1>(ss);   // the row's 8 lanes: quad_perm [1,0,3,2], [2,3,0,1], row_half_mirror
+        ss += dpp_f<0x4E>(ss);
+        ss += dpp_f<0x141>(ss);
+        const float inv = 1.f / sqrtf(ss * (1.f / 128.f) + p.eps);
+        numbers(rwa, p.w_dt, wa);
+        numbers(rwb, p.w_dt, wb);
+        numbers(rc, p.cs_dt, c);
+        numbers(rs, p.cs_dt, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float2 z = rotate(a[e] * (inv * wa[e]), b[e] * (inv * wb[e]), c[e], s[e]);
+            a[e] = round_to(z.x, DT);
+            b[e] = round_to(z.y, DT);
+        }
+    } else {
+        numbers(ra, DT, a);
+        numbers(rb, DT, b);
+    }
+    const int64_t o = (t * (isq ? p.H : p.Hkv) + h) * 128 + d;
+    void* full = isq ? p.q_out : isv ? nullptr : p.k_out;
+    if (full) {
+        store8(full, o, DT, a);
+        store8(full, o + 64, DT, b);
+    }
+    if (isq) return;
+    uint16_t* x16 = isv ? p.v16 : p.k16;
+    if (x16) {
+        store8(x16, o, STARKV_F16, a);
+        store8(x16, o + 64, STARKV_F16, b);
+    }
+    if (slot >= 0 && slot < p.num_blocks * p.block_size) {
+        const int64_t to = (slot / p.block_size) * p.c_s0 + (slot % p.block_size) * p.c_s1 + h * p.c_s2 + d;
+        store8(isv ? p.vc : p.kc, to, DT, a);
+        store8(isv ? p.vc : p.kc, to + 64, DT, b);
     }
 }
 
@@ -453,11 +536,15 @@ int rope_call(void* stream, const void* q, int64_t q_s0, int64_t q_s1, const voi
     p.k16 = (uint16_t*)k_half; p.v16 = (uint16_t*)v_half;
     p.qw = q_weight; p.kw = k_weight; p.w_dt = w_dtype; p.eps = eps;
     const int rows = num_heads + (k ? num_kv_heads : 0) + (v ? num_kv_heads : 0);
-    const dim3 grid(num_tokens, (8 * rows + 255) / 256);
-    if (q_weight)
-        hipLaunchKernelGGL(rope_qkv_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    const int passes = (rows + 31) / 32;  // of a workgroup over a token's rows
+    if (q_weight && dtype == STARKV_BF16)
+        hipLaunchKernelGGL(norm_rope_kernel<STARKV_BF16>, dim3(num_tokens, passes), dim3(256), 0, (hipStream_t)stream, p);
+    else if (q_weight && dtype == STARKV_F16)
+        hipLaunchKernelGGL(norm_rope_kernel<STARKV_F16>, dim3(num_tokens, passes), dim3(256), 0, (hipStream_t)stream, p);
+    else if (q_weight)
+        hipLaunchKernelGGL(norm_rope_kernel<STARKV_F32>, dim3(num_tokens, passes), dim3(256), 0, (hipStream_t)stream, p);
     else
-        hipLaunchKernelGGL(rope_qkv_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL(rope_qkv_kernel, dim3(num_tokens, passes), dim3(256), 0, (hipStream_t)stream, p);
     SKV_HIP(hipGetLastError());
     return STARKV_OK;
 }

@@ -10,20 +10,20 @@
 //
 // Both products run on v_mfma_f32_16x16x32 with nothing but registers between memory and the matrix
 // unit: S^T = K q^T takes 16 tokens as rows, so a lane holds row l % 16 of the page's keys as they lie
-// in memory (64 bytes of each of 16 rows a load) and the 16 columns are the query heads, zeros past
-// the G-th. The result gives lane l the scores of head l % 16 at tokens 4 (l / 16) .. + 3 of either
-// page, which is the B operand of out^T = V^T P^T with the product's 32 terms in the order (l / 16,
-// page, token): P goes from one product into the other in place. V^T's rows are the head's dimensions
-// in the order 8 (l % 16) + i for the i-th of 8 products, so the A operand is dimension i of the 16
-// bytes that lane l loaded of each of its 8 tokens (4 rows of 256 bytes a load), gathered with 4 byte
-// permutes. A lane ends with 32 consecutive dimensions of one head. Any G costs the same instructions,
-// far below memory's time.
+// in memory (64 bytes of each of 16 rows a load) and the 16 columns are the query heads. The result
+// gives lane l the scores of column l % 16 at tokens 4 (l / 16) .. + 3 of either page, which is the B
+// operand of out^T = V^T P^T with the product's 32 terms in the order (l / 16, page, token): P goes
+// from one product into the other in place. V^T's rows are the head's dimensions in the order
+// 8 (l % 16) + i for the i-th of 8 products, so the A operand is dimension i of the 16 bytes that lane
+// l loaded of each of its 8 tokens (4 rows of 256 bytes a load), gathered with 4 byte permutes. A lane
+// ends with 32 consecutive dimensions of one column.
 //
-// Rounding: scores, references and sums are fp32. The weights are rounded to the cache's type for the
-// second product (2^-8 relative for bf16, 2^-11 for fp16, as the output is in the end), and the
-// sum that divides takes the rounded weights, so that they sum to one. The reference lies 2^7 below
-// the largest score seen when it was set and moves when a score passes it by 2^15 (fp16 weights stay
-// finite, and small ones keep 22 bits of range above its subnormals).
+// Rounding: scores, references and sums are fp32. The weights enter the second product as two values
+// of the cache's type, the rounded weight and what the rounding left (16 bits of a bf16 weight, 22 of an
+// fp16 one): up to 8 query heads the second value takes the other 8 columns, whose scores are the same
+// heads' again, and costs no instruction of the matrix unit; 9 to 16 heads take a product each. The
+// reference lies 2^7 below the largest score seen when it was set and moves when a score passes it by
+// 2^15 (fp16 weights stay finite, and small ones keep 22 bits of range above its subnormals).
 #pragma once
 
 #include <algorithm>
@@ -34,7 +34,7 @@ namespace starkv {
 
 constexpr int AT_THR = 256;
 constexpr int AT_CHUNK = 512;      // pages whose places are looked up at a time
-constexpr int AT_PART = 132;       // floats of a partial: reference, sum of rounded weights, sum of weights, 0, out[128]
+constexpr int AT_PART = 132;       // floats of a partial: reference, sum of weights, 0, 0, out[128]
 constexpr int AT_MAX_SPLITS = 128;
 constexpr int AT_MAX_GROUP = 16;   // query heads per KV head: the columns of a matrix product
 constexpr float AT_LOG2E = 1.4426950408889634f;
@@ -48,7 +48,7 @@ struct AttendParams {
     int n, Hkv, G, splits, pps;                                          // pps: pages per split
     float sc;                                                            // scale * log2(e)
     const int32_t* sel; int64_t sel_s0, sel_s1; int keep;                // SPARSE: logical blocks [n][Hkv][keep]
-    float* lg; int64_t lg_row;                                           // else: scores [n][H][lg_row]
+    float* lg; int64_t lg_row;                                           // else: scores [n][Hkv][page][G][16], lg_row a unit
     float* part;                                                         // [n][H][splits][AT_PART]
     uint16_t* out; int64_t o_s0, o_s1;
 };
@@ -67,31 +67,45 @@ __device__ __forceinline__ f32x4_t attend_mfma(uint4 a, uint4 b, f32x4_t c) {
                                                       0, 0, 0);
 }
 
-// Two values rounded to DT, packed, and their sum as rounded.
+// Two values in DT, packed, and as they became: bf16 by its upper bits (what they leave goes into the second
+// product too), fp16 to the nearest (its subnormals leave nothing).
 template <int DT>
-__device__ __forceinline__ uint32_t attend_pack(float a, float b, float& sum) {
+__device__ __forceinline__ uint32_t attend_pack(float a, float b, float& ra, float& rb) {
     if constexpr (DT == STARKV_BF16) {
-        const uint32_t lo = f32_to_bf16_rne(a), hi = f32_to_bf16_rne(b);
-        sum += bf16_bits_to_f32(lo) + bf16_bits_to_f32(hi);
-        return lo | (hi << 16);
+        ra = __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+        rb = __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+        return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
     } else {
         const _Float16 lo = (_Float16)a, hi = (_Float16)b;
-        sum += (float)lo + (float)hi;
+        ra = (float)lo;
+        rb = (float)hi;
         return (uint32_t)__builtin_bit_cast(uint16_t, lo) | ((uint32_t)__builtin_bit_cast(uint16_t, hi) << 16);
     }
+}
+
+// What a .. d leave of their packed forms, packed: the second value of a weight.
+template <int DT>
+__device__ __forceinline__ uint2 attend_rest(const float (&p)[4], float of) {
+    float r[4], x[4];
+    attend_pack<DT>(p[0], p[1], r[0], r[1]);
+    attend_pack<DT>(p[2], p[3], r[2], r[3]);
+    return make_uint2(attend_pack<DT>(fmaf(-of, r[0], p[0]), fmaf(-of, r[1], p[1]), x[0], x[1]),
+                      attend_pack<DT>(fmaf(-of, r[2], p[2]), fmaf(-of, r[3], p[3]), x[2], x[3]));
 }
 
 // Component i of a 16-byte register row.
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // The workgroup's unit: (request, KV head, split) from the block index.
-template <int DT, bool SPARSE>
-__global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p) {
+// MANY: 9 to 16 query heads.
+template <int DT, bool SPARSE, bool MANY>
+__global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const AttendParams p) {
     __shared__ int2 s_page[AT_CHUNK];           // a page's block, and its tokens | its place in the block << 8
     extern __shared__ float s_dyn[];            // [4 waves][G][AT_PART] for the merge
     const int id = blockIdx.x, s = id % p.splits, u = id / p.splits, h = u % p.Hkv, b = u / p.Hkv;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int col = lane & 15, quad = lane >> 4;
+    const int col = MANY ? lane & 15 : lane & 7, quad = lane >> 4;  // the lane's query head
+    const float rest = lane & 8 ? 1.f : 0.f;                        // not MANY: its column takes the weights' second values
     const int H = p.Hkv * p.G;
     const int L = attend_length(p, b);
     const int pages = SPARSE ? p.keep << p.bs_shift : (L + 15) >> 4;
@@ -103,12 +117,12 @@ __global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p)
     for (int st = 0; st < 4; ++st)
         qf[st] = col < p.G ? *(const uint4*)(p.q + b * p.q_s0 + (int64_t)(h * p.G + col) * p.q_s1 + 32 * st + 8 * quad)
                            : make_uint4(0, 0, 0, 0);
-    float m = -INFINITY, l = 0.f, lx = 0.f;
+    float m = -INFINITY, l = 0.f;
     f32x4_t acc[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     const uint16_t* kh = p.kc + (int64_t)h * p.c_s2 + 8 * quad;
-    const uint16_t* vh = p.vc + (int64_t)h * p.c_s2 + 8 * col;
+    const uint16_t* vh = p.vc + (int64_t)h * p.c_s2 + 8 * (lane & 15);
 
     for (int c0 = k0; c0 < k1; c0 += AT_CHUNK) {
         const int count = min(AT_CHUNK, k1 - c0);
@@ -135,11 +149,12 @@ __global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p)
                 e[x].y = __builtin_amdgcn_readfirstlane(v.y);
                 nt[x] = i + x < count ? e[x].y & 255 : 0;
             }
-            float* lg = p.lg + ((int64_t)b * H + h * p.G + col) * p.lg_row + 16 * (c0 + i) + 4 * quad;
+            const bool own = col < p.G && (MANY || !(lane & 8));
+            float* lg = p.lg + ((int64_t)b * p.Hkv + h) * p.lg_row + ((int64_t)(c0 + i) * p.G + col) * 16 + 4 * quad;
             if (nt[0] + nt[1] == 0) {
-                if (!SPARSE && col < p.G)
+                if (!SPARSE && own)
                     for (int x = 0; x < 2 && i + x < count; ++x)
-                        *(float4*)(lg + 16 * x) = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                        *(float4*)(lg + 16 * x * p.G) = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                 continue;
             }
             uint4 kr[2][4], vr[2][4];
@@ -152,7 +167,7 @@ __global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p)
                 const int64_t base = at.x * p.c_s0 + (int64_t)((at.y >> 8) << 4) * p.c_s1;
 #pragma unroll
                 for (int st = 0; st < 4; ++st)
-                    kr[x][st] = *(const uint4*)(kh + base + min(col, last) * p.c_s1 + 32 * st);
+                    kr[x][st] = *(const uint4*)(kh + base + min(lane & 15, last) * p.c_s1 + 32 * st);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     vr[x][j] = *(const uint4*)(vh + base + min(4 * quad + j, last) * p.c_s1);
@@ -173,8 +188,10 @@ __global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p)
                         vr[x][r] = ok ? vr[x][r] : make_uint4(0, 0, 0, 0);
                     }
                 }
-                if (!SPARSE && col < p.G && i + x < count)
-                    *(float4*)(lg + 16 * x) = make_float4(sv[x][0], sv[x][1], sv[x][2], sv[x][3]);
+            }
+            if (!SPARSE && own) {
+                *(float4*)lg = make_float4(sv[0][0], sv[0][1], sv[0][2], sv[0][3]);
+                if (i + 1 < count) *(float4*)(lg + 16 * p.G) = make_float4(sv[1][0], sv[1][1], sv[1][2], sv[1][3]);
             }
             float mx = sv[0][0];
 #pragma unroll
@@ -185,7 +202,6 @@ __global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p)
                 const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
                 m = mn;
                 l *= alpha;
-                lx *= alpha;
 #pragma unroll
                 for (int i8 = 0; i8 < 8; ++i8) acc[i8] *= alpha;
             }
@@ -195,10 +211,15 @@ __global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     pe[x][r] = 4 * quad + r < nt[x] ? exp2f(sv[x][r] - m) : 0.f;
-                    if (!SPARSE) lx += pe[x][r];
+                    l += pe[x][r];
                 }
-            const uint4 pf = make_uint4(attend_pack<DT>(pe[0][0], pe[0][1], l), attend_pack<DT>(pe[0][2], pe[0][3], l),
-                                        attend_pack<DT>(pe[1][0], pe[1][1], l), attend_pack<DT>(pe[1][2], pe[1][3], l));
+            const uint2 p0 = attend_rest<DT>(pe[0], MANY ? 0.f : rest), p1 = attend_rest<DT>(pe[1], MANY ? 0.f : rest);
+            const uint4 pf = make_uint4(p0.x, p0.y, p1.x, p1.y);
+            uint4 pl = make_uint4(0, 0, 0, 0);
+            if constexpr (MANY) {
+                const uint2 q0 = attend_rest<DT>(pe[0], 1.f), q1 = attend_rest<DT>(pe[1], 1.f);
+                pl = make_uint4(q0.x, q0.y, q1.x, q1.y);
+            }
 #pragma unroll
             for (int i8 = 0; i8 < 8; ++i8) {
                 const uint32_t pick = i8 & 1 ? 0x07060302u : 0x05040100u;  // both high halves, or both low ones
@@ -208,17 +229,22 @@ __global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p)
                 vt.z = __builtin_amdgcn_perm(word_of(vr[1][1], i8 >> 1), word_of(vr[1][0], i8 >> 1), pick);
                 vt.w = __builtin_amdgcn_perm(word_of(vr[1][3], i8 >> 1), word_of(vr[1][2], i8 >> 1), pick);
                 acc[i8] = attend_mfma<DT>(vt, pf, acc[i8]);
+                if constexpr (MANY) acc[i8] = attend_mfma<DT>(vt, pl, acc[i8]);
             }
         }
     }
     l = sum_rows(l);
-    lx = sum_rows(lx);
-    if (col < p.G) {
+    if constexpr (!MANY) {  // both columns of a head: lanes 8 apart in a row of 16
+#pragma unroll
+        for (int i8 = 0; i8 < 8; ++i8)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[i8][x] += dpp_f<0x128>(acc[i8][x]);  // row_ror:8
+    }
+    if (col < p.G && (MANY || !(lane & 8))) {
         float* w = s_dyn + (wave * p.G + col) * AT_PART;
         if (quad == 0) {
             w[0] = m;
             w[1] = l;
-            w[2] = lx;
         }
 #pragma unroll
         for (int x = 0; x < 4; ++x) {  // dimensions 32 quad + 8 x + i
@@ -230,7 +256,7 @@ __global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p)
     for (int i = tid; i < p.G * 128; i += AT_THR) {
         const int g = i >> 7, d = i & 127;
         const float* w = s_dyn + g * AT_PART;
-        float M = -INFINITY, lt = 0.f, lxt = 0.f, a = 0.f;
+        float M = -INFINITY, lt = 0.f, a = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) M = fmaxf(M, w[k * p.G * AT_PART]);
 #pragma unroll
@@ -239,42 +265,67 @@ __global__ __launch_bounds__(AT_THR, 2) void attend_kernel(const AttendParams p)
             // A wave without tokens has reference -inf and sums 0; NaN scores leave sums of NaN.
             const float f = r[0] == -INFINITY ? 1.f : exp2f(r[0] - M);
             lt = fmaf(r[1], f, lt);
-            lxt = fmaf(r[2], f, lxt);
             a = fmaf(r[4 + d], f, a);
         }
         const int hq = h * p.G + g;
         if (p.splits == 1) store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, DT, lt == 0.f ? 0.f : a / lt);
         if (p.splits > 1 || !SPARSE) {
             float* pp = p.part + (((int64_t)b * H + hq) * p.splits + s) * AT_PART;
-            if (d == 0) *(float4*)pp = make_float4(M, lt, lxt, 0.f);
+            if (d == 0) *(float4*)pp = make_float4(M, lt, 0.f, 0.f);
             pp[4 + d] = a;
         }
     }
 }
 
-// A head's splits joined: thread d sums dimension d, every thread the references and sums.
+// A head's splits joined by one wave: lane s holds the factors of splits s and s + 64, and sums dimensions 2 s
+// and 2 s + 1, eight splits' loads in flight.
 template <int DT>
-__device__ __forceinline__ void attend_merge_head(const AttendParams& p, int b, int hq, int d) {
+__device__ __forceinline__ void attend_merge_head(const AttendParams& p, int b, int hq) {
+    static_assert(AT_MAX_SPLITS <= 128, "two splits a lane");
+    const int lane = threadIdx.x & 63;
     const float* pp = p.part + ((int64_t)b * p.Hkv * p.G + hq) * p.splits * AT_PART;
-    float M = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, pp[s * AT_PART]);
-    float lt = 0.f, a = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-        const float m = pp[s * AT_PART], f = m == -INFINITY ? 1.f : exp2f(m - M);
-        lt = fmaf(pp[s * AT_PART + 1], f, lt);
-        a = fmaf(pp[s * AT_PART + 4 + d], f, a);
+    float m[2], f[2], lt = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int s = lane + 64 * x;
+        m[x] = s < p.splits ? pp[s * AT_PART] : -INFINITY;
+        f[x] = s < p.splits ? pp[s * AT_PART + 1] : 0.f;
     }
-    store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, DT, lt == 0.f ? 0.f : a / lt);
+    const float M = wave_max(fmaxf(m[0], m[1]));
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const float l = f[x];
+        f[x] = m[x] == -INFINITY ? 1.f : exp2f(m[x] - M);
+        lt = fmaf(l, f[x], lt);
+    }
+    lt = wave_sum(lt);
+    float2 a = make_float2(0.f, 0.f);
+    for (int s0 = 0; s0 < p.splits; s0 += 8) {
+        float2 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = *(const float2*)(pp + min(s0 + u, p.splits - 1) * AT_PART + 4 + 2 * lane);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(s0 < 64 ? f[0] : f[1]), (s0 + u) & 63));
+            if (s0 + u < p.splits) {
+                a.x = fmaf(v[u].x, fs, a.x);
+                a.y = fmaf(v[u].y, fs, a.y);
+            }
+        }
+    }
+    const int64_t o = b * p.o_s0 + hq * p.o_s1 + 2 * lane;
+    store_f(p.out, o, DT, lt == 0.f ? 0.f : a.x / lt);
+    store_f(p.out, o + 1, DT, lt == 0.f ? 0.f : a.y / lt);
 }
 
-// Splits per unit (request and KV head) of at most `pages` pages: workgroups for two a CU, 8 pages a
+// Splits per unit (request and KV head) of at most `pages` pages: workgroups for `per_cu` a CU, `least` pages a
 // split at least.
-inline int attend_splits(int64_t units, int pages) {
+inline int attend_splits(int64_t units, int pages, int per_cu, int least) {
     int dev = 0, cus = 256, c = 0;
     if (hipGetDevice(&dev) == hipSuccess &&
         hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && c > 0)
         cus = c;
-    const int64_t s = std::min<int64_t>((2 * (int64_t)cus + units - 1) / units, (pages + 7) / 8);
+    const int64_t s = std::min<int64_t>((per_cu * (int64_t)cus + units - 1) / units, (pages + least - 1) / least);
     return (int)std::max<int64_t>(1, std::min<int64_t>(s, AT_MAX_SPLITS));
 }
 
@@ -318,11 +369,13 @@ inline int attend_launch(void* stream, int dtype, const AttendParams& p) {
     SKV_CHECK((int64_t)p.n * p.Hkv * p.splits < 1 << 23, "%d requests of %d KV heads in one call", p.n, p.Hkv);
     const dim3 grid((unsigned)((int64_t)p.n * p.Hkv * p.splits));
     const size_t lds = (size_t)4 * p.G * AT_PART * 4;
-    if (dtype == STARKV_BF16)
-        hipLaunchKernelGGL((attend_kernel<STARKV_BF16, SPARSE>), grid, dim3(AT_THR), lds, (hipStream_t)stream, p);
-    else
-        hipLaunchKernelGGL((attend_kernel<STARKV_F16, SPARSE>), grid, dim3(AT_THR), lds, (hipStream_t)stream, p);
-    SKV_HIP(hipGetLastError());
+    const bool bf = dtype == STARKV_BF16;
+    const void* fn = p.G <= 8 ? bf ? (const void*)&attend_kernel<STARKV_BF16, SPARSE, false>
+                                   : (const void*)&attend_kernel<STARKV_F16, SPARSE, false>
+                              : bf ? (const void*)&attend_kernel<STARKV_BF16, SPARSE, true>
+                                   : (const void*)&attend_kernel<STARKV_F16, SPARSE, true>;
+    void* args[] = {(void*)&p};
+    SKV_HIP(hipLaunchKernel(fn, grid, dim3(AT_THR), args, lds, (hipStream_t)stream));
     return STARKV_OK;
 }
 

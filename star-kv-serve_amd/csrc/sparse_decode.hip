@@ -81,9 +81,9 @@ __global__ __launch_bounds__(256) void key_bounds_kernel(const BoundsParams p) {
     uint32_t w[2][4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        float none = 0.f;
-        w[0][e] = attend_pack<DT>(lo[2 * e], lo[2 * e + 1], none);
-        w[1][e] = attend_pack<DT>(hi[2 * e], hi[2 * e + 1], none);
+        float x, y;  // values of DT already
+        w[0][e] = attend_pack<DT>(lo[2 * e], lo[2 * e + 1], x, y);
+        w[1][e] = attend_pack<DT>(hi[2 * e], hi[2 * e + 1], x, y);
     }
     uint16_t* o = p.bounds + blk * p.b_s0 + h * p.b_s1 + d;
     *(uint4*)o = make_uint4(w[0][0], w[0][1], w[0][2], w[0][3]);
@@ -109,89 +109,101 @@ __device__ __forceinline__ int select_blocks_of(const SelectParams& p, int b) {
     return (int)(((int64_t)L + (16 << p.bs_shift) - 1) >> (p.bs_shift + 4));
 }
 
-constexpr int SC_U = 4;        // blocks a 16-lane row has in flight
-constexpr int SC_BLOCKS = 16 * SC_U;
+constexpr int SC_U = 4;  // blocks a 16-lane row has in flight
 
-// 16 lanes a block, 8 dimensions of both bounds each; a workgroup of 16 rows takes 64 blocks of one
-// (request, KV head).
+template <int CTL>
+__device__ __forceinline__ double add_dpp(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTL, 0xF, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTL, 0xF, 0xF, true);
+    return v + __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
+// 16 lanes a (block, head), 8 dimensions of both bounds each. A workgroup of 16 rows takes a request's
+// blocks for `heads` KV heads at once (a power of two up to 16), as they lie in memory: 4 heads of a
+// block are 2 KB that a wave reads as one run (one head a workgroup read 512 bytes here and there). A row
+// takes SC_U consecutive blocks at a time, with its head's query part in registers.
 template <int DT>
-__global__ __launch_bounds__(256) void score_kernel(const SelectParams p) {
-    const int h = blockIdx.y, b = blockIdx.z;
-    const int nb = select_blocks_of(p, b);
-    const int first = blockIdx.x * SC_BLOCKS;
-    if (nb <= p.keep || first >= nb - p.recent) return;
-    const int row = threadIdx.x >> 4, d = 8 * (threadIdx.x & 15);
-    uint4 lo[SC_U], hi[SC_U];
-    int blk[SC_U];
-#pragma unroll
-    for (int u = 0; u < SC_U; ++u) {
-        blk[u] = p.bt[b * p.bt_s0 + min(first + 16 * u + row, nb - 1) * p.bt_s1];
-        if (blk[u] < 0 || blk[u] >= p.num_blocks) blk[u] = -1;
-    }
-#pragma unroll
-    for (int u = 0; u < SC_U; ++u) {
-        const uint16_t* x = p.bounds + max(blk[u], 0) * p.b_s0 + h * p.b_s1 + d;
-        lo[u] = *(const uint4*)x;
-        hi[u] = *(const uint4*)(x + p.b_s2);
-    }
+__global__ __launch_bounds__(256) void score_kernel(const SelectParams p, int heads) {
+    const int b = blockIdx.z, row = threadIdx.x >> 4, d = 8 * (threadIdx.x & 15);
+    const int nb = select_blocks_of(p, b), last = nb - p.recent;  // blocks behind `last` are read unscored
+    const int h = blockIdx.y * heads + (row & (heads - 1)), step = 16 / heads * SC_U;
+    int j0 = blockIdx.x * step + row / heads * SC_U;
+    if (nb <= p.keep || h >= p.Hkv) return;
     double up[8], down[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) up[e] = down[e] = 0.0;
-    for (int g = 0; g < p.G; ++g) {
-        float f[8];
-        values8<DT>(*(const uint4*)(p.q + b * p.q_s0 + (int64_t)(h * p.G + g) * p.q_s1 + d), f);
+    for (int g0 = 0; g0 < p.G; g0 += 4) {  // four rows on their way at a time
+        uint4 w[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            up[e] += (double)__builtin_elementwise_maximum(f[e], 0.f);
-            down[e] += (double)__builtin_elementwise_minimum(f[e], 0.f);
+        for (int g = 0; g < 4; ++g)
+            w[g] = *(const uint4*)(p.q + b * p.q_s0 + (int64_t)(h * p.G + min(g0 + g, p.G - 1)) * p.q_s1 + d);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if (g0 + g >= p.G) continue;
+            float f[8];
+            values8<DT>(w[g], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                up[e] += (double)__builtin_elementwise_maximum(f[e], 0.f);
+                down[e] += (double)__builtin_elementwise_minimum(f[e], 0.f);
+            }
         }
     }
+    float* score = p.score + ((int64_t)b * p.Hkv + h) * p.cap;
+    for (; j0 < last; j0 += step * gridDim.x) {
+        uint4 lo[SC_U], hi[SC_U];
+        int blk[SC_U];
 #pragma unroll
-    for (int u = 0; u < SC_U; ++u) {
-        float a[8], c[8];
-        values8<DT>(lo[u], a);
-        values8<DT>(hi[u], c);
-        double s = 0.0;
+        for (int u = 0; u < SC_U; ++u) {
+            blk[u] = p.bt[b * p.bt_s0 + min(j0 + u, nb - 1) * p.bt_s1];
+            if (blk[u] < 0 || blk[u] >= p.num_blocks) blk[u] = -1;
+        }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s = fma(up[e], (double)c[e], fma(down[e], (double)a[e], s));
+        for (int u = 0; u < SC_U; ++u) {
+            const uint16_t* x = p.bounds + max(blk[u], 0) * p.b_s0 + h * p.b_s1 + d;
+            lo[u] = *(const uint4*)x;
+            hi[u] = *(const uint4*)(x + p.b_s2);
+        }
 #pragma unroll
-        for (int o = 1; o < 16; o <<= 1) s += __shfl_xor(s, o);
-        const int j = first + 16 * u + row;
-        if (d == 0 && j < nb) p.score[((int64_t)b * p.Hkv + h) * p.cap + j] = blk[u] < 0 ? -INFINITY : (float)s;
+        for (int u = 0; u < SC_U; ++u) {
+            float a[8], c[8];
+            values8<DT>(lo[u], a);
+            values8<DT>(hi[u], c);
+            double s = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fma(up[e], (double)c[e], fma(down[e], (double)a[e], s));
+            s = add_dpp<0xB1>(s);
+            s = add_dpp<0x4E>(s);
+            s = add_dpp<0x141>(s);
+            s = add_dpp<0x140>(s);
+            if (d == 0 && j0 + u < last) score[j0 + u] = blk[u] < 0 ? -INFINITY : (float)s;
+        }
     }
 }
 
-constexpr int SEL_THR = 1024;
-constexpr int SEL_LDS = 12288;  // keys of a row kept in LDS
-
-template <bool IN_LDS>
-__global__ __launch_bounds__(SEL_THR) void select_kernel(const SelectParams p) {
-    __shared__ TopkShared<SEL_THR> sh;
-    __shared__ uint32_t s_key[IN_LDS ? SEL_LDS : 1];
+template <bool KEPT>
+__global__ __launch_bounds__(TK_THR) void select_kernel(const SelectParams p) {
+    __shared__ TopkShared sh;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
     const int nb = select_blocks_of(p, b);
     int32_t* sel = p.sel + ((int64_t)b * p.Hkv + h) * p.keep;
     if (nb <= p.keep) {
-        for (int i = tid; i < p.keep; i += SEL_THR) sel[i] = i < nb ? i : -1;
+        for (int i = tid; i < p.keep; i += TK_THR) sel[i] = i < nb ? i : -1;
         return;
     }
     const int middle = nb - p.sink - p.recent, k = p.keep - p.sink - p.recent;
-    for (int i = tid; i < p.sink + p.recent; i += SEL_THR)
+    for (int i = tid; i < p.sink + p.recent; i += TK_THR)
         sel[i < p.sink ? i : k + i] = i < p.sink ? i : middle + i;
     if (k == 0) return;
     const float* score = p.score + ((int64_t)b * p.Hkv + h) * p.cap + p.sink;
-    if constexpr (IN_LDS) {
-        for (int i = tid; i < middle; i += SEL_THR) s_key[i] = order_key(score[i]);
-        __syncthreads();
-    }
-    topk_ascending<SEL_THR>(
-        sh, middle, k, [&](int i) { return IN_LDS ? s_key[i] : order_key(score[i]); },
-        [&](int pos, int i) { sel[p.sink + pos] = p.sink + i; });
+    topk_ascending<KEPT>(sh, middle, k, [&](int i) { return score[i]; },
+                         [&](int pos, int i, float) { sel[p.sink + pos] = p.sink + i; });
 }
 
 template <int DT>
-__global__ __launch_bounds__(128) void attend_merge_kernel(const AttendParams p) {
-    attend_merge_head<DT>(p, blockIdx.y, blockIdx.x, threadIdx.x);
+__global__ __launch_bounds__(64) void attend_merge_kernel(const AttendParams p) {
+    attend_merge_head<DT>(p, blockIdx.y, blockIdx.x);
 }
 
 }  // namespace
@@ -274,25 +286,35 @@ int starkv_select_blocks(void* stream, const void* query, int64_t q_s0, int64_t 
     p.keep = keep; p.sink = sink; p.recent = recent;
     p.score = (float*)workspace; p.sel = selected;
     if (p.cap > keep && keep > sink + recent) {
-        const dim3 grid((p.cap + SC_BLOCKS - 1) / SC_BLOCKS, num_kv_heads, n);
+        int heads = 1;
+        while (heads < num_kv_heads && heads < 16) heads *= 2;
+        const int64_t groups = (num_kv_heads + heads - 1) / heads, step = 16 / heads * SC_U, most = (p.cap + step - 1) / step;
+        const int64_t want = 2048 / (groups * n);
+        const dim3 grid((unsigned)std::min<int64_t>(most, std::max<int64_t>(1, want)), (unsigned)groups, n);
         if (dtype == STARKV_BF16)
-            hipLaunchKernelGGL(score_kernel<STARKV_BF16>, grid, dim3(256), 0, (hipStream_t)stream, p);
+            hipLaunchKernelGGL(score_kernel<STARKV_BF16>, grid, dim3(256), 0, (hipStream_t)stream, p, heads);
         else
-            hipLaunchKernelGGL(score_kernel<STARKV_F16>, grid, dim3(256), 0, (hipStream_t)stream, p);
+            hipLaunchKernelGGL(score_kernel<STARKV_F16>, grid, dim3(256), 0, (hipStream_t)stream, p, heads);
         SKV_HIP(hipGetLastError());
     }
-    if (p.cap <= SEL_LDS)
-        hipLaunchKernelGGL(select_kernel<true>, dim3(num_kv_heads, n), dim3(SEL_THR), 0, (hipStream_t)stream, p);
+    if (p.cap <= TK_KEPT)
+        hipLaunchKernelGGL(select_kernel<true>, dim3(num_kv_heads, n), dim3(TK_THR), 0, (hipStream_t)stream, p);
     else
-        hipLaunchKernelGGL(select_kernel<false>, dim3(num_kv_heads, n), dim3(SEL_THR), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL(select_kernel<false>, dim3(num_kv_heads, n), dim3(TK_THR), 0, (hipStream_t)stream, p);
     SKV_HIP(hipGetLastError());
     return STARKV_OK;
+}
+
+// Requests of one call have about the same work, so one round of the device is even: 64 requests of 4096 selected
+// tokens over 8 KV heads 189 us with workgroups for 2 a CU, 194 for 4, 205 for 8.
+static int sparse_splits(int n, int num_kv_heads, int pages) {
+    return attend_splits((int64_t)n * num_kv_heads, pages, 2, 8);
 }
 
 size_t starkv_sparse_decode_workspace_bytes(int n, int num_heads, int num_kv_heads, int block_size, int keep) {
     if (n < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || block_size < 16 || keep < 1) return 256;
     const int64_t pages = (int64_t)keep * (block_size / 16);
-    const int splits = attend_splits((int64_t)n * num_kv_heads, (int)std::min<int64_t>(pages, 1 << 27));
+    const int splits = sparse_splits(n, num_kv_heads, (int)std::min<int64_t>(pages, 1 << 27));
     return splits == 1 ? 256 : (size_t)n * num_heads * splits * AT_PART * 4;
 }
 
@@ -316,15 +338,15 @@ int starkv_sparse_decode(void* stream, const void* query, int64_t q_s0, int64_t 
     SKV_CHECK(workspace_bytes >= need, "sparse_decode: workspace %zu bytes < %zu", workspace_bytes, need);
     const int pages = keep << p.bs_shift;
     p.sel = selected; p.sel_s0 = sel_s0; p.sel_s1 = sel_s1; p.keep = keep;
-    p.splits = attend_splits((int64_t)n * num_kv_heads, pages);
+    p.splits = sparse_splits(n, num_kv_heads, pages);
     p.pps = (pages + p.splits - 1) / p.splits;
     p.part = (float*)workspace;
     const int err = attend_launch<true>(stream, dtype, p);
     if (err != STARKV_OK || p.splits == 1) return err;
     if (dtype == STARKV_BF16)
-        hipLaunchKernelGGL(attend_merge_kernel<STARKV_BF16>, dim3(num_heads, n), dim3(128), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL(attend_merge_kernel<STARKV_BF16>, dim3(num_heads, n), dim3(64), 0, (hipStream_t)stream, p);
     else
-        hipLaunchKernelGGL(attend_merge_kernel<STARKV_F16>, dim3(num_heads, n), dim3(128), 0, (hipStream_t)stream, p);
+        hipLaunchKernelGGL(attend_merge_kernel<STARKV_F16>, dim3(num_heads, n), dim3(64), 0, (hipStream_t)stream, p);
     SKV_HIP(hipGetLastError());
     return STARKV_OK;
 }

@@ -2,11 +2,13 @@
 // blocks a query reads, which tokens a cache keeps. Equal values go to the lowest index, NaN counts as
 // the largest value and -0 as 0, so the choice is a function of the values alone.
 //
-// Values are compared as integers of the same order. The k-th largest is found by halving its range
-// eight bits at a time: 256 buckets over [least, largest], a histogram in LDS, the bucket that holds it
-// becomes the range. Scores of one sign and a few binades spread over the buckets from the first round
-// on (buckets of the number's upper bits would put them all in one, whose counter is then added to one
-// lane at a time), and two or three rounds do.
+// Values are compared as integers of the same order. 2048 buckets over [least, largest] (scores of one
+// sign and a few binades spread over them, where buckets of the number's upper bits would be a handful)
+// are counted in LDS; the bucket that holds the k-th largest becomes the range, until it is taken
+// whole, holds 64 values or fewer, which one wave ranks, or one value. One round does for most rows.
+// A thread keeps a run of consecutive values in registers (rows of up to RUN values a thread; longer
+// ones are read again in every pass). A row's time is that of its barriers and first reads: 4096 scores 8
+// us from launch to end (a kernel of three dependent reads and nothing else takes 4).
 #pragma once
 
 #include "common.hpp"
@@ -19,109 +21,186 @@ __device__ __forceinline__ uint32_t order_key(float v) {
     return v != v ? 0xffffffffu : k;
 }
 
-template <int THR>
+// Over the lanes of a wave with data-parallel moves (a cross-lane load through LDS costs a hundred cycles a
+// step): the inclusive sum, the least and the largest.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, true);  // row_shr:1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, true);
+    const uint32_t a = __builtin_amdgcn_readlane(v, 15), b = __builtin_amdgcn_readlane(v, 31), c = __builtin_amdgcn_readlane(v, 47);
+    const int row = (threadIdx.x >> 4) & 3;
+    return v + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
+}
+
+template <int CTL>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTL, 0xF, 0xF, true);
+}
+
+__device__ __forceinline__ uint32_t wave_least(uint32_t v) {
+    v = min(v, dpp_u<0xB1>(v));  // as row16_max
+    v = min(v, dpp_u<0x4E>(v));
+    v = min(v, dpp_u<0x141>(v));
+    v = min(v, dpp_u<0x140>(v));
+    const uint32_t a = __builtin_amdgcn_readlane(v, 0), b = __builtin_amdgcn_readlane(v, 16),
+                   c = __builtin_amdgcn_readlane(v, 32), d = __builtin_amdgcn_readlane(v, 48);
+    return min(min(a, b), min(c, d));
+}
+
+constexpr int TK_BITS = 11, TK_BINS = 1 << TK_BITS;
+
+constexpr int TK_THR = 1024, TK_WAVES = TK_THR / 64;
+constexpr int TK_RUN = 16;                       // values a thread keeps
+constexpr int TK_KEPT = TK_THR * TK_RUN;         // the longest row that is kept
+
 struct TopkShared {
-    uint32_t hist[256];
-    uint32_t lo[THR / 64], hi[THR / 64];
-    uint32_t bin, above, inside;
-    unsigned long long scan[THR / 64];
+    uint32_t hist[TK_BINS];
+    uint32_t lo[TK_WAVES], hi[TK_WAVES];
+    uint32_t above[TK_WAVES];           // values in a wave's buckets
+    uint32_t bin, over, inside;
+    uint32_t few, key[64], at[64];      // a small bucket's values
+    uint32_t sure[TK_WAVES], tie[TK_WAVES];
 };
 
-// emit(position, index) for the k values chosen, positions 0 .. k - 1 by ascending index; 0 < k <= count. `key(i)`
-// gives value i's key. Every thread of the workgroup calls it.
-template <int THR, class Key, class Emit>
-__device__ __forceinline__ void topk_ascending(TopkShared<THR>& sh, int count, int k, Key key, Emit emit) {
+// The sum of t[w] over the waves w after (before) `wave`.
+__device__ __forceinline__ uint32_t sum_of_waves(const uint32_t* t, int wave, bool after) {
+    static_assert(TK_WAVES == 16, "a wave a lane of a row");
+    const int w = threadIdx.x & 15;
+    uint32_t v = (after ? w > wave : w < wave) ? t[w] : 0;
+    v += dpp_u<0xB1>(v);
+    v += dpp_u<0x4E>(v);
+    v += dpp_u<0x141>(v);
+    return v + dpp_u<0x140>(v);
+}
+
+// emit(position, index, value) for the k values chosen of value(0) .. value(count - 1), positions 0 .. k - 1 by
+// ascending index; 0 < k <= count, and count <= TK_KEPT where KEPT. Every thread of the workgroup calls it.
+template <bool KEPT, class Value, class Emit>
+__device__ __forceinline__ void topk_ascending(TopkShared& sh, int count, int k, Value value, Emit emit) {
+    constexpr int PER = TK_BINS / TK_THR;  // buckets a thread
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int run = (count + TK_THR - 1) / TK_THR, i0 = min(tid * run, count), mine = min(run, count - i0);
+    float kept[KEPT ? TK_RUN : 1];
+    if constexpr (KEPT) {
+#pragma unroll
+        for (int u = 0; u < TK_RUN; ++u)
+            if (u < run) kept[u] = u < mine ? value(i0 + u) : 0.f;
+    }
+    // f(key, index, value) of the thread's values, in order.
+    const auto each = [&](auto f) {
+        if constexpr (KEPT) {
+#pragma unroll
+            for (int u = 0; u < TK_RUN; ++u)
+                if (u < run && u < mine) f(order_key(kept[u]), i0 + u, kept[u]);
+        } else {
+            for (int u = 0; u < mine; ++u) {
+                const float v = value(i0 + u);
+                f(order_key(v), i0 + u, v);
+            }
+        }
+    };
+#pragma unroll
+    for (int x = 0; x < PER; ++x) sh.hist[x * TK_THR + tid] = 0;
+    if (tid == 0) sh.few = 0;
     uint32_t lo = 0xffffffffu, hi = 0;
-    for (int i = tid; i < count; i += THR) {
-        const uint32_t v = key(i);
+    each([&](uint32_t v, int, float) {
         lo = min(lo, v);
         hi = max(hi, v);
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
-        hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
-    }
+    });
+    lo = wave_least(lo);
+    hi = ~wave_least(~hi);
     if (lane == 0) {
         sh.lo[wave] = lo;
         sh.hi[wave] = hi;
     }
     __syncthreads();
-    for (int w = 0; w < THR / 64; ++w) {
-        lo = min(lo, sh.lo[w]);
-        hi = max(hi, sh.hi[w]);
-    }
-    // The values above `hi` are chosen; `need` more come from [lo, hi].
-    int need = k;
+    lo = wave_least(sh.lo[lane & 15]);
+    hi = ~wave_least(~sh.hi[lane & 15]);
+    // The values above `hi` are chosen; `need` more come from [lo, hi]: all of them, the first `need` of one
+    // value's, or those before (key, index) = (lo, limit).
+    int need = k, limit = -1;
     bool all = k == count;
     while (!all && lo != hi) {
-        const int shift = max(0, 24 - __clz((int)(hi - lo)));
-        for (int i = tid; i < 256; i += THR) sh.hist[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < count; i += THR) {
-            const uint32_t v = key(i);
+        const int shift = max(0, 32 - TK_BITS - __clz((int)(hi - lo)));
+        each([&](uint32_t v, int, float) {
             if (v >= lo && v <= hi) atomicAdd(&sh.hist[(v - lo) >> shift], 1u);
-        }
+        });
         __syncthreads();
-        if (wave == 0) {  // lane: buckets 4 lane .. + 3; from the top, the bucket that passes `need`
-            uint32_t c[4], sum = 0;
+        // From the top, the bucket that passes `need`: a thread's buckets, its wave's, the waves above.
+        uint32_t c[PER], sum = 0;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) sum += c[x] = sh.hist[4 * lane + x];
-            uint32_t from = sum;  // of this lane's buckets and the lanes above
+        for (int x = 0; x < PER; ++x) sum += c[x] = sh.hist[tid * PER + x];
+        const uint32_t upto = wave_prefix(sum), whole = __builtin_amdgcn_readlane(upto, 63);
+        if (lane == 0) sh.above[wave] = whole;
+        __syncthreads();
+        uint32_t over = whole - upto + sum_of_waves(sh.above, wave, true);
+        if (over < (uint32_t)need && over + sum >= (uint32_t)need) {
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint32_t o = (uint32_t)__shfl_down((int)from, d);
-                if (lane + d < 64) from += o;
-            }
-            uint32_t above = from - sum;
-            if (above < (uint32_t)need && from >= (uint32_t)need) {
-#pragma unroll
-                for (int x = 3; x >= 0; --x) {
-                    if (above < (uint32_t)need && above + c[x] >= (uint32_t)need) {
-                        sh.bin = 4 * lane + x;
-                        sh.above = above;
-                        sh.inside = c[x];
-                    }
-                    above += c[x];
+            for (int x = PER - 1; x >= 0; --x) {
+                if (over < (uint32_t)need && over + c[x] >= (uint32_t)need) {
+                    sh.bin = tid * PER + x;
+                    sh.over = over;
+                    sh.inside = c[x];
                 }
+                over += c[x];
             }
         }
+#pragma unroll
+        for (int x = 0; x < PER; ++x) sh.hist[tid * PER + x] = 0;
         __syncthreads();
-        need -= (int)sh.above;
+        need -= (int)sh.over;
         lo += sh.bin << shift;
         if (hi - lo >= 1u << shift) hi = lo + ((1u << shift) - 1);
-        all = need == (int)sh.inside;  // the bucket whole
+        const int inside = (int)sh.inside;
+        all = need == inside;  // the bucket whole
+        if (all || inside > 64) continue;
+        each([&](uint32_t v, int i, float) {
+            if (v >= lo && v <= hi) {
+                const uint32_t s = atomicAdd(&sh.few, 1u);
+                sh.key[s] = v;
+                sh.at[s] = i;
+            }
+        });
+        __syncthreads();
+        if (wave == 0) {  // a lane's value has as many before it as are larger, or equal at a lower index
+            const uint32_t v = lane < inside ? sh.key[lane] : 0, at = lane < inside ? sh.at[lane] : 0;
+            int before = 0;
+            for (int i = 0; i < inside; ++i) {
+                const uint32_t o = __builtin_amdgcn_readlane(v, i), oat = __builtin_amdgcn_readlane(at, i);
+                before += o > v || (o == v && oat < at);
+            }
+            if (lane < inside && before == need - 1) {  // the last one chosen
+                sh.bin = v;
+                sh.over = at;
+            }
+        }
+        __syncthreads();
+        lo = hi = sh.bin;
+        limit = (int)sh.over;
     }
-    // Chosen: keys above `hi`, and of those in [lo, hi] all, or (one value) the first `need`.
-    // A thread takes a run of consecutive indices, so that positions ascend with them.
-    const int run = (count + THR - 1) / THR, i0 = min(tid * run, count), i1 = min(i0 + run, count);
-    unsigned long long mine = 0;  // chosen above | candidates << 32
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t v = key(i);
-        if (v > hi || (all && v >= lo))
-            mine += 1;
-        else if (!all && v == lo)
-            mine += 1ull << 32;
+    const auto sure = [&](uint32_t v, int i) { return v > hi || (v >= lo && (all || i <= limit)); };
+    const bool first = !all && limit < 0;  // the first `need` of the values equal to lo
+    uint32_t in = 0, equal = 0;
+    each([&](uint32_t v, int i, float) {
+        const bool s = sure(v, i);
+        in += s;
+        equal += !s && first && v == lo;
+    });
+    const uint32_t ins = wave_prefix(in), equals = wave_prefix(equal);
+    if (lane == 63) {
+        sh.sure[wave] = ins;
+        sh.tie[wave] = equals;
     }
-    unsigned long long incl = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const unsigned long long o = __shfl_up(incl, d);
-        if (lane >= d) incl += o;
-    }
-    if (lane == 63) sh.scan[wave] = incl;
     __syncthreads();
-    unsigned long long before = incl - mine;
-    for (int w = 0; w < wave; ++w) before += sh.scan[w];
-    int sure = (int)(uint32_t)before, ties = (int)(before >> 32);
-    for (int i = i0; i < i1; ++i) {
-        const uint32_t v = key(i);
-        const bool in = v > hi || (all && v >= lo), tie = !in && !all && v == lo;
-        if (in || (tie && ties < need)) emit(sure + min(ties, need), i);
-        sure += in;
+    int chosen = (int)(ins - in + sum_of_waves(sh.sure, wave, false));
+    int ties = (int)(equals - equal + sum_of_waves(sh.tie, wave, false));
+    each([&](uint32_t v, int i, float x) {
+        const bool s = sure(v, i), tie = !s && first && v == lo;
+        if (s || (tie && ties < need)) emit(chosen + min(ties, need), i, x);
+        chosen += s;
         ties += tie;
-    }
+    });
 }
 
 }  // namespace starkv

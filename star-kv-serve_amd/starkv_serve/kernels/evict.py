@@ -22,7 +22,7 @@ def paged_decode_weighted(query: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     A request without tokens gives zeros and leaves its weights."""
     _hip.require_cuda(query, k_cache, v_cache, block_table, seq_lens, weights)
     _hip.refuse_grad("paged_decode_weighted", query, k_cache, v_cache, weights)
-    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if query.shape[0]:
         _hip.ops().weighted_decode(query, k_cache, v_cache, _as_i32(block_table), _as_i32(seq_lens), int(max_seq_len),
                                    float(scale), weights, out)
@@ -42,8 +42,8 @@ def evict(k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tenso
     _hip.refuse_grad("evict", k_cache, v_cache, weights)
     if sink < 0 or recent < 0 or keep < 1 or sink + recent > keep:
         raise ValueError(f"evict: keep={keep} tokens, sink={sink} and recent={recent} among them")
-    lens = torch.empty(seq_lens.shape, dtype=torch.int32, device=seq_lens.device)
-    kept = torch.empty(weights.shape, dtype=torch.float32, device=weights.device)
+    lens = seq_lens.new_empty(seq_lens.shape, dtype=torch.int32)
+    kept = torch.empty_like(weights, memory_format=torch.contiguous_format)
     if block_table.shape[0]:
         _hip.ops().evict(k_cache, v_cache, _as_i32(block_table), _as_i32(seq_lens), weights, int(keep), int(sink),
                          int(recent), lens, kept)

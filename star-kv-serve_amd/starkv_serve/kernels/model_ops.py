@@ -81,26 +81,16 @@ def rope_write(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: tor
     return q_out, k_out, kv16[0], kv16[1]
 
 
-def _norm_rope_check(what: str, positions: torch.Tensor, cos_sin: torch.Tensor, rows: tuple, weights: tuple) -> None:
-    _hip.require_cuda(*rows, positions, cos_sin, *weights)
-    _hip.refuse_grad(what, *rows, *weights)
-    if not rope_fits(cos_sin, positions, *rows):
-        raise NotImplementedError(f"{what}: rows [T, heads, 128] of one dtype (bf16, fp16 or fp32) and cos_sin "
-                                  "[positions, 128], 16-byte aligned, int positions [T], not traced or mapped")
-    for w in weights:
-        if w.shape != (128,) or not w.is_contiguous() or w.dtype not in _FLOATS or w.dtype != weights[0].dtype:
-            raise ValueError(f"{what}: norm weights [128] of one dtype")
-
-
 def norm_rope(positions: torch.Tensor, q: torch.Tensor, k: Optional[torch.Tensor], cos_sin: torch.Tensor,
               q_weight: torch.Tensor, k_weight: Optional[torch.Tensor], eps: float) -> tuple:
     """q [T, H, 128] and k [T, H_kv, 128] (or None) with the RMS norm of each row (x / sqrt(mean(x^2) + eps) *
     weight [128]) and its rotation at `positions` [T], in one launch: fp32 arithmetic, rounded once to their
     dtype. Returns (q, k). No gradient: calls that want one raise."""
-    _norm_rope_check("norm_rope", positions, cos_sin, (q,) if k is None else (q, k),
-                     (q_weight,) if k is None else (q_weight, k_weight))
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    ts = (q, positions, cos_sin, q_weight) if k is None else (q, positions, cos_sin, q_weight, k, k_weight)
+    _hip.require_cuda(*ts)
+    _hip.refuse_grad("norm_rope", *ts)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     if q.shape[0]:
         _hip.ops().norm_rope_qkv(q, k, None, q_weight, k_weight, float(eps), positions, cos_sin, q_out, k_out, None,
                                  None, None, None, None)
@@ -113,15 +103,12 @@ def norm_rope_write(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     """``norm_rope`` with the step's cache write, one launch: the normed and rotated k and v [T, H_kv, 128] into the
     paged caches [num_blocks, block_size, H_kv, 128] at `slots` [T] (distinct; one outside the cache: nothing).
     Returns (q, k when `keep_k`, and with `half` k and v in fp16), as ``rope_write``."""
-    _norm_rope_check("norm_rope_write", positions, cos_sin, (q, k, v), (q_weight, k_weight))
-    _hip.require_cuda(q, k_cache, v_cache, slots)
-    if not rope_write_fits(cos_sin, positions, q, k, v, k_cache, v_cache, slots):
-        raise NotImplementedError("norm_rope_write: bf16 or fp16 rows and caches [blocks, block_size, heads, 128] of one "
-                                  "dtype and layout, 16-byte aligned, blocks of a power of two from 16 tokens")
+    _hip.require_cuda(q, k, v, positions, cos_sin, q_weight, k_weight, k_cache, v_cache, slots)
+    _hip.refuse_grad("norm_rope_write", q, k, v, cos_sin, q_weight, k_weight, k_cache, v_cache)
     if slots.dim() != 1 or slots.shape[0] != q.shape[0]:
         raise ValueError(f"norm_rope_write: slots {tuple(slots.shape)} for {q.shape[0]} tokens")
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if keep_k else None
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if keep_k else None
     kv16 = torch.empty((2, *k.shape), dtype=torch.float16, device=k.device) if half else (None, None)
     if q.shape[0]:
         slots = slots.contiguous() if slots.dtype == torch.int64 else _as_i32(slots)

@@ -56,12 +56,12 @@ def select_blocks(query: torch.Tensor, bounds: torch.Tensor, block_table: torch.
     ``sum_g sum_d max(q_gd lo_d, q_gd hi_d)``, an upper bound of the block's scores summed over the KV head's query
     heads. Scores are summed in 64 bits and compared in fp32, equal ones go to the lower block, so
     the choice does not depend on batch or launch. Requests of at most `keep` blocks read all of them."""
-    n, H = query.shape[:2]
+    n = query.shape[0]
     _hip.require_cuda(query, bounds, block_table, seq_lens)
     _hip.refuse_grad("select_blocks", query, bounds)
     if sink < 0 or recent < 0 or keep < 1 or sink + recent > keep:
         raise ValueError(f"select_blocks: keep={keep} blocks, sink={sink} and recent={recent} among them")
-    selected = torch.empty((n, bounds.shape[1], int(keep)), dtype=torch.int32, device=query.device)
+    selected = query.new_empty((n, bounds.shape[1], int(keep)), dtype=torch.int32)
     if n:
         _hip.ops().select_blocks(query, bounds, _as_i32(block_table), _as_i32(seq_lens), int(max_seq_len),
                                  int(block_size), int(sink), int(recent), selected)
@@ -76,7 +76,7 @@ def paged_decode_sparse(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     tokens is zero."""
     _hip.require_cuda(query, k_cache, v_cache, block_table, seq_lens, selected)
     _hip.refuse_grad("paged_decode_sparse", query, k_cache, v_cache)
-    out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if query.shape[0]:
         _hip.ops().sparse_decode(query, k_cache, v_cache, _as_i32(block_table), _as_i32(seq_lens), selected,
                                  float(scale), out)

@@ -234,9 +234,10 @@ def test_select_blocks(cuda, dt, small, Hkv, G, bs, lens, keep, sink, recent):
         assert torch.equal(got.cpu(), select_plain(q, bounds, bt, lens, span, bs, keep, sink, recent))
 
 
-def test_select_blocks_long(cuda):
-    """More blocks than a row keeps in LDS, and a table of more columns than the span needs."""
-    lens = [16 * 12800 + 5, 16 * 12288, 16 * 9000 - 3]
+@pytest.mark.parametrize("blocks", [12800, 16384, 16387, 33000])
+def test_select_blocks_long(cuda, blocks):
+    """Rows of as many values as the choice keeps in registers, and of more; a table of more columns than needed."""
+    lens = [16 * blocks - 11, 16 * 12288, 16 * 9000 - 3]
     bounds, bt, sl = make_bounds(cuda, lens, 1, 16, BF16, 31)
     q = torch.randn(3, 2, D, generator=torch.Generator().manual_seed(32)).to(BF16).to(cuda)
     got = select_blocks(q, bounds, bt.long(), sl.long(), max(lens), 16, 513, 1, 2)
@@ -447,14 +448,15 @@ def test_evict(cuda, dt, Hkv, bs, lens, keep, sink, recent, layout, ties):
     assert same(kc, want[0]) and same(vc, want[1])
 
 
-def test_evict_long_and_extreme_weights(cuda):
-    """More tokens than a row keeps in LDS; weights of NaN, infinity and zeros of both signs; int64 tables."""
-    lens = [13000, 12400]
+@pytest.mark.parametrize("lens,keep", [([13000, 12400], 12000), ([17000, 16385], 16000)])
+def test_evict_long_and_extreme_weights(cuda, lens, keep):
+    """Rows that the choice keeps in registers and longer ones; weights of NaN, infinity and zeros of both signs; int64
+    tables."""
     kc, vc, bt, sl = make_caches(cuda, lens, 1, 16, BF16, 121)
-    w = torch.rand(2, 1, 13000, generator=torch.Generator().manual_seed(122))
+    w = torch.rand(2, 1, lens[0], generator=torch.Generator().manual_seed(122))
     w[0, 0, 500], w[0, 0, 700], w[0, 0, 900:1000], w[0, 0, 1000:1100] = math.nan, math.inf, -0.0, 0.0
-    want = evict_plain(kc, vc, bt, lens, w, 12000, 2, 50)
-    got_lens, got_w = evict(kc, vc, bt.long(), sl.long(), w.to(cuda), 12000, 2, 50)
+    want = evict_plain(kc, vc, bt, lens, w, keep, 2, 50)
+    got_lens, got_w = evict(kc, vc, bt.long(), sl.long(), w.to(cuda), keep, 2, 50)
     assert torch.equal(got_lens.cpu(), want[2]) and same(got_w, want[3]) and same(kc, want[0]) and same(vc, want[1])
 
 
