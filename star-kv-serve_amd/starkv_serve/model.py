@@ -26,6 +26,17 @@ Two kinds of step: ``decode_step`` (every request contributes its one next token
 compressed layer writes the prompt's codes and runs its dense prefill,
 attention.py:219-251; a full layer writes K/V and runs causal attention over the prompt,
 here on this library's prefill kernel where vLLM would run FlashAttention).
+
+Three options of the uncompressed layers that the reference does not have:
+
+- ``LlamaShape.qk_norm``: an RMS norm of each query and key head in front of the rotation, in the rotation's launch
+  (``model_ops.norm_rope_write``). A compressed layer's keys are lifted from codes as a linear map, which a norm of
+  each key is not: such a shape takes no compressed layer.
+- ``sparse``: decode steps attend to the blocks of each request whose key bounds promise the largest scores
+  (``kernels/sparse_decode.py``); every step keeps the bounds of the blocks it writes.
+- ``weigh``: steps sum up what each cached token weighs (``kernels/evict.py``); ``evict`` cuts the caches of all layers
+  to the tokens that weigh most. After a cut a request's next position is no longer its cache length:
+  ``decode_metadata`` and ``DecodeGraph`` take the lengths apart.
 """
 import math
 from dataclasses import dataclass
@@ -37,7 +48,10 @@ import torch.nn.functional as F
 from starkv_serve.attention import StarKVAttentionImpl, StarKVMetadata
 from starkv_serve.checkpoint import StarKVCheckpoint
 from starkv_serve.kernels import model_ops
+from starkv_serve.kernels.evict import evict, paged_decode_weighted
 from starkv_serve.kernels.prefill import prefill_attention
+from starkv_serve.kernels.sparse_decode import (BlockSelection, key_bounds_like, paged_decode_sparse, select_blocks,
+                                                update_key_bounds)
 from starkv_serve.kernels.stock_decode import paged_decode_full, write_kv_full
 from starkv_serve.workloads import cos_sin_table
 
@@ -53,11 +67,13 @@ class LlamaShape:
     vocab_size: int = 32000
     rms_norm_eps: float = 1e-5
     rope_theta: float = 10000.0
+    qk_norm: bool = False  # an RMS norm of each query and key head (uncompressed layers only)
 
 
 LLAMA2_7B = LlamaShape()
 
 FEW_MAX_TOKENS = 16  # decode steps up to this many tokens take few_linear
+OBSERVED = 16        # a prompt's last tokens, whose attention a model that weighs sums up first
 
 
 class Rotary:
@@ -87,6 +103,8 @@ class Layer:
     q_proj: Optional[torch.Tensor] = None    # compressed: [H * D, hidden]
     impl: Optional[StarKVAttentionImpl] = None
     qkv_proj: Optional[torch.Tensor] = None  # uncompressed: [(H + 2 H_kv) * D, hidden]
+    q_norm: Optional[torch.Tensor] = None    # qk_norm: [D]
+    k_norm: Optional[torch.Tensor] = None
 
     @property
     def compressed(self) -> bool:
@@ -97,9 +115,19 @@ class StarKVLlamaForCausalLM:
     """Decode steps of a Llama with STAR-KV attention in its compressed layers."""
 
     def __init__(self, shape: LlamaShape, starkv: Optional[StarKVCheckpoint], max_model_len: int, device,
-                 dtype: torch.dtype = torch.bfloat16, seed: int = 0, stock: bool = False):
-        """`starkv` = None or `stock` = True: every layer uncompressed (the stock model)."""
+                 dtype: torch.dtype = torch.bfloat16, seed: int = 0, stock: bool = False,
+                 sparse: Optional[BlockSelection] = None, weigh: bool = False):
+        """`starkv` = None or `stock` = True: every layer uncompressed (the stock model). `sparse`: decode steps of
+        the uncompressed layers read selected blocks. `weigh`: steps sum up their tokens' weights, for ``evict``."""
+        compressed = starkv is not None and not stock and any(map(starkv.is_compressed, range(shape.num_layers)))
+        if sparse is not None and weigh:
+            raise ValueError("sparse or weigh: a decode over selected blocks does not weigh the others' tokens")
+        if compressed and shape.qk_norm:
+            raise NotImplementedError("qk_norm: a compressed layer's keys are a linear map of its codes, not normed ones")
+        if compressed and weigh:
+            raise NotImplementedError("weigh: a compressed layer's cache row holds every head's codes and is not cut by head")
         self.shape, self.device, self.dtype = shape, torch.device(device), dtype
+        self.sparse, self.weigh = sparse, weigh
         self.max_model_len = max_model_len
         H, Hkv, D, hid = shape.num_heads, shape.num_kv_heads, shape.head_dim, shape.hidden_size
         self.scale = D ** -0.5
@@ -129,8 +157,12 @@ class StarKVLlamaForCausalLM:
                 layer.impl.to_device(self.device, dtype)
             else:
                 layer.qkv_proj = w((H + 2 * Hkv) * D, hid, fan_in=hid)
+                if shape.qk_norm:
+                    layer.q_norm, layer.k_norm = (torch.ones(D, device=self.device, dtype=dtype) for _ in range(2))
             self.layers.append(layer)
         self.kv_caches: List = []
+        self.key_bounds: List = []  # sparse: per layer, None for a compressed one
+        self.weights: List = []     # weigh: per layer [requests, H_kv, max_model_len], in the order of a step's rows
 
     # -- caches ---------------------------------------------------------------------------
     def cache_bytes_per_token(self) -> int:
@@ -145,10 +177,13 @@ class StarKVLlamaForCausalLM:
                 total += 2 * s.num_kv_heads * s.head_dim * 2
         return total
 
-    def allocate_kv_cache(self, num_blocks: int, block_size: int = 16) -> None:
+    def allocate_kv_cache(self, num_blocks: int, block_size: int = 16, num_requests: int = 0) -> None:
+        """`num_requests`: the most rows of a step of a model that weighs; a request keeps its row from its prompt on."""
         s = self.shape
+        if self.weigh and num_requests < 1:
+            raise ValueError("a model that weighs needs num_requests")
         self.block_size = block_size
-        self.kv_caches = []
+        self.kv_caches, self.key_bounds, self.weights = [], [], []
         for layer in self.layers:
             if layer.compressed:
                 imp = layer.impl
@@ -162,10 +197,29 @@ class StarKVLlamaForCausalLM:
                 kc = torch.zeros(num_blocks, block_size, s.num_kv_heads, s.head_dim, dtype=self.dtype,
                                  device=self.device)
                 self.kv_caches.append((kc, torch.zeros_like(kc)))
+            if self.sparse is not None:
+                self.key_bounds.append(None if layer.compressed else key_bounds_like(kc))
+            if self.weigh:
+                self.weights.append(torch.zeros(num_requests, s.num_kv_heads, self.max_model_len, device=self.device))
+
+    @torch.no_grad()
+    def evict(self, block_table: torch.Tensor, seq_lens: torch.Tensor, keep: int, sink: int = 4,
+              recent: int = 32) -> torch.Tensor:
+        """The caches of every layer cut to `keep` tokens a request and KV head (``kernels.evict.evict``; rows of
+        `block_table` and `seq_lens` as in the steps), their summed weights with them. Returns the cache lengths
+        [n] int32, which the next step takes apart from the positions."""
+        if not self.weights:
+            raise RuntimeError("evict: a model built with weigh=True, its caches allocated")
+        n = seq_lens.shape[0]
+        lens = seq_lens
+        for (kc, vc), weights in zip(self.kv_caches, self.weights):
+            lens, kept = evict(kc, vc, block_table[:n], seq_lens, weights[:n], keep, sink, recent)
+            weights[:n].copy_(kept)
+        return lens
 
     # -- the step ---------------------------------------------------------------------------
     def _attention(self, li: int, x: torch.Tensor, positions: torch.Tensor, md: StarKVMetadata,
-                   capture: Optional[list], in_graph: bool, few: bool) -> torch.Tensor:
+                   capture: Optional[list], in_graph: bool, few: bool, observed=None) -> torch.Tensor:
         """The layer's attention from its residual stream x [T, hidden], up to o_proj's input.
         Inside a graph (`in_graph`) no launch depends on the step's lengths: every layer
         decodes over the span max_model_len, the lengths are read on the device."""
@@ -186,21 +240,72 @@ class StarKVLlamaForCausalLM:
             slots = md.slot_mapping[:T]
             own = getattr(self.rotary.apply, "__func__", None) is Rotary.apply  # not a rotation of the caller's
             if own and model_ops.rope_write_fits(self.rotary.cos_sin_cache, positions, q, k, v, kc, vc, slots):
-                q, k, ka, va = model_ops.rope_write(positions, q, k, v, self.rotary.cos_sin_cache, kc, vc, slots,
-                                                    capture is not None, bool(md.num_prefills))
+                if layer.q_norm is None:
+                    q, k, ka, va = model_ops.rope_write(positions, q, k, v, self.rotary.cos_sin_cache, kc, vc, slots,
+                                                        capture is not None, bool(md.num_prefills))
+                else:
+                    q, k, ka, va = model_ops.norm_rope_write(positions, q, k, v, self.rotary.cos_sin_cache, layer.q_norm,
+                                                             layer.k_norm, s.rms_norm_eps, kc, vc, slots,
+                                                             capture is not None, bool(md.num_prefills))
             else:
+                q, k = self._normed(layer, q, k)
                 q, k = self.rotary.apply(positions, q), self.rotary.apply(positions, k)
                 ka = k
                 write_kv_full(k, v, kc, vc, slots)
             if md.num_prefills:  # whole prompts only (prefill_step): causal attention over each prompt
                 out = prefill_attention(q, ka, va, md.prefill_seq_lens_cpu, self.scale).view(T, H * D)
+                if self.sparse is not None:
+                    update_key_bounds(kc, self.key_bounds[li], md.block_table[:md.num_prefills], md.seq_lens,
+                                      md.max_seq_len)
+                if self.weigh:
+                    self._observe(li, q, md, observed)
             else:
                 span = self.max_model_len if in_graph else max(md.max_seq_len, 1)
-                out = paged_decode_full(q, kc, vc, md.block_table[:T], md.seq_lens[:T], span,
-                                        self.scale).view(T, H * D)
+                out = self._decode_attention(li, q, md, span).view(T, H * D)
         if capture is not None:
             capture.append(dict(layer=li, q=q.view(T, H, D), out=out.view(T, H, D), h=h, k=k, v=v))
         return out
+
+    def _normed(self, layer: Layer, q: torch.Tensor, k: torch.Tensor) -> tuple:
+        """q and k behind their norms, where a rotation of the caller's follows (rounded between the two)."""
+        if layer.q_norm is None:
+            return q, k
+        eps, D = self.shape.rms_norm_eps, self.shape.head_dim
+        return F.rms_norm(q, (D,), layer.q_norm, eps), F.rms_norm(k, (D,), layer.k_norm, eps)
+
+    def _decode_attention(self, li: int, q: torch.Tensor, md: StarKVMetadata, span: int) -> torch.Tensor:
+        """An uncompressed layer's attention of a decode step, its keys and values written."""
+        T = q.shape[0]
+        kc, vc = self.kv_caches[li]
+        table, lens = md.block_table[:T], md.seq_lens[:T]
+        if self.sparse is not None:
+            update_key_bounds(kc, self.key_bounds[li], table, lens, 1)
+            sel = select_blocks(q, self.key_bounds[li], table, lens, span, self.block_size, self.sparse.keep,
+                                self.sparse.sink, self.sparse.recent)
+            return paged_decode_sparse(q, kc, vc, table, lens, sel, self.scale)
+        if self.weigh:
+            return paged_decode_weighted(q, kc, vc, table, lens, span, self.scale, self.weights[li][:T])
+        return paged_decode_full(q, kc, vc, table, lens, span, self.scale)
+
+    @staticmethod
+    def _observed_rows(md: StarKVMetadata, device) -> list:
+        """Per observed token of each prompt, the last first seen latest: (its row of the step, the tokens it sees),
+        0 tokens where the prompt is shorter."""
+        ends = torch.tensor(md.prefill_query_start_loc_cpu[1:])
+        lens = torch.tensor(md.prefill_seq_lens_cpu)
+        back = torch.arange(OBSERVED - 1, -1, -1)[:, None]
+        seen = (lens - back).clamp(min=0)
+        rows = (ends - 1 - torch.minimum(back, lens - 1)).to(device, non_blocking=True)
+        return list(zip(rows, seen.to(torch.int32).to(device, non_blocking=True)))
+
+    def _observe(self, li: int, q: torch.Tensor, md: StarKVMetadata, observed: list) -> None:
+        """The weights of prompts just written: what their last ``OBSERVED`` tokens give, a decode form each."""
+        kc, vc = self.kv_caches[li]
+        n = md.num_prefills
+        weights = self.weights[li][:n]
+        weights.zero_()
+        for rows, seen in observed:
+            paged_decode_weighted(q[rows], kc, vc, md.block_table[:n], seen, md.max_seq_len, self.scale, weights)
 
     # -- the weight products ------------------------------------------------------------------
     def _few(self, T: int, md: StarKVMetadata) -> bool:
@@ -253,8 +358,9 @@ class StarKVLlamaForCausalLM:
                 res.append((q.reshape(T, H * D), None, None))
             else:
                 q, k, v = F.linear(hidden, layer.qkv_proj).split([H * D, Hkv * D, Hkv * D], dim=-1)
-                res.append((self.rotary.apply(positions, q.reshape(T, H, D)),
-                            self.rotary.apply(positions, k.reshape(T, Hkv, D)), v.reshape(T, Hkv, D).contiguous()))
+                q, k = self._normed(layer, q.reshape(T, H, D), k.reshape(T, Hkv, D))
+                res.append((self.rotary.apply(positions, q), self.rotary.apply(positions, k),
+                            v.reshape(T, Hkv, D).contiguous()))
         return res
 
     @torch.no_grad()
@@ -275,15 +381,16 @@ class StarKVLlamaForCausalLM:
             else:
                 kc, vc = self.kv_caches[li]
                 write_kv_full(k, v, kc, vc, md.slot_mapping[:T])
-                span = self.max_model_len if in_graph else max(md.max_seq_len, 1)
-                paged_decode_full(q, kc, vc, md.block_table[:T], md.seq_lens[:T], span, self.scale)
+                self._decode_attention(li, q, md, self.max_model_len if in_graph else max(md.max_seq_len, 1))
 
     @torch.no_grad()
     def _layers(self, x: torch.Tensor, positions: torch.Tensor, md: StarKVMetadata, capture: Optional[list],
                 in_graph: bool) -> torch.Tensor:
         few = self._few(x.shape[0], md)
+        observed = self._observed_rows(md, x.device) if self.weigh and md.num_prefills else None
         for li, layer in enumerate(self.layers):
-            x = self._add_linear(x, self._attention(li, x, positions, md, capture, in_graph, few), layer.o_proj, few)
+            a = self._attention(li, x, positions, md, capture, in_graph, few, observed)
+            x = self._add_linear(x, a, layer.o_proj, few)
             x = self._mlp(x, layer, few)
         return x
 
@@ -293,8 +400,8 @@ class StarKVLlamaForCausalLM:
     def decode_step(self, tokens: torch.Tensor, positions: torch.Tensor, md: StarKVMetadata,
                     capture: Optional[list] = None, in_graph: bool = False) -> torch.Tensor:
         """Logits [n, vocab] for one new token per request: tokens [n] at `positions` [n];
-        `md` has every row as a decode (seq_lens = positions + 1, slot_mapping the new
-        tokens' slots)."""
+        `md` has every row as a decode (slot_mapping the new tokens' slots, seq_lens the cached
+        tokens with them: positions + 1, fewer where caches were cut)."""
         x = self._layers(self.embed[tokens], positions, md, capture, in_graph)
         return self._logits(x, self._few(x.shape[0], md))
 
@@ -318,19 +425,24 @@ class DecodeGraph:
     advances the static tokens and positions in place, so consecutive replays decode
     consecutive tokens with no host work between them; `logits` holds the last replay's
     logits. The block table is static: its rows must cover every position the replays
-    reach (up to max_model_len - 1)."""
+    reach (up to max_model_len - 1). `lens`: cached tokens of each session where they are not its
+    positions (``StarKVLlamaForCausalLM.evict`` cut its caches; ``lens`` of the graph takes what a later
+    cut returns); they advance with the positions."""
 
     def __init__(self, model: StarKVLlamaForCausalLM, block_table: torch.Tensor, tokens: torch.Tensor,
-                 positions: torch.Tensor):
+                 positions: torch.Tensor, lens: Optional[torch.Tensor] = None):
         if model.max_model_len > block_table.shape[1] * model.block_size:
             raise ValueError("the block table's rows must cover max_model_len positions")
         self.model, self.block_table = model, block_table
         self.tokens = tokens.clone()
         self.positions = positions.clone().long()
+        self.lens = None if lens is None else lens.clone().long()
         self.graph = torch.cuda.CUDAGraph()
+        weights = [w.clone() for w in model.weights]
         self._body()  # eager first: every lazy initialisation outside the capture
-        self.tokens.copy_(tokens)
-        self.positions.copy_(positions)
+        for w, before in zip(model.weights, weights):  # that step is run again: its weights count once
+            w.copy_(before)
+        self.reset(tokens, positions, lens)
         torch.cuda.synchronize()
         with torch.cuda.graph(self.graph):
             self._body()
@@ -338,27 +450,36 @@ class DecodeGraph:
     @torch.no_grad()
     def _body(self) -> None:
         m = self.model
-        md = decode_metadata(self.block_table, self.positions, m.block_size, m.max_model_len)
+        md = decode_metadata(self.block_table, self.positions, m.block_size, m.max_model_len, self.lens)
         self.logits = m.decode_step(self.tokens, self.positions, md, in_graph=True)
         if model_ops.greedy_fits(self.logits, self.tokens):
             model_ops.greedy_step(self.logits, self.tokens, self.positions)
         else:
             self.tokens.copy_(self.logits.argmax(-1))
             self.positions.add_(1)
+        if self.lens is not None:
+            self.lens.add_(1)
 
-    def reset(self, tokens: torch.Tensor, positions: torch.Tensor) -> None:
+    def reset(self, tokens: torch.Tensor, positions: torch.Tensor, lens: Optional[torch.Tensor] = None) -> None:
+        if (lens is None) != (self.lens is None):
+            raise ValueError("a graph of sessions with lengths of their own takes them at every reset, another none")
         self.tokens.copy_(tokens)
         self.positions.copy_(positions)
+        if lens is not None:
+            self.lens.copy_(lens)
 
     def replay(self) -> None:
         self.graph.replay()
 
 
 def decode_metadata(block_table: torch.Tensor, positions: torch.Tensor, block_size: int,
-                    max_seq_len: int) -> StarKVMetadata:
+                    max_seq_len: int, lens: Optional[torch.Tensor] = None) -> StarKVMetadata:
     """A decode-only batch's metadata: request b's new token at positions[b] (slot from its
-    block-table row), seq_lens = positions + 1."""
+    block-table row), seq_lens = positions + 1. `lens` [n]: the tokens cached before it, where a cut left fewer than
+    positions[b]; the slot and seq_lens go by them."""
     n = positions.shape[0]
+    if lens is not None:
+        positions = lens.long()
     if max_seq_len > block_table.shape[1] * block_size:
         raise ValueError(f"positions up to {max_seq_len - 1} need more than the block table's "
                          f"{block_table.shape[1]} blocks of {block_size}")

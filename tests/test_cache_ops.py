@@ -111,3 +111,40 @@ def test_norm_rope_refuses_bad_arguments():
         assert L.starkv_norm_rope_qkv(*dict(good, **{arg: value}).values()) != 0, arg
         assert message in L.starkv_last_error(), (arg, L.starkv_last_error())
     assert L.starkv_norm_rope_qkv(*dict(good, T=0).values()) == 0
+
+
+def test_model_options_that_do_not_go_together():
+    from starkv_serve import model as M
+
+    class Compressed:
+        @staticmethod
+        def is_compressed(li):
+            return li == 0
+
+    shape = M.LlamaShape(hidden_size=64, num_layers=1, num_heads=1, num_kv_heads=1, intermediate_size=64, vocab_size=10)
+    normed = M.LlamaShape(**{**shape.__dict__, "qk_norm": True})
+    with pytest.raises(ValueError, match="sparse or weigh"):
+        M.StarKVLlamaForCausalLM(shape, None, 32, "cpu", sparse=BlockSelection(4), weigh=True)
+    with pytest.raises(NotImplementedError, match="qk_norm"):
+        M.StarKVLlamaForCausalLM(normed, Compressed, 32, "cpu")
+    with pytest.raises(NotImplementedError, match="weigh"):
+        M.StarKVLlamaForCausalLM(shape, Compressed, 32, "cpu", weigh=True)
+    model = M.StarKVLlamaForCausalLM(normed, None, 32, "cpu", weigh=True)
+    assert model.layers[0].q_norm.shape == model.layers[0].k_norm.shape == (128,)
+    with pytest.raises(ValueError, match="num_requests"):
+        model.allocate_kv_cache(4)
+    with pytest.raises(RuntimeError, match="weigh=True"):
+        model.evict(torch.zeros(1, 2, dtype=torch.int32), torch.ones(1), 16)
+    model.allocate_kv_cache(4, 16, 3)
+    assert model.weights[0].shape == (3, 1, 32)
+    plain = M.StarKVLlamaForCausalLM(shape, None, 32, "cpu", sparse=BlockSelection(4))
+    plain.allocate_kv_cache(4)
+    assert plain.key_bounds[0].shape == (4, 1, 2, 128) and plain.weights == [] and plain.layers[0].q_norm is None
+
+
+def test_decode_metadata_of_cut_caches():
+    from starkv_serve import model as M
+    bt = torch.arange(8, dtype=torch.int32).view(2, 4)
+    md = M.decode_metadata(bt, torch.tensor([50, 20]), 16, 64, torch.tensor([17, 20], dtype=torch.int32))
+    assert md.slot_mapping.tolist() == [1 * 16 + 1, 5 * 16 + 4] and md.seq_lens.tolist() == [18, 21]
+    assert M.decode_metadata(bt, torch.tensor([50, 20]), 16, 64).seq_lens.tolist() == [51, 21]
