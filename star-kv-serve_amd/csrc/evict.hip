@@ -97,16 +97,10 @@ struct EvictParams {
     const float* w; int64_t w_s0, w_s1;
     int Hkv, cap, keep, sink, recent;
     int32_t* new_lens; float* new_w;  // [n], [n][Hkv][cap]
-    int32_t* kept;                    // [n][Hkv][keep]: the kept tokens' rows of the cache, -1 for none
+    int32_t* kept;                    // [n][Hkv][keep]: the kept tokens, ascending
 };
 
 __device__ __forceinline__ int evict_length(const EvictParams& p, int b) { return min(max(p.seq_lens[b], 0), p.span); }
-
-// Token t's row in a cache of rows, -1 where its block is none of the cache's.
-__device__ __forceinline__ int evict_row(const EvictParams& p, const int32_t* bt, int t) {
-    const int blk = bt[(t >> p.block_shift) * p.bt_s1];
-    return blk < 0 || blk >= p.num_blocks ? -1 : (blk << p.block_shift) + (t & ((1 << p.block_shift) - 1));
-}
 
 template <bool KEPT>
 __global__ __launch_bounds__(TK_THR) void evict_select_kernel(const EvictParams p) {
@@ -122,18 +116,17 @@ __global__ __launch_bounds__(TK_THR) void evict_select_kernel(const EvictParams 
         return;
     }
     int32_t* kept = p.kept + ((int64_t)b * p.Hkv + h) * p.keep;
-    const int32_t* bt = p.bt + b * p.bt_s0;
     const int middle = L - p.sink - p.recent, k = p.keep - p.sink - p.recent;
     for (int i = tid; i < p.sink + p.recent; i += TK_THR) {
         const int from = i < p.sink ? i : middle + i, to = i < p.sink ? i : k + i;
-        kept[to] = evict_row(p, bt, from);
+        kept[to] = from;
         nw[to] = w[from];
     }
     if (k == 0) return;
     w += p.sink;
     topk_ascending<KEPT>(sh, middle, k, [&](int i) { return w[i]; },
                          [&](int pos, int i, float x) {
-                             kept[p.sink + pos] = evict_row(p, bt, p.sink + i);
+                             kept[p.sink + pos] = p.sink + i;
                              nw[p.sink + pos] = x;
                          });
 }
@@ -156,24 +149,30 @@ __global__ __launch_bounds__(CP_THR) void compact_kernel(const EvictParams p, in
     const int mask = (1 << p.block_shift) - 1, chunk = CP_U * step;
     const int32_t* kept = p.kept + ((int64_t)b * p.Hkv + h) * p.keep;
     const int32_t* bt = p.bt + b * p.bt_s0;
-    int from[CP_U], to[CP_U];  // the rows of the chunk after those on their way
+    int64_t from[CP_U], to[CP_U];  // element offsets of the chunk after those on their way, from < 0: stays
     const auto places = [&](int j0) {
+        int t[CP_U], sb[CP_U], db[CP_U];
+#pragma unroll
+        for (int u = 0; u < CP_U; ++u) t[u] = kept[min(j0 + u * step + row, p.keep - 1)];
 #pragma unroll
         for (int u = 0; u < CP_U; ++u) {
-            const int j = min(j0 + u * step + row, p.keep - 1);
-            from[u] = kept[j];
-            to[u] = evict_row(p, bt, j);
-            if (j0 + u * step + row >= p.keep) from[u] = -1;
+            sb[u] = bt[(t[u] >> p.block_shift) * p.bt_s1];
+            db[u] = bt[(min(j0 + u * step + row, p.keep - 1) >> p.block_shift) * p.bt_s1];
+        }
+#pragma unroll
+        for (int u = 0; u < CP_U; ++u) {
+            const int j = j0 + u * step + row;
+            const bool moves = j < p.keep && t[u] != j && sb[u] >= 0 && sb[u] < p.num_blocks && db[u] >= 0 && db[u] < p.num_blocks;
+            from[u] = moves ? sb[u] * p.c_s0 + (t[u] & mask) * p.c_s1 : -1;
+            to[u] = moves ? db[u] * p.c_s0 + (j & mask) * p.c_s1 : -1;
         }
     };
-    const auto offset = [&](int r) { return (r >> p.block_shift) * p.c_s0 + (r & mask) * p.c_s1; };
     const auto read = [&](Round& r) {
 #pragma unroll
         for (int u = 0; u < CP_U; ++u) {
-            const bool moves = from[u] >= 0 && to[u] >= 0 && from[u] != to[u];
-            r.to[u] = moves ? offset(to[u]) : -1;
+            r.to[u] = to[u];
             r.v[u] = make_uint4(0, 0, 0, 0);
-            if (moves) r.v[u] = *(const uint4*)(c + offset(from[u]));
+            if (from[u] >= 0) r.v[u] = *(const uint4*)(c + from[u]);
         }
     };
     const auto write = [&](Round& r) {
@@ -283,8 +282,8 @@ int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64
               "evict: null pointer");
     SKV_CHECK(dtype == STARKV_BF16 || dtype == STARKV_F16, "evict: bf16 or fp16");
     SKV_CHECK(block_shift(block_size) >= 0, "evict: block_size must be 16 times a power of two");
-    SKV_CHECK(num_blocks >= 1 && num_blocks * block_size <= 0x7fffffff && bt_width >= 1 && weights_len >= 1,
-              "evict: empty cache, block table or weights, or a cache of more than 2^31 rows");
+    SKV_CHECK(num_blocks >= 1 && num_blocks <= 0x7fffffff && bt_width >= 1 && weights_len >= 1,
+              "evict: empty cache, block table or weights");
     SKV_CHECK(((uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 && (c_s0 | c_s1 | c_s2) % 8 == 0,
               "evict: cache rows must be 16-byte aligned");
     const size_t need = starkv_evict_workspace_bytes(n, num_kv_heads, keep);

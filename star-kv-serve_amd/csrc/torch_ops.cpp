@@ -6,6 +6,7 @@
 // c10::Error carrying the library's message. Registered for the CUDA (ROCm) dispatch
 // key only: a CPU tensor has no kernel here and raises. The Python wrappers in
 // starkv_serve/kernels/ keep the reference signatures and call these operators.
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/core/DeviceGuard.h>
@@ -324,6 +325,10 @@ void rope_call(const at::Tensor& q, const std::optional<at::Tensor>& k, const st
         for (const auto* w : {q_weight, k_weight})
             TORCH_CHECK(!w || (w->is_contiguous() && w->numel() == 128 && w->scalar_type() == q_weight->scalar_type()),
                         "starkv.norm_rope_qkv: weights [128] of one dtype");
+        if (k_cache) {
+            at::assert_no_internal_overlap(*k_cache);
+            at::assert_no_internal_overlap(*v_cache);
+        }
         check(starkv_norm_rope_qkv(stream_of(q), q.data_ptr(), q.stride(0), q.stride(1), data_of(k), s0, s1, data_of(v),
                                    v0, v1, dtype_code(q), (int)T, (int)H, (int)Hkv, q_weight->data_ptr(),
                                    k_weight ? k_weight->data_ptr() : nullptr, dtype_code(*q_weight), (float)eps,
@@ -396,6 +401,7 @@ void key_bounds(const at::Tensor& k_cache, const at::Tensor& bounds, const at::T
                     bounds.size(2) == 2 && bounds.size(3) == 128 && bounds.stride(3) == 1 &&
                     bounds.scalar_type() == k_cache.scalar_type(),
                 "starkv.key_bounds: bounds [blocks, heads, 2, 128] of the cache's dtype");
+    at::assert_no_internal_overlap(bounds);
     check(starkv_key_bounds(stream_of(k_cache), k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
                             k_cache.stride(2), dtype_code(k_cache), (int)k_cache.size(1), k_cache.size(0),
                             bounds.data_ptr(), bounds.stride(0), bounds.stride(1), bounds.stride(2),
@@ -443,6 +449,7 @@ void sparse_decode(const at::Tensor& query, const at::Tensor& k_cache, const at:
     check_query(out, k_cache, Hkv, "sparse_decode");
     check_table(block_table, seq_lens, n, "sparse_decode");
     TORCH_CHECK(out.sizes() == query.sizes(), "starkv.sparse_decode: out as query");
+    at::assert_no_internal_overlap(out);
     TORCH_CHECK(selected.dim() == 3 && selected.size(0) == n && selected.size(1) == Hkv && selected.size(2) >= 1 &&
                     selected.stride(2) == 1 && selected.scalar_type() == at::kInt,
                 "starkv.sparse_decode: selected [n, heads, keep] int32");
@@ -477,6 +484,8 @@ void weighted_decode(const at::Tensor& query, const at::Tensor& k_cache, const a
     check_table(block_table, seq_lens, n, "weighted_decode");
     check_weights(weights, n, Hkv, "weighted_decode");
     TORCH_CHECK(out.sizes() == query.sizes(), "starkv.weighted_decode: out as query");
+    at::assert_no_internal_overlap(weights);
+    at::assert_no_internal_overlap(out);
     const int span = as_int(max_seq_len, "max_seq_len");
     const at::Tensor ws = workspace(query, starkv_weighted_decode_workspace_bytes((int)n, H, Hkv, span));
     check(starkv_weighted_decode(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1),
@@ -502,6 +511,8 @@ void evict(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tenso
     TORCH_CHECK(new_lens.sizes() == seq_lens.sizes() && new_weights.sizes() == weights.sizes() &&
                     new_weights.is_contiguous() && new_weights.scalar_type() == at::kFloat,
                 "starkv.evict: new_lens and new_weights as seq_lens and weights");
+    at::assert_no_internal_overlap(k_cache);
+    at::assert_no_internal_overlap(v_cache);
     const int k = as_int(keep, "keep");
     const at::Tensor ws = workspace(k_cache, starkv_evict_workspace_bytes((int)n, (int)k_cache.size(2), k));
     check(starkv_evict(stream_of(k_cache), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),

@@ -105,8 +105,8 @@ def norm_rope_write(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     Returns (q, k when `keep_k`, and with `half` k and v in fp16), as ``rope_write``."""
     _hip.require_cuda(q, k, v, positions, cos_sin, q_weight, k_weight, k_cache, v_cache, slots)
     _hip.refuse_grad("norm_rope_write", q, k, v, cos_sin, q_weight, k_weight, k_cache, v_cache)
-    if slots.dim() != 1 or slots.shape[0] != q.shape[0]:
-        raise ValueError(f"norm_rope_write: slots {tuple(slots.shape)} for {q.shape[0]} tokens")
+    if slots.dim() != 1 or slots.shape[0] != q.shape[0] or slots.is_floating_point():
+        raise ValueError(f"norm_rope_write: slots {tuple(slots.shape)} of {slots.dtype} for {q.shape[0]} tokens")
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if keep_k else None
     kv16 = torch.empty((2, *k.shape), dtype=torch.float16, device=k.device) if half else (None, None)

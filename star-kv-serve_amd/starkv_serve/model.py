@@ -178,7 +178,8 @@ class StarKVLlamaForCausalLM:
         return total
 
     def allocate_kv_cache(self, num_blocks: int, block_size: int = 16, num_requests: int = 0) -> None:
-        """`num_requests`: the most rows of a step of a model that weighs; a request keeps its row from its prompt on."""
+        """`num_requests`: the most rows of a step of a model that weighs; a request keeps its row of the weights from its
+        prompt on (decode steps take rows 0 .. n - 1)."""
         s = self.shape
         if self.weigh and num_requests < 1:
             raise ValueError("a model that weighs needs num_requests")
@@ -289,8 +290,8 @@ class StarKVLlamaForCausalLM:
 
     @staticmethod
     def _observed_rows(md: StarKVMetadata, device) -> list:
-        """Per observed token of each prompt, the last first seen latest: (its row of the step, the tokens it sees),
-        0 tokens where the prompt is shorter."""
+        """The last tokens of each prompt in their order: (their rows of the step, the tokens they see), 0 tokens where
+        the prompt is shorter."""
         ends = torch.tensor(md.prefill_query_start_loc_cpu[1:])
         lens = torch.tensor(md.prefill_seq_lens_cpu)
         back = torch.arange(OBSERVED - 1, -1, -1)[:, None]
@@ -298,14 +299,15 @@ class StarKVLlamaForCausalLM:
         rows = (ends - 1 - torch.minimum(back, lens - 1)).to(device, non_blocking=True)
         return list(zip(rows, seen.to(torch.int32).to(device, non_blocking=True)))
 
-    def _observe(self, li: int, q: torch.Tensor, md: StarKVMetadata, observed: list) -> None:
+    def _observe(self, li: int, q: torch.Tensor, md: StarKVMetadata, observed: tuple) -> None:
         """The weights of prompts just written: what their last ``OBSERVED`` tokens give, a decode form each."""
         kc, vc = self.kv_caches[li]
         n = md.num_prefills
-        weights = self.weights[li][:n]
-        weights.zero_()
-        for rows, seen in observed:
-            paged_decode_weighted(q[rows], kc, vc, md.block_table[:n], seen, md.max_seq_len, self.scale, weights)
+        steps, rows = observed
+        weights = torch.zeros(n, *self.weights[li].shape[1:], device=q.device)
+        for at, seen in steps:
+            paged_decode_weighted(q[at], kc, vc, md.block_table[:n], seen, md.max_seq_len, self.scale, weights)
+        self.weights[li].index_copy_(0, rows, weights)
 
     # -- the weight products ------------------------------------------------------------------
     def _few(self, T: int, md: StarKVMetadata) -> bool:
@@ -385,9 +387,12 @@ class StarKVLlamaForCausalLM:
 
     @torch.no_grad()
     def _layers(self, x: torch.Tensor, positions: torch.Tensor, md: StarKVMetadata, capture: Optional[list],
-                in_graph: bool) -> torch.Tensor:
+                in_graph: bool, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         few = self._few(x.shape[0], md)
-        observed = self._observed_rows(md, x.device) if self.weigh and md.num_prefills else None
+        observed = None
+        if self.weigh and md.num_prefills:
+            rows = torch.arange(md.num_prefills, device=x.device) if rows is None else rows.to(x.device, torch.int64)
+            observed = self._observed_rows(md, x.device), rows
         for li, layer in enumerate(self.layers):
             a = self._attention(li, x, positions, md, capture, in_graph, few, observed)
             x = self._add_linear(x, a, layer.o_proj, few)
@@ -407,14 +412,15 @@ class StarKVLlamaForCausalLM:
 
     @torch.no_grad()
     def prefill_step(self, tokens: torch.Tensor, positions: torch.Tensor, md: StarKVMetadata,
-                     capture: Optional[list] = None) -> torch.Tensor:
+                     capture: Optional[list] = None, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Logits [P, vocab] at the last token of each of P whole prompts: tokens [T] and
         positions [T] (0 .. L - 1 per prompt) laid end to end, `md` from
         ``prefill_metadata``. Every layer writes the prompts' cache rows (compressed: the
-        codes through the fused write; full: K and V), so decode steps can follow."""
+        codes through the fused write; full: K and V), so decode steps can follow. `rows` [P]: the
+        prompts' rows of a weighing model's weights (0 .. P - 1)."""
         if md.num_decodes or not md.num_prefills:
             raise ValueError("prefill_step: a prompts-only batch (prefill_metadata)")
-        x = self._layers(self.embed[tokens], positions, md, capture, False)
+        x = self._layers(self.embed[tokens], positions, md, capture, False, rows)
         last = torch.tensor([e - 1 for e in md.prefill_query_start_loc_cpu[1:]]).to(x.device, non_blocking=True)
         return self._logits(x[last], False)
 

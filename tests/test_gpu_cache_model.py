@@ -177,6 +177,19 @@ def test_weighing_and_cuts(cuda):
         tokens, positions = logits.argmax(-1), positions + 1
 
 
+def test_prompts_of_a_later_batch_take_their_rows(cuda):
+    """A prompt that joins running sessions sets its own row of the weights and no other."""
+    model, bt = build(cuda, weigh=True)
+    prefill(model, bt)
+    before = [w.clone() for w in model.weights]
+    md, pos = M.prefill_metadata(bt[1:2], [50], 16)
+    model.prefill_step(torch.arange(50, device=cuda), pos, md, rows=torch.tensor([1]))
+    for w, old in zip(model.weights, before):
+        assert torch.equal(w[0], old[0]) and torch.equal(w[2], old[2]) and not torch.equal(w[1], old[1])
+        assert (w[1, :, :50] > 0).all() and (w[1, :, 50:] == 0).all()
+        assert ((w[1].sum(-1) - 4 * M.OBSERVED).abs() < 4 * M.OBSERVED).all()
+
+
 @pytest.mark.parametrize("mode", ["norm", "sparse", "weigh"])
 def test_captured_steps_are_the_eager_ones(cuda, mode):
     """A captured step of each option, replayed with cuts between the replays where it weighs, against eager steps of a

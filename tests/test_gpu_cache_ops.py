@@ -559,3 +559,77 @@ def test_no_requests(cuda):
     assert paged_decode_weighted(q, x["kc"], x["vc"], bt, sl, 1000, SCALE, x["weights"][:0]).shape == q.shape
     lens, kept = evict(x["kc"], x["vc"], bt, sl, x["weights"][:0], 500)
     assert lens.shape == (0,) and kept.shape == (0, 4, 1000)
+
+
+# -- refusals ---------------------------------------------------------------------------------
+def calls(x):
+    """Each operator as a function of one tensor to put in another's place."""
+    slots = torch.arange(3, device=x["q"].device)
+    k = x["q"][:, :4]
+    return dict(
+        norm=lambda **r: mo.norm_rope(r.get("pos", x["pos"]), r.get("q", x["q"]), r.get("k"), r.get("table", x["table"]),
+                                      r.get("w", x["w"]), r.get("kw"), 1e-6),
+        write=lambda **r: mo.norm_rope_write(x["pos"], r.get("q", x["q"]), r.get("k", k), r.get("v", k), x["table"], x["w"],
+                                             r.get("kw", x["w"]), 1e-6, r.get("kc", x["kc"]), r.get("vc", x["vc"]),
+                                             r.get("slots", slots), False, False),
+        bounds=lambda **r: update_key_bounds(r.get("kc", x["kc"]), r.get("bounds", x["bounds"]), r.get("bt", x["bt"]),
+                                             r.get("sl", x["sl"]), 1),
+        select=lambda **r: select_blocks(r.get("q", x["q"]), r.get("bounds", x["bounds"]), r.get("bt", x["bt"]),
+                                         r.get("sl", x["sl"]), 1000, r.get("bs", 16), r.get("keep", 5), 1, 2),
+        sparse=lambda **r: paged_decode_sparse(r.get("q", x["q"]), r.get("kc", x["kc"]), r.get("vc", x["vc"]), r.get("bt", x["bt"]),
+                                               r.get("sl", x["sl"]), r.get("sel", x["sel"]), SCALE),
+        weighted=lambda **r: paged_decode_weighted(r.get("q", x["q"]), r.get("kc", x["kc"]), r.get("vc", x["vc"]),
+                                                   r.get("bt", x["bt"]), r.get("sl", x["sl"]), r.get("span", 1000), SCALE,
+                                                   r.get("weights", x["weights"])),
+        evict=lambda **r: evict(r.get("kc", x["kc"]), r.get("vc", x["vc"]), r.get("bt", x["bt"]), r.get("sl", x["sl"]),
+                                r.get("weights", x["weights"]), r.get("keep", 500)))
+
+
+def test_refusals(cuda):
+    """What the operators cannot run raises before anything is launched, and leaves everything as it was."""
+    x = make_all(cuda, 171)
+    x["sel"] = torch.zeros(3, 4, 2, dtype=torch.int32, device=cuda)
+    before = {k: v.clone() for k, v in x.items()}
+    f = calls(x)
+    q, kc = x["q"], x["kc"]
+    grad = q.clone().requires_grad_()
+    for name in ("norm", "write", "select", "sparse", "weighted"):
+        with pytest.raises(NotImplementedError, match="gradient"):
+            f[name](q=grad)
+    for name in ("bounds", "sparse", "weighted", "evict"):
+        with pytest.raises(NotImplementedError, match="gradient"):
+            f[name](kc=kc.clone().requires_grad_())
+    with pytest.raises(NotImplementedError, match="transforms"):
+        torch.func.vmap(lambda t: f["sparse"](q=t))(q[None].expand(2, -1, -1, -1))
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        f["weighted"]()
+    for name, key, t in (("norm", "table", x["table"]), ("write", "kc", kc), ("write", "slots", x["pos"]), ("bounds", "bt", x["bt"]),
+                         ("select", "sl", x["sl"]), ("sparse", "sel", x["sel"]), ("weighted", "weights", x["weights"]),
+                         ("evict", "weights", x["weights"])):  # a tensor of another device
+        with pytest.raises(RuntimeError):
+            f[name](**{key: t.cpu()})
+    bad = [
+        ("norm", dict(q=q[..., :64])), ("norm", dict(q=q.double())), ("norm", dict(w=x["w"][:64])), ("norm", dict(pos=x["pos"][:2])),
+        ("norm", dict(table=x["table"][:, :64])), ("norm", dict(k=q, kw=x["w"].half())), ("norm", dict(pos=x["pos"].float())),
+        ("write", dict(k=q)), ("write", dict(kc=kc.half())), ("write", dict(slots=x["pos"][:2])), ("write", dict(v=q[:, :3])),
+        ("write", dict(vc=x["vc"][1:])), ("write", dict(slots=x["pos"].float())),
+        ("write", dict(kc=kc[:1].expand(5, -1, -1, -1), vc=kc[:1].expand(5, -1, -1, -1))),
+        ("bounds", dict(bounds=x["bounds"].half())), ("bounds", dict(bounds=x["bounds"][1:])), ("bounds", dict(sl=x["sl"][:2])),
+        ("bounds", dict(bounds=x["bounds"][:, :1].expand(-1, 4, -1, -1))), ("bounds", dict(kc=kc[:, :8])),
+        ("select", dict(bounds=x["bounds"].half())), ("select", dict(q=q[:, :3])), ("select", dict(bs=24)),
+        ("select", dict(bt=x["bt"][:2])), ("select", dict(keep=2)), ("select", dict(keep=0)),
+        ("sparse", dict(q=q.half())), ("sparse", dict(sel=x["sel"].long())), ("sparse", dict(sel=x["sel"][:, :2])),
+        ("sparse", dict(sel=x["sel"][..., :0])), ("sparse", dict(vc=x["vc"][:, :, :2])), ("sparse", dict(q=q[:, :7])),
+        ("sparse", dict(q=q.repeat(1, 6, 1))), ("sparse", dict(kc=kc.transpose(0, 1).contiguous().transpose(0, 1))),
+        ("weighted", dict(span=1001)), ("weighted", dict(weights=x["weights"].double())), ("weighted", dict(span=0)),
+        ("weighted", dict(weights=x["weights"][:, :1].expand(-1, 4, -1))), ("weighted", dict(weights=x["weights"][:2])),
+        ("weighted", dict(q=q.float())), ("weighted", dict(sl=x["sl"][None])),
+        ("evict", dict(keep=35)), ("evict", dict(weights=x["weights"][:, :3])), ("evict", dict(bt=x["bt"][0])),
+        ("evict", dict(kc=kc[:1].expand(5, -1, -1, -1), vc=kc[:1].expand(5, -1, -1, -1))), ("evict", dict(vc=x["vc"].half())),
+    ]
+    for name, wrong in bad:
+        with pytest.raises((RuntimeError, ValueError, IndexError)):
+            f[name](**wrong)
+    torch.cuda.synchronize()
+    for k, v in before.items():
+        assert same(x[k], v), k
