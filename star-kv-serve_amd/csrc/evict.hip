@@ -44,12 +44,29 @@ __global__ __launch_bounds__(256) void weigh_kernel(const WeighParams wp) {
     }
     const int L = attend_length(p, b), t0 = blockIdx.x * WG_TOKENS;
     if (t0 >= L) return;
+    // The tokens' sums so far and the first heads' scores are on their way while the heads' sums are formed.
+    constexpr int U = WG_TOKENS / 256, AHEAD = 4;
+    const float* lg = p.lg + ((int64_t)b * p.Hkv + h) * p.lg_row;
+    float* w = wp.w + b * wp.w_s0 + h * wp.w_s1;
+    const float* at[U];
+    float old[U], sum[U], ahead[AHEAD][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int t = min(t0 + 256 * u + tid, L - 1);
+        at[u] = lg + (int64_t)(t >> 4) * p.G * 16 + (t & 15);
+        old[u] = w[t];
+        sum[u] = 0.f;
+    }
+#pragma unroll
+    for (int g = 0; g < AHEAD; ++g)
+#pragma unroll
+        for (int u = 0; u < U; ++u) ahead[g][u] = at[u][16 * min(g, p.G - 1)];
     // Each head's log2 of its sum of weights, 16 lanes a head.
     __shared__ float s_lse[AT_MAX_GROUP];
     const int g16 = tid >> 4;
     if (g16 < p.G) {
         const float* pp = p.part + ((int64_t)b * H + h * p.G + g16) * p.splits * AT_PART;
-        float m[AT_MAX_SPLITS / 16], l[AT_MAX_SPLITS / 16], M = -INFINITY, sum = 0.f;
+        float m[AT_MAX_SPLITS / 16], l[AT_MAX_SPLITS / 16], M = -INFINITY, all = 0.f;
 #pragma unroll
         for (int x = 0; x < AT_MAX_SPLITS / 16; ++x) {
             const int s = (tid & 15) + 16 * x;
@@ -59,24 +76,18 @@ __global__ __launch_bounds__(256) void weigh_kernel(const WeighParams wp) {
         }
         M = row16_max(M);
 #pragma unroll
-        for (int x = 0; x < AT_MAX_SPLITS / 16; ++x) sum = fmaf(l[x], m[x] == -INFINITY ? 1.f : exp2f(m[x] - M), sum);
-        sum = row16_sum(sum);
-        if ((tid & 15) == 0) s_lse[g16] = sum == 0.f ? 0.f : M + log2f(sum);  // no block of the cache: weights of 0
+        for (int x = 0; x < AT_MAX_SPLITS / 16; ++x) all = fmaf(l[x], m[x] == -INFINITY ? 1.f : exp2f(m[x] - M), all);
+        all = row16_sum(all);
+        if ((tid & 15) == 0) s_lse[g16] = all == 0.f ? 0.f : M + log2f(all);  // no block of the cache: weights of 0
     }
     __syncthreads();
-    const float* lg = p.lg + ((int64_t)b * p.Hkv + h) * p.lg_row;
-    float* w = wp.w + b * wp.w_s0 + h * wp.w_s1;
-    constexpr int U = WG_TOKENS / 256;
-    float old[U], sum[U];
-    const float* at[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int t = min(t0 + 256 * u + tid, L - 1);
-        at[u] = lg + (int64_t)(t >> 4) * p.G * 16 + (t & 15);
-        old[u] = w[t];
-        sum[u] = 0.f;
-    }
-    for (int g = 0; g < p.G; ++g) {
+    for (int g = 0; g < AHEAD; ++g)
+        if (g < p.G) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) sum[u] += exp2f(ahead[g][u] - s_lse[g]);
+        }
+    for (int g = AHEAD; g < p.G; ++g) {
         float s[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) s[u] = at[u][16 * g];
@@ -102,7 +113,7 @@ struct EvictParams {
 
 __device__ __forceinline__ int evict_length(const EvictParams& p, int b) { return min(max(p.seq_lens[b], 0), p.span); }
 
-template <bool KEPT>
+template <int RUN>
 __global__ __launch_bounds__(TK_THR) void evict_select_kernel(const EvictParams p) {
     __shared__ TopkShared sh;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
@@ -124,7 +135,7 @@ __global__ __launch_bounds__(TK_THR) void evict_select_kernel(const EvictParams 
     }
     if (k == 0) return;
     w += p.sink;
-    topk_ascending<KEPT>(sh, middle, k, [&](int i) { return w[i]; },
+    topk_ascending<RUN>(sh, middle, k, [&](int i) { return w[i]; },
                          [&](int pos, int i, float x) {
                              kept[p.sink + pos] = p.sink + i;
                              nw[p.sink + pos] = x;
@@ -296,11 +307,12 @@ int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64
     p.w = weights; p.w_s0 = w_s0; p.w_s1 = w_s1;
     p.Hkv = num_kv_heads; p.cap = weights_len; p.keep = keep; p.sink = sink; p.recent = recent;
     p.new_lens = new_lens; p.new_w = new_weights; p.kept = (int32_t*)workspace;
-    if (p.span <= TK_KEPT)
-        hipLaunchKernelGGL(evict_select_kernel<true>, dim3(num_kv_heads, n), dim3(TK_THR), 0, (hipStream_t)stream, p);
-    else
-        hipLaunchKernelGGL(evict_select_kernel<false>, dim3(num_kv_heads, n), dim3(TK_THR), 0, (hipStream_t)stream, p);
-    SKV_HIP(hipGetLastError());
+    const int run = topk_run(p.span);
+    const void* fn = run == TK_FEW ? (const void*)&evict_select_kernel<TK_FEW>
+                     : run         ? (const void*)&evict_select_kernel<TK_MANY>
+                                   : (const void*)&evict_select_kernel<0>;
+    void* args[] = {(void*)&p};
+    SKV_HIP(hipLaunchKernel(fn, dim3(num_kv_heads, n), dim3(TK_THR), args, 0, (hipStream_t)stream));
     if (p.span > keep) {
         // Whole rows a workgroup where those fill 256 CUs, else their halves: 8192 -> 2048 tokens of 16 requests of
         // 8 KV heads 81 us whole, 85 in halves; 4096 -> 2048 of 64 requests 255, 265, of 8 53, 42; one of

@@ -182,7 +182,7 @@ __global__ __launch_bounds__(256) void score_kernel(const SelectParams p, int he
     }
 }
 
-template <bool KEPT>
+template <int RUN>
 __global__ __launch_bounds__(TK_THR) void select_kernel(const SelectParams p) {
     __shared__ TopkShared sh;
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
@@ -197,8 +197,8 @@ __global__ __launch_bounds__(TK_THR) void select_kernel(const SelectParams p) {
         sel[i < p.sink ? i : k + i] = i < p.sink ? i : middle + i;
     if (k == 0) return;
     const float* score = p.score + ((int64_t)b * p.Hkv + h) * p.cap + p.sink;
-    topk_ascending<KEPT>(sh, middle, k, [&](int i) { return score[i]; },
-                         [&](int pos, int i, float) { sel[p.sink + pos] = p.sink + i; });
+    topk_ascending<RUN>(sh, middle, k, [&](int i) { return score[i]; },
+                        [&](int pos, int i, float) { sel[p.sink + pos] = p.sink + i; });
 }
 
 template <int DT>
@@ -289,7 +289,7 @@ int starkv_select_blocks(void* stream, const void* query, int64_t q_s0, int64_t 
         int heads = 1;
         while (heads < num_kv_heads && heads < 16) heads *= 2;
         const int64_t groups = (num_kv_heads + heads - 1) / heads, step = 16 / heads * SC_U, most = (p.cap + step - 1) / step;
-        const int64_t want = 2048 / (groups * n);
+        const int64_t want = 4096 / (groups * n);
         const dim3 grid((unsigned)std::min<int64_t>(most, std::max<int64_t>(1, want)), (unsigned)groups, n);
         if (dtype == STARKV_BF16)
             hipLaunchKernelGGL(score_kernel<STARKV_BF16>, grid, dim3(256), 0, (hipStream_t)stream, p, heads);
@@ -297,11 +297,12 @@ int starkv_select_blocks(void* stream, const void* query, int64_t q_s0, int64_t 
             hipLaunchKernelGGL(score_kernel<STARKV_F16>, grid, dim3(256), 0, (hipStream_t)stream, p, heads);
         SKV_HIP(hipGetLastError());
     }
-    if (p.cap <= TK_KEPT)
-        hipLaunchKernelGGL(select_kernel<true>, dim3(num_kv_heads, n), dim3(TK_THR), 0, (hipStream_t)stream, p);
-    else
-        hipLaunchKernelGGL(select_kernel<false>, dim3(num_kv_heads, n), dim3(TK_THR), 0, (hipStream_t)stream, p);
-    SKV_HIP(hipGetLastError());
+    const int run = topk_run(p.cap);
+    const void* fn = run == TK_FEW ? (const void*)&select_kernel<TK_FEW>
+                     : run         ? (const void*)&select_kernel<TK_MANY>
+                                   : (const void*)&select_kernel<0>;
+    void* args[] = {(void*)&p};
+    SKV_HIP(hipLaunchKernel(fn, dim3(num_kv_heads, n), dim3(TK_THR), args, 0, (hipStream_t)stream));
     return STARKV_OK;
 }
 

@@ -6,8 +6,8 @@
 // sign and a few binades spread over them, where buckets of the number's upper bits would be a handful)
 // are counted in LDS; the bucket that holds the k-th largest becomes the range, until it is taken
 // whole, holds 64 values or fewer, which one wave ranks, or one value. One round does for most rows.
-// A thread keeps a run of consecutive values in registers (rows of up to RUN values a thread; longer
-// ones are read again in every pass). A row's time is that of its barriers and first reads: 4096 scores 8
+// A thread keeps a run of consecutive values in registers (rows past 16384 values are read again in
+// every pass). A row's time is that of its barriers and first reads: 4096 scores 8
 // us from launch to end (a kernel of three dependent reads and nothing else takes 4).
 #pragma once
 
@@ -51,8 +51,11 @@ __device__ __forceinline__ uint32_t wave_least(uint32_t v) {
 constexpr int TK_BITS = 11, TK_BINS = 1 << TK_BITS;
 
 constexpr int TK_THR = 1024, TK_WAVES = TK_THR / 64;
-constexpr int TK_RUN = 16;                       // values a thread keeps
-constexpr int TK_KEPT = TK_THR * TK_RUN;         // the longest row that is kept
+// Values a thread keeps, by the longest row: straight code over 4 or 16 of them (a row of 2000 values steps over
+// what it does not have of 16 in every pass), longer rows none.
+constexpr int TK_FEW = 4, TK_MANY = 16;
+
+inline int topk_run(int longest) { return longest <= TK_THR * TK_FEW ? TK_FEW : longest <= TK_THR * TK_MANY ? TK_MANY : 0; }
 
 struct TopkShared {
     uint32_t hist[TK_BINS];
@@ -75,24 +78,32 @@ __device__ __forceinline__ uint32_t sum_of_waves(const uint32_t* t, int wave, bo
 }
 
 // emit(position, index, value) for the k values chosen of value(0) .. value(count - 1), positions 0 .. k - 1 by
-// ascending index; 0 < k <= count, and count <= TK_KEPT where KEPT. Every thread of the workgroup calls it.
-template <bool KEPT, class Value, class Emit>
+// ascending index; 0 < k <= count, and count <= TK_THR RUN where RUN is not 0. Every thread of the workgroup
+// calls it.
+template <int RUN, class Value, class Emit>
 __device__ __forceinline__ void topk_ascending(TopkShared& sh, int count, int k, Value value, Emit emit) {
     constexpr int PER = TK_BINS / TK_THR;  // buckets a thread
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int run = (count + TK_THR - 1) / TK_THR, i0 = min(tid * run, count), mine = min(run, count - i0);
-    float kept[KEPT ? TK_RUN : 1];
-    if constexpr (KEPT) {
+    float kept[RUN ? RUN : 1];
+    if constexpr (RUN) {
 #pragma unroll
-        for (int u = 0; u < TK_RUN; ++u)
-            if (u < run) kept[u] = u < mine ? value(i0 + u) : 0.f;
+        for (int u0 = 0; u0 < RUN; u0 += 4)
+            if (u0 < run) {
+#pragma unroll
+                for (int u = u0; u < u0 + 4; ++u) kept[u] = value(min(i0 + u, count - 1));
+            }
     }
     // f(key, index, value) of the thread's values, in order.
     const auto each = [&](auto f) {
-        if constexpr (KEPT) {
+        if constexpr (RUN) {
 #pragma unroll
-            for (int u = 0; u < TK_RUN; ++u)
-                if (u < run && u < mine) f(order_key(kept[u]), i0 + u, kept[u]);
+            for (int u0 = 0; u0 < RUN; u0 += 4)
+                if (u0 < run) {
+#pragma unroll
+                    for (int u = u0; u < u0 + 4; ++u)
+                        if (u < mine) f(order_key(kept[u]), i0 + u, kept[u]);
+                }
         } else {
             for (int u = 0; u < mine; ++u) {
                 const float v = value(i0 + u);
