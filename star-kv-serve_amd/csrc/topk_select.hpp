@@ -6,9 +6,12 @@
 // sign and a few binades spread over them, where buckets of the number's upper bits would be a handful)
 // are counted in LDS; the bucket that holds the k-th largest becomes the range, until it is taken
 // whole, holds 64 values or fewer, which one wave ranks, or one value. One round does for most rows.
-// A thread keeps a run of consecutive values in registers (rows past 16384 values are read again in
-// every pass). A row's time is that of its barriers and first reads: 4096 scores 8
-// us from launch to end (a kernel of three dependent reads and nothing else takes 4).
+// A wave takes a run of consecutive values, 64 at a time, so that loads are whole lines and a value's
+// place among the chosen is a count of bits; its lanes keep their values in registers (rows past 16384
+// values are read again in every pass). The one CU's instructions, barriers and first reads are a row's
+// time: 4096 scores 5.3 us from launch to end, where a kernel of three dependent reads and nothing else
+// takes 4 (9.0 with a thread's run of consecutive values read from LDS in every pass; 8192 weights 11.2,
+// from 17.6).
 #pragma once
 
 #include "common.hpp"
@@ -48,6 +51,11 @@ __device__ __forceinline__ uint32_t wave_least(uint32_t v) {
     return min(min(a, b), min(c, d));
 }
 
+// The set lanes of a mask below this one.
+__device__ __forceinline__ int lanes_below(unsigned long long mask) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+}
+
 constexpr int TK_BITS = 11, TK_BINS = 1 << TK_BITS;
 
 constexpr int TK_THR = 1024, TK_WAVES = TK_THR / 64;
@@ -84,30 +92,31 @@ template <int RUN, class Value, class Emit>
 __device__ __forceinline__ void topk_ascending(TopkShared& sh, int count, int k, Value value, Emit emit) {
     constexpr int PER = TK_BINS / TK_THR;  // buckets a thread
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int run = (count + TK_THR - 1) / TK_THR, i0 = min(tid * run, count), mine = min(run, count - i0);
+    const int run = (count + TK_THR - 1) / TK_THR, i0 = wave * run * 64 + lane;  // the lane's values: i0 + 64 u, u < run
     float kept[RUN ? RUN : 1];
+    uint32_t keys[RUN ? RUN : 1];
     if constexpr (RUN) {
 #pragma unroll
         for (int u0 = 0; u0 < RUN; u0 += 4)
             if (u0 < run) {
 #pragma unroll
-                for (int u = u0; u < u0 + 4; ++u) kept[u] = value(min(i0 + u, count - 1));
+                for (int u = u0; u < u0 + 4; ++u) kept[u] = value(min(i0 + 64 * u, count - 1));
             }
     }
-    // f(key, index, value) of the thread's values, in order.
+    // f(key, index, value) of the lane's values, in order; every lane calls it. A value that the lane has not has
+    // key 0, below every value's.
     const auto each = [&](auto f) {
         if constexpr (RUN) {
 #pragma unroll
             for (int u0 = 0; u0 < RUN; u0 += 4)
                 if (u0 < run) {
 #pragma unroll
-                    for (int u = u0; u < u0 + 4; ++u)
-                        if (u < mine) f(order_key(kept[u]), i0 + u, kept[u]);
+                    for (int u = u0; u < u0 + 4; ++u) f(keys[u], i0 + 64 * u, kept[u]);
                 }
         } else {
-            for (int u = 0; u < mine; ++u) {
-                const float v = value(i0 + u);
-                f(order_key(v), i0 + u, v);
+            for (int u = 0; u < run; ++u) {
+                const float v = value(min(i0 + 64 * u, count - 1));
+                f(i0 + 64 * u < count ? order_key(v) : 0, i0 + 64 * u, v);
             }
         }
     };
@@ -115,10 +124,24 @@ __device__ __forceinline__ void topk_ascending(TopkShared& sh, int count, int k,
     for (int x = 0; x < PER; ++x) sh.hist[x * TK_THR + tid] = 0;
     if (tid == 0) sh.few = 0;
     uint32_t lo = 0xffffffffu, hi = 0;
-    each([&](uint32_t v, int, float) {
-        lo = min(lo, v);
-        hi = max(hi, v);
-    });
+    if constexpr (RUN) {
+#pragma unroll
+        for (int u0 = 0; u0 < RUN; u0 += 4)
+            if (u0 < run) {
+#pragma unroll
+                for (int u = u0; u < u0 + 4; ++u) {
+                    const uint32_t v = order_key(kept[u]);  // of a lane's own or the row's last value
+                    lo = min(lo, v);
+                    hi = max(hi, v);
+                    keys[u] = u < run && i0 + 64 * u < count ? v : 0;
+                }
+            }
+    } else {
+        each([&](uint32_t v, int, float) {
+            lo = min(lo, v ? v : lo);
+            hi = max(hi, v);
+        });
+    }
     lo = wave_least(lo);
     hi = ~wave_least(~hi);
     if (lane == 0) {
@@ -135,7 +158,7 @@ __device__ __forceinline__ void topk_ascending(TopkShared& sh, int count, int k,
     while (!all && lo != hi) {
         const int shift = max(0, 32 - TK_BITS - __clz((int)(hi - lo)));
         each([&](uint32_t v, int, float) {
-            if (v >= lo && v <= hi) atomicAdd(&sh.hist[(v - lo) >> shift], 1u);
+            if (v - lo <= hi - lo) atomicAdd(&sh.hist[(v - lo) >> shift], 1u);
         });
         __syncthreads();
         // From the top, the bucket that passes `need`: a thread's buckets, its wave's, the waves above.
@@ -167,7 +190,7 @@ __device__ __forceinline__ void topk_ascending(TopkShared& sh, int count, int k,
         all = need == inside;  // the bucket whole
         if (all || inside > 64) continue;
         each([&](uint32_t v, int i, float) {
-            if (v >= lo && v <= hi) {
+            if (v - lo <= hi - lo) {
                 const uint32_t s = atomicAdd(&sh.few, 1u);
                 sh.key[s] = v;
                 sh.at[s] = i;
@@ -190,27 +213,33 @@ __device__ __forceinline__ void topk_ascending(TopkShared& sh, int count, int k,
         lo = hi = sh.bin;
         limit = (int)sh.over;
     }
-    const auto sure = [&](uint32_t v, int i) { return v > hi || (v >= lo && (all || i <= limit)); };
     const bool first = !all && limit < 0;  // the first `need` of the values equal to lo
-    uint32_t in = 0, equal = 0;
+    if (all) hi = lo - 1;                  // all from lo on; one that equals hi comes after `limit`
+    const auto sure = [&](uint32_t v, int i) { return v > hi || (v == hi && i <= limit); };
+    int chosen = 0, ties = 0;  // of the wave's values
     each([&](uint32_t v, int i, float) {
-        const bool s = sure(v, i);
-        in += s;
-        equal += !s && first && v == lo;
+        chosen += __builtin_popcountll(__builtin_amdgcn_ballot_w64(sure(v, i)));
+        if (first) ties += __builtin_popcountll(__builtin_amdgcn_ballot_w64(v == hi));
     });
-    const uint32_t ins = wave_prefix(in), equals = wave_prefix(equal);
-    if (lane == 63) {
-        sh.sure[wave] = ins;
-        sh.tie[wave] = equals;
+    if (lane == 0) {
+        sh.sure[wave] = chosen;
+        sh.tie[wave] = ties;
     }
     __syncthreads();
-    int chosen = (int)(ins - in + sum_of_waves(sh.sure, wave, false));
-    int ties = (int)(equals - equal + sum_of_waves(sh.tie, wave, false));
+    chosen = (int)sum_of_waves(sh.sure, wave, false);
+    ties = (int)sum_of_waves(sh.tie, wave, false);
     each([&](uint32_t v, int i, float x) {
-        const bool s = sure(v, i), tie = !s && first && v == lo;
-        if (s || (tie && ties < need)) emit(chosen + min(ties, need), i, x);
-        chosen += s;
-        ties += tie;
+        const bool s = sure(v, i);
+        const unsigned long long in = __builtin_amdgcn_ballot_w64(s);
+        if (!first) {
+            if (s) emit(chosen + lanes_below(in), i, x);
+        } else {
+            const unsigned long long equal = __builtin_amdgcn_ballot_w64(v == hi);
+            const int before = ties + lanes_below(equal);
+            if (s || (v == hi && before < need)) emit(chosen + lanes_below(in) + min(before, need), i, x);
+            ties += __builtin_popcountll(equal);
+        }
+        chosen += __builtin_popcountll(in);
     });
 }
 
