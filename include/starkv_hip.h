@@ -539,7 +539,7 @@ int starkv_weighted_decode(void *stream, const void *query, int64_t q_s0, int64_
                            const int32_t *seq_lens, int n, int num_heads, int num_kv_heads, int max_seq_len,
                            float scale, float *weights, int64_t w_s0, int64_t w_s1, int weights_len, void *out,
                            int64_t o_s0, int64_t o_s1, void *workspace, size_t workspace_bytes);
-size_t starkv_evict_workspace_bytes(int n, int num_kv_heads, int keep);
+size_t starkv_evict_workspace_bytes(int n, int num_kv_heads, int weights_len, int keep);
 int starkv_evict(void *stream, void *k_cache, void *v_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype,
                  int block_size, int64_t num_blocks, const int32_t *block_table, int64_t bt_s0, int64_t bt_s1,
                  int bt_width, const int32_t *seq_lens, int n, int num_kv_heads, const float *weights, int64_t w_s0,

@@ -273,9 +273,9 @@ int starkv_weighted_decode(void* stream, const void* query, int64_t q_s0, int64_
     return STARKV_OK;
 }
 
-size_t starkv_evict_workspace_bytes(int n, int num_kv_heads, int keep) {
-    if (n < 1 || num_kv_heads < 1 || keep < 1) return 256;
-    return std::max<size_t>(256, (size_t)n * num_kv_heads * keep * 4);
+size_t starkv_evict_workspace_bytes(int n, int num_kv_heads, int weights_len, int keep) {
+    if (n < 1 || num_kv_heads < 1 || weights_len < 1 || keep < 1) return 256;
+    return std::max<size_t>(256, (size_t)n * num_kv_heads * std::min(keep, weights_len) * 4);
 }
 
 int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype,
@@ -297,7 +297,7 @@ int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64
               "evict: empty cache, block table or weights");
     SKV_CHECK(((uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 && (c_s0 | c_s1 | c_s2) % 8 == 0,
               "evict: cache rows must be 16-byte aligned");
-    const size_t need = starkv_evict_workspace_bytes(n, num_kv_heads, keep);
+    const size_t need = starkv_evict_workspace_bytes(n, num_kv_heads, weights_len, keep);
     SKV_CHECK(workspace_bytes >= need, "evict: workspace %zu bytes < %zu", workspace_bytes, need);
     EvictParams p = {};
     p.kc = (uint16_t*)k_cache; p.vc = (uint16_t*)v_cache; p.c_s0 = c_s0; p.c_s1 = c_s1; p.c_s2 = c_s2;

@@ -514,7 +514,7 @@ void evict(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tenso
     at::assert_no_internal_overlap(k_cache);
     at::assert_no_internal_overlap(v_cache);
     const int k = as_int(keep, "keep");
-    const at::Tensor ws = workspace(k_cache, starkv_evict_workspace_bytes((int)n, (int)k_cache.size(2), k));
+    const at::Tensor ws = workspace(k_cache, starkv_evict_workspace_bytes((int)n, (int)k_cache.size(2), as_int(weights.size(2), "weights"), k));
     check(starkv_evict(stream_of(k_cache), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),
                        k_cache.stride(2), dtype_code(k_cache), (int)k_cache.size(1), k_cache.size(0),
                        i32(block_table, "block_table"), block_table.stride(0), block_table.stride(1),

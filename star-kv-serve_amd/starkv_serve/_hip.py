@@ -80,7 +80,7 @@ SIGNATURES = {
     "starkv_weighted_decode_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "starkv_weighted_decode": (_I, [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _I64, _P, _I64, _I64, _I, _P,
                                     _I, _I, _I, _I, _F, _P, _I64, _I64, _I, _P, _I64, _I64, _P, _SZ]),
-    "starkv_evict_workspace_bytes": (_SZ, [_I, _I, _I]),
+    "starkv_evict_workspace_bytes": (_SZ, [_I, _I, _I, _I]),
     "starkv_evict": (_I, [_P, _P, _P, _I64, _I64, _I64, _I, _I, _I64, _P, _I64, _I64, _I, _P, _I, _I, _P, _I64, _I64,
                           _I, _I, _I, _I, _P, _P, _P, _SZ]),
     "starkv_profile_begin": (_I, [_I, _I]),

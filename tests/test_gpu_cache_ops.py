@@ -223,7 +223,8 @@ def make_bounds(cuda, lens, Hkv, bs, dt, seed, small=False):
 @pytest.mark.parametrize("Hkv,G,bs,lens,keep,sink,recent", [
     (1, 1, 16, [1, 0, 16, 17, 4000], 3, 1, 2), (2, 4, 32, [5000, 3000, 64, 33], 17, 1, 2), (3, 7, 16, [2000, 1999], 50, 0, 0),
     (8, 1, 64, [9000, 128, 65], 5, 2, 3), (1, 16, 16, [1600], 99, 0, 1), (2, 2, 16, [640, 500], 1, 0, 1),
-    (4, 8, 16, [20000, 333], 700, 4, 9)])
+    (4, 8, 16, [20000, 333], 700, 4, 9), (20, 2, 16, [3000, 500], 40, 1, 2), (32, 1, 32, [5000], 12, 0, 1),
+    (5, 3, 16, [1200, 1100, 90], 9, 2, 1), (2, 9, 16, [900], 20, 1, 1)])
 def test_select_blocks(cuda, dt, small, Hkv, G, bs, lens, keep, sink, recent):
     bounds, bt, sl = make_bounds(cuda, lens, Hkv, bs, dt, 21, small)
     g = torch.Generator().manual_seed(22)
@@ -264,7 +265,8 @@ def test_select_blocks_extremes(cuda):
 # -- the decode over selected blocks ----------------------------------------------------------
 SPARSE = [(1, 1, 16, [1, 0, 15, 17, 200], 4, "plain"), (2, 4, 16, [700, 333, 16], 9, "pairs"),
           (3, 7, 32, [1000, 31], 5, "heads"), (8, 2, 64, [900, 64, 129], 6, "plain"), (1, 16, 16, [2500], 120, "plain"),
-          (4, 1, 16, [5000, 4999], 301, "pairs")]
+          (4, 1, 16, [5000, 4999], 301, "pairs"), (2, 9, 16, [300, 77], 11, "heads"), (1, 12, 1024, [3000], 3, "plain"),
+          (5, 3, 16, [400], 25, "plain")]
 
 
 def pick(lens, Hkv, bs, keep, seed):
@@ -375,7 +377,8 @@ def test_infinite_and_nan_values_stay_in_their_rows(cuda):
 @pytest.mark.parametrize("Hkv,G,bs,lens,span,layout", [
     (1, 1, 16, [1, 0, 15, 17, 200], 200, "plain"), (2, 4, 16, [700, 333, 16], 700, "pairs"),
     (3, 7, 32, [1000, 31], 900, "heads"), (8, 2, 64, [900, 64, 129], 2000, "plain"), (1, 16, 16, [5000], 5000, "plain"),
-    (32, 1, 16, [1300, 1025], 1300, "plain"), (1, 5, 16, [9000], 9001, "heads")])
+    (32, 1, 16, [1300, 1025], 1300, "plain"), (1, 5, 16, [9000], 9001, "heads"), (2, 11, 16, [300, 77], 300, "pairs"),
+    (1, 3, 256, [700], 700, "plain"), (1, 1, 16, [70000], 70000, "plain")])
 def test_weighted_decode(cuda, dt, Hkv, G, bs, lens, span, layout):
     kc, vc, bt, sl = make_caches(cuda, lens, Hkv, bs, dt, 101, layout)
     g = torch.Generator().manual_seed(102)
@@ -406,6 +409,34 @@ def test_weighted_decode(cuda, dt, Hkv, G, bs, lens, span, layout):
     assert torch.equal(again, wide)  # the same bits every time
 
 
+def test_long_ranges_of_a_workgroup(cuda):
+    """So many requests that each one's head is one workgroup's, over more pages than are looked up at a time. The
+    requests read the same blocks, each with a query of its own."""
+    bs, Hkv, L, blocks = 256, 8, 8900, 36
+    g = torch.Generator(device=cuda).manual_seed(191)
+    kc, vc = (torch.empty(blocks, bs, Hkv, D, device=cuda).normal_(generator=g).to(BF16) for _ in range(2))
+    one = torch.randperm(blocks, generator=torch.Generator().manual_seed(192))[:35].int().to(cuda)
+    k, v = (t[one.long()].reshape(-1, Hkv, D)[:L].permute(1, 0, 2).cpu() for t in (kc, vc))
+    for n, weighted in ((70, False), (520, True)):
+        q = torch.empty(n, Hkv, D, device=cuda).normal_(generator=g).to(BF16)
+        bt, sl = one.expand(n, -1), torch.full((n,), L, dtype=torch.int32, device=cuda)
+        sl[1] = 8193
+        if weighted:
+            w = torch.zeros(n, Hkv, L, device=cuda)
+            got = paged_decode_weighted(q, kc, vc, bt, sl, L, SCALE, w)
+        else:
+            sel = torch.arange(35, dtype=torch.int32, device=cuda).expand(n, Hkv, -1)
+            got = paged_decode_sparse(q, kc, vc, bt, sl, sel, SCALE)
+        for b in (0, 1, n // 2, n - 1):
+            for h in (0, 3, 7):
+                t = int(sl[b])
+                out, tol, p, ptol = attention64(q[b, h:h + 1].cpu(), k[h, :t].double(), v[h, :t].double(), BF16)
+                check(got[b, h:h + 1], out, tol, (n, b, h))
+                if weighted:
+                    check(w[b, h, :t], p[0], ptol[0] + 4 * E * p[0] + 1e-37, (n, b, h, "w"))
+                    assert (w[b, h, t:] == 0).all()
+
+
 # -- eviction ---------------------------------------------------------------------------------
 def evict_plain(kc, vc, bt, lens, w, keep, sink, recent):
     kc, vc, bt, w = kc.cpu().clone(), vc.cpu().clone(), bt.cpu().long(), w.cpu()
@@ -434,7 +465,8 @@ def same(a, b):
     (1, 16, [1, 0, 15, 17, 200], 16, 1, 2, "plain", False), (2, 16, [700, 333, 16], 300, 4, 32, "pairs", True),
     (3, 32, [1000, 31], 1, 0, 1, "heads", False), (8, 64, [900, 64, 129], 128, 0, 128, "plain", True),
     (1, 16, [2500, 2049], 2048, 0, 0, "plain", False), (2, 16, [1500], 1499, 4, 32, "plain", True),
-    (4, 16, [700], 20, 10, 10, "heads", False)])
+    (4, 16, [700], 20, 10, 10, "heads", False), (1, 16, [90, 40], 1 << 30, 0, 0, "plain", False),
+    (33, 16, [300, 170, 290, 100], 128, 2, 9, "plain", True), (1, 512, [1200], 700, 1, 1, "plain", False)])
 def test_evict(cuda, dt, Hkv, bs, lens, keep, sink, recent, layout, ties):
     kc, vc, bt, sl = make_caches(cuda, lens, Hkv, bs, dt, 111, layout)
     g = torch.Generator().manual_seed(112)
