@@ -18,6 +18,11 @@
 // l loaded of each of its 8 tokens (4 rows of 256 bytes a load), gathered with 4 byte permutes. A lane
 // ends with 32 consecutive dimensions of one column.
 //
+// Memory bounds it: 512 bytes of keys and values a token and KV head, far above the instructions' time for
+// any G. 32 requests of up to 2048 selected tokens over 32 KV heads (1.07 GB) 189 us, 5.7 TB/s; 24 of 1000
+// to 8191 tokens over 8 KV heads with their scores left behind (445 MB) 97. The next tile's loads ahead of a
+// tile's products gained nothing (189 -> 193, at half the waves), nor did loads past the caches.
+//
 // Rounding: scores, references and sums are fp32. The weights enter the second product as two values
 // of the cache's type, the rounded weight and what the rounding left (16 bits of a bf16 weight, 22 of an
 // fp16 one): up to 8 query heads the second value takes the other 8 columns, whose scores are the same
@@ -105,7 +110,6 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
     const int id = blockIdx.x, s = id % p.splits, u = id / p.splits, h = u % p.Hkv, b = u / p.Hkv;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = MANY ? lane & 15 : lane & 7, quad = lane >> 4;  // the lane's query head
-    const float rest = lane & 8 ? 1.f : 0.f;                        // not MANY: its column takes the weights' second values
     const int H = p.Hkv * p.G;
     const int L = attend_length(p, b);
     const int pages = SPARSE ? p.keep << p.bs_shift : (L + 15) >> 4;
@@ -134,7 +138,7 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
             if (lb >= 0 && lb < blocks) {
                 tokens = min(max(L - 16 * ((lb << p.bs_shift) + (pg & mask)), 0), 16);
                 blk = p.bt[b * p.bt_s0 + lb * p.bt_s1];
-                if (blk < 0 || blk >= p.num_blocks) tokens = 0;  // no block of the cache: no tokens
+                if (blk < 0 || blk >= p.num_blocks) blk = tokens = 0;  // no block of the cache: no tokens
             }
             s_page[i] = make_int2(blk, tokens | (pg & mask) << 8);
         }
@@ -149,21 +153,17 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
                 e[x].y = __builtin_amdgcn_readfirstlane(v.y);
                 nt[x] = i + x < count ? e[x].y & 255 : 0;
             }
+            float* lg = p.lg + ((int64_t)b * p.Hkv + h) * p.lg_row + (int64_t)(c0 + i) * p.G * 16;  // page i's scores
+            if (SPARSE && nt[0] + nt[1] == 0) continue;
             const bool own = col < p.G && (MANY || !(lane & 8));
-            float* lg = p.lg + ((int64_t)b * p.Hkv + h) * p.lg_row + ((int64_t)(c0 + i) * p.G + col) * 16 + 4 * quad;
-            if (nt[0] + nt[1] == 0) {
-                if (!SPARSE && own)
-                    for (int x = 0; x < 2 && i + x < count; ++x)
-                        *(float4*)(lg + 16 * x * p.G) = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                continue;
-            }
             uint4 kr[2][4], vr[2][4];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 // A page without tokens reads the other one's rows, one with fewer than 16 its last row
-                // again: every address lies in the request's tokens, and nothing of them is used.
+                // again: every address lies in the request's tokens (or, where neither page has a block of the
+                // cache, in block 0), and nothing of them is used.
                 const int2 at = nt[x] ? e[x] : e[x ^ 1];
-                const int last = (nt[x] ? nt[x] : nt[x ^ 1]) - 1;
+                const int last = max(nt[x] ? nt[x] : nt[x ^ 1], 1) - 1;
                 const int64_t base = at.x * p.c_s0 + (int64_t)((at.y >> 8) << 4) * p.c_s1;
 #pragma unroll
                 for (int st = 0; st < 4; ++st)
@@ -190,8 +190,8 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
                 }
             }
             if (!SPARSE && own) {
-                *(float4*)lg = make_float4(sv[0][0], sv[0][1], sv[0][2], sv[0][3]);
-                if (i + 1 < count) *(float4*)(lg + 16 * p.G) = make_float4(sv[1][0], sv[1][1], sv[1][2], sv[1][3]);
+                *(float4*)(lg + 16 * col + 4 * quad) = make_float4(sv[0][0], sv[0][1], sv[0][2], sv[0][3]);
+                if (i + 1 < count) *(float4*)(lg + 16 * p.G + 16 * col + 4 * quad) = make_float4(sv[1][0], sv[1][1], sv[1][2], sv[1][3]);
             }
             float mx = sv[0][0];
 #pragma unroll
@@ -213,7 +213,8 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
                     pe[x][r] = 4 * quad + r < nt[x] ? exp2f(sv[x][r] - m) : 0.f;
                     l += pe[x][r];
                 }
-            const uint2 p0 = attend_rest<DT>(pe[0], MANY ? 0.f : rest), p1 = attend_rest<DT>(pe[1], MANY ? 0.f : rest);
+            const float rest = !MANY && lane & 8 ? 1.f : 0.f;  // the lane's column takes the weights' second values
+            const uint2 p0 = attend_rest<DT>(pe[0], rest), p1 = attend_rest<DT>(pe[1], rest);
             const uint4 pf = make_uint4(p0.x, p0.y, p1.x, p1.y);
             uint4 pl = make_uint4(0, 0, 0, 0);
             if constexpr (MANY) {
