@@ -492,6 +492,59 @@ def test_evict_long_and_extreme_weights(cuda, lens, keep):
     assert torch.equal(got_lens.cpu(), want[2]) and same(got_w, want[3]) and same(kc, want[0]) and same(vc, want[1])
 
 
+@pytest.mark.parametrize("gone", [[3], [2, 3], [0, 1, 2, 3, 4, 5, 6], [6], [5, 6]])
+def test_blocks_outside_the_cache_hold_no_tokens(cuda, gone):
+    """Block ids outside the cache (a table's padding that a length runs into): no bounds, the lowest score, no attention,
+    a weight of 0, no move."""
+    L, Hkv, bs = 100, 2, 16
+    kc, vc, bt, sl = make_caches(cuda, [L, 40], Hkv, bs, BF16, 201)
+    g = torch.Generator().manual_seed(202)
+    q = torch.randn(2, 4, D, generator=g).to(BF16).to(cuda)
+    bt2 = bt.clone()
+    bt2[0, gone] = torch.tensor([-1, kc.shape[0], 1 << 30, -1 << 31, -7, kc.shape[0] + 1, -1], dtype=torch.int32, device=cuda)[:len(gone)]
+    there = [t for t in range(L) if t // bs not in gone]
+    bounds = key_bounds_like(kc).fill_(3.0)
+    update_key_bounds(kc, bounds, bt2, sl, L)
+    want = key_bounds_like(kc).fill_(3.0)
+    update_key_bounds(kc, want, bt, sl, L)
+    want[bt[0, gone].long()] = 3.0
+    assert torch.equal(bounds, want)
+    keep = max(1, 7 - len(gone))
+    sel = select_blocks(q, bounds, bt2, sl, L, bs, keep, 0, 0)
+    if len(gone) < 7:
+        assert sel[0].tolist() == [[j for j in range(7) if j not in gone]] * Hkv
+    w = torch.rand(2, Hkv, 128, generator=g).to(cuda)
+    old = w.clone()
+    out = paged_decode_weighted(q, kc, vc, bt2, sl, 128, SCALE, w)
+    for h in range(Hkv):
+        if there:
+            want_out, tol, p, ptol = attention64(q[0, 2 * h:2 * h + 2].cpu(), rows_of(kc, bt, 0, h, there), rows_of(vc, bt, 0, h, there), BF16)
+            check(out[0, 2 * h:2 * h + 2], want_out, tol, h)
+        else:
+            assert (out[0] == 0).all()
+        new = old[0, h].double().cpu()
+        new[L - 1] = 0
+        slack = 4 * E * new
+        if there:
+            new[there] += p.sum(0)
+            slack[there] += ptol.sum(0) + 4 * E * p.sum(0)
+        check(w[0, h], new, slack + 1e-37, h)
+    before = kc.clone(), vc.clone()
+    lens, kept = evict(kc, vc, bt2, sl, w, 50, 2, 10)
+    assert lens.tolist() == [50, 40]
+    for h in range(Hkv):
+        mid = sorted(range(2, 90), key=lambda i: (-w[0, h, i].item(), i))[:38]
+        order = [0, 1, *sorted(mid), *range(90, 100)]
+        assert torch.equal(kept[0, h, :50], w[0, h, order])
+        for now, then in zip((kc, vc), before):
+            for j, t in enumerate(order):
+                if j // bs in gone:
+                    continue
+                row = now[bt[0, j // bs].long(), j % bs, h]
+                source = t if t // bs not in gone else j  # a row without a source stays
+                assert torch.equal(row, then[bt[0, source // bs].long(), source % bs, h])
+
+
 # -- uses -------------------------------------------------------------------------------------
 def test_offsets_past_32_bits(cuda):
     """Blocks behind 2^31 elements of the caches."""
