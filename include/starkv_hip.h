@@ -490,7 +490,8 @@ int starkv_norm_rope_qkv(void *stream, const void *q, int64_t q_s0, int64_t q_s1
  *
  * starkv_key_bounds: bounds [num_blocks, num_kv_heads, 2, 128] (element strides b_s0, b_s1, b_s2; the cache's
  * dtype) of every block that holds one of a request's last max_new tokens: the elementwise least and largest
- * of the block's keys up to the request's length (NaN stays NaN). max_new 1 after a decode step, the longest
+ * of the block's keys up to the request's length (NaN stays NaN; a block with an infinite key scores infinite or
+ * NaN). max_new 1 after a decode step, the longest
  * prompt after a prefill.
  *
  * starkv_select_blocks: for each request and KV head the `keep` logical blocks (indices into the request's

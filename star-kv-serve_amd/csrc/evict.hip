@@ -62,8 +62,8 @@ __global__ __launch_bounds__(256) void weigh_kernel(const WeighParams wp) {
     for (int g = 0; g < AHEAD; ++g)
 #pragma unroll
         for (int u = 0; u < U; ++u) ahead[g][u] = at[u][16 * min(g, p.G - 1)];
-    // Each head's log2 of its sum of weights, 16 lanes a head.
-    __shared__ float s_lse[AT_MAX_GROUP];
+    // Each head's largest reference and the inverse of its sum of weights above it, 16 lanes a head.
+    __shared__ float s_ref[AT_MAX_GROUP], s_inv[AT_MAX_GROUP];
     const int g16 = tid >> 4;
     if (g16 < p.G) {
         const float* pp = p.part + ((int64_t)b * H + h * p.G + g16) * p.splits * AT_PART;
@@ -79,21 +79,24 @@ __global__ __launch_bounds__(256) void weigh_kernel(const WeighParams wp) {
 #pragma unroll
         for (int x = 0; x < AT_MAX_SPLITS / 16; ++x) all = fmaf(l[x], m[x] == -INFINITY ? 1.f : exp2f(m[x] - M), all);
         all = row16_sum(all);
-        if ((tid & 15) == 0) s_lse[g16] = all == 0.f ? 0.f : M + log2f(all);  // no block of the cache: weights of 0
+        if ((tid & 15) == 0) {
+            s_ref[g16] = all == 0.f ? 0.f : M;  // no block of the cache: weights of 0
+            s_inv[g16] = all == 0.f ? 0.f : 1.f / all;
+        }
     }
     __syncthreads();
 #pragma unroll
     for (int g = 0; g < AHEAD; ++g)
         if (g < p.G) {
 #pragma unroll
-            for (int u = 0; u < U; ++u) sum[u] += exp2f(ahead[g][u] - s_lse[g]);
+            for (int u = 0; u < U; ++u) sum[u] = fmaf(exp2f(ahead[g][u] - s_ref[g]), s_inv[g], sum[u]);
         }
     for (int g = AHEAD; g < p.G; ++g) {
         float s[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) s[u] = at[u][16 * g];
 #pragma unroll
-        for (int u = 0; u < U; ++u) sum[u] += exp2f(s[u] - s_lse[g]);
+        for (int u = 0; u < U; ++u) sum[u] = fmaf(exp2f(s[u] - s_ref[g]), s_inv[g], sum[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {

@@ -24,8 +24,8 @@
 // tile's products gained nothing (189 -> 193, at half the waves), nor did loads past the caches.
 //
 // Rounding: scores, references and sums are fp32. The weights enter the second product as two values
-// of the cache's type, the rounded weight and what the rounding left (16 bits of a bf16 weight, 22 of an
-// fp16 one): up to 8 query heads the second value takes the other 8 columns, whose scores are the same
+// of the cache's type, the weight in it and what that left (16 bits of a bf16 weight, cut, and 22 of an
+// fp16 one, rounded): up to 8 query heads the second value takes the other 8 columns, whose scores are the same
 // heads' again, and costs no instruction of the matrix unit; 9 to 16 heads take a product each. The
 // reference lies 2^7 below the largest score seen when it was set and moves when a score passes it by
 // 2^15 (fp16 weights stay finite, and small ones keep 22 bits of range above its subnormals).

@@ -328,6 +328,7 @@ void rope_call(const at::Tensor& q, const std::optional<at::Tensor>& k, const st
         if (k_cache) {
             at::assert_no_internal_overlap(*k_cache);
             at::assert_no_internal_overlap(*v_cache);
+            at::assert_no_overlap(*k_cache, *v_cache);
         }
         check(starkv_norm_rope_qkv(stream_of(q), q.data_ptr(), q.stride(0), q.stride(1), data_of(k), s0, s1, data_of(v),
                                    v0, v1, dtype_code(q), (int)T, (int)H, (int)Hkv, q_weight->data_ptr(),
@@ -513,6 +514,7 @@ void evict(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tenso
                 "starkv.evict: new_lens and new_weights as seq_lens and weights");
     at::assert_no_internal_overlap(k_cache);
     at::assert_no_internal_overlap(v_cache);
+    at::assert_no_overlap(k_cache, v_cache);  // each tensor's rows move by themselves
     const int k = as_int(keep, "keep");
     const at::Tensor ws = workspace(k_cache, starkv_evict_workspace_bytes((int)n, (int)k_cache.size(2), as_int(weights.size(2), "weights"), k));
     check(starkv_evict(stream_of(k_cache), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1),

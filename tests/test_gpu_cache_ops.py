@@ -711,6 +711,7 @@ def test_refusals(cuda):
         ("weighted", dict(q=q.float())), ("weighted", dict(sl=x["sl"][None])),
         ("evict", dict(keep=35)), ("evict", dict(weights=x["weights"][:, :3])), ("evict", dict(bt=x["bt"][0])),
         ("evict", dict(kc=kc[:1].expand(5, -1, -1, -1), vc=kc[:1].expand(5, -1, -1, -1))), ("evict", dict(vc=x["vc"].half())),
+        ("evict", dict(vc=kc)), ("write", dict(vc=kc)),
     ]
     for name, wrong in bad:
         with pytest.raises((RuntimeError, ValueError, IndexError)):
