@@ -11,7 +11,8 @@
 // those of the largest weights between (topk_select.hpp). The order of tokens stays, so `recent` means the
 // same at the next eviction, and kept[j] >= j ascends: compact_kernel moves row kept[j] to row j in place,
 // reading rows of a chunk before any of them is written; a later chunk's sources lie behind every
-// earlier chunk's targets. Columns are independent of each other, so K and V, and for few requests their
+// earlier chunk's targets (a handful of heads moves all rows at once instead, through the workspace:
+// stage_kernel). Columns are independent of each other, so K and V, and for few requests their
 // halves of 128 bytes, go to workgroups of their own. 16 requests of 8 KV heads cut from 4097 to 8192 tokens
 // to 2048: the choice 11 us (one CU a head), the move 60 (268 MB, 4.4 TB/s; a large copy's rate is 5.0).
 #include <algorithm>
@@ -113,6 +114,7 @@ struct EvictParams {
     int Hkv, cap, keep, sink, recent;
     int32_t* new_lens; float* new_w;  // [n], [n][Hkv][cap]
     int32_t* kept;                    // [n][Hkv][keep]: the kept tokens, ascending
+    uint16_t* aside;                  // stage_kernel: [n][Hkv][keep][2][128]
 };
 
 __device__ __forceinline__ int evict_length(const EvictParams& p, int b) { return min(max(p.seq_lens[b], 0), p.span); }
@@ -212,6 +214,48 @@ __global__ __launch_bounds__(CP_THR) void compact_kernel(const EvictParams p, in
     }
 }
 
+constexpr int ST_ROWS = 64;  // rows a workgroup, four a lane
+
+// A few long rows of caches: one workgroup a column slice moves a chunk after the other, and a handful of them
+// leave the device idle. Here every row moves at once, in two launches: the sources that are targets too (token
+// kept[j] < keep) are copied aside, then all rows are written, from there or from behind the kept part.
+// 16 lanes a row.
+template <bool BACK>
+__global__ __launch_bounds__(256) void stage_kernel(const EvictParams p) {
+    const int h = blockIdx.y, b = blockIdx.z;
+    if (evict_length(p, b) <= p.keep) return;
+    const int d = 8 * (threadIdx.x & 15), j0 = blockIdx.x * ST_ROWS + (threadIdx.x >> 4), mask = (1 << p.block_shift) - 1;
+    const int64_t unit = (int64_t)b * p.Hkv + h;
+    const int32_t* kept = p.kept + unit * p.keep;
+    const int32_t* bt = p.bt + b * p.bt_s0;
+    uint16_t* aside = p.aside + unit * p.keep * 256 + d;  // [keep][K, V][128]
+    uint4 vk[4], vv[4];
+    int64_t to[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int j = min(j0 + 16 * u, p.keep - 1), t = kept[j];
+        const int sb = bt[(t >> p.block_shift) * p.bt_s1], db = bt[(j >> p.block_shift) * p.bt_s1];
+        const bool saved = t < p.keep;
+        const bool moves = j0 + 16 * u < p.keep && t != j && sb >= 0 && sb < p.num_blocks && db >= 0 &&
+                           db < p.num_blocks && (BACK || saved);
+        const int64_t from = sb * p.c_s0 + (t & mask) * p.c_s1 + h * p.c_s2 + d;
+        const uint16_t* k = BACK && saved ? aside + (int64_t)j * 256 : p.kc + from;
+        const uint16_t* v = BACK && saved ? aside + (int64_t)j * 256 + 128 : p.vc + from;
+        to[u] = moves ? BACK ? db * p.c_s0 + (j & mask) * p.c_s1 + h * p.c_s2 + d : (int64_t)j * 256 : -1;
+        vk[u] = vv[u] = make_uint4(0, 0, 0, 0);
+        if (moves) {
+            vk[u] = *(const uint4*)k;
+            vv[u] = *(const uint4*)v;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        if (to[u] >= 0) {
+            *(uint4*)((BACK ? p.kc : aside) + to[u]) = vk[u];
+            *(uint4*)((BACK ? p.vc : aside + 128) + to[u]) = vv[u];
+        }
+}
+
 }  // namespace
 
 }  // namespace starkv
@@ -277,9 +321,20 @@ int starkv_weighted_decode(void* stream, const void* query, int64_t q_s0, int64_
     return STARKV_OK;
 }
 
+// Up to 16 heads in a call their rows move through the workspace, all at once (up to twice the bytes). In order / at
+// once, us a call, choice included: 1 head 65536 -> 57000 tokens 360 / 72, 8 heads 32768 -> 28000 292 / 116, 8192 -> 7000
+// 57 / 32, 2176 -> 2048 21 / 20, 16 heads 8192 -> 7000 59 / 48, 2176 -> 2048 24 / 25, 32 heads 16384 -> 14000 181 / 191,
+// 2176 -> 2048 25 / 31.
+static bool evict_staged(int n, int num_kv_heads) { return (int64_t)n * num_kv_heads <= 16; }
+
+static size_t evict_kept_bytes(int n, int num_kv_heads, int weights_len, int keep) {
+    return ((size_t)n * num_kv_heads * std::min(keep, weights_len) * 4 + 255) / 256 * 256;
+}
+
 size_t starkv_evict_workspace_bytes(int n, int num_kv_heads, int weights_len, int keep) {
     if (n < 1 || num_kv_heads < 1 || weights_len < 1 || keep < 1) return 256;
-    return std::max<size_t>(256, (size_t)n * num_kv_heads * std::min(keep, weights_len) * 4);
+    const size_t rows = keep < weights_len && evict_staged(n, num_kv_heads) ? (size_t)n * num_kv_heads * keep : 0;
+    return evict_kept_bytes(n, num_kv_heads, weights_len, keep) + rows * 512;
 }
 
 int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype,
@@ -302,7 +357,8 @@ int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64
     SKV_CHECK(((uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0 && (c_s0 | c_s1 | c_s2) % 8 == 0,
               "evict: cache rows must be 16-byte aligned");
     const size_t need = starkv_evict_workspace_bytes(n, num_kv_heads, weights_len, keep);
-    SKV_CHECK(workspace_bytes >= need, "evict: workspace %zu bytes < %zu", workspace_bytes, need);
+    SKV_CHECK(workspace_bytes >= need && (uintptr_t)workspace % 16 == 0, "evict: workspace %zu bytes < %zu, or unaligned",
+              workspace_bytes, need);
     EvictParams p = {};
     p.kc = (uint16_t*)k_cache; p.vc = (uint16_t*)v_cache; p.c_s0 = c_s0; p.c_s1 = c_s1; p.c_s2 = c_s2;
     p.block_shift = block_shift(block_size) + 4; p.num_blocks = num_blocks;
@@ -313,11 +369,19 @@ int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64
     p.new_lens = new_lens; p.new_w = new_weights; p.kept = (int32_t*)workspace;
     const int run = topk_run(p.span);
     const void* fn = run == TK_FEW ? (const void*)&evict_select_kernel<TK_FEW>
-                     : run         ? (const void*)&evict_select_kernel<TK_MANY>
+                     : run == TK_MANY ? (const void*)&evict_select_kernel<TK_MANY>
+                     : run         ? (const void*)&evict_select_kernel<TK_MOST>
                                    : (const void*)&evict_select_kernel<0>;
     void* args[] = {(void*)&p};
     SKV_HIP(hipLaunchKernel(fn, dim3(num_kv_heads, n), dim3(TK_THR), args, 0, (hipStream_t)stream));
-    if (p.span > keep) {
+    if (p.span > keep && evict_staged(n, num_kv_heads)) {
+        p.aside = (uint16_t*)((char*)workspace + evict_kept_bytes(n, num_kv_heads, weights_len, keep));
+        const dim3 grid((keep + ST_ROWS - 1) / ST_ROWS, num_kv_heads, n);
+        hipLaunchKernelGGL(stage_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, p);
+        SKV_HIP(hipGetLastError());
+        hipLaunchKernelGGL(stage_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, p);
+        SKV_HIP(hipGetLastError());
+    } else if (p.span > keep) {
         // Whole rows a workgroup where those fill 256 CUs, else their halves: 8192 -> 2048 tokens of 16 requests of
         // 8 KV heads 81 us whole, 85 in halves; 4096 -> 2048 of 64 requests 255, 265, of 8 53, 42; one of
         // 32 heads 2176 -> 2048 34, 25 (in quarters 29).

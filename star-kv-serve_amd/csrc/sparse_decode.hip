@@ -302,7 +302,8 @@ int starkv_select_blocks(void* stream, const void* query, int64_t q_s0, int64_t 
     }
     const int run = topk_run(p.cap);
     const void* fn = run == TK_FEW ? (const void*)&select_kernel<TK_FEW>
-                     : run         ? (const void*)&select_kernel<TK_MANY>
+                     : run == TK_MANY ? (const void*)&select_kernel<TK_MANY>
+                     : run         ? (const void*)&select_kernel<TK_MOST>
                                    : (const void*)&select_kernel<0>;
     void* args[] = {(void*)&p};
     SKV_HIP(hipLaunchKernel(fn, dim3(num_kv_heads, n), dim3(TK_THR), args, 0, (hipStream_t)stream));

@@ -7,7 +7,7 @@
 // are counted in LDS; the bucket that holds the k-th largest becomes the range, until it is taken
 // whole, holds 64 values or fewer, which one wave ranks, or one value. One round does for most rows.
 // A wave takes a run of consecutive values, 64 at a time, so that loads are whole lines and a value's
-// place among the chosen is a count of bits; its lanes keep their values in registers (rows past 16384
+// place among the chosen is a count of bits; its lanes keep their values in registers (rows past 32768
 // values are read again in every pass). The one CU's instructions, barriers and first reads are a row's
 // time: 4096 scores 5.3 us from launch to end, where a kernel of three dependent reads and nothing else
 // takes 4 (9.0 with a thread's run of consecutive values read from LDS in every pass; 8192 weights 11.2,
@@ -59,11 +59,13 @@ __device__ __forceinline__ int lanes_below(unsigned long long mask) {
 constexpr int TK_BITS = 11, TK_BINS = 1 << TK_BITS;
 
 constexpr int TK_THR = 1024, TK_WAVES = TK_THR / 64;
-// Values a thread keeps, by the longest row: straight code over 4 or 16 of them (a row of 2000 values steps over
-// what it does not have of 16 in every pass), longer rows none.
-constexpr int TK_FEW = 4, TK_MANY = 16;
+// Values a thread keeps, by the longest row: straight code over 4, 16 or 32 of them (a row of 2000 values steps
+// over what it does not have of 16 in every pass), longer rows none.
+constexpr int TK_FEW = 4, TK_MANY = 16, TK_MOST = 32;
 
-inline int topk_run(int longest) { return longest <= TK_THR * TK_FEW ? TK_FEW : longest <= TK_THR * TK_MANY ? TK_MANY : 0; }
+inline int topk_run(int longest) {
+    return longest <= TK_THR * TK_FEW ? TK_FEW : longest <= TK_THR * TK_MANY ? TK_MANY : longest <= TK_THR * TK_MOST ? TK_MOST : 0;
+}
 
 struct TopkShared {
     uint32_t hist[TK_BINS];
@@ -114,9 +116,16 @@ __device__ __forceinline__ void topk_ascending(TopkShared& sh, int count, int k,
                     for (int u = u0; u < u0 + 4; ++u) f(keys[u], i0 + 64 * u, kept[u]);
                 }
         } else {
-            for (int u = 0; u < run; ++u) {
-                const float v = value(min(i0 + 64 * u, count - 1));
-                f(i0 + 64 * u < count ? order_key(v) : 0, i0 + 64 * u, v);
+            constexpr int AT_ONCE = 16;  // reads on their way
+            for (int u0 = 0; u0 < run; u0 += AT_ONCE) {
+                float v[AT_ONCE];
+#pragma unroll
+                for (int x = 0; x < AT_ONCE; ++x) v[x] = value(min(i0 + 64 * (u0 + x), count - 1));
+#pragma unroll
+                for (int x = 0; x < AT_ONCE; ++x) {
+                    const int i = i0 + 64 * (u0 + x);
+                    f(u0 + x < run && i < count ? order_key(v[x]) : 0, i, v[x]);
+                }
             }
         }
     };

@@ -235,7 +235,7 @@ def test_select_blocks(cuda, dt, small, Hkv, G, bs, lens, keep, sink, recent):
         assert torch.equal(got.cpu(), select_plain(q, bounds, bt, lens, span, bs, keep, sink, recent))
 
 
-@pytest.mark.parametrize("blocks", [12800, 16384, 16387, 33000])
+@pytest.mark.parametrize("blocks", [12800, 16384, 16387, 32768, 33000])
 def test_select_blocks_long(cuda, blocks):
     """Rows of as many values as the choice keeps in registers, and of more; a table of more columns than needed."""
     lens = [16 * blocks - 11, 16 * 12288, 16 * 9000 - 3]
@@ -466,7 +466,8 @@ def same(a, b):
     (3, 32, [1000, 31], 1, 0, 1, "heads", False), (8, 64, [900, 64, 129], 128, 0, 128, "plain", True),
     (1, 16, [2500, 2049], 2048, 0, 0, "plain", False), (2, 16, [1500], 1499, 4, 32, "plain", True),
     (4, 16, [700], 20, 10, 10, "heads", False), (1, 16, [90, 40], 1 << 30, 0, 0, "plain", False),
-    (33, 16, [300, 170, 290, 100], 128, 2, 9, "plain", True), (1, 512, [1200], 700, 1, 1, "plain", False)])
+    (33, 16, [300, 170, 290, 100], 128, 2, 9, "plain", True), (1, 512, [1200], 700, 1, 1, "plain", False),
+    (8, 16, [1300, 900, 1250, 40], 600, 3, 20, "pairs", True), (17, 16, [1200], 1100, 3, 20, "heads", False)])
 def test_evict(cuda, dt, Hkv, bs, lens, keep, sink, recent, layout, ties):
     kc, vc, bt, sl = make_caches(cuda, lens, Hkv, bs, dt, 111, layout)
     g = torch.Generator().manual_seed(112)
@@ -480,7 +481,7 @@ def test_evict(cuda, dt, Hkv, bs, lens, keep, sink, recent, layout, ties):
     assert same(kc, want[0]) and same(vc, want[1])
 
 
-@pytest.mark.parametrize("lens,keep", [([13000, 12400], 12000), ([17000, 16385], 16000)])
+@pytest.mark.parametrize("lens,keep", [([13000, 12400], 12000), ([17000, 16385], 16000), ([33000, 32769], 30000)])
 def test_evict_long_and_extreme_weights(cuda, lens, keep):
     """Rows that the choice keeps in registers and longer ones; weights of NaN, infinity and zeros of both signs; int64
     tables."""
