@@ -14,7 +14,7 @@
 // earlier chunk's targets (a handful of heads moves all rows at once instead, through the workspace:
 // stage_kernel). Columns are independent of each other, so K and V, and for few requests their
 // halves of 128 bytes, go to workgroups of their own. 16 requests of 8 KV heads cut from 4097 to 8192 tokens
-// to 2048: the choice 11 us (one CU a head), the move 60 (268 MB, 4.4 TB/s; a large copy's rate is 5.0).
+// to 2048: the choice 11 us (one CU a head), the move 57 (268 MB, 4.7 TB/s; a large copy's rate is 5.0).
 #include <algorithm>
 
 #include "common.hpp"
@@ -157,7 +157,9 @@ struct Round {
 };
 
 // 2^lanes lanes a row's slice of 16 << lanes bytes, CP_U slices a lane and chunk. Two chunks are on their way
-// at a time: a chunk is written behind a barrier that waits for its own rows only.
+// at a time: a chunk is written behind a barrier that waits for its own rows only. A chunk's tokens and their
+// blocks are read two and one chunk ahead and before the rows that are on their way: reads arrive in their
+// order, and one that is waited for behind rows waits for the rows.
 __global__ __launch_bounds__(CP_THR) void compact_kernel(const EvictParams p, int lanes) {
     const int h = blockIdx.y, b = blockIdx.z;
     if (evict_length(p, b) <= p.keep) return;
@@ -166,28 +168,34 @@ __global__ __launch_bounds__(CP_THR) void compact_kernel(const EvictParams p, in
     const int mask = (1 << p.block_shift) - 1, chunk = CP_U * step;
     const int32_t* kept = p.kept + ((int64_t)b * p.Hkv + h) * p.keep;
     const int32_t* bt = p.bt + b * p.bt_s0;
-    int64_t from[CP_U], to[CP_U];  // element offsets of the chunk after those on their way, from < 0: stays
-    const auto places = [&](int j0) {
-        int t[CP_U], sb[CP_U], db[CP_U];
+    int t1[CP_U], t2[CP_U], sb[CP_U], db[CP_U];  // tokens of the next chunk and the one after, blocks of the next
+    const auto tokens = [&](int j0, int (&t)[CP_U]) {
 #pragma unroll
         for (int u = 0; u < CP_U; ++u) t[u] = kept[min(j0 + u * step + row, p.keep - 1)];
+    };
+    const auto blocks = [&](int j0, const int (&t)[CP_U]) {
 #pragma unroll
         for (int u = 0; u < CP_U; ++u) {
             sb[u] = bt[(t[u] >> p.block_shift) * p.bt_s1];
             db[u] = bt[(min(j0 + u * step + row, p.keep - 1) >> p.block_shift) * p.bt_s1];
         }
+    };
+    // The chunk at j0 sets out; behind it wait the tokens of the third and the blocks of the second after it.
+    const auto read = [&](int j0, Round& r) {
+        int64_t from[CP_U];
 #pragma unroll
         for (int u = 0; u < CP_U; ++u) {
             const int j = j0 + u * step + row;
-            const bool moves = j < p.keep && t[u] != j && sb[u] >= 0 && sb[u] < p.num_blocks && db[u] >= 0 && db[u] < p.num_blocks;
-            from[u] = moves ? sb[u] * p.c_s0 + (t[u] & mask) * p.c_s1 : -1;
-            to[u] = moves ? db[u] * p.c_s0 + (j & mask) * p.c_s1 : -1;
+            const bool moves = j < p.keep && t1[u] != j && sb[u] >= 0 && sb[u] < p.num_blocks && db[u] >= 0 && db[u] < p.num_blocks;
+            from[u] = moves ? sb[u] * p.c_s0 + (t1[u] & mask) * p.c_s1 : -1;
+            r.to[u] = moves ? db[u] * p.c_s0 + (j & mask) * p.c_s1 : -1;
+            t1[u] = t2[u];
         }
-    };
-    const auto read = [&](Round& r) {
+        tokens(j0 + 2 * chunk, t2);
+        blocks(j0 + chunk, t1);
+        asm volatile("" ::: "memory");
 #pragma unroll
         for (int u = 0; u < CP_U; ++u) {
-            r.to[u] = to[u];
             r.v[u] = make_uint4(0, 0, 0, 0);
             if (from[u] >= 0) r.v[u] = *(const uint4*)(c + from[u]);
         }
@@ -201,15 +209,14 @@ __global__ __launch_bounds__(CP_THR) void compact_kernel(const EvictParams p, in
             if (r.to[u] >= 0) *(uint4*)(c + r.to[u]) = r.v[u];
     };
     Round x, y;
-    places(0);
-    read(x);
-    places(chunk);
+    tokens(0, t1);
+    tokens(chunk, t2);
+    blocks(0, t1);
+    read(0, x);
     for (int j0 = 0; j0 < p.keep; j0 += 2 * chunk) {
-        read(y);
-        places(j0 + 2 * chunk);
+        read(j0 + chunk, y);
         write(x);
-        read(x);
-        places(j0 + 3 * chunk);
+        read(j0 + 2 * chunk, x);
         write(y);
     }
 }
@@ -321,11 +328,10 @@ int starkv_weighted_decode(void* stream, const void* query, int64_t q_s0, int64_
     return STARKV_OK;
 }
 
-// Up to 16 heads in a call their rows move through the workspace, all at once (up to twice the bytes). In order / at
-// once, us a call, choice included: 1 head 65536 -> 57000 tokens 360 / 72, 8 heads 32768 -> 28000 292 / 116, 8192 -> 7000
-// 57 / 32, 2176 -> 2048 21 / 20, 16 heads 8192 -> 7000 59 / 48, 2176 -> 2048 24 / 25, 32 heads 16384 -> 14000 181 / 191,
-// 2176 -> 2048 25 / 31.
-static bool evict_staged(int n, int num_kv_heads) { return (int64_t)n * num_kv_heads <= 16; }
+// Up to 8 heads in a call their rows move through the workspace, all at once (up to twice the bytes). In order / at
+// once, us a call, choice included: 1 head 65536 -> 57000 tokens 360 / 72, 8 heads 32768 -> 28000 292 / 105, 8192 -> 7000
+// 46 / 32, 2176 -> 2048 20 / 20, 16 heads 8192 -> 7000 46 / 46, 2176 -> 2048 22 / 25.
+static bool evict_staged(int n, int num_kv_heads) { return (int64_t)n * num_kv_heads <= 8; }
 
 static size_t evict_kept_bytes(int n, int num_kv_heads, int weights_len, int keep) {
     return ((size_t)n * num_kv_heads * std::min(keep, weights_len) * 4 + 255) / 256 * 256;
@@ -382,9 +388,9 @@ int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64
         hipLaunchKernelGGL(stage_kernel<true>, grid, dim3(256), 0, (hipStream_t)stream, p);
         SKV_HIP(hipGetLastError());
     } else if (p.span > keep) {
-        // Whole rows a workgroup where those fill 256 CUs, else their halves: 8192 -> 2048 tokens of 16 requests of
-        // 8 KV heads 81 us whole, 85 in halves; 4096 -> 2048 of 64 requests 255, 265, of 8 53, 42; one of
-        // 32 heads 2176 -> 2048 34, 25 (in quarters 29).
+        // Whole rows a workgroup where those fill 256 CUs, else their halves: 4097 to 8192 -> 2048 tokens of 16 requests
+        // of 8 KV heads 72 us whole, 77 in halves; 4096 -> 2048 of 64 requests 239, 251; 8192 -> 7000 of 8 requests
+        // 127, 117; one of 32 heads 2176 -> 2048 29, 22 (in quarters 27).
         const int lanes = (int64_t)n * num_kv_heads >= 128 ? 4 : 3;
         hipLaunchKernelGGL(compact_kernel, dim3(32 >> lanes, num_kv_heads, n), dim3(CP_THR), 0, (hipStream_t)stream, p,
                            lanes);
