@@ -330,8 +330,11 @@ int starkv_weighted_decode(void* stream, const void* query, int64_t q_s0, int64_
 
 // Up to 8 heads in a call their rows move through the workspace, all at once (up to twice the bytes). In order / at
 // once, us a call, choice included: 1 head 65536 -> 57000 tokens 360 / 72, 8 heads 32768 -> 28000 292 / 105, 8192 -> 7000
-// 46 / 32, 2176 -> 2048 20 / 20, 16 heads 8192 -> 7000 46 / 46, 2176 -> 2048 22 / 25.
-static bool evict_staged(int n, int num_kv_heads) { return (int64_t)n * num_kv_heads <= 8; }
+// 46 / 32, 2176 -> 2048 20 / 20, 16 heads 8192 -> 7000 46 / 46, 2176 -> 2048 22 / 25. Not past 1 GiB of workspace.
+static bool evict_staged(int n, int num_kv_heads, int keep) {
+    const int64_t units = (int64_t)n * num_kv_heads;
+    return units <= 8 && units * keep <= 1 << 21;
+}
 
 static size_t evict_kept_bytes(int n, int num_kv_heads, int weights_len, int keep) {
     return ((size_t)n * num_kv_heads * std::min(keep, weights_len) * 4 + 255) / 256 * 256;
@@ -339,7 +342,7 @@ static size_t evict_kept_bytes(int n, int num_kv_heads, int weights_len, int kee
 
 size_t starkv_evict_workspace_bytes(int n, int num_kv_heads, int weights_len, int keep) {
     if (n < 1 || num_kv_heads < 1 || weights_len < 1 || keep < 1) return 256;
-    const size_t rows = keep < weights_len && evict_staged(n, num_kv_heads) ? (size_t)n * num_kv_heads * keep : 0;
+    const size_t rows = keep < weights_len && evict_staged(n, num_kv_heads, keep) ? (size_t)n * num_kv_heads * keep : 0;
     return evict_kept_bytes(n, num_kv_heads, weights_len, keep) + rows * 512;
 }
 
@@ -380,7 +383,7 @@ int starkv_evict(void* stream, void* k_cache, void* v_cache, int64_t c_s0, int64
                                    : (const void*)&evict_select_kernel<0>;
     void* args[] = {(void*)&p};
     SKV_HIP(hipLaunchKernel(fn, dim3(num_kv_heads, n), dim3(TK_THR), args, 0, (hipStream_t)stream));
-    if (p.span > keep && evict_staged(n, num_kv_heads)) {
+    if (p.span > keep && evict_staged(n, num_kv_heads, keep)) {
         p.aside = (uint16_t*)((char*)workspace + evict_kept_bytes(n, num_kv_heads, weights_len, keep));
         const dim3 grid((keep + ST_ROWS - 1) / ST_ROWS, num_kv_heads, n);
         hipLaunchKernelGGL(stage_kernel<false>, grid, dim3(256), 0, (hipStream_t)stream, p);
