@@ -486,7 +486,8 @@ int starkv_norm_rope_qkv(void *stream, const void *q, int64_t q_s0, int64_t q_s1
  * fp16, element strides c_s0, c_s1, c_s2 shared by K and V, rows 16-byte aligned, block_size 16 * 2^s). Common
  * to them: block_table [n, bt_width] int32; seq_lens [n] int32, clamped to the table's row; num_heads a
  * multiple of num_kv_heads; query and out of the cache's dtype. A block id outside [0, num_blocks) stands for
- * no tokens. n is at most 65535, workspaces are 16-byte aligned.
+ * no tokens. n is at most 65535, workspaces are 16-byte aligned. In the decodes a token whose score is -inf (an
+ * infinite key) weighs 0; a row whose scores are all -inf is NaN, as are its weights.
  *
  * starkv_key_bounds: bounds [num_blocks, num_kv_heads, 2, 128] (element strides b_s0, b_s1, b_s2; the cache's
  * dtype) of every block that holds one of a request's last max_new tokens: the elementwise least and largest

@@ -81,8 +81,8 @@ __global__ __launch_bounds__(256) void weigh_kernel(const WeighParams wp) {
         for (int x = 0; x < AT_MAX_SPLITS / 16; ++x) all = fmaf(l[x], m[x] == -INFINITY ? 1.f : exp2f(m[x] - M), all);
         all = row16_sum(all);
         if ((tid & 15) == 0) {
-            s_ref[g16] = all == 0.f ? 0.f : M;  // no block of the cache: weights of 0
-            s_inv[g16] = all == 0.f ? 0.f : 1.f / all;
+            s_ref[g16] = M == -INFINITY ? 0.f : M;  // no block of the cache: weights of 0
+            s_inv[g16] = M == -INFINITY ? 0.f : 1.f / all;
         }
     }
     __syncthreads();

@@ -29,6 +29,10 @@
 // heads' again, and costs no instruction of the matrix unit; 9 to 16 heads take a product each. The
 // reference lies 2^7 below the largest score seen when it was set and moves when a score passes it by
 // 2^15 (fp16 weights stay finite, and small ones keep 22 bits of range above its subnormals).
+//
+// A wave that has seen tokens has a finite reference or +inf: scores of -inf (an infinite key) weigh 0 against it,
+// and where a row has no others its sums are 0 and the result 0 / 0. A reference of -inf says that there were no
+// tokens, whose result is 0.
 #pragma once
 
 #include <algorithm>
@@ -43,6 +47,7 @@ constexpr int AT_PART = 132;       // floats of a partial: reference, sum of wei
 constexpr int AT_MAX_SPLITS = 128;
 constexpr int AT_MAX_GROUP = 16;   // query heads per KV head: the columns of a matrix product
 constexpr float AT_LOG2E = 1.4426950408889634f;
+constexpr float AT_LEAST = -3.402823466e38f;  // the reference of tokens whose scores are all -inf
 
 struct AttendParams {
     const uint16_t* q; int64_t q_s0, q_s1;                               // elements, as all strides here
@@ -197,9 +202,10 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
 #pragma unroll
             for (int r = 1; r < 8; ++r) mx = fmaxf(mx, sv[r >> 2][r & 3]);
             mx = max_rows(mx);
+            if (nt[0] + nt[1] > 0) m = fmaxf(m, AT_LEAST);
             if (__builtin_amdgcn_ballot_w64(mx > m + 15.f) != 0) {
                 const float mn = mx > m + 15.f ? mx - 7.f : m;
-                const float alpha = mn == -INFINITY ? 1.f : exp2f(m - mn);
+                const float alpha = mn == m ? 1.f : exp2f(m - mn);
                 m = mn;
                 l *= alpha;
 #pragma unroll
@@ -263,13 +269,13 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const float* r = w + k * p.G * AT_PART;
-            // A wave without tokens has reference -inf and sums 0; NaN scores leave sums of NaN.
+            // A wave without tokens has reference -inf and sums 0; NaN scores leave sums of NaN, scores of -inf alone 0.
             const float f = r[0] == -INFINITY ? 1.f : exp2f(r[0] - M);
             lt = fmaf(r[1], f, lt);
             a = fmaf(r[4 + d], f, a);
         }
         const int hq = h * p.G + g;
-        if (p.splits == 1) store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, DT, lt == 0.f ? 0.f : a / lt);
+        if (p.splits == 1) store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, DT, M == -INFINITY ? 0.f : a / lt);
         if (p.splits > 1 || !SPARSE) {
             float* pp = p.part + (((int64_t)b * H + hq) * p.splits + s) * AT_PART;
             if (d == 0) *(float4*)pp = make_float4(M, lt, 0.f, 0.f);
@@ -315,8 +321,8 @@ __device__ __forceinline__ void attend_merge_head(const AttendParams& p, int b, 
         }
     }
     const int64_t o = b * p.o_s0 + hq * p.o_s1 + 2 * lane;
-    store_f(p.out, o, DT, lt == 0.f ? 0.f : a.x / lt);
-    store_f(p.out, o + 1, DT, lt == 0.f ? 0.f : a.y / lt);
+    store_f(p.out, o, DT, M == -INFINITY ? 0.f : a.x / lt);
+    store_f(p.out, o + 1, DT, M == -INFINITY ? 0.f : a.y / lt);
 }
 
 // Splits per unit (request and KV head) of at most `pages` pages: workgroups for `per_cu` a CU, `least` pages a
