@@ -81,3 +81,42 @@ def test_rows_whose_scores_are_all_minus_infinity(cuda, dt):
                 assert torch.isfinite(w[b, 0]).all() and (w[b, 1, L:] == 0).all()
                 assert w[b, 1, :L].isnan().all() if b < 3 else torch.isfinite(w[b, 1]).all()
         assert (out[3] == 0).all()
+
+
+# (length, {token: its score's distance above the others', or None for one among them}); the infinite values' tokens
+INFINITE = [(1, {0: None}), (2, {1: None}), (37, {19: None}), (300, {0: None, 299: None}), (5000, {4999: None}),
+            (700, {123: 30.0}), (700, {5: -30.0}), (64, {t: None for t in range(64)}), (5000, {40: -12.0, 3000: 12.0})]
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("G", GROUPS)
+def test_infinite_values(cuda, dt, G):
+    """Dimension 0 holds +inf at the named tokens, 1 -inf, 2 NaN, 3 both infinities by turns (of a single token +inf), 127
+    +inf at one that scores -inf besides. Scores below the largest by 30 leave weights that fp16 does not hold."""
+    lens = [L for L, _ in INFINITE]
+    kc, vc, bt, sl = make_caches(cuda, lens, 1, 16, dt, 321)
+    q = queries(len(lens), G, dt, 322, cuda)
+    for b, (L, at) in enumerate(INFINITE):
+        for i, (t, above) in enumerate(at.items()):
+            if above is not None:
+                token(kc, bt, b, t, 0)[0] += above / SCALE
+            row = token(vc, bt, b, t, 0)
+            row[0], row[1], row[2], row[3] = math.inf, -math.inf, math.nan, -math.inf if i % 2 else math.inf
+    last = len(lens) - 1
+    token(kc, bt, last, 1, 0)[0] = -math.inf
+    token(vc, bt, last, 1, 0)[127] = math.inf
+    for name, out, w in decodes(q, kc, vc, bt, sl, max(lens)):
+        for b, (L, at) in enumerate(INFINITE):
+            both = len(at) > 1
+            for d, want in ((0, math.inf), (1, -math.inf), (2, math.nan), (3, math.nan if both else math.inf)):
+                got = out[b, :, d]
+                assert got.isnan().all() if math.isnan(want) else (got == want).all(), (name, b, d)
+            k, v = rows_of(kc, bt, b, 0, range(L)), rows_of(vc, bt, b, 0, range(L))
+            if b == last:
+                assert out[b, :, 127].isnan().all()  # 0 inf
+                there = [t for t in range(L) if t != 1]
+                k, v = k[there], v[there]
+            want, tol, p, _ = attention64(q[b].cpu(), k, v[:, 4:127], dt)
+            check(out[b, :, 4:127], want, tol, (name, b))
+            if w is not None:
+                assert torch.isfinite(w).all() and abs(w[b, 0].sum().item() - G) < 1e-3 * G
