@@ -23,19 +23,20 @@
 // to 8191 tokens over 8 KV heads with their scores left behind (445 MB) 97. The next tile's loads ahead of a
 // tile's products gained nothing (189 -> 193, at half the waves), nor did loads past the caches.
 //
-// Rounding: scores, references and sums are fp32. The weights enter the second product as two values
-// of the cache's type, the weight in it and what that left (16 bits of a bf16 weight, cut, and 22 of an
-// fp16 one, rounded): up to 8 query heads the second value takes the other 8 columns, whose scores are the same
-// heads' again, and costs no instruction of the matrix unit; 9 to 16 heads take a product each. The
-// reference lies 2^7 below the largest score seen when it was set and moves when a score passes it by
-// 2^15 (fp16 weights stay finite, and small ones keep 22 bits of range above its subnormals).
+// Rounding: scores, references and sums are fp32. The weights enter the second product as three values
+// of the cache's type, the weight in it, what that left and what that left: all 24 bits of a bf16 weight
+// (each value cut) and of an fp16 one (rounded) down to 2^-24, where fp16 ends. Up to 8 query heads the second and
+// third values take the other 8 columns, whose scores are the same heads' again, so that two products do; 9 to 16
+// heads take a product each. Two values, 16 bits of a bf16 weight, made results low by up to 2^-15 and were
+// 1 % faster at most. The reference lies 2^7 below the largest score seen when it was set and moves when a score
+// passes it by 2^15 (fp16 weights stay finite, and small ones keep 22 bits of range above its subnormals).
 //
 // A wave that has seen tokens has a finite reference or +inf: scores of -inf (an infinite key) weigh 0 against it,
 // and where a row has no others its sums are 0 and the result 0 / 0. A reference of -inf says that there were no
 // tokens, whose result is 0.
 //
-// An infinite value times a weight's second value would be NaN or an infinity of the other sign where that is 0 or
-// negative. A workgroup whose sums are not finite though its weights are goes over its pages once more, the finite
+// An infinite value times a weight's second or third value would be NaN or an infinity of the other sign where that
+// is 0 or negative. A workgroup whose sums are not finite though its weights are goes over its pages once more, the finite
 // values as before and the others times 1 where their token's weight is not 0: what the weight's bits are no
 // longer matters. Finite values pay for the look at the sums alone (32 requests 190 us with and without it, one
 // request of 4096 tokens 17.4 -> 17.8).
@@ -99,14 +100,14 @@ __device__ __forceinline__ uint32_t attend_pack(float a, float b, float& ra, flo
     }
 }
 
-// What a .. d leave of their packed forms, packed: the second value of a weight.
+// Four weights packed, and `own` of that taken off them: all of it or nothing.
 template <int DT>
-__device__ __forceinline__ uint2 attend_rest(const float (&p)[4], float of) {
-    float r[4], x[4];
-    attend_pack<DT>(p[0], p[1], r[0], r[1]);
-    attend_pack<DT>(p[2], p[3], r[2], r[3]);
-    return make_uint2(attend_pack<DT>(fmaf(-of, r[0], p[0]), fmaf(-of, r[1], p[1]), x[0], x[1]),
-                      attend_pack<DT>(fmaf(-of, r[2], p[2]), fmaf(-of, r[3], p[3]), x[2], x[3]));
+__device__ __forceinline__ uint2 attend_take(float (&p)[4], float own) {
+    float r[4];
+    const uint2 v = make_uint2(attend_pack<DT>(p[0], p[1], r[0], r[1]), attend_pack<DT>(p[2], p[3], r[2], r[3]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = fmaf(-own, r[i], p[i]);
+    return v;
 }
 
 // The halves of a word that hold infinities or NaN.
@@ -268,19 +269,25 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
                                        v.w & ~attend_odd<DT>(v.w));
                     }
                 }
-                const float rest = !MANY && lane & 8 ? 1.f : 0.f;  // the lane's column takes the weights' second values
-                const uint2 p0 = attend_rest<DT>(pe[0], rest), p1 = attend_rest<DT>(pe[1], rest);
-                const uint4 pf = make_uint4(p0.x, p0.y, p1.x, p1.y);
-                uint4 pl = make_uint4(0, 0, 0, 0);
-                if constexpr (MANY) {
-                    const uint2 q0 = attend_rest<DT>(pe[0], 1.f), q1 = attend_rest<DT>(pe[1], 1.f);
-                    pl = make_uint4(q0.x, q0.y, q1.x, q1.y);
+                // The weights' values, largest first, one a product; up to 8 heads the lanes of the second columns take
+                // the second in the first product, the third in the second, the others' second operand being 0.
+                uint4 pw[MANY ? 3 : 2];
+                if constexpr (!MANY) {
+                    const float second = lane & 8 ? 1.f : 0.f;
+                    attend_take<DT>(pe[0], second);
+                    attend_take<DT>(pe[1], second);
                 }
+#pragma unroll
+                for (int k = 0; k < (MANY ? 3 : 2); ++k) {
+                    const uint2 lo = attend_take<DT>(pe[0], 1.f), hi = attend_take<DT>(pe[1], 1.f);
+                    pw[k] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+                }
+                if (!MANY && !(lane & 8)) pw[1] = make_uint4(0, 0, 0, 0);
 #pragma unroll
                 for (int i8 = 0; i8 < 8; ++i8) {
                     const uint4 vt = attend_column(vr, i8);
-                    acc[i8] = attend_mfma<DT>(vt, pf, acc[i8]);
-                    if constexpr (MANY) acc[i8] = attend_mfma<DT>(vt, pl, acc[i8]);
+#pragma unroll
+                    for (int k = 0; k < (MANY ? 3 : 2); ++k) acc[i8] = attend_mfma<DT>(vt, pw[k], acc[i8]);
                 }
             }
         }
