@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void weigh_kernel(const WeighParams wp) {
         all = row16_sum(all);
         if ((tid & 15) == 0) {
             s_ref[g16] = M == -INFINITY ? 0.f : M;  // no block of the cache: weights of 0
-            s_inv[g16] = M == -INFINITY ? 0.f : 1.f / all;
+            s_inv[g16] = M == -INFINITY ? 0.f : AT_DOWN<DT> / all;
         }
     }
     __syncthreads();

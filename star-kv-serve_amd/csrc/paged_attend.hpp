@@ -54,6 +54,10 @@ constexpr int AT_PART = 132;       // floats of a partial: reference, sum of wei
 constexpr int AT_MAX_SPLITS = 128;
 constexpr int AT_MAX_GROUP = 16;   // query heads per KV head: the columns of a matrix product
 constexpr float AT_LOG2E = 1.4426950408889634f;
+// What weights are multiplied by. bf16 values reach fp32's largest: times weights of 2^15 and summed, those past 2^100 or
+// so left it. fp16 values are far from it, and fp16 weights have no such range.
+template <int DT>
+constexpr float AT_DOWN = DT == STARKV_BF16 ? 0x1p-40f : 1.f;
 constexpr float AT_LEAST = -3.402823466e38f;  // the reference of tokens whose scores are all -inf
 
 struct AttendParams {
@@ -249,7 +253,7 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        pe[x][r] = 4 * quad + r < nt[x] ? exp2f(sv[x][r] - m) : 0.f;
+                        pe[x][r] = 4 * quad + r < nt[x] ? exp2f(sv[x][r] - m) * AT_DOWN<DT> : 0.f;
                         l += pe[x][r];
                     }
                 if (__builtin_expect(careful, 0)) {

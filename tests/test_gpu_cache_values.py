@@ -120,3 +120,22 @@ def test_infinite_values(cuda, dt, G):
             check(out[b, :, 4:127], want, tol, (name, b))
             if w is not None:
                 assert torch.isfinite(w).all() and abs(w[b, 0].sum().item() - G) < 1e-3 * G
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("G", [1, 8, 13])
+@pytest.mark.parametrize("part", [1.0, 2.0 ** -9, 2.0 ** -14])
+def test_largest_values(cuda, dt, G, part):
+    """A mean of the type's largest values is no larger, whatever the sums on the way to it are."""
+    lens = [1, 40, 3000, 20000]
+    kc, vc, bt, sl = make_caches(cuda, lens, 1, 16, dt, 331)
+    vc.copy_(torch.where(vc.isnan(), vc, vc.sign() * (torch.finfo(dt).max * part)))
+    vc[:, :, :, :64] = vc[:, :, :, :64].abs()
+    q = queries(len(lens), G, dt, 332, cuda)
+    for name, out, w in decodes(q, kc, vc, bt, sl, max(lens)):
+        for b, L in enumerate(lens):
+            want, tol, _, _ = attention64(q[b].cpu(), rows_of(kc, bt, b, 0, range(L)), rows_of(vc, bt, b, 0, range(L)), dt)
+            top = torch.finfo(dt).max * part
+            got = out[b].double().cpu()
+            assert ((got - want).abs() <= tol).all(), (name, b)
+            assert (got[:, :64] >= top * 0.98).all() and (got.abs() <= top).all(), (name, b)
