@@ -10,6 +10,7 @@ import torch
 
 from starkv_serve.kernels.evict import paged_decode_weighted
 from starkv_serve.kernels.sparse_decode import paged_decode_sparse
+from starkv_serve.kernels.stock_decode import paged_decode_full
 from test_gpu_cache_ops import BF16, D, E, F16, SCALE, attention64, check, make_caches, rows_of
 
 pytestmark = pytest.mark.gpu
@@ -139,3 +140,23 @@ def test_largest_values(cuda, dt, G, part):
             got = out[b].double().cpu()
             assert ((got - want).abs() <= tol).all(), (name, b)
             assert (got[:, :64] >= top * 0.98).all() and (got.abs() <= top).all(), (name, b)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("G", [1, 2, 4, 8])
+def test_whole_decode_with_scores_of_minus_infinity(cuda, dt, G):
+    """``paged_decode_full``: one length a call, so that every split of it is a case."""
+    for L, lost in LOST:
+        kc, vc, bt, sl = make_caches(cuda, [L, L], 2, 16, dt, 341)
+        for t in lost:
+            token(kc, bt, 0, t, 1)[0] = -math.inf
+        for t in range(L):
+            token(kc, bt, 1, t, 0)[0] = -math.inf
+        q = queries(2, 2 * G, dt, 342, cuda)
+        out = paged_decode_full(q, kc, vc, bt, sl, L, SCALE)
+        there = sorted(set(range(L)) - set(lost))
+        for b, h, tokens in ((0, 0, range(L)), (0, 1, there), (1, 1, range(L))):
+            mine = out[b, h * G:(h + 1) * G]
+            want, tol, _, _ = attention64(q[b, h * G:(h + 1) * G].cpu(), rows_of(kc, bt, b, h, tokens), rows_of(vc, bt, b, h, tokens), dt)
+            check(mine, want, tol, (L, b, h))
+        assert out[1, :G].isnan().all()
