@@ -66,6 +66,8 @@ class StarKVMetadata:
     slot_mapping: torch.Tensor   # [>= num_actual_tokens] int64 (-1: padding token)
     prefill_seq_lens_cpu: Optional[List[int]] = None
     prefill_query_start_loc_cpu: Optional[List[int]] = None
+    positions_apart: bool = False        # the tokens' positions are not seq_lens - 1: caches were cut
+    max_position: Optional[int] = None   # an upper bound of the positions, where the caller has one
 
     def decode_lens(self, nd: int) -> torch.Tensor:
         """seq_lens[:nd] with padding rows (length 0) given one (null-block) position to

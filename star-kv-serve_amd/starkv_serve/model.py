@@ -36,7 +36,8 @@ Three options of the uncompressed layers that the reference does not have:
   (``kernels/sparse_decode.py``); every step keeps the bounds of the blocks it writes.
 - ``weigh``: steps sum up what each cached token weighs (``kernels/evict.py``); ``evict`` cuts the caches of all layers
   to the tokens that weigh most. After a cut a request's next position is no longer its cache length:
-  ``decode_metadata`` and ``DecodeGraph`` take the lengths apart.
+  ``decode_metadata`` and ``DecodeGraph`` take the lengths apart. Positions then go on past ``max_model_len`` while the
+  cache does not; ``max_positions`` says how far, and a step past it raises.
 """
 import math
 from dataclasses import dataclass
@@ -116,9 +117,11 @@ class StarKVLlamaForCausalLM:
 
     def __init__(self, shape: LlamaShape, starkv: Optional[StarKVCheckpoint], max_model_len: int, device,
                  dtype: torch.dtype = torch.bfloat16, seed: int = 0, stock: bool = False,
-                 sparse: Optional[BlockSelection] = None, weigh: bool = False):
+                 sparse: Optional[BlockSelection] = None, weigh: bool = False, max_positions: Optional[int] = None):
         """`starkv` = None or `stock` = True: every layer uncompressed (the stock model). `sparse`: decode steps of
-        the uncompressed layers read selected blocks. `weigh`: steps sum up their tokens' weights, for ``evict``."""
+        the uncompressed layers read selected blocks. `weigh`: steps sum up their tokens' weights, for ``evict``.
+        `max_positions`: the last position of a session whose cuts keep its cache within max_model_len tokens
+        (max_model_len, and never less)."""
         compressed = starkv is not None and not stock and any(map(starkv.is_compressed, range(shape.num_layers)))
         if sparse is not None and weigh:
             raise ValueError("sparse or weigh: a decode over selected blocks does not weigh the others' tokens")
@@ -131,7 +134,7 @@ class StarKVLlamaForCausalLM:
         self.max_model_len = max_model_len
         H, Hkv, D, hid = shape.num_heads, shape.num_kv_heads, shape.head_dim, shape.hidden_size
         self.scale = D ** -0.5
-        self.rotary = Rotary(max_model_len + 1, dtype, self.device, shape.rope_theta)
+        self.rotary = Rotary(max(max_model_len, max_positions or 0) + 1, dtype, self.device, shape.rope_theta)
         g = torch.Generator(device=self.device).manual_seed(seed)
 
         def w(*size, fan_in):
@@ -239,8 +242,7 @@ class StarKVLlamaForCausalLM:
             kc, vc = self.kv_caches[li]
             ka, va = k, v  # the prefill attention's operands
             slots = md.slot_mapping[:T]
-            own = getattr(self.rotary.apply, "__func__", None) is Rotary.apply  # not a rotation of the caller's
-            if own and model_ops.rope_write_fits(self.rotary.cos_sin_cache, positions, q, k, v, kc, vc, slots):
+            if self._own_rotation() and model_ops.rope_write_fits(self.rotary.cos_sin_cache, positions, q, k, v, kc, vc, slots):
                 if layer.q_norm is None:
                     q, k, ka, va = model_ops.rope_write(positions, q, k, v, self.rotary.cos_sin_cache, kc, vc, slots,
                                                         capture is not None, bool(md.num_prefills))
@@ -266,6 +268,24 @@ class StarKVLlamaForCausalLM:
         if capture is not None:
             capture.append(dict(layer=li, q=q.view(T, H, D), out=out.view(T, H, D), h=h, k=k, v=v))
         return out
+
+    def _own_rotation(self) -> bool:
+        """Whether rows are rotated by the rotary table, not by a rotation of the caller's."""
+        return getattr(self.rotary.apply, "__func__", None) is Rotary.apply
+
+    def _check_positions(self, positions: torch.Tensor, md: StarKVMetadata) -> None:
+        """Refuses positions behind the rotary table, where the kernels would end the launch and the process with it. The
+        block table bounds a position that is its cache's length; one that lies apart is read here where the
+        caller gives no bound (a wait for the device; inside a capture ``DecodeGraph.replay`` counts)."""
+        if not (md.positions_apart or md.max_position is not None) or not self._own_rotation():
+            return
+        top, rows = md.max_position, self.rotary.cos_sin_cache.shape[0]
+        if top is None:
+            if not positions.numel() or positions.is_cuda and torch.cuda.is_current_stream_capturing():
+                return
+            top = int(positions.max())
+        if top >= rows:
+            raise ValueError(f"position {top} is behind the rotary table's {rows} rows (max_positions)")
 
     def _normed(self, layer: Layer, q: torch.Tensor, k: torch.Tensor) -> tuple:
         """q and k behind their norms, where a rotation of the caller's follows (rounded between the two)."""
@@ -407,6 +427,7 @@ class StarKVLlamaForCausalLM:
         """Logits [n, vocab] for one new token per request: tokens [n] at `positions` [n];
         `md` has every row as a decode (slot_mapping the new tokens' slots, seq_lens the cached
         tokens with them: positions + 1, fewer where caches were cut)."""
+        self._check_positions(positions, md)
         x = self._layers(self.embed[tokens], positions, md, capture, in_graph)
         return self._logits(x, self._few(x.shape[0], md))
 
@@ -433,7 +454,8 @@ class DecodeGraph:
     logits. The block table is static: its rows must cover every position the replays
     reach (up to max_model_len - 1). `lens`: cached tokens of each session where they are not its
     positions (``StarKVLlamaForCausalLM.evict`` cut its caches; ``lens`` of the graph takes what a later
-    cut returns); they advance with the positions."""
+    cut returns); they advance with the positions, and ``replay`` raises before a length passes max_model_len or a
+    position the rotary table."""
 
     def __init__(self, model: StarKVLlamaForCausalLM, block_table: torch.Tensor, tokens: torch.Tensor,
                  positions: torch.Tensor, lens: Optional[torch.Tensor] = None):
@@ -443,6 +465,8 @@ class DecodeGraph:
         self.tokens = tokens.clone()
         self.positions = positions.clone().long()
         self.lens = None if lens is None else lens.clone().long()
+        if lens is not None:
+            self._steps_left()
         self.graph = torch.cuda.CUDAGraph()
         weights = [w.clone() for w in model.weights]
         self._body()  # eager first: every lazy initialisation outside the capture
@@ -473,17 +497,37 @@ class DecodeGraph:
         self.positions.copy_(positions)
         if lens is not None:
             self.lens.copy_(lens)
+        self._left = 0
+
+    def _steps_left(self) -> int:
+        """Replays that stay in the cache and the rotary table; raises where there are none."""
+        m = self.model
+        length, top = int(self.lens.max()), int(self.positions.max())
+        if length >= m.max_model_len:
+            raise ValueError(f"a session's cache holds {length} tokens, the model's max_model_len; cut it or reset")
+        left = m.max_model_len - length
+        if m._own_rotation():
+            rows = m.rotary.cos_sin_cache.shape[0]
+            if top >= rows:
+                raise ValueError(f"position {top} is behind the rotary table's {rows} rows (max_positions)")
+            left = min(left, rows - top)
+        return left
 
     def replay(self) -> None:
+        if self.lens is not None:
+            # Counted on the host and read from the device only where the count runs out: a cut since shortened lengths.
+            self._left = (self._left or self._steps_left()) - 1
         self.graph.replay()
 
 
 def decode_metadata(block_table: torch.Tensor, positions: torch.Tensor, block_size: int,
-                    max_seq_len: int, lens: Optional[torch.Tensor] = None) -> StarKVMetadata:
+                    max_seq_len: int, lens: Optional[torch.Tensor] = None,
+                    max_position: Optional[int] = None) -> StarKVMetadata:
     """A decode-only batch's metadata: request b's new token at positions[b] (slot from its
     block-table row), seq_lens = positions + 1. `lens` [n]: the tokens cached before it, where a cut left fewer than
-    positions[b]; the slot and seq_lens go by them."""
-    n = positions.shape[0]
+    positions[b]; the slot and seq_lens go by them. `max_position`: an upper bound of positions that lie apart from
+    `lens`, so that the step need not read them back to see that they are in the rotary table."""
+    n, apart = positions.shape[0], lens is not None
     if lens is not None:
         positions = lens.long()
     if max_seq_len > block_table.shape[1] * block_size:
@@ -496,7 +540,8 @@ def decode_metadata(block_table: torch.Tensor, positions: torch.Tensor, block_si
         slots = block_table[rows, positions // block_size].long() * block_size + positions % block_size
         seq_lens = (positions + 1).to(torch.int32)
     return StarKVMetadata(num_actual_tokens=n, num_decodes=n, num_decode_tokens=n, num_prefills=0,
-                          max_seq_len=int(max_seq_len), seq_lens=seq_lens, block_table=block_table, slot_mapping=slots)
+                          max_seq_len=int(max_seq_len), seq_lens=seq_lens, block_table=block_table, slot_mapping=slots,
+                          positions_apart=apart, max_position=max_position)
 
 
 def prefill_metadata(block_table: torch.Tensor, prompt_lens: List[int], block_size: int):
