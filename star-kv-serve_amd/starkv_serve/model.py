@@ -319,6 +319,23 @@ class StarKVLlamaForCausalLM:
         rows = (ends - 1 - torch.minimum(back, lens - 1)).to(device, non_blocking=True)
         return list(zip(rows, seen.to(torch.int32).to(device, non_blocking=True)))
 
+    def _prompt_rows(self, n: int, rows) -> torch.Tensor:
+        """`rows` of n prompts on the device. One outside the weights would end the process there, and of two prompts with
+        one row either might win: refused before the step writes anything."""
+        if not self.weights:
+            raise RuntimeError("prompts of a model that weighs need allocate_kv_cache first")
+        have = self.weights[0].shape[0]
+        if n > have:
+            raise ValueError(f"{n} prompts for {have} rows of weights (num_requests of allocate_kv_cache)")
+        if rows is None:
+            return torch.arange(n, device=self.device)
+        rows = torch.as_tensor(rows)
+        whole = not rows.is_floating_point() and rows.dtype != torch.bool and rows.shape == (n,)
+        at = rows.tolist() if whole else []
+        if len(set(at)) != n or min(at) < 0 or max(at) >= have:
+            raise ValueError(f"prefill_step: rows {rows.tolist()} of {n} prompts: each one of its own of 0 .. {have - 1}")
+        return rows.to(self.device, torch.int64)
+
     def _observe(self, li: int, q: torch.Tensor, md: StarKVMetadata, observed: tuple) -> None:
         """The weights of prompts just written: what their last ``OBSERVED`` tokens give, a decode form each."""
         kc, vc = self.kv_caches[li]
@@ -411,7 +428,6 @@ class StarKVLlamaForCausalLM:
         few = self._few(x.shape[0], md)
         observed = None
         if self.weigh and md.num_prefills:
-            rows = torch.arange(md.num_prefills, device=x.device) if rows is None else rows.to(x.device, torch.int64)
             observed = self._observed_rows(md, x.device), rows
         for li, layer in enumerate(self.layers):
             a = self._attention(li, x, positions, md, capture, in_graph, few, observed)
@@ -433,14 +449,16 @@ class StarKVLlamaForCausalLM:
 
     @torch.no_grad()
     def prefill_step(self, tokens: torch.Tensor, positions: torch.Tensor, md: StarKVMetadata,
-                     capture: Optional[list] = None, rows: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     capture: Optional[list] = None, rows=None) -> torch.Tensor:
         """Logits [P, vocab] at the last token of each of P whole prompts: tokens [T] and
         positions [T] (0 .. L - 1 per prompt) laid end to end, `md` from
         ``prefill_metadata``. Every layer writes the prompts' cache rows (compressed: the
         codes through the fused write; full: K and V), so decode steps can follow. `rows` [P]: the
-        prompts' rows of a weighing model's weights (0 .. P - 1)."""
+        prompts' rows of a weighing model's weights (0 .. P - 1; a list or a tensor, which is read back)."""
         if md.num_decodes or not md.num_prefills:
             raise ValueError("prefill_step: a prompts-only batch (prefill_metadata)")
+        if self.weigh:
+            rows = self._prompt_rows(md.num_prefills, rows)
         x = self._layers(self.embed[tokens], positions, md, capture, False, rows)
         last = torch.tensor([e - 1 for e in md.prefill_query_start_loc_cpu[1:]]).to(x.device, non_blocking=True)
         return self._logits(x[last], False)

@@ -121,3 +121,30 @@ def test_a_graph_does_not_start_behind_the_limits(monkeypatch):
     with pytest.raises(ValueError, match="position 70"):
         M.DecodeGraph(model, TABLE, tokens, torch.tensor([70, 3]), torch.tensor([20, 3]))
     assert not model.ran
+
+
+def prompts(model, lens, **kw):
+    table = torch.arange(4 * len(lens), dtype=torch.int32).view(len(lens), 4)
+    md, positions = M.prefill_metadata(table, lens, 16)
+    return model.prefill_step(torch.zeros(sum(lens), dtype=torch.int64), positions, md, **kw)
+
+
+@pytest.mark.parametrize("lens,rows,message", [
+    ([5, 3, 4], None, "3 prompts"), ([5, 3], [0, 2], "rows"), ([5, 3], torch.tensor([0, 7]), "rows"),
+    ([5, 3], [-1, 0], "rows"), ([5, 3], [1, 1], "rows"), ([5, 3], [0], "rows"), ([5], torch.tensor([0, 1]), "rows"),
+    ([5, 3], torch.tensor([[0, 1]]), "rows"), ([5, 3], torch.tensor([0.0, 1.0]), "rows"), ([5, 3], [True, False], "rows")])
+def test_prompts_take_rows_that_are_there(monkeypatch, lens, rows, message):
+    model = weighing(monkeypatch)
+    with pytest.raises(ValueError, match=message):
+        prompts(model, lens, rows=rows)
+    assert not model.ran
+
+
+def test_prompts_rows(monkeypatch):
+    model = weighing(monkeypatch)
+    for lens, rows in (([5, 3], None), ([5, 3], [1, 0]), ([5], torch.tensor([1])), ([5], (0,)),
+                       ([5, 3], torch.tensor([1, 0], dtype=torch.int32))):
+        prompts(model, lens, rows=rows)
+    assert len(model.ran) == 5
+    with pytest.raises(RuntimeError, match="allocate_kv_cache"):
+        prompts(M.StarKVLlamaForCausalLM(SHAPE, None, 64, "cpu", weigh=True), [5])
