@@ -486,9 +486,10 @@ class DecodeGraph:
         if lens is not None:
             self._steps_left()
         self.graph = torch.cuda.CUDAGraph()
-        weights = [w.clone() for w in model.weights]
+        weights = getattr(model, "weights", [])  # any model with these steps will do
+        kept = [w.clone() for w in weights]
         self._body()  # eager first: every lazy initialisation outside the capture
-        for w, before in zip(model.weights, weights):  # that step is run again: its weights count once
+        for w, before in zip(weights, kept):  # that step is run again: its weights count once
             w.copy_(before)
         self.reset(tokens, positions, lens)
         torch.cuda.synchronize()

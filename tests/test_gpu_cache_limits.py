@@ -58,3 +58,21 @@ def test_a_full_cache_ends_the_replays(cuda):
     graph.replay()
     torch.cuda.synchronize()
     assert graph.lens.tolist() == [41, 12, 41] and torch.isfinite(graph.logits).all()
+
+
+def test_a_graph_of_another_models_steps(cuda):
+    """``DecodeGraph`` takes any model with ``decode_step``, ``block_size`` and ``max_model_len``."""
+    model, bt = build(cuda)
+
+    class Steps:
+        block_size, max_model_len, decode_step = model.block_size, model.max_model_len, model.decode_step
+
+    tokens, positions = prefill(model, bt), torch.tensor(PROMPTS, device=cuda)
+    graph = M.DecodeGraph(Steps(), bt, tokens, positions)
+    graph.replay()
+    want = graph.logits.clone()
+    graph.reset(tokens, positions)
+    logits, _, _ = decode(model, bt, tokens, positions, in_graph=True)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(want, logits) and torch.equal(graph.logits, logits)
