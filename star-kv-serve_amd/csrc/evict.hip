@@ -14,7 +14,7 @@
 // earlier chunk's targets (a handful of heads moves all rows at once instead, through the workspace:
 // stage_kernel). Columns are independent of each other, so K and V, and for few requests their
 // halves of 128 bytes, go to workgroups of their own. 16 requests of 8 KV heads cut from 4097 to 8192 tokens
-// to 2048: the choice 11 us (one CU a head), the move 57 (268 MB, 4.7 TB/s; a large copy's rate is 5.0).
+// to 2048: the choice 11 us (one CU a head), the move 55 (268 MB, 4.9 TB/s; a large copy's rate is 5.0).
 #include <algorithm>
 
 #include "common.hpp"

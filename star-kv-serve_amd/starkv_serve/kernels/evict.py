@@ -19,7 +19,8 @@ def paged_decode_weighted(query: torch.Tensor, k_cache: torch.Tensor, v_cache: t
     """``paged_decode_full`` (query of the cache's dtype, up to 16 query heads per KV head, any number), and weights
     [n, H_kv, >= max_seq_len] += each token's softmax weight, summed over its KV head's query heads. The newest
     token's entry (seq_lens[b] - 1) is set, as its sum starts with this step; entries behind it stay as they are.
-    Lengths are cut to max_seq_len. A request without tokens gives zeros and leaves its weights."""
+    Lengths are cut to max_seq_len. A request without tokens gives zeros and leaves its weights; a head whose scores
+    are all -inf gives NaN, and NaN weights."""
     _hip.require_cuda(query, k_cache, v_cache, block_table, seq_lens, weights)
     _hip.refuse_grad("paged_decode_weighted", query, k_cache, v_cache, weights)
     out = torch.empty_like(query, memory_format=torch.contiguous_format)

@@ -73,7 +73,7 @@ def paged_decode_sparse(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     """``[n, H_q, 128]``: ``paged_decode_full`` over the tokens of the blocks that `selected` [n, H_kv, keep] names for
     each request and KV head (each at most once; a place outside the request's blocks, such as -1, holds no
     tokens). Up to 16 query heads per KV head, any number; query of the cache's dtype. A row without
-    tokens is zero."""
+    tokens is zero, one whose scores are all -inf NaN."""
     _hip.require_cuda(query, k_cache, v_cache, block_table, seq_lens, selected)
     _hip.refuse_grad("paged_decode_sparse", query, k_cache, v_cache)
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
