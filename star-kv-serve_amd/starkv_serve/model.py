@@ -324,17 +324,17 @@ class StarKVLlamaForCausalLM:
         one row either might win: refused before the step writes anything."""
         if not self.weights:
             raise RuntimeError("prompts of a model that weighs need allocate_kv_cache first")
-        have = self.weights[0].shape[0]
+        have, dev = self.weights[0].shape[0], self.weights[0].device
         if n > have:
             raise ValueError(f"{n} prompts for {have} rows of weights (num_requests of allocate_kv_cache)")
         if rows is None:
-            return torch.arange(n, device=self.device)
+            return torch.arange(n, device=dev)
         rows = torch.as_tensor(rows)
         whole = not rows.is_floating_point() and rows.dtype != torch.bool and rows.shape == (n,)
         at = rows.tolist() if whole else []
         if len(set(at)) != n or min(at) < 0 or max(at) >= have:
             raise ValueError(f"prefill_step: rows {rows.tolist()} of {n} prompts: each one of its own of 0 .. {have - 1}")
-        return rows.to(self.device, torch.int64)
+        return rows.to(dev, torch.int64)
 
     def _observe(self, li: int, q: torch.Tensor, md: StarKVMetadata, observed: tuple) -> None:
         """The weights of prompts just written: what their last ``OBSERVED`` tokens give, a decode form each."""
