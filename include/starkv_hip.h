@@ -26,6 +26,10 @@ extern "C" {
 #define STARKV_F16 1
 #define STARKV_BF16 2
 
+/* Code types of an 8-bit cache: int8 in [-127, 127], e4m3 (no infinities) up to 448. */
+#define STARKV_I8 3
+#define STARKV_E4M3 4
+
 /* Cache kinds of starkv_decode_workspace_bytes / starkv_decode_two_pass: STARKV_BF16 or
  * STARKV_F16 low-rank codes, or the 3.2-bit QuantRow cache. */
 #define STARKV_CACHE_Q3_2 16
@@ -547,6 +551,66 @@ int starkv_evict(void *stream, void *k_cache, void *v_cache, int64_t c_s0, int64
                  int bt_width, const int32_t *seq_lens, int n, int num_kv_heads, const float *weights, int64_t w_s0,
                  int64_t w_s1, int weights_len, int keep, int sink, int recent, int32_t *new_lens, float *new_weights,
                  void *workspace, size_t workspace_bytes);
+
+/*
+ * Attention through a window, and 8-bit caches of uncompressed layers (the reference has neither). Block tables, lengths,
+ * block ids and n as above.
+ *
+ * Through a window the token at place t of its request sees place s <= t where t - s < window or s < sinks. A
+ * decode's token is at place length - 1. Blocks of which it sees nothing are not read, nor their table entries.
+ *
+ * starkv_window_decode: the decode over a bf16 or fp16 cache through a window; lengths are clamped to max_seq_len. At
+ * most 16 query heads a KV head. A row that sees no token gives zeros, one whose scores are all -inf NaN.
+ *
+ * starkv_prefill_window: starkv_prefill_attention through a window.
+ *
+ * An 8-bit cache: k_codes and v_codes [num_blocks, block_size, num_kv_heads, 128] of one byte (code_type; byte strides
+ * c_s0, c_s1, c_s2 shared by both, multiples of 16, rows 16-byte aligned; block_size 16 * 2^s up to 1024), and exponents
+ * [num_blocks, num_kv_heads, 2] int8 (strides x_s0, x_s1; last dimension contiguous): a key is code * 2^exponents[..][0], a
+ * value code * 2^exponents[..][1]. Exponents are at least -126; -128 stands for NaN, whatever the codes.
+ *
+ * starkv_write_kv8: key and value [n, num_kv_heads, 128] (bf16 or fp16, element strides) into their slots. Per block
+ * that is touched, head, and of the two: the exponent of the call's tokens is the least at which the largest
+ * magnitude has a code (-128 where one is infinite or NaN). Where the block's first token is among them the block begins
+ * anew with it, its other rows staying as they are; else the exponent becomes the larger of this and its own (-128 stays),
+ * and where it grows the codes of the other rows are rounded to it. Slots of one call are distinct; one outside
+ * the cache takes nothing. Codes are rounded to the nearest, ties to even.
+ *
+ * starkv_read_kv8: the values at n slots as contiguous key_out and value_out [n, num_kv_heads, 128] (bf16, fp16 or fp32,
+ * rounded once); a slot outside the cache gives zeros.
+ *
+ * starkv_decode_kv8: the decode over an 8-bit cache, through a window where window > 0 (0: all tokens); query and out
+ * bf16 or fp16, lengths clamped to max_seq_len. At most 16 query heads a KV head. A row that sees a token of a block whose
+ * exponent is -128 is NaN; one that sees no token gives zeros.
+ */
+size_t starkv_window_decode_workspace_bytes(int n, int num_heads, int num_kv_heads, int max_seq_len, int window, int sinks);
+int starkv_window_decode(void *stream, const void *query, int64_t q_s0, int64_t q_s1, const void *k_cache,
+                         const void *v_cache, int64_t c_s0, int64_t c_s1, int64_t c_s2, int dtype, int block_size,
+                         int64_t num_blocks, const int32_t *block_table, int64_t bt_s0, int64_t bt_s1, int bt_width,
+                         const int32_t *seq_lens, int n, int num_heads, int num_kv_heads, int max_seq_len, int window,
+                         int sinks, float scale, void *out, int64_t o_s0, int64_t o_s1, void *workspace,
+                         size_t workspace_bytes);
+int starkv_prefill_window(void *stream, const void *query, int64_t q_s0, int64_t q_s1, int q_dtype, const void *key,
+                          const void *value, int64_t kv_s0, int64_t kv_s1, int kv_dtype, const int32_t *cu_seqlens,
+                          const int32_t *blocks, int num_blocks, int num_heads, int num_kv_heads, int head_size,
+                          int window, int sinks, float scale, void *out, int64_t o_s0, int64_t o_s1, int out_dtype);
+size_t starkv_write_kv8_workspace_bytes(int n, int64_t num_blocks, int block_size);
+int starkv_write_kv8(void *stream, const void *key, int64_t k_s0, int64_t k_s1, const void *value, int64_t v_s0,
+                     int64_t v_s1, int dtype, void *k_codes, void *v_codes, int64_t c_s0, int64_t c_s1, int64_t c_s2,
+                     int code_type, int8_t *exponents, int64_t x_s0, int64_t x_s1, int block_size, int64_t num_blocks,
+                     const void *slot_mapping, int slot_bits, int n, int num_kv_heads, void *workspace,
+                     size_t workspace_bytes);
+int starkv_read_kv8(void *stream, const void *k_codes, const void *v_codes, int64_t c_s0, int64_t c_s1, int64_t c_s2,
+                    int code_type, const int8_t *exponents, int64_t x_s0, int64_t x_s1, int block_size,
+                    int64_t num_blocks, const void *slot_mapping, int slot_bits, int n, int num_kv_heads, void *key_out,
+                    void *value_out, int out_dtype);
+size_t starkv_decode_kv8_workspace_bytes(int n, int num_heads, int num_kv_heads, int max_seq_len, int window, int sinks);
+int starkv_decode_kv8(void *stream, const void *query, int64_t q_s0, int64_t q_s1, int dtype, const void *k_codes,
+                      const void *v_codes, int64_t c_s0, int64_t c_s1, int64_t c_s2, int code_type,
+                      const int8_t *exponents, int64_t x_s0, int64_t x_s1, int block_size, int64_t num_blocks,
+                      const int32_t *block_table, int64_t bt_s0, int64_t bt_s1, int bt_width, const int32_t *seq_lens,
+                      int n, int num_heads, int num_kv_heads, int max_seq_len, int window, int sinks, float scale,
+                      void *out, int64_t o_s0, int64_t o_s1, void *workspace, size_t workspace_bytes);
 
 /*
  * Timing for benchmarks (no counterpart in the reference, whose benchmark reads profiler

@@ -1,0 +1,374 @@
+// The 8-bit cache's write and read back (cache8.hpp has what it holds).
+//
+// A write puts n tokens' keys and values into their slots. Per block that it touches, head, and of keys and values: e_new
+// is the exponent of its own tokens' largest magnitude; where the block's first token is among them the block
+// begins anew with it, else the exponent becomes max(e_old, e_new), and where that is more than e_old the codes
+// that are there are rounded to it. All tokens of a block have to be known together: one workgroup does a whole
+// block, the one of the block's token that leads (its other tokens' workgroups end).
+//
+// Up to WR_FEW tokens (a decode step) each workgroup finds its block's tokens by looking through all slots (2 KB that
+// every workgroup reads from L2): one launch. More (prompts) write each token's index to its slot of a map first,
+// [num_blocks * block_size] of the workspace, which is not cleared: an entry counts where the slot of the token that
+// it names is the entry's own.
+//
+// A wave takes a (head, keys or values) of the block: four rows of 256 bytes a load, largest magnitude as integer bits
+// (NaN is above infinity, which is above all others), rows kept in registers from the first look to the rounding where there
+// are at most 16.
+#include <algorithm>
+
+#include "cache8.hpp"
+
+namespace starkv {
+
+namespace {
+
+constexpr int WR_THR = 256;
+constexpr int WR_FEW = 256;  // tokens that a workgroup looks through
+constexpr int WR_RUN = 16;   // tokens of a workgroup of a larger write
+
+struct Write8Params {
+    const uint8_t* src[2]; int64_t s0[2], s1[2];   // keys, values: bytes
+    uint8_t* codes[2]; int64_t c_s0, c_s1, c_s2;   // bytes
+    int8_t* ex; int64_t x_s0, x_s1;                // [num_blocks][H][2]
+    int shift; int64_t num_blocks;                 // block_size = 1 << shift
+    const void* slots; int slot64;
+    int n, H;
+    int32_t* map;                                  // larger writes
+};
+
+__device__ __forceinline__ int64_t slot_of(const Write8Params& p, int t) {
+    const int64_t s = p.slot64 ? ((const int64_t*)p.slots)[t] : (int64_t)((const int32_t*)p.slots)[t];
+    return s >= 0 && s >> p.shift < p.num_blocks ? s : -1;
+}
+
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    return v;
+}
+
+// Eight 16-bit values as fp32.
+template <int DT>
+__device__ __forceinline__ void values8(const uint4& w, float (&f)[8]) {
+    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if constexpr (DT == STARKV_BF16) {
+            f[2 * k] = __uint_as_float(ws[k] << 16);
+            f[2 * k + 1] = __uint_as_float(ws[k] & 0xffff0000u);
+        } else {
+            f[2 * k] = (float)__builtin_bit_cast(_Float16, (uint16_t)(ws[k] & 0xffffu));
+            f[2 * k + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(ws[k] >> 16));
+        }
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t top_of(const uint4& w) {
+    float f[8];
+    values8<DT>(w, f);
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
+    return top;
+}
+
+template <int CT, int DT>
+__device__ __forceinline__ uint2 encode(const uint4& w, float inv) {
+    float f[8];
+    values8<DT>(w, f);
+    return make_uint2(c8_pack<CT>(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                      c8_pack<CT>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+}
+
+// One block's (head, keys or values) by one wave. tok[offset]: the token of each place or -1; list: the places that
+// have one, `count` of them.
+template <int CT, int DT>
+__device__ __forceinline__ void write_unit(const Write8Params& p, int blk, int unit, const int* tok, const uint16_t* list,
+                                           int count) {
+    const int lane = threadIdx.x & 63, row = lane >> 4, d = lane & 15, h = unit >> 1, z = unit & 1;
+    int8_t* ex = p.ex + blk * p.x_s0 + h * p.x_s1 + z;
+    const int old = *ex;
+    const uint8_t* src = p.src[z] + h * p.s1[z] + 16 * d;
+    uint8_t* dst = p.codes[z] + blk * p.c_s0 + h * p.c_s2 + 8 * d;
+    constexpr int KEEP = 4;
+    uint4 kept[KEEP];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) {
+        const int at = 4 * i + row;
+        kept[i] = at < count ? *(const uint4*)(src + tok[list[at]] * p.s0[z]) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) top = max(top, top_of<DT>(kept[i]));
+    for (int at = 4 * KEEP + row; at < count; at += 4) top = max(top, top_of<DT>(*(const uint4*)(src + tok[list[at]] * p.s0[z])));
+    int e = c8_exponent<CT>(wave_umax(top));
+    const bool fresh = tok[0] >= 0;
+    if (!fresh) e = old == C8_NAN || e == C8_NAN ? C8_NAN : max(old, e);
+    if (!fresh && e != old && e != C8_NAN) {  // the codes that are there, to the new exponent
+        const float less = c8_scale(-min(e - old, 126));
+        for (int at = row; at < 1 << p.shift; at += 4) {
+            if (tok[at] >= 0) continue;
+            uint2* c = (uint2*)(dst + at * p.c_s1);
+            const uint2 w = *c;
+            float a[4], b[4];
+            c8_values<CT>(w.x, a);
+            c8_values<CT>(w.y, b);
+            *c = make_uint2(c8_pack<CT>(a[0] * less, a[1] * less, a[2] * less, a[3] * less),
+                            c8_pack<CT>(b[0] * less, b[1] * less, b[2] * less, b[3] * less));
+        }
+    }
+    const float inv = e == C8_NAN ? 0.f : c8_scale(-e);
+    const auto put = [&](int at, const uint4& w) {
+        *(uint2*)(dst + list[at] * p.c_s1) = e == C8_NAN ? make_uint2(0, 0) : encode<CT, DT>(w, inv);
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+        if (4 * i + row < count) put(4 * i + row, kept[i]);
+    for (int at = 4 * KEEP + row; at < count; at += 4) put(at, *(const uint4*)(src + tok[list[at]] * p.s0[z]));
+    if (lane == 0 && e != old) *ex = (int8_t)e;
+}
+
+struct Block8Shared {
+    int tok[C8_MAX_BLOCK];        // the token of each place, -1
+    uint16_t list[C8_MAX_BLOCK];  // the places that have one
+    int count, lead;
+};
+
+// The places with tokens, from tok; the workgroup's threads meet on both sides.
+__device__ __forceinline__ void list_places(Block8Shared& sh, int shift) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < 1 << shift; i += WR_THR)
+        if (sh.tok[i] >= 0) sh.list[atomicAdd(&sh.count, 1)] = (uint16_t)i;
+    __syncthreads();
+}
+
+// A workgroup a token and 4 units (of 2 H): the block's tokens by looking through all slots.
+template <int CT, int DT>
+__global__ __launch_bounds__(WR_THR) void write8_few_kernel(const Write8Params p) {
+    __shared__ Block8Shared sh;
+    const int t = blockIdx.x, tid = threadIdx.x;
+    const int64_t slot = slot_of(p, t);
+    if (slot < 0) return;
+    const int blk = (int)(slot >> p.shift), size = 1 << p.shift;
+    for (int i = tid; i < size; i += WR_THR) sh.tok[i] = -1;
+    if (tid == 0) {
+        sh.count = 0;
+        sh.lead = p.n;
+    }
+    __syncthreads();
+    for (int i = tid; i < p.n; i += WR_THR) {
+        const int64_t s = slot_of(p, i);
+        if (s >= 0 && s >> p.shift == blk) {
+            atomicMax(&sh.tok[s & (size - 1)], i);  // of two tokens with one slot the later
+            atomicMin(&sh.lead, i);
+        }
+    }
+    list_places(sh, p.shift);
+    if (sh.lead != t) return;
+    const int unit = blockIdx.y * 4 + (tid >> 6);
+    if (unit < 2 * p.H) write_unit<CT, DT>(p, blk, unit, sh.tok, sh.list, sh.count);
+}
+
+__global__ __launch_bounds__(WR_THR) void write8_map_kernel(const Write8Params p) {
+    const int t = blockIdx.x * WR_THR + threadIdx.x;
+    if (t >= p.n) return;
+    const int64_t slot = slot_of(p, t);
+    if (slot >= 0) p.map[slot] = t;
+}
+
+// The token of a slot by the map, -1 where it has none.
+__device__ __forceinline__ int mapped(const Write8Params& p, int64_t slot) {
+    const int t = p.map[slot];
+    return (uint32_t)t < (uint32_t)p.n && slot_of(p, t) == slot ? t : -1;
+}
+
+// A workgroup WR_RUN tokens: the blocks that one of them leads (has the lowest place of), each with the units of
+// blockIdx.y.
+template <int CT, int DT>
+__global__ __launch_bounds__(WR_THR) void write8_kernel(const Write8Params p, int units) {
+    __shared__ Block8Shared sh;
+    __shared__ int s_follows[WR_RUN];
+    const int tid = threadIdx.x, size = 1 << p.shift;
+    {
+        const int j = tid / WR_RUN, t = blockIdx.x * WR_RUN + j;
+        if (tid < WR_RUN) s_follows[tid] = 0;
+        __syncthreads();
+        const int64_t slot = t < p.n ? slot_of(p, t) : -1;
+        if (slot < 0 || p.map[slot] != t) {
+            s_follows[j] = 1;
+        } else {
+            for (int64_t s = (slot & ~(int64_t)(size - 1)) + tid % WR_RUN; s < slot; s += WR_RUN)
+                if (mapped(p, s) >= 0) s_follows[j] = 1;
+        }
+        __syncthreads();
+    }
+    for (int j = 0; j < WR_RUN; ++j) {
+        if (s_follows[j]) continue;
+        const int blk = (int)(slot_of(p, blockIdx.x * WR_RUN + j) >> p.shift);
+        if (tid == 0) sh.count = 0;
+        for (int i = tid; i < size; i += WR_THR) sh.tok[i] = mapped(p, ((int64_t)blk << p.shift) + i);
+        list_places(sh, p.shift);
+        const int end = min((int)(blockIdx.y + 1) * units, 2 * p.H);
+        for (int u = blockIdx.y * units + (tid >> 6); u < end; u += 4) write_unit<CT, DT>(p, blk, u, sh.tok, sh.list, sh.count);
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Rows back: code * 2^exponent, rounded once to 16 or 32 bits
+// ---------------------------------------------------------------------------
+struct Read8Params {
+    const uint8_t* codes[2]; int64_t c_s0, c_s1, c_s2;  // bytes
+    const int8_t* ex; int64_t x_s0, x_s1;
+    int shift; int64_t num_blocks;
+    const void* slots; int slot64;
+    int n, H, out_dt;
+    void* out[2];                                       // [n][H][128]
+};
+
+// 8 dimensions a lane, 16 lanes a row, rows of a token side by side. The bound is HBM: 128 bytes read and 256 written.
+template <int CT, int ODT>
+__global__ __launch_bounds__(256) void read8_kernel(const Read8Params p) {
+    const int64_t pieces = (int64_t)p.n * p.H * 16;
+    const int z = blockIdx.y;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i >> 4;
+        const int t = (int)(row / p.H), h = (int)(row - (int64_t)t * p.H), d = 8 * (int)(i & 15);
+        const int64_t slot = p.slot64 ? ((const int64_t*)p.slots)[t] : (int64_t)((const int32_t*)p.slots)[t];
+        const bool there = slot >= 0 && slot >> p.shift < p.num_blocks;
+        float f[8];
+        if (there) {
+            const int64_t blk = slot >> p.shift;
+            const uint2 w = *(const uint2*)(p.codes[z] + blk * p.c_s0 + (slot & ((1 << p.shift) - 1)) * p.c_s1 + h * p.c_s2 + d);
+            const float scale = c8_scale(p.ex[blk * p.x_s0 + h * p.x_s1 + z]);
+            float a[4], b[4];
+            c8_values<CT>(w.x, a);
+            c8_values<CT>(w.y, b);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                f[e] = a[e] * scale;
+                f[4 + e] = b[e] * scale;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = 0.f;
+        }
+        if constexpr (ODT == STARKV_F32) {
+            float4* o = (float4*)((float*)p.out[z] + 8 * i);
+            o[0] = make_float4(f[0], f[1], f[2], f[3]);
+            o[1] = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint16_t lo = ODT == STARKV_BF16 ? f32_to_bf16_rne(f[2 * e]) : __builtin_bit_cast(uint16_t, (_Float16)f[2 * e]);
+                const uint16_t hi = ODT == STARKV_BF16 ? f32_to_bf16_rne(f[2 * e + 1]) : __builtin_bit_cast(uint16_t, (_Float16)f[2 * e + 1]);
+                w[e] = (uint32_t)lo | (uint32_t)hi << 16;
+            }
+            *(uint4*)((uint16_t*)p.out[z] + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+template <int CT>
+const void* read_pick(int dt) {
+    return dt == STARKV_F32 ? (const void*)&read8_kernel<CT, STARKV_F32>
+           : dt == STARKV_F16 ? (const void*)&read8_kernel<CT, STARKV_F16>
+                              : (const void*)&read8_kernel<CT, STARKV_BF16>;
+}
+
+}  // namespace
+
+}  // namespace starkv
+
+using namespace starkv;
+
+extern "C" {
+
+size_t starkv_write_kv8_workspace_bytes(int n, int64_t num_blocks, int block_size) {
+    if (n <= WR_FEW || num_blocks < 1 || block_size < 1) return 256;
+    return std::max<size_t>(256, (size_t)num_blocks * block_size * 4);
+}
+
+int starkv_write_kv8(void* stream, const void* key, int64_t k_s0, int64_t k_s1, const void* value, int64_t v_s0,
+                     int64_t v_s1, int dtype, void* k_codes, void* v_codes, int64_t c_s0, int64_t c_s1, int64_t c_s2,
+                     int code_type, int8_t* exponents, int64_t x_s0, int64_t x_s1, int block_size, int64_t num_blocks,
+                     const void* slot_mapping, int slot_bits, int n, int num_kv_heads, void* workspace,
+                     size_t workspace_bytes) {
+    clear_error();
+    SKV_CHECK(n >= 0 && num_kv_heads >= 1 && num_kv_heads <= 65535, "write_kv8: n=%d num_kv_heads=%d (up to 65535)", n, num_kv_heads);
+    if (n == 0) return STARKV_OK;
+    SKV_CHECK(key && value && k_codes && v_codes && exponents && slot_mapping && workspace, "write_kv8: null pointer");
+    SKV_CHECK(dtype == STARKV_BF16 || dtype == STARKV_F16, "write_kv8: keys and values must be bf16 or fp16");
+    SKV_CHECK(code_type == STARKV_I8 || code_type == STARKV_E4M3, "write_kv8: codes must be int8 or e4m3");
+    SKV_CHECK(slot_bits == 32 || slot_bits == 64, "write_kv8: slot_mapping must be int32 or int64");
+    SKV_CHECK(c8_block_shift(block_size) >= 0, "write_kv8: block_size must be 16 times a power of two, at most %d", C8_MAX_BLOCK);
+    SKV_CHECK(num_blocks >= 1 && num_blocks <= 0x7fffffff, "write_kv8: empty cache");
+    SKV_CHECK(((uintptr_t)key | (uintptr_t)value) % 16 == 0 && (k_s0 | k_s1 | v_s0 | v_s1) % 8 == 0 &&
+                  ((uintptr_t)k_codes | (uintptr_t)v_codes) % 16 == 0 && (c_s0 | c_s1 | c_s2) % 16 == 0,
+              "write_kv8: rows must be 16-byte aligned");
+    const size_t need = starkv_write_kv8_workspace_bytes(n, num_blocks, block_size);
+    SKV_CHECK(workspace_bytes >= need && (uintptr_t)workspace % 16 == 0, "write_kv8: workspace %zu bytes < %zu", workspace_bytes, need);
+    Write8Params p;
+    p.src[0] = (const uint8_t*)key; p.s0[0] = 2 * k_s0; p.s1[0] = 2 * k_s1;
+    p.src[1] = (const uint8_t*)value; p.s0[1] = 2 * v_s0; p.s1[1] = 2 * v_s1;
+    p.codes[0] = (uint8_t*)k_codes; p.codes[1] = (uint8_t*)v_codes;
+    p.c_s0 = c_s0; p.c_s1 = c_s1; p.c_s2 = c_s2;
+    p.ex = exponents; p.x_s0 = x_s0; p.x_s1 = x_s1;
+    p.shift = c8_block_shift(block_size); p.num_blocks = num_blocks;
+    p.slots = slot_mapping; p.slot64 = slot_bits == 64;
+    p.n = n; p.H = num_kv_heads;
+    p.map = (int32_t*)workspace;
+    const bool i8 = code_type == STARKV_I8, bf = dtype == STARKV_BF16;
+    if (n <= WR_FEW) {
+        const void* fn = i8 ? bf ? (const void*)&write8_few_kernel<STARKV_I8, STARKV_BF16> : (const void*)&write8_few_kernel<STARKV_I8, STARKV_F16>
+                            : bf ? (const void*)&write8_few_kernel<STARKV_E4M3, STARKV_BF16> : (const void*)&write8_few_kernel<STARKV_E4M3, STARKV_F16>;
+        void* args[] = {(void*)&p};
+        SKV_HIP(hipLaunchKernel(fn, dim3(n, (2 * num_kv_heads + 3) / 4), dim3(WR_THR), args, 0, (hipStream_t)stream));
+        return STARKV_OK;
+    }
+    hipLaunchKernelGGL(write8_map_kernel, dim3((n + WR_THR - 1) / WR_THR), dim3(WR_THR), 0, (hipStream_t)stream, p);
+    SKV_HIP(hipGetLastError());
+    const void* fn = i8 ? bf ? (const void*)&write8_kernel<STARKV_I8, STARKV_BF16> : (const void*)&write8_kernel<STARKV_I8, STARKV_F16>
+                        : bf ? (const void*)&write8_kernel<STARKV_E4M3, STARKV_BF16> : (const void*)&write8_kernel<STARKV_E4M3, STARKV_F16>;
+    int units = 16;  // four a wave: the search for a block's tokens is made once for them
+    void* args[] = {(void*)&p, (void*)&units};
+    SKV_HIP(hipLaunchKernel(fn, dim3((n + WR_RUN - 1) / WR_RUN, (2 * num_kv_heads + units - 1) / units), dim3(WR_THR), args, 0,
+                            (hipStream_t)stream));
+    return STARKV_OK;
+}
+
+int starkv_read_kv8(void* stream, const void* k_codes, const void* v_codes, int64_t c_s0, int64_t c_s1, int64_t c_s2,
+                    int code_type, const int8_t* exponents, int64_t x_s0, int64_t x_s1, int block_size,
+                    int64_t num_blocks, const void* slot_mapping, int slot_bits, int n, int num_kv_heads, void* key_out,
+                    void* value_out, int out_dtype) {
+    clear_error();
+    SKV_CHECK(n >= 0 && num_kv_heads >= 1, "read_kv8: n=%d num_kv_heads=%d", n, num_kv_heads);
+    if (n == 0) return STARKV_OK;
+    SKV_CHECK(k_codes && v_codes && exponents && slot_mapping && key_out && value_out, "read_kv8: null pointer");
+    SKV_CHECK(out_dtype >= STARKV_F32 && out_dtype <= STARKV_BF16, "read_kv8: rows of bf16, fp16 or fp32");
+    SKV_CHECK(code_type == STARKV_I8 || code_type == STARKV_E4M3, "read_kv8: codes must be int8 or e4m3");
+    SKV_CHECK(slot_bits == 32 || slot_bits == 64, "read_kv8: slot_mapping must be int32 or int64");
+    SKV_CHECK(c8_block_shift(block_size) >= 0, "read_kv8: block_size must be 16 times a power of two, at most %d", C8_MAX_BLOCK);
+    SKV_CHECK(num_blocks >= 1 && num_blocks <= 0x7fffffff, "read_kv8: empty cache");
+    SKV_CHECK(((uintptr_t)k_codes | (uintptr_t)v_codes | (uintptr_t)key_out | (uintptr_t)value_out) % 16 == 0 &&
+                  (c_s0 | c_s1 | c_s2) % 16 == 0,
+              "read_kv8: rows must be 16-byte aligned");
+    Read8Params p;
+    p.codes[0] = (const uint8_t*)k_codes; p.codes[1] = (const uint8_t*)v_codes;
+    p.c_s0 = c_s0; p.c_s1 = c_s1; p.c_s2 = c_s2;
+    p.ex = exponents; p.x_s0 = x_s0; p.x_s1 = x_s1;
+    p.shift = c8_block_shift(block_size); p.num_blocks = num_blocks;
+    p.slots = slot_mapping; p.slot64 = slot_bits == 64;
+    p.n = n; p.H = num_kv_heads; p.out_dt = out_dtype;
+    p.out[0] = key_out; p.out[1] = value_out;
+    const void* fn = code_type == STARKV_I8 ? read_pick<STARKV_I8>(out_dtype) : read_pick<STARKV_E4M3>(out_dtype);
+    void* args[] = {(void*)&p};
+    const int64_t pieces = (int64_t)n * num_kv_heads * 16;
+    SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 20), 2), dim3(256), args, 0,
+                            (hipStream_t)stream));
+    return STARKV_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,452 @@
+// One token's attention over an 8-bit cache (cache8.hpp has what it holds), whole or through a window
+// (window_pages.hpp), on matrix instructions.
+//
+// For a request b, a KV head h and its G <= 16 query heads, over the places t that the newest token sees, with K_t =
+// k_t 2^a, V_t = v_t 2^c (k, v codes; a, c the exponents of t's block):
+//     s_t = scale log2(e) 2^a (q . k_t),  out = sum_t 2^(s_t - m) 2^c v_t / sum_t 2^(s_t - m).
+// Codes are never multiplied by their scales: 2^a goes onto the 4 scores that a lane has of a page, 2^c into its
+// weights. A page is 16 tokens of one block. A workgroup of 4 waves takes a range of the unit's pages (a split);
+// a wave takes two pages, 32 tokens, at a time and keeps references and sums of its own; the waves meet in LDS at
+// the end, the splits in merge8_kernel.
+//
+// Both products run on v_mfma_f32_16x16x32_f16, for which every code and fp16 query is exact; a bf16 query row goes to fp16
+// by a power of two that brings its largest value to 2^14, which leaves values down to 2^-28 of that exact. S^T =
+// K q^T has 16 tokens as rows: lane l holds 16 bytes of row l % 16 at a time, two operands of 8 dimensions. Its result
+// gives lane l the scores of column l % 16 (a query head) at tokens 4 (l / 16) .. + 3 of either page, which is the B
+// operand of out^T = V^T P^T with that product's 32 terms in the order (l / 16, page, token). V^T's rows are the
+// head's dimensions in the order 8 (l % 16) + i for the i-th of 8 products: lane l loads 8 bytes of each of its 8
+// tokens, and 4x4 byte transposes (8 permutes each) make words of 4 tokens' dimension i before they become halves.
+//
+// Rounding: scores, references and sums are fp32. A weight enters the second product as two fp16 values, itself rounded and what
+// that left, 22 bits; up to 8 query heads the lanes of the other 8 columns, whose scores are the same heads'
+// again, take the second one, so that one product does. Two references are kept for that: m of the scores s for
+// the sum of weights, and r of s + c for the weights of the values, each 2^7 below the largest when it was set and moved
+// when that passes it by 2^15, so that neither overflows fp16 and what a value contributes keeps its bits whatever the
+// blocks' exponents are (a first token with a large weight and values of 2^-40 of the others' keeps them). Partials
+// are divided by their sum and scaled by 2^(r - m) where they are left, so values near fp32's largest stay finite.
+//
+// A block whose exponent says NaN makes every row NaN that sees one of its tokens. A row that sees no token is zero; one
+// whose scores are all -inf is 0 / 0, NaN.
+#include <algorithm>
+
+#include "cache8.hpp"
+#include "window_pages.hpp"
+
+namespace starkv {
+
+namespace {
+
+constexpr int D8_THR = 256;
+constexpr int D8_CHUNK = 512;       // pages whose places are looked up at a time
+constexpr int D8_PART = 132;        // floats of a partial: reference, sum of weights, 0, 0, out[128]
+constexpr int D8_MAX_SPLITS = 128;
+constexpr int D8_MAX_GROUP = 16;    // query heads per KV head: the columns of a matrix product
+constexpr float D8_LEAST = -3.402823466e38f;  // the reference of tokens whose scores are all -inf
+
+struct Decode8Params {
+    const uint16_t* q; int64_t q_s0, q_s1;                              // elements
+    const uint8_t* kc; const uint8_t* vc; int64_t c_s0, c_s1, c_s2;     // bytes
+    const int8_t* ex; int64_t x_s0, x_s1;                               // [num_blocks][Hkv][2]
+    int bs_shift; int64_t num_blocks;                                   // block_size = 16 << bs_shift
+    const int32_t* bt; int64_t bt_s0, bt_s1;
+    const int32_t* seq_lens; int span;                                  // lengths are clamped to span
+    int n, Hkv, G, splits, window, sinks;
+    float sc;                                                           // scale * log2(e)
+    float* part;                                                        // [n][H][splits][D8_PART]
+    uint16_t* out; int64_t o_s0, o_s1;
+};
+
+// Pages of a split: the request's, shared out evenly, 8 at least (two a wave). The splits behind the last have none.
+__device__ __forceinline__ int pages_per_split(int pages, int splits) { return max((pages + splits - 1) / splits, 8); }
+
+__device__ __forceinline__ SeenPages seen_by(const Decode8Params& p, int b) {
+    return seen_pages(min(max(p.seq_lens[b], 0), p.span), p.window, p.sinks);
+}
+
+__device__ __forceinline__ f32x4_t mfma_f16(uint4 a, uint4 b, f32x4_t c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+// Two floats to fp16, packed, and what the rounding left of them.
+__device__ __forceinline__ uint32_t split_half(float& a, float& b) {
+    const _Float16 x = (_Float16)a, y = (_Float16)b;
+    a -= (float)x;
+    b -= (float)y;
+    return (uint32_t)__builtin_bit_cast(uint16_t, x) | (uint32_t)__builtin_bit_cast(uint16_t, y) << 16;
+}
+
+// Words of 4 dimensions of tokens 0 .. 3 to words of 4 tokens of dimensions 0 .. 3.
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
+    const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    const uint32_t c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+
+// The workgroup's unit: (request, KV head, split) from the block index. MANY: 9 to 16 query heads.
+template <int CT, int QDT, bool MANY>
+__global__ __launch_bounds__(D8_THR, 4) void decode8_kernel(const Decode8Params p) {
+    __shared__ int4 s_page[D8_CHUNK];  // block, place in the block, places that are seen, exponents
+    extern __shared__ float s_dyn[];   // [4 waves][G][D8_PART] for the merge
+    const int id = blockIdx.x, s = id % p.splits, u = id / p.splits, h = u % p.Hkv, b = u / p.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = MANY ? lane & 15 : lane & 7, quad = lane >> 4;  // the lane's query head
+    const int H = p.Hkv * p.G;
+    const SeenPages seen = seen_by(p, b);
+    const int pps = pages_per_split(seen.pages, p.splits);
+    const int k0 = min(s * pps, seen.pages), k1 = min(k0 + pps, seen.pages);
+    if (k0 >= k1 && s > 0) return;  // the merge reads the splits that have pages
+    const int mask = (1 << p.bs_shift) - 1;
+
+    // The head's row: dimensions 64 st + 16 quad .. + 15, two operands; their fp16 values times 2^up.
+    uint4 qf[2][2];
+    float sc = p.sc;
+    {
+        uint4 w[2][2];
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                w[st][x] = col < p.G ? *(const uint4*)(p.q + b * p.q_s0 + (int64_t)(h * p.G + col) * p.q_s1 + 64 * st + 16 * quad + 8 * x)
+                                     : make_uint4(0, 0, 0, 0);
+        if constexpr (QDT == STARKV_F16) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) qf[i >> 1][i & 1] = w[i >> 1][i & 1];
+        } else {
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t v = ((const uint32_t*)&w[i >> 1][i & 1])[k];
+                    top = fmaxf(top, fmaxf(fabsf(__uint_as_float(v << 16)), fabsf(__uint_as_float(v & 0xffff0000u))));
+                }
+            top = max_rows(top);
+            // 2^14 <= top 2^up < 2^15; of zeros, subnormal numbers and infinities the nearest power there is.
+            const int x = (int)(__float_as_uint(top) >> 23), up = min(max(141 - x, -126), 126);
+            const float by = __uint_as_float((uint32_t)(up + 127) << 23);
+            sc *= __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                half8_t o;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t v = ((const uint32_t*)&w[i >> 1][i & 1])[k];
+                    o[2 * k] = (_Float16)(__uint_as_float(v << 16) * by);
+                    o[2 * k + 1] = (_Float16)(__uint_as_float(v & 0xffff0000u) * by);
+                }
+                qf[i >> 1][i & 1] = __builtin_bit_cast(uint4, o);
+            }
+        }
+    }
+    const uint8_t* kh = p.kc + h * p.c_s2 + 16 * quad + (int64_t)(lane & 15) * p.c_s1;
+    const uint8_t* vh = p.vc + h * p.c_s2 + 8 * (lane & 15) + (int64_t)(4 * quad) * p.c_s1;
+    float m = -INFINITY, r = -INFINITY, l = 0.f;
+    f32x4_t acc[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+    for (int c0 = k0; c0 < k1; c0 += D8_CHUNK) {
+        const int count = min(D8_CHUNK, k1 - c0);
+        if (c0 != k0) __syncthreads();
+        for (int i = tid; i < count; i += D8_THR) {
+            const int pg = seen.page(c0 + i);
+            int blk = p.bt[b * p.bt_s0 + (pg >> p.bs_shift) * p.bt_s1];
+            uint32_t see = seen.mask(pg);
+            int ex = 0;
+            if (blk < 0 || blk >= p.num_blocks) {
+                blk = 0;  // no block of the cache: no tokens
+                see = 0;
+            } else {
+                const int8_t* e = p.ex + blk * p.x_s0 + h * p.x_s1;
+                ex = (uint8_t)e[0] | (int)e[1] << 8;
+            }
+            s_page[i] = make_int4(blk, pg & mask, (int)see, ex);
+        }
+        __syncthreads();
+        for (int i = 2 * wave; i < count; i += 8) {
+            uint32_t see[2];
+            int at[2], place[2], ex[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int4 v = s_page[min(i + x, count - 1)];
+                at[x] = __builtin_amdgcn_readfirstlane(v.x);
+                place[x] = __builtin_amdgcn_readfirstlane(v.y);
+                see[x] = i + x < count ? (uint32_t)__builtin_amdgcn_readfirstlane(v.z) : 0u;
+                ex[x] = __builtin_amdgcn_readfirstlane(v.w);
+            }
+            if ((see[0] | see[1]) == 0) continue;
+            uint4 kr[2][2];
+            uint2 vr[2][4];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                // A page of which nothing is seen reads the other one again. A page lies within its block whatever
+                // the request's length, so every row of it can be read.
+                const int y = see[x] ? x : x ^ 1;
+                const int64_t base = at[y] * p.c_s0 + (int64_t)(16 * place[y]) * p.c_s1;
+#pragma unroll
+                for (int st = 0; st < 2; ++st) kr[x][st] = *(const uint4*)(kh + base + 64 * st);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) vr[x][j] = *(const uint2*)(vh + base + j * p.c_s1);
+            }
+            float sv[2][4], up[2];  // scores; the exponents of the values
+            float mx = -INFINITY, rx = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    const uint2 a = c8_halves<CT>(kr[x][st].x), c = c8_halves<CT>(kr[x][st].y);
+                    const uint2 e = c8_halves<CT>(kr[x][st].z), f = c8_halves<CT>(kr[x][st].w);
+                    d = mfma_f16(make_uint4(a.x, a.y, c.x, c.y), qf[st][0], d);
+                    d = mfma_f16(make_uint4(e.x, e.y, f.x, f.y), qf[st][1], d);
+                }
+                const float by = sc * c8_scale((int)(int8_t)ex[x]);
+                const int ev = ex[x] >> 8;
+                up[x] = ev == C8_NAN ? __builtin_nanf("") : (float)ev;
+                if (see[x] == 0) up[x] = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sv[x][k] = d[k] * by;
+                if (see[x] != 0xffffu) {  // tokens out of sight: no score, and codes of 0 (an e4m3 code may be NaN)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const bool ok = see[x] >> (4 * quad + k) & 1u;
+                        sv[x][k] = ok ? sv[x][k] : -INFINITY;
+                        vr[x][k] = ok ? vr[x][k] : make_uint2(0, 0);
+                    }
+                }
+                const float px = fmaxf(fmaxf(sv[x][0], sv[x][1]), fmaxf(sv[x][2], sv[x][3]));
+                mx = fmaxf(mx, px);
+                rx = fmaxf(rx, px + up[x]);
+            }
+            mx = max_rows(mx);
+            rx = max_rows(rx);
+            m = fmaxf(m, D8_LEAST);
+            r = fmaxf(r, D8_LEAST);
+            if (__builtin_amdgcn_ballot_w64(mx > m + 15.f || rx > r + 15.f) != 0) {
+                const float mn = mx > m + 15.f ? mx - 7.f : m, rn = rx > r + 15.f ? rx - 7.f : r;
+                l *= mn == m ? 1.f : exp2f(m - mn);
+                const float alpha = rn == r ? 1.f : exp2f(r - rn);
+                m = mn;
+                r = rn;
+#pragma unroll
+                for (int i8 = 0; i8 < 8; ++i8) acc[i8] *= alpha;
+            }
+            float pe[2][4];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const float f = exp2f(up[x] + (m - r));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const bool ok = see[x] >> (4 * quad + k) & 1u;
+                    const float w = ok ? exp2f(sv[x][k] - m) : 0.f;
+                    l += w;
+                    pe[x][k] = ok ? w * f : 0.f;
+                }
+            }
+            // The weights' values: the first, and what it left; up to 8 heads the lanes of the second columns take that.
+            uint4 pw[MANY ? 2 : 1];
+            pw[0] = make_uint4(split_half(pe[0][0], pe[0][1]), split_half(pe[0][2], pe[0][3]),
+                               split_half(pe[1][0], pe[1][1]), split_half(pe[1][2], pe[1][3]));
+            const uint4 rest = make_uint4(split_half(pe[0][0], pe[0][1]), split_half(pe[0][2], pe[0][3]),
+                                          split_half(pe[1][0], pe[1][1]), split_half(pe[1][2], pe[1][3]));
+            if constexpr (MANY) {
+                pw[1] = rest;
+            } else if (lane & 8) {
+                pw[0] = rest;
+            }
+#pragma unroll
+            for (int hd = 0; hd < 2; ++hd) {
+                uint32_t w[2][4];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[x][j] = hd ? vr[x][j].y : vr[x][j].x;
+                    transpose4(w[x]);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint2 a = c8_halves<CT>(w[0][i]), c = c8_halves<CT>(w[1][i]);
+                    const uint4 vt = make_uint4(a.x, a.y, c.x, c.y);
+#pragma unroll
+                    for (int k = 0; k < (MANY ? 2 : 1); ++k) acc[4 * hd + i] = mfma_f16(vt, pw[k], acc[4 * hd + i]);
+                }
+            }
+        }
+    }
+    l = sum_rows(l);
+    if constexpr (!MANY) {  // both columns of a head: lanes 8 apart in a row of 16
+#pragma unroll
+        for (int i8 = 0; i8 < 8; ++i8)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[i8][x] += dpp_f<0x128>(acc[i8][x]);  // row_ror:8
+    }
+    if (col < p.G && (MANY || !(lane & 8))) {
+        float* w = s_dyn + (wave * p.G + col) * D8_PART;
+        if (quad == 0) *(float4*)w = make_float4(m, l, r, 0.f);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {  // dimensions 32 quad + 8 x + i
+            *(float4*)(w + 4 + 32 * quad + 8 * x) = make_float4(acc[0][x], acc[1][x], acc[2][x], acc[3][x]);
+            *(float4*)(w + 8 + 32 * quad + 8 * x) = make_float4(acc[4][x], acc[5][x], acc[6][x], acc[7][x]);
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < p.G * 128; i += D8_THR) {
+        const int g = i >> 7, d = i & 127;
+        const float* w = s_dyn + g * D8_PART;
+        float M = -INFINITY, R = -INFINITY, lt = 0.f, a = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            M = fmaxf(M, w[k * p.G * D8_PART]);
+            R = fmaxf(R, w[k * p.G * D8_PART + 2]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float* x = w + k * p.G * D8_PART;
+            // A wave without tokens has references of -inf and sums of 0.
+            lt = fmaf(x[1], x[0] == -INFINITY ? 1.f : exp2f(x[0] - M), lt);
+            a = fmaf(x[4 + d], x[2] == -INFINITY ? 1.f : exp2f(x[2] - R), a);
+        }
+        const int hq = h * p.G + g;
+        const float half = exp2f(0.5f * (R - M));  // in two steps: its square may be past fp32's range where the result is not
+        // A split without weight (scores of -inf alone) adds 0 to the others', not 0 times 0 / 0.
+        const float o = M == -INFINITY || (lt == 0.f && p.splits > 1) ? 0.f : a / lt * half * half;
+        if (p.splits == 1) {
+            store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, QDT, o);
+        } else {
+            float* pp = p.part + (((int64_t)b * H + hq) * p.splits + s) * D8_PART;
+            if (d == 0) *(float4*)pp = make_float4(M, lt, 0.f, 0.f);
+            pp[4 + d] = o;
+        }
+    }
+}
+
+// A head's splits joined by one wave: out = sum_s l_s 2^(m_s - M) out_s / sum_s l_s 2^(m_s - M). Lane s holds the factors of
+// splits s and s + 64 and sums dimensions 2 s and 2 s + 1, eight splits' loads in flight.
+template <int QDT>
+__global__ __launch_bounds__(64) void merge8_kernel(const Decode8Params p) {
+    static_assert(D8_MAX_SPLITS <= 128, "two splits a lane");
+    const int lane = threadIdx.x, hq = blockIdx.x, b = blockIdx.y;
+    const SeenPages seen = seen_by(p, b);
+    const int pps = pages_per_split(seen.pages, p.splits), splits = max((seen.pages + pps - 1) / pps, 1);
+    const float* pp = p.part + ((int64_t)b * p.Hkv * p.G + hq) * p.splits * D8_PART;
+    float m[2], f[2], lt = 0.f;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        const int s = lane + 64 * x;
+        m[x] = s < splits ? pp[s * D8_PART] : -INFINITY;
+        f[x] = s < splits ? pp[s * D8_PART + 1] : 0.f;
+    }
+    const float M = wave_max(fmaxf(m[0], m[1]));
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        f[x] *= m[x] == -INFINITY ? 1.f : exp2f(m[x] - M);
+        lt += f[x];
+    }
+    lt = wave_sum(lt);
+    float2 a = make_float2(0.f, 0.f);
+    for (int s0 = 0; s0 < splits; s0 += 8) {
+        float2 v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = *(const float2*)(pp + min(s0 + u, splits - 1) * D8_PART + 4 + 2 * lane);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(s0 < 64 ? f[0] : f[1]), (s0 + u) & 63)) / lt;
+            if (s0 + u < splits) {
+                a.x = fmaf(v[u].x, fs, a.x);
+                a.y = fmaf(v[u].y, fs, a.y);
+            }
+        }
+    }
+    const int64_t o = b * p.o_s0 + hq * p.o_s1 + 2 * lane;
+    store_f(p.out, o, QDT, M == -INFINITY ? 0.f : a.x);
+    store_f(p.out, o + 1, QDT, M == -INFINITY ? 0.f : a.y);
+}
+
+// Splits per unit (request and KV head): workgroups for `per_cu` a CU, 8 pages a split at least.
+int decode8_splits(int n, int num_kv_heads, int span, int window, int sinks) {
+    int dev = 0, cus = 256, c = 0;
+    if (hipGetDevice(&dev) == hipSuccess &&
+        hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && c > 0)
+        cus = c;
+    const int64_t units = (int64_t)n * num_kv_heads, pages = seen_pages_most(span, window, sinks);
+    const int64_t s = std::min<int64_t>((2 * (int64_t)cus + units - 1) / units, (pages + 7) / 8);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(s, D8_MAX_SPLITS));
+}
+
+template <int CT, int QDT>
+const void* decode_pick(int G) {
+    return G <= 8 ? (const void*)&decode8_kernel<CT, QDT, false> : (const void*)&decode8_kernel<CT, QDT, true>;
+}
+
+}  // namespace
+
+}  // namespace starkv
+
+using namespace starkv;
+
+extern "C" {
+
+size_t starkv_decode_kv8_workspace_bytes(int n, int num_heads, int num_kv_heads, int max_seq_len, int window, int sinks) {
+    if (n < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || max_seq_len < 1 || window < 0 || sinks < 0) return 256;
+    const int splits = decode8_splits(n, num_kv_heads, max_seq_len, window, sinks);
+    return splits == 1 ? 256 : (size_t)n * num_heads * splits * D8_PART * 4;
+}
+
+int starkv_decode_kv8(void* stream, const void* query, int64_t q_s0, int64_t q_s1, int dtype, const void* k_codes,
+                      const void* v_codes, int64_t c_s0, int64_t c_s1, int64_t c_s2, int code_type,
+                      const int8_t* exponents, int64_t x_s0, int64_t x_s1, int block_size, int64_t num_blocks,
+                      const int32_t* block_table, int64_t bt_s0, int64_t bt_s1, int bt_width, const int32_t* seq_lens,
+                      int n, int num_heads, int num_kv_heads, int max_seq_len, int window, int sinks, float scale,
+                      void* out, int64_t o_s0, int64_t o_s1, void* workspace, size_t workspace_bytes) {
+    clear_error();
+    SKV_CHECK(n >= 0 && n <= 65535 && max_seq_len >= 1, "decode_kv8: n=%d (up to 65535) max_seq_len=%d", n, max_seq_len);
+    SKV_CHECK(window >= 0 && sinks >= 0, "decode_kv8: window=%d sinks=%d", window, sinks);
+    if (n == 0) return STARKV_OK;
+    SKV_CHECK(query && k_codes && v_codes && exponents && block_table && seq_lens && out && workspace, "decode_kv8: null pointer");
+    SKV_CHECK(num_kv_heads >= 1 && num_heads >= num_kv_heads && num_heads % num_kv_heads == 0 &&
+                  num_heads / num_kv_heads <= D8_MAX_GROUP,
+              "decode_kv8: %d query heads over %d KV heads (1 to 16 each)", num_heads, num_kv_heads);
+    SKV_CHECK(dtype == STARKV_BF16 || dtype == STARKV_F16, "decode_kv8: queries must be bf16 or fp16");
+    SKV_CHECK(code_type == STARKV_I8 || code_type == STARKV_E4M3, "decode_kv8: codes must be int8 or e4m3");
+    SKV_CHECK(c8_block_shift(block_size) >= 0, "decode_kv8: block_size must be 16 times a power of two, at most %d", C8_MAX_BLOCK);
+    SKV_CHECK(num_blocks >= 1 && num_blocks <= 0x7fffffff && bt_width >= 1, "decode_kv8: empty cache or block table");
+    SKV_CHECK(((uintptr_t)query | (uintptr_t)k_codes | (uintptr_t)v_codes) % 16 == 0 && (q_s0 | q_s1) % 8 == 0 &&
+                  (c_s0 | c_s1 | c_s2) % 16 == 0 && (uintptr_t)workspace % 16 == 0,
+              "decode_kv8: rows must be 16-byte aligned");
+    const size_t need = starkv_decode_kv8_workspace_bytes(n, num_heads, num_kv_heads, max_seq_len, window, sinks);
+    SKV_CHECK(workspace_bytes >= need, "decode_kv8: workspace %zu bytes < %zu", workspace_bytes, need);
+    Decode8Params p;
+    p.q = (const uint16_t*)query; p.q_s0 = q_s0; p.q_s1 = q_s1;
+    p.kc = (const uint8_t*)k_codes; p.vc = (const uint8_t*)v_codes;
+    p.c_s0 = c_s0; p.c_s1 = c_s1; p.c_s2 = c_s2;
+    p.ex = exponents; p.x_s0 = x_s0; p.x_s1 = x_s1;
+    p.bs_shift = c8_block_shift(block_size) - 4; p.num_blocks = num_blocks;
+    p.bt = block_table; p.bt_s0 = bt_s0; p.bt_s1 = bt_s1;
+    p.seq_lens = seq_lens;
+    p.span = (int)std::min<int64_t>({(int64_t)bt_width * block_size, 0x7ffffff0, (int64_t)max_seq_len});
+    p.n = n; p.Hkv = num_kv_heads; p.G = num_heads / num_kv_heads;
+    p.splits = decode8_splits(n, num_kv_heads, max_seq_len, window, sinks);
+    p.window = window; p.sinks = sinks;
+    p.sc = scale * 1.4426950408889634f;
+    p.part = (float*)workspace;
+    p.out = (uint16_t*)out; p.o_s0 = o_s0; p.o_s1 = o_s1;
+    SKV_CHECK((int64_t)n * num_kv_heads * p.splits < 1 << 23, "decode_kv8: %d requests of %d KV heads in one call", n, num_kv_heads);
+    const bool bf = dtype == STARKV_BF16;
+    const void* fn = code_type == STARKV_I8 ? bf ? decode_pick<STARKV_I8, STARKV_BF16>(p.G) : decode_pick<STARKV_I8, STARKV_F16>(p.G)
+                                            : bf ? decode_pick<STARKV_E4M3, STARKV_BF16>(p.G) : decode_pick<STARKV_E4M3, STARKV_F16>(p.G);
+    void* args[] = {(void*)&p};
+    SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)((int64_t)n * num_kv_heads * p.splits)), dim3(D8_THR), args,
+                            (size_t)4 * p.G * D8_PART * 4, (hipStream_t)stream));
+    if (p.splits == 1) return STARKV_OK;
+    if (bf)
+        hipLaunchKernelGGL(merge8_kernel<STARKV_BF16>, dim3(num_heads, n), dim3(64), 0, (hipStream_t)stream, p);
+    else
+        hipLaunchKernelGGL(merge8_kernel<STARKV_F16>, dim3(num_heads, n), dim3(64), 0, (hipStream_t)stream, p);
+    SKV_HIP(hipGetLastError());
+    return STARKV_OK;
+}
+
+}  // extern "C"

@@ -2,7 +2,7 @@
 //
 // starkv_weighted_decode is a paged decode over a request's whole cache that also sums up what each
 // cached token weighs: weights[b, h, t] += sum_g softmax_g(t) over the G query heads of KV head h (the
-// newest token's entry starts there: it is set). attend_kernel<.., false> (paged_attend.hpp) leaves every
+// newest token's entry starts there: it is set). attend_kernel<.., AT_SCORES, ..> (paged_attend.hpp) leaves every
 // score behind (4 bytes a query head and token beside 512 bytes of keys and values), weigh_kernel turns
 // them into weights once the splits' references and sums are known, and joins the splits' outputs. A
 // token's entry belongs to one thread, which sums the heads in order: no atomics, the same bits every run.
@@ -317,7 +317,7 @@ int starkv_weighted_decode(void* stream, const void* query, int64_t q_s0, int64_
     p.part = (float*)((char*)workspace + weighted_logits_bytes(n, num_heads, max_seq_len));
     wp.w = weights; wp.w_s0 = w_s0; wp.w_s1 = w_s1;
     wp.chunks = (p.span + WG_TOKENS - 1) / WG_TOKENS;
-    const int err = attend_launch<false>(stream, dtype, p);
+    const int err = attend_launch<AT_SCORES>(stream, dtype, p);
     if (err != STARKV_OK) return err;
     const dim3 grid(wp.chunks + (p.splits > 1 ? (p.G + 3) / 4 : 0), num_kv_heads, n);
     if (dtype == STARKV_BF16)

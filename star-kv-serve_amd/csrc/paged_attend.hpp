@@ -1,6 +1,6 @@
 // One token's attention over pages of an uncompressed paged cache, on matrix instructions: the body
-// that the decode over selected blocks (sparse_decode.hip) and the decode that weighs its tokens
-// (evict.hip) share.
+// that the decode over selected blocks (sparse_decode.hip), the decode that weighs its tokens
+// (evict.hip) and the one through a window (window_decode.hip) share.
 //
 // For a request b, a KV head h and its G <= 16 query heads: s_g(t) = scale log2(e) q_g . k_t over the
 // tokens t of the unit's pages, p = 2^(s - m), out_g = sum p v / sum p. A page is 16 tokens of one
@@ -45,6 +45,7 @@
 #include <algorithm>
 
 #include "common.hpp"
+#include "window_pages.hpp"
 
 namespace starkv {
 
@@ -60,6 +61,10 @@ template <int DT>
 constexpr float AT_DOWN = DT == STARKV_BF16 ? 0x1p-40f : 1.f;
 constexpr float AT_LEAST = -3.402823466e38f;  // the reference of tokens whose scores are all -inf
 
+// Which pages a unit has: all of its request, with the scores left behind; those of selected blocks; those seen
+// through a window.
+enum { AT_SCORES, AT_SPARSE, AT_WINDOW };
+
 struct AttendParams {
     const uint16_t* q; int64_t q_s0, q_s1;                               // elements, as all strides here
     const uint16_t* kc; const uint16_t* vc; int64_t c_s0, c_s1, c_s2;
@@ -69,7 +74,8 @@ struct AttendParams {
     int n, Hkv, G, splits, pps;                                          // pps: pages per split
     float sc;                                                            // scale * log2(e)
     const int32_t* sel; int64_t sel_s0, sel_s1; int keep;                // SPARSE: logical blocks [n][Hkv][keep]
-    float* lg; int64_t lg_row;                                           // else: scores [n][Hkv][page][G][16], lg_row a unit
+    float* lg; int64_t lg_row;                                           // SCORES: [n][Hkv][page][G][16], lg_row a unit
+    int window, sinks;                                                   // WINDOW
     float* part;                                                         // [n][H][splits][AT_PART]
     uint16_t* out; int64_t o_s0, o_s1;
 };
@@ -142,18 +148,23 @@ __device__ __forceinline__ uint4 attend_column(const uint4 (&v)[2][4], int i) {
 
 // The workgroup's unit: (request, KV head, split) from the block index.
 // MANY: 9 to 16 query heads.
-template <int DT, bool SPARSE, bool MANY>
-__global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const AttendParams p) {
+template <int DT, int MODE, bool MANY>
+__global__ __launch_bounds__(AT_THR, MODE == AT_SPARSE ? 4 : 3) void attend_kernel(const AttendParams p) {
     __shared__ int2 s_page[AT_CHUNK];           // a page's block, and its tokens | its place in the block << 8
     extern __shared__ float s_dyn[];            // [4 waves][G][AT_PART] for the merge
     __shared__ int s_odd;                       // a wave's sums are not finite
+    __shared__ uint32_t s_seen[MODE == AT_WINDOW ? AT_CHUNK : 1];  // a page's places that are seen
+    constexpr bool SPARSE = MODE == AT_SPARSE, WINDOW = MODE == AT_WINDOW;
     const int id = blockIdx.x, s = id % p.splits, u = id / p.splits, h = u % p.Hkv, b = u / p.Hkv;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = MANY ? lane & 15 : lane & 7, quad = lane >> 4;  // the lane's query head
     const int H = p.Hkv * p.G;
     const int L = attend_length(p, b);
-    const int pages = SPARSE ? p.keep << p.bs_shift : (L + 15) >> 4;
-    const int k0 = min(s * p.pps, pages), k1 = min(k0 + p.pps, pages);
+    const SeenPages seen = seen_pages(L, WINDOW ? p.window : 0, WINDOW ? p.sinks : 0);
+    const int pages = SPARSE ? p.keep << p.bs_shift : seen.pages;
+    // Through a window a request's pages are shared out evenly, eight a split at least: a span may be far longer.
+    const int pps = WINDOW ? max((pages + p.splits - 1) / p.splits, 8) : p.pps;
+    const int k0 = min(s * pps, pages), k1 = min(k0 + pps, pages);
     const int mask = (1 << p.bs_shift) - 1, blocks = (((L + 15) >> 4) + mask) >> p.bs_shift;
 
     uint4 qf[4];
@@ -174,7 +185,7 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
             const int count = min(AT_CHUNK, k1 - c0);
             if (c0 != k0) __syncthreads();
             for (int i = tid; i < count; i += AT_THR) {
-                const int pg = c0 + i;
+                const int pg = WINDOW ? seen.page(c0 + i) : c0 + i;
                 const int lb = SPARSE ? p.sel[b * p.sel_s0 + h * p.sel_s1 + (pg >> p.bs_shift)] : pg >> p.bs_shift;
                 int blk = 0, tokens = 0;
                 if (lb >= 0 && lb < blocks) {
@@ -183,20 +194,23 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
                     if (blk < 0 || blk >= p.num_blocks) blk = tokens = 0;  // no block of the cache: no tokens
                 }
                 s_page[i] = make_int2(blk, tokens | (pg & mask) << 8);
+                if constexpr (WINDOW) s_seen[i] = seen.mask(pg);
             }
             __syncthreads();
             for (int i = 2 * wave; i < count; i += 8) {
                 int2 e[2];
                 int nt[2];
+                uint32_t see[2];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
                     const int2 v = s_page[min(i + x, count - 1)];
                     e[x].x = __builtin_amdgcn_readfirstlane(v.x);
                     e[x].y = __builtin_amdgcn_readfirstlane(v.y);
                     nt[x] = i + x < count ? e[x].y & 255 : 0;
+                    if constexpr (WINDOW) see[x] = nt[x] ? __builtin_amdgcn_readfirstlane(s_seen[min(i + x, count - 1)]) : 0u;
                 }
                 float* lg = p.lg + ((int64_t)b * p.Hkv + h) * p.lg_row + (int64_t)(c0 + i) * p.G * 16;  // page i's scores
-                if (SPARSE && nt[0] + nt[1] == 0) continue;
+                if (MODE != AT_SCORES && nt[0] + nt[1] == 0) continue;
                 const bool own = col < p.G && (MANY || !(lane & 8));
                 uint4 kr[2][4], vr[2][4];
 #pragma unroll
@@ -222,16 +236,16 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
                     for (int st = 0; st < 4; ++st) d = attend_mfma<DT>(kr[x][st], qf[st], d);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) sv[x][r] = d[r] * p.sc;
-                    if (nt[x] < 16) {  // tokens past the end: no score, and no value that a weight of 0 could turn into NaN
+                    if (WINDOW ? see[x] != 0xffffu : nt[x] < 16) {  // tokens past the end or out of sight: no score, and no value that a weight of 0 could turn into NaN
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const bool ok = 4 * quad + r < nt[x];
+                            const bool ok = WINDOW ? see[x] >> (4 * quad + r) & 1u : 4 * quad + r < nt[x];
                             sv[x][r] = ok ? sv[x][r] : -INFINITY;
                             vr[x][r] = ok ? vr[x][r] : make_uint4(0, 0, 0, 0);
                         }
                     }
                 }
-                if (!SPARSE && own) {
+                if (MODE == AT_SCORES && own) {
                     *(float4*)(lg + 16 * col + 4 * quad) = make_float4(sv[0][0], sv[0][1], sv[0][2], sv[0][3]);
                     if (i + 1 < count) *(float4*)(lg + 16 * p.G + 16 * col + 4 * quad) = make_float4(sv[1][0], sv[1][1], sv[1][2], sv[1][3]);
                 }
@@ -253,7 +267,8 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        pe[x][r] = 4 * quad + r < nt[x] ? exp2f(sv[x][r] - m) * AT_DOWN<DT> : 0.f;
+                        const bool ok = WINDOW ? see[x] >> (4 * quad + r) & 1u : 4 * quad + r < nt[x];
+                        pe[x][r] = ok ? exp2f(sv[x][r] - m) * AT_DOWN<DT> : 0.f;
                         l += pe[x][r];
                     }
                 if (__builtin_expect(careful, 0)) {
@@ -339,7 +354,7 @@ __global__ __launch_bounds__(AT_THR, SPARSE ? 4 : 3) void attend_kernel(const At
         }
         const int hq = h * p.G + g;
         if (p.splits == 1) store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, DT, M == -INFINITY ? 0.f : a / lt);
-        if (p.splits > 1 || !SPARSE) {
+        if (p.splits > 1 || MODE == AT_SCORES) {
             float* pp = p.part + (((int64_t)b * H + hq) * p.splits + s) * AT_PART;
             if (d == 0) *(float4*)pp = make_float4(M, lt, 0.f, 0.f);
             pp[4 + d] = a;
@@ -434,16 +449,16 @@ inline int attend_setup(AttendParams& p, const char* what, const void* query, in
     return STARKV_OK;
 }
 
-template <bool SPARSE>
+template <int MODE>
 inline int attend_launch(void* stream, int dtype, const AttendParams& p) {
     SKV_CHECK((int64_t)p.n * p.Hkv * p.splits < 1 << 23, "%d requests of %d KV heads in one call", p.n, p.Hkv);
     const dim3 grid((unsigned)((int64_t)p.n * p.Hkv * p.splits));
     const size_t lds = (size_t)4 * p.G * AT_PART * 4;
     const bool bf = dtype == STARKV_BF16;
-    const void* fn = p.G <= 8 ? bf ? (const void*)&attend_kernel<STARKV_BF16, SPARSE, false>
-                                   : (const void*)&attend_kernel<STARKV_F16, SPARSE, false>
-                              : bf ? (const void*)&attend_kernel<STARKV_BF16, SPARSE, true>
-                                   : (const void*)&attend_kernel<STARKV_F16, SPARSE, true>;
+    const void* fn = p.G <= 8 ? bf ? (const void*)&attend_kernel<STARKV_BF16, MODE, false>
+                                   : (const void*)&attend_kernel<STARKV_F16, MODE, false>
+                              : bf ? (const void*)&attend_kernel<STARKV_BF16, MODE, true>
+                                   : (const void*)&attend_kernel<STARKV_F16, MODE, true>;
     void* args[] = {(void*)&p};
     SKV_HIP(hipLaunchKernel(fn, grid, dim3(AT_THR), args, lds, (hipStream_t)stream));
     return STARKV_OK;

@@ -34,6 +34,12 @@
 // other, a swizzle whose V reads met in one bank quarter, and heads spread over the XCDs took
 // 3214 us there against 2237 now, on one box; 4096 tokens 291 against 158, 2048 tokens 82 against 53.
 // At the end the two halves of each query's sum are added and O / l is written.
+//
+// Through a window (prefill_kernel<.., true>, starkv_prefill_window) token t sees place s <= t where t - s < window or
+// s < sinks: a workgroup takes the tiles that hold the first tokens and those from its first query's window on, and
+// tiles across an edge are masked (its later waves mask up to two whole ones). The scale goes onto
+// the fp32 scores there (one fused multiply-add in front of the exponential in place of a subtraction) and not into q, whose
+// fp16 values are then those of bf16 and fp16 queries themselves.
 #include <algorithm>
 #include <array>
 #include <type_traits>
@@ -64,6 +70,7 @@ struct PrefillParams {
     int Hq, G;
     float sc;                                                 // scale * log2(e)
     void* out; int64_t o_s0, o_s1; int out_dt;                // elements
+    int window, sinks;
 };
 
 // A row's granules (16 bytes, 16 a row) lie XOR-swizzled by its low 4 bits, their two halves
@@ -76,9 +83,9 @@ __device__ __forceinline__ int pf_swz(int row) { return ((row & 3) << 2) | ((row
 // Physical byte of (row, granule g) in a K or V tile.
 __device__ __forceinline__ uint32_t pf_addr(int row, int g) { return (uint32_t)(row * 256 + ((g ^ pf_swz(row)) << 4)); }
 
-// 8 query dimensions times scale * log2(e), as fp16 (zeros past the prompt).
+// 8 query dimensions times `by`, as fp16 (zeros past the prompt).
 template <int QDT>
-__device__ __forceinline__ half8_t pf_load_q(const PrefillParams& p, int64_t tok, int hq, int d0, bool ok) {
+__device__ __forceinline__ half8_t pf_load_q(const PrefillParams& p, int64_t tok, int hq, int d0, bool ok, float by) {
     half8_t r;
     if (!ok) {
 #pragma unroll
@@ -104,7 +111,7 @@ __device__ __forceinline__ half8_t pf_load_q(const PrefillParams& p, int64_t tok
         for (int e = 0; e < 8; ++e) f[e] = ((const float*)p.q)[off + e];
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) r[e] = (_Float16)(f[e] * p.sc);
+    for (int e = 0; e < 8; ++e) r[e] = (_Float16)(f[e] * by);
     return r;
 }
 
@@ -132,7 +139,7 @@ __device__ __forceinline__ void pf_work(const PrefillParams& p, int& entry, int&
     }
 }
 
-template <int QDT, int ODT>
+template <int QDT, int ODT, bool WINDOW>
 __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) void prefill_kernel(const PrefillParams p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t s_kv[];  // K tiles 0, 1, V tiles 0, 1
     const int tid = threadIdx.x, lane = tid & 63, wave = rfl(tid >> 6);
@@ -148,8 +155,14 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
     const int nq = min(32, L - qw);         // its rows (<= 0: none)
     const int qi = qw + n;                  // this lane's query
     const int kend = min(L, q0 + PF_QB);    // keys the workgroup needs: [0, kend)
-    const int ntile = (kend + PF_KT - 1) / PF_KT;
-    const int last = nq > 0 ? (qw + nq - 1) / PF_KT : -1;  // the wave's last tile with a visible key
+    // Tiles of keys: all up to kend; through a window the first tokens' (tiles below `first`) and those from `second` on.
+    const int qlo = WINDOW ? max(q0 - p.window + 1, 0) : 0;
+    const int first = WINDOW ? (min(p.sinks, qlo) + PF_KT - 1) / PF_KT : 0, second = WINDOW ? max(qlo / PF_KT, first) : 0;
+    const int ntile = first + (kend + PF_KT - 1) / PF_KT - second;
+    const auto tile_of = [&](int i) { return !WINDOW || i < first ? i : i - first + second; };
+    const int last = nq > 0 ? (qw + nq - 1) / PF_KT - second + first : -1;  // the wave's last tile with a visible key
+    // The factors of q (a scale's sign, or 0) and of the scores (not 0: a masked score is -inf).
+    const float sq = WINDOW ? (float)((p.sc > 0.f) - (p.sc < 0.f)) : p.sc, ss = WINDOW && p.sc != 0.f ? fabsf(p.sc) : 1.f;
 
     // Copies: a K or V tile is 16 KB, 16 copies of 1 KB, PF_CPW per wave. Copy c of wave w moves
     // LDS bytes [1024 (PF_WAVES c + w), + 1024): rows 4 (PF_WAVES c + w) .. + 3; lane j writes
@@ -164,7 +177,7 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
     const int64_t kv0 = (int64_t)s * p.kv_s0 + (int64_t)hk * p.kv_s1;
     // Tile t of K (or V) into its buffer at LDS address dst.
     auto issue = [&](const uint8_t* src, int t, uint32_t dst) {
-        const int r0 = t * PF_KT;
+        const int r0 = tile_of(t) * PF_KT;
         const int rows = max(0, min(PF_KT, L - r0));
         int4v_t rs = buffer_rsrc(src + kv0 + (int64_t)r0 * p.kv_s0, (int)(rows * p.kv_s0));
 #pragma unroll
@@ -177,7 +190,7 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
     // Q as the B operand of S^T = K Q^T: query n, dimensions 16 ks + 8 h .. + 7.
     half8_t qb[8];
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) qb[ks] = pf_load_q<QDT>(p, (int64_t)s + qi, hq, 16 * ks + 8 * h, qi < L);
+    for (int ks = 0; ks < 8; ++ks) qb[ks] = pf_load_q<QDT>(p, (int64_t)s + qi, hq, 16 * ks + 8 * h, qi < L, sq);
 
     // Per-lane LDS addresses of buffer 0; the other buffer and the row blocks are immediates.
     // A of S^T: key row 32 mb + n, granule 2 ks + h (block mb = 1 is 32 rows further: the same
@@ -217,7 +230,7 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
     // Tile t, its scores in sc, its V in buffer B; the next tile's scores (NEXT, into nx) are formed
     // beside the exponentials: matrix and vector work of one wave with no dependence between them.
     auto tile = [&](auto B, int t, f32x16_t* sc, f32x16_t* nx) {
-        const int k0 = t * PF_KT;
+        const int k0 = tile_of(t) * PF_KT;
         // Scores of this lane's query (already scaled through q): key k0 + 32 mb + 8 (r / 4) +
         // 4 h + r % 4. Only a tile that reaches past the wave's first query or the prompt's
         // end needs the causal / end mask.
@@ -229,6 +242,16 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
                 for (int r = 0; r < 16; ++r)
                     if (32 * mb + 8 * (r >> 2) + (r & 3) > lim) sc[mb][r] = -INFINITY;
         }
+        if (WINDOW && k0 < qw + 32 - p.window && k0 + PF_KT > p.sinks) {  // keys before a query's window, not among the first
+            const int lo = qi - p.window - k0 - 4 * h, head = p.sinks - k0 - 4 * h;
+#pragma unroll
+            for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int c = 32 * mb + 8 * (r >> 2) + (r & 3);
+                    if (c <= lo && c >= head) sc[mb][r] = -INFINITY;
+                }
+        }
         float mx = -INFINITY;
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb)
@@ -236,7 +259,7 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
             for (int r = 0; r < 16; ++r) mx = fmaxf(mx, sc[mb][r]);
         {  // with the partner lane's half: x[0] holds lane l % 32's value, x[1] lane 32 + l % 32's
             const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-            mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+            mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])) * ss;
         }
         if (__builtin_amdgcn_ballot_w64(mx > m + PF_LAZY) != 0) {
             const float mn = fmaxf(m, mx);
@@ -256,7 +279,8 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
         for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(sc[mb][r] - mr), e1 = __builtin_amdgcn_exp2f(sc[mb][r + 1] - mr);
+                const float e0 = __builtin_amdgcn_exp2f(WINDOW ? fmaf(sc[mb][r], ss, -mr) : sc[mb][r] - mr);
+                const float e1 = __builtin_amdgcn_exp2f(WINDOW ? fmaf(sc[mb][r + 1], ss, -mr) : sc[mb][r + 1] - mr);
                 l += e0;
                 l += e1;
                 const half2_t hh = cvt_h2(e0, e1);
@@ -373,11 +397,18 @@ __global__ __launch_bounds__(256) void to_half_kernel(const ToHalfParams p) {
     }
 }
 
-template <int QDT>
+template <int QDT, bool WINDOW>
 const void* pf_pick(int odt) {
-    if (odt == STARKV_F32) return (const void*)&prefill_kernel<QDT, STARKV_F32>;
-    if (odt == STARKV_F16) return (const void*)&prefill_kernel<QDT, STARKV_F16>;
-    return (const void*)&prefill_kernel<QDT, STARKV_BF16>;
+    if (odt == STARKV_F32) return (const void*)&prefill_kernel<QDT, STARKV_F32, WINDOW>;
+    if (odt == STARKV_F16) return (const void*)&prefill_kernel<QDT, STARKV_F16, WINDOW>;
+    return (const void*)&prefill_kernel<QDT, STARKV_BF16, WINDOW>;
+}
+
+template <bool WINDOW>
+const void* pf_pick(int qdt, int odt) {
+    return qdt == STARKV_F32 ? pf_pick<STARKV_F32, WINDOW>(odt)
+           : qdt == STARKV_F16 ? pf_pick<STARKV_F16, WINDOW>(odt)
+                               : pf_pick<STARKV_BF16, WINDOW>(odt);
 }
 
 }  // namespace
@@ -410,11 +441,12 @@ int starkv_prefill_block_list(const int32_t* cu_seqlens, int num_prompts, int32_
     return (int)all.size();
 }
 
-int starkv_prefill_attention(void* stream, const void* query, int64_t q_s0, int64_t q_s1, int q_dtype,
-                             const void* key, const void* value, int64_t kv_s0, int64_t kv_s1, int kv_dtype,
-                             const int32_t* cu_seqlens, const int32_t* blocks, int num_blocks, int num_heads,
-                             int num_kv_heads, int head_size, float scale, void* out, int64_t o_s0, int64_t o_s1,
-                             int out_dtype) {
+// window 0: every key up to the query.
+static int prefill_call(void* stream, const void* query, int64_t q_s0, int64_t q_s1, int q_dtype,
+                        const void* key, const void* value, int64_t kv_s0, int64_t kv_s1, int kv_dtype,
+                        const int32_t* cu_seqlens, const int32_t* blocks, int num_blocks, int num_heads,
+                        int num_kv_heads, int head_size, int window, int sinks, float scale, void* out, int64_t o_s0, int64_t o_s1,
+                        int out_dtype) {
     clear_error();
     SKV_CHECK(num_blocks >= 0, "prefill: num_blocks=%d", num_blocks);
     if (num_blocks == 0) return STARKV_OK;
@@ -440,21 +472,39 @@ int starkv_prefill_attention(void* stream, const void* query, int64_t q_s0, int6
     p.Hq = num_heads; p.G = num_heads / num_kv_heads;
     p.sc = scale * 1.4426950408889634f;
     p.out = out; p.o_s0 = o_s0; p.o_s1 = o_s1; p.out_dt = out_dtype;
-    const void* fn = q_dtype == STARKV_F32 ? pf_pick<STARKV_F32>(out_dtype)
-                     : q_dtype == STARKV_F16 ? pf_pick<STARKV_F16>(out_dtype)
-                                             : pf_pick<STARKV_BF16>(out_dtype);
+    p.window = window; p.sinks = sinks;
+    const void* fn = window > 0 ? pf_pick<true>(q_dtype, out_dtype) : pf_pick<false>(q_dtype, out_dtype);
     const int lds = PF_LDS;
-    static const void* raised[16];
+    static const void* raised[32];
     static int nraised = 0;
     bool seen = false;
     for (int i = 0; i < nraised; ++i) seen = seen || raised[i] == fn;
     if (!seen) {
         SKV_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-        if (nraised < 16) raised[nraised++] = fn;
+        if (nraised < 32) raised[nraised++] = fn;
     }
     void* args[] = {(void*)&p};
     SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)(num_blocks * num_heads)), dim3(PF_THR), args, (size_t)lds, (hipStream_t)stream));
     return STARKV_OK;
+}
+
+int starkv_prefill_attention(void* stream, const void* query, int64_t q_s0, int64_t q_s1, int q_dtype,
+                             const void* key, const void* value, int64_t kv_s0, int64_t kv_s1, int kv_dtype,
+                             const int32_t* cu_seqlens, const int32_t* blocks, int num_blocks, int num_heads,
+                             int num_kv_heads, int head_size, float scale, void* out, int64_t o_s0, int64_t o_s1,
+                             int out_dtype) {
+    return prefill_call(stream, query, q_s0, q_s1, q_dtype, key, value, kv_s0, kv_s1, kv_dtype, cu_seqlens, blocks,
+                        num_blocks, num_heads, num_kv_heads, head_size, 0, 0, scale, out, o_s0, o_s1, out_dtype);
+}
+
+int starkv_prefill_window(void* stream, const void* query, int64_t q_s0, int64_t q_s1, int q_dtype, const void* key,
+                          const void* value, int64_t kv_s0, int64_t kv_s1, int kv_dtype, const int32_t* cu_seqlens,
+                          const int32_t* blocks, int num_blocks, int num_heads, int num_kv_heads, int head_size,
+                          int window, int sinks, float scale, void* out, int64_t o_s0, int64_t o_s1, int out_dtype) {
+    clear_error();
+    SKV_CHECK(window >= 1 && sinks >= 0, "prefill_window: window=%d sinks=%d", window, sinks);
+    return prefill_call(stream, query, q_s0, q_s1, q_dtype, key, value, kv_s0, kv_s1, kv_dtype, cu_seqlens, blocks,
+                        num_blocks, num_heads, num_kv_heads, head_size, window, sinks, scale, out, o_s0, o_s1, out_dtype);
 }
 
 int starkv_prefill_to_half(void* stream, const void* key, int64_t k_s0, int64_t k_s1, void* key_out, const void* value,

@@ -7,7 +7,7 @@
 //     score = sum_g sum_d max(q_gd lo_d, q_gd hi_d) = sum_d (sum_g max(q_gd, 0)) hi_d + (sum_g min(q_gd, 0)) lo_d:
 // one product of 256 terms a block, whatever G. score_kernel forms it, select_kernel keeps the blocks of
 // the largest scores (topk_select.hpp) between the first `sink` and the last `recent` ones, and
-// attend_kernel<.., true> (paged_attend.hpp) attends to their tokens.
+// attend_kernel<.., AT_SPARSE, ..> (paged_attend.hpp) attends to their tokens.
 //
 // Scores are summed in 64 bits and rounded once to fp32: a choice must not change with the order of a
 // sum (a block that one order puts first and another second changes the output by its whole weight).
@@ -346,7 +346,7 @@ int starkv_sparse_decode(void* stream, const void* query, int64_t q_s0, int64_t 
     p.splits = sparse_splits(n, num_kv_heads, pages);
     p.pps = (pages + p.splits - 1) / p.splits;
     p.part = (float*)workspace;
-    const int err = attend_launch<true>(stream, dtype, p);
+    const int err = attend_launch<AT_SPARSE>(stream, dtype, p);
     if (err != STARKV_OK || p.splits == 1) return err;
     if (dtype == STARKV_BF16)
         hipLaunchKernelGGL(attend_merge_kernel<STARKV_BF16>, dim3(num_heads, n), dim3(64), 0, (hipStream_t)stream, p);

@@ -238,6 +238,21 @@ void prefill(const at::Tensor& query, const at::Tensor& key, const at::Tensor& v
           "prefill");
 }
 
+// The same through a window.
+void prefill_window(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, const at::Tensor& cu_seqlens,
+                    const at::Tensor& blocks, int64_t window, int64_t sinks, double scale, const at::Tensor& out) {
+    const c10::DeviceGuard guard(query.device());
+    TORCH_CHECK(key.strides() == value.strides(), "starkv.prefill_window: K and V must share strides");
+    TORCH_CHECK(blocks.dim() == 2 && blocks.size(1) == 2, "starkv.prefill_window: blocks must be [num_blocks, 2]");
+    for (const int64_t v : {window, sinks}) TORCH_CHECK(v >= 0 && v <= INT32_MAX, "starkv.prefill_window: window ", window, ", sinks ", sinks);
+    check(starkv_prefill_window(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), dtype_code(query),
+                                key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), dtype_code(key),
+                                i32(cu_seqlens, "cu_seqlens"), i32(blocks, "blocks"), (int)blocks.size(0),
+                                (int)query.size(1), (int)key.size(1), (int)query.size(2), (int)window, (int)sinks,
+                                (float)scale, out.data_ptr(), out.stride(0), out.stride(1), dtype_code(out)),
+          "prefill_window");
+}
+
 // K and V [T, H, 128] of one dtype (bf16 or fp32) as contiguous fp16.
 void prefill_to_half(const at::Tensor& key, const at::Tensor& value, const at::Tensor& key_out,
                      const at::Tensor& value_out) {
@@ -528,6 +543,110 @@ void evict(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tenso
           "evict");
 }
 
+// One token's attention over a 16-bit cache through a window.
+void window_decode(const at::Tensor& query, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                   const at::Tensor& block_table, const at::Tensor& seq_lens, int64_t max_seq_len, int64_t window,
+                   int64_t sinks, double scale, const at::Tensor& out) {
+    const c10::DeviceGuard guard(query.device());
+    const int64_t n = query.size(0);
+    check_caches(k_cache, v_cache, "window_decode");
+    const int H = (int)query.size(1), Hkv = (int)k_cache.size(2);
+    check_query(query, k_cache, Hkv, "window_decode");
+    check_query(out, k_cache, Hkv, "window_decode");
+    check_table(block_table, seq_lens, n, "window_decode");
+    TORCH_CHECK(out.sizes() == query.sizes(), "starkv.window_decode: out as query");
+    at::assert_no_internal_overlap(out);
+    const int span = as_int(max_seq_len, "max_seq_len"), w = as_int(window, "window"), s = as_int(sinks, "sinks");
+    const at::Tensor ws = workspace(query, starkv_window_decode_workspace_bytes((int)n, H, Hkv, span, w, s));
+    check(starkv_window_decode(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), k_cache.data_ptr(),
+                               v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+                               dtype_code(k_cache), (int)k_cache.size(1), k_cache.size(0), i32(block_table, "block_table"),
+                               block_table.stride(0), block_table.stride(1), (int)block_table.size(1),
+                               i32(seq_lens, "seq_lens"), (int)n, H, Hkv, span, w, s, (float)scale, out.data_ptr(),
+                               out.stride(0), out.stride(1), ws.data_ptr(), (size_t)ws.numel()),
+          "window_decode");
+}
+
+// An 8-bit cache's codes [blocks, block_size, heads, 128] and exponents [blocks, heads, 2]; its code type.
+int check_cache8(const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& exponents, const char* what) {
+    check_caches(k_codes, v_codes, what);
+    TORCH_CHECK(exponents.scalar_type() == at::kChar && exponents.dim() == 3 && exponents.size(0) == k_codes.size(0) &&
+                    exponents.size(1) == k_codes.size(2) && exponents.size(2) == 2 && exponents.stride(2) == 1,
+                "starkv.", what, ": exponents [blocks, heads, 2] int8");
+    if (k_codes.scalar_type() == at::kChar) return STARKV_I8;
+    TORCH_CHECK(k_codes.scalar_type() == at::kFloat8_e4m3fn, "starkv.", what, ": codes of int8 or float8_e4m3fn");
+    return STARKV_E4M3;
+}
+
+int slots_of(const at::Tensor& slots, int64_t n, const char* what) {
+    TORCH_CHECK(slots.dim() == 1 && slots.size(0) == n, "starkv.", what, ": slots [n]");
+    return slot_bits(slots);
+}
+
+// A step's keys and values into an 8-bit cache.
+void write_kv8(const at::Tensor& key, const at::Tensor& value, const at::Tensor& k_codes, const at::Tensor& v_codes,
+               const at::Tensor& exponents, const at::Tensor& slots) {
+    const c10::DeviceGuard guard(key.device());
+    const int code = check_cache8(k_codes, v_codes, exponents, "write_kv8");
+    const int64_t n = key.dim() == 3 ? key.size(0) : -1, H = k_codes.size(2);
+    for (const auto* t : {&key, &value})
+        TORCH_CHECK(t->dim() == 3 && t->size(0) == n && t->size(1) == H && t->size(2) == 128 && t->stride(2) == 1 &&
+                        t->scalar_type() == key.scalar_type(),
+                    "starkv.write_kv8: key and value [n, heads, 128] of one dtype");
+    const int bits = slots_of(slots, n, "write_kv8"), tokens = as_int(n, "tokens");
+    for (const auto* t : {&k_codes, &v_codes, &exponents}) at::assert_no_internal_overlap(*t);
+    at::assert_no_overlap(k_codes, v_codes);
+    const at::Tensor ws = workspace(key, starkv_write_kv8_workspace_bytes(tokens, k_codes.size(0), (int)k_codes.size(1)));
+    check(starkv_write_kv8(stream_of(key), key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+                           value.stride(1), dtype_code(key), k_codes.data_ptr(), v_codes.data_ptr(), k_codes.stride(0),
+                           k_codes.stride(1), k_codes.stride(2), code, exponents.data_ptr<int8_t>(), exponents.stride(0),
+                           exponents.stride(1), (int)k_codes.size(1), k_codes.size(0), slots.data_ptr(), bits, tokens,
+                           (int)H, ws.data_ptr(), (size_t)ws.numel()),
+          "write_kv8");
+}
+
+// Rows of an 8-bit cache back.
+void read_kv8(const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& exponents, const at::Tensor& slots,
+              const at::Tensor& key_out, const at::Tensor& value_out) {
+    const c10::DeviceGuard guard(k_codes.device());
+    const int code = check_cache8(k_codes, v_codes, exponents, "read_kv8");
+    const int64_t n = slots.dim() == 1 ? slots.size(0) : -1, H = k_codes.size(2);
+    for (const auto* t : {&key_out, &value_out})
+        TORCH_CHECK(t->dim() == 3 && t->size(0) == n && t->size(1) == H && t->size(2) == 128 && t->is_contiguous() &&
+                        t->scalar_type() == key_out.scalar_type(),
+                    "starkv.read_kv8: the results are contiguous [n, heads, 128] of one dtype");
+    check(starkv_read_kv8(stream_of(k_codes), k_codes.data_ptr(), v_codes.data_ptr(), k_codes.stride(0), k_codes.stride(1),
+                          k_codes.stride(2), code, exponents.data_ptr<int8_t>(), exponents.stride(0), exponents.stride(1),
+                          (int)k_codes.size(1), k_codes.size(0), slots.data_ptr(), slots_of(slots, n, "read_kv8"),
+                          as_int(n, "tokens"), (int)H, key_out.data_ptr(), value_out.data_ptr(), dtype_code(key_out)),
+          "read_kv8");
+}
+
+// One token's attention over an 8-bit cache; window 0: all tokens.
+void decode_kv8(const at::Tensor& query, const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& exponents,
+                const at::Tensor& block_table, const at::Tensor& seq_lens, int64_t max_seq_len, int64_t window,
+                int64_t sinks, double scale, const at::Tensor& out) {
+    const c10::DeviceGuard guard(query.device());
+    const int code = check_cache8(k_codes, v_codes, exponents, "decode_kv8");
+    const int64_t n = query.size(0);
+    const int H = (int)query.size(1), Hkv = (int)k_codes.size(2);
+    check_query(query, query, Hkv, "decode_kv8");
+    check_query(out, query, Hkv, "decode_kv8");
+    check_table(block_table, seq_lens, n, "decode_kv8");
+    TORCH_CHECK(out.sizes() == query.sizes(), "starkv.decode_kv8: out as query");
+    at::assert_no_internal_overlap(out);
+    const int span = as_int(max_seq_len, "max_seq_len"), w = as_int(window, "window"), s = as_int(sinks, "sinks");
+    const at::Tensor ws = workspace(query, starkv_decode_kv8_workspace_bytes((int)n, H, Hkv, span, w, s));
+    check(starkv_decode_kv8(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), dtype_code(query),
+                            k_codes.data_ptr(), v_codes.data_ptr(), k_codes.stride(0), k_codes.stride(1),
+                            k_codes.stride(2), code, exponents.data_ptr<int8_t>(), exponents.stride(0),
+                            exponents.stride(1), (int)k_codes.size(1), k_codes.size(0), i32(block_table, "block_table"),
+                            block_table.stride(0), block_table.stride(1), (int)block_table.size(1),
+                            i32(seq_lens, "seq_lens"), (int)n, H, Hkv, span, w, s, (float)scale, out.data_ptr(),
+                            out.stride(0), out.stride(1), ws.data_ptr(), (size_t)ws.numel()),
+          "decode_kv8");
+}
+
 // A decode step's slots (int64) and lengths (int32) from its positions (int64).
 void decode_slots(const at::Tensor& block_table, const at::Tensor& positions, int64_t block_size,
                   const at::Tensor& slots, const at::Tensor& seq_lens) {
@@ -631,6 +750,16 @@ TORCH_LIBRARY(starkv, m) {
           "int max_seq_len, float scale, Tensor(a!) weights, Tensor(b!) out) -> ()");
     m.def("evict(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor seq_lens, Tensor weights, "
           "int keep, int sink, int recent, Tensor(c!) new_lens, Tensor(d!) new_weights) -> ()");
+    m.def("window_decode(Tensor query, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, "
+          "int max_seq_len, int window, int sinks, float scale, Tensor(a!) out) -> ()");
+    m.def("prefill_window(Tensor query, Tensor key, Tensor value, Tensor cu_seqlens, Tensor blocks, int window, "
+          "int sinks, float scale, Tensor(a!) out) -> ()");
+    m.def("write_kv8(Tensor key, Tensor value, Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) exponents, "
+          "Tensor slots) -> ()");
+    m.def("read_kv8(Tensor k_codes, Tensor v_codes, Tensor exponents, Tensor slots, Tensor(a!) key_out, "
+          "Tensor(b!) value_out) -> ()");
+    m.def("decode_kv8(Tensor query, Tensor k_codes, Tensor v_codes, Tensor exponents, Tensor block_table, "
+          "Tensor seq_lens, int max_seq_len, int window, int sinks, float scale, Tensor(a!) out) -> ()");
     m.def("decode_slots(Tensor block_table, Tensor positions, int block_size, Tensor(a!) slots, "
           "Tensor(b!) seq_lens) -> ()");
     m.def("greedy_step(Tensor logits, Tensor(a!) tokens, Tensor(b!) positions) -> ()");
@@ -659,6 +788,11 @@ TORCH_LIBRARY_IMPL(starkv, CUDA, m) {
     m.impl("sparse_decode", &sparse_decode);
     m.impl("weighted_decode", &weighted_decode);
     m.impl("evict", &evict);
+    m.impl("window_decode", &window_decode);
+    m.impl("prefill_window", &prefill_window);
+    m.impl("write_kv8", &write_kv8);
+    m.impl("read_kv8", &read_kv8);
+    m.impl("decode_kv8", &decode_kv8);
     m.impl("decode_slots", &decode_slots);
     m.impl("greedy_step", &greedy_step);
     m.impl("silu_mul", &silu_mul);

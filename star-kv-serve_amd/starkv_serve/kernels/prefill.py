@@ -10,6 +10,7 @@ from typing import List, Optional
 import torch
 
 from starkv_serve import _hip
+from starkv_serve.kernels.window import Window, sizes
 
 
 def block_list(query_lens: List[int]) -> List[int]:
@@ -61,8 +62,10 @@ def prefill_lift(k_codes: torch.Tensor, v_codes: torch.Tensor, cu_seqlens: torch
 
 
 def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_lens: List[int], scale: float,
-                      out: Optional[torch.Tensor] = None, tables: Optional[tuple] = None) -> torch.Tensor:
-    """Causal attention of each prompt to itself.
+                      out: Optional[torch.Tensor] = None, tables: Optional[tuple] = None,
+                      window: Optional[Window] = None) -> torch.Tensor:
+    """Causal attention of each prompt to itself, through `window` where there is one (which has no gradient: calls that want
+    one raise).
 
     q [T, H_q, 128] (bf16, fp16 or fp32); k, v [T, H_kv, 128] (converted to fp16 once
     here when they are not); query_lens: the prompts' token counts (host ints, summing to
@@ -71,6 +74,8 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_l
     T, Hq, D = q.shape
     assert D == 128 and k.shape == v.shape and k.shape[0] == T and k.shape[2] == D and Hq % k.shape[1] == 0
     assert sum(query_lens) == T
+    if window is not None:
+        _hip.refuse_grad("prefill_attention through a window", q, k, v)
     if out is None:
         out = torch.empty_like(q)
     if T == 0:
@@ -84,5 +89,8 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_l
     q = q if q.stride(-1) == 1 else q.contiguous()
     k, v = k.contiguous(), v.contiguous()
     cu_d, blk_d = prompt_tables(query_lens, q.device) if tables is None else tables
-    _hip.ops().prefill(q, k, v, cu_d, blk_d, float(scale), out)
+    if window is None:
+        _hip.ops().prefill(q, k, v, cu_d, blk_d, float(scale), out)
+    else:
+        _hip.ops().prefill_window(q, k, v, cu_d, blk_d, *sizes(window), float(scale), out)
     return out
