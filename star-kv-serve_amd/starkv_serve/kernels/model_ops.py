@@ -117,6 +117,21 @@ def norm_rope_write(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v
     return q_out, k_out, kv16[0], kv16[1]
 
 
+def rope_rows(positions: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos_sin: torch.Tensor, half: bool,
+              norms: Optional[tuple] = None) -> tuple:
+    """q and k rotated in one launch, behind the RMS norms `norms` (q_weight, k_weight, eps) where given, for a cache
+    that another call writes. Returns (q, k, and with `half` k and v in fp16, the prefill attention's operands)."""
+    q_out, k_out = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    kv16 = torch.empty((2, *k.shape), dtype=torch.float16, device=k.device) if half else (None, None)
+    v = v if half else None  # rows that nothing is made of
+    if q.shape[0] and norms is None:
+        _hip.ops().rope_qkv(q, k, v, positions, cos_sin, q_out, k_out, None, None, None, kv16[0], kv16[1])
+    elif q.shape[0]:
+        _hip.ops().norm_rope_qkv(q, k, v, norms[0], norms[1], float(norms[2]), positions, cos_sin, q_out, k_out, None, None,
+                                 None, kv16[0], kv16[1])
+    return q_out, k_out, kv16[0], kv16[1]
+
+
 def silu_mul(gate_up: torch.Tensor) -> torch.Tensor:
     """silu(gate) * up of gate_up [T, 2 I] (bf16 / fp16, I a multiple of 8)."""
     T, w = gate_up.shape

@@ -27,7 +27,7 @@ compressed layer writes the prompt's codes and runs its dense prefill,
 attention.py:219-251; a full layer writes K/V and runs causal attention over the prompt,
 here on this library's prefill kernel where vLLM would run FlashAttention).
 
-Three options of the uncompressed layers that the reference does not have:
+Options of the uncompressed layers that the reference does not have:
 
 - ``LlamaShape.qk_norm``: an RMS norm of each query and key head in front of the rotation, in the rotation's launch
   (``model_ops.norm_rope_write``). A compressed layer's keys are lifted from codes as a linear map, which a norm of
@@ -38,6 +38,10 @@ Three options of the uncompressed layers that the reference does not have:
   to the tokens that weigh most. After a cut a request's next position is no longer its cache length:
   ``decode_metadata`` and ``DecodeGraph`` take the lengths apart. Positions then go on past ``max_model_len`` while the
   cache does not; ``max_positions`` says how far, and a step past it raises.
+- ``cache8``: their caches hold 8 bits a value (``kernels/cache8.py``): torch.int8 or torch.float8_e4m3fn codes. Steps
+  quantise keys and values as they write them; prompts attend to their own in 16 bits.
+- ``window``: their tokens see the last ones and a few first ones (``kernels/window.py``), in prompts and in steps. It goes with
+  either kind of cache.
 """
 import math
 from dataclasses import dataclass
@@ -49,11 +53,13 @@ import torch.nn.functional as F
 from starkv_serve.attention import StarKVAttentionImpl, StarKVMetadata
 from starkv_serve.checkpoint import StarKVCheckpoint
 from starkv_serve.kernels import model_ops
+from starkv_serve.kernels.cache8 import CODE_TYPES, Cache8, paged_decode_8, write_kv8
 from starkv_serve.kernels.evict import evict, paged_decode_weighted
 from starkv_serve.kernels.prefill import prefill_attention
 from starkv_serve.kernels.sparse_decode import (BlockSelection, key_bounds_like, paged_decode_sparse, select_blocks,
                                                 update_key_bounds)
 from starkv_serve.kernels.stock_decode import paged_decode_full, write_kv_full
+from starkv_serve.kernels.window import Window, paged_decode_window
 from starkv_serve.workloads import cos_sin_table
 
 
@@ -117,20 +123,27 @@ class StarKVLlamaForCausalLM:
 
     def __init__(self, shape: LlamaShape, starkv: Optional[StarKVCheckpoint], max_model_len: int, device,
                  dtype: torch.dtype = torch.bfloat16, seed: int = 0, stock: bool = False,
-                 sparse: Optional[BlockSelection] = None, weigh: bool = False, max_positions: Optional[int] = None):
+                 sparse: Optional[BlockSelection] = None, weigh: bool = False, max_positions: Optional[int] = None,
+                 cache8: Optional[torch.dtype] = None, window: Optional[Window] = None):
         """`starkv` = None or `stock` = True: every layer uncompressed (the stock model). `sparse`: decode steps of
         the uncompressed layers read selected blocks. `weigh`: steps sum up their tokens' weights, for ``evict``.
         `max_positions`: the last position of a session whose cuts keep its cache within max_model_len tokens
-        (max_model_len, and never less)."""
+        (max_model_len, and never less). `cache8`: the code type of the uncompressed layers' 8-bit caches. `window`: what
+        the uncompressed layers' tokens see."""
         compressed = starkv is not None and not stock and any(map(starkv.is_compressed, range(shape.num_layers)))
         if sparse is not None and weigh:
             raise ValueError("sparse or weigh: a decode over selected blocks does not weigh the others' tokens")
+        if (sparse is not None or weigh) and (cache8 is not None or window is not None):
+            raise ValueError("sparse and weigh read whole caches of 16 bits: neither goes with cache8 or window")
+        if cache8 is not None and cache8 not in CODE_TYPES:
+            raise ValueError(f"cache8: torch.int8 or torch.float8_e4m3fn, not {cache8}")
         if compressed and shape.qk_norm:
             raise NotImplementedError("qk_norm: a compressed layer's keys are a linear map of its codes, not normed ones")
         if compressed and weigh:
             raise NotImplementedError("weigh: a compressed layer's cache row holds every head's codes and is not cut by head")
         self.shape, self.device, self.dtype = shape, torch.device(device), dtype
         self.sparse, self.weigh = sparse, weigh
+        self.cache8, self.window = cache8, window
         self.max_model_len = max_model_len
         H, Hkv, D, hid = shape.num_heads, shape.num_kv_heads, shape.head_dim, shape.hidden_size
         self.scale = D ** -0.5
@@ -169,7 +182,7 @@ class StarKVLlamaForCausalLM:
 
     # -- caches ---------------------------------------------------------------------------
     def cache_bytes_per_token(self) -> int:
-        """KV-cache bytes per token over all layers."""
+        """KV-cache bytes per token over all layers (an 8-bit cache's exponents, 2 bytes a head and block, apart)."""
         s = self.shape
         total = 0
         for layer in self.layers:
@@ -177,7 +190,7 @@ class StarKVLlamaForCausalLM:
                 imp = layer.impl
                 total += imp.row.nbytes if imp.row is not None else (imp.k_width + imp.w.v_rank) * 2
             else:
-                total += 2 * s.num_kv_heads * s.head_dim * 2
+                total += 2 * s.num_kv_heads * s.head_dim * (2 if self.cache8 is None else 1)
         return total
 
     def allocate_kv_cache(self, num_blocks: int, block_size: int = 16, num_requests: int = 0) -> None:
@@ -197,6 +210,8 @@ class StarKVLlamaForCausalLM:
                     c = torch.zeros(num_blocks, block_size, imp.k_width + imp.w.v_rank, dtype=self.dtype,
                                     device=self.device)
                 self.kv_caches.append(c)
+            elif self.cache8 is not None:
+                self.kv_caches.append(Cache8.zeros(num_blocks, block_size, s.num_kv_heads, self.cache8, self.device, s.head_dim))
             else:
                 kc = torch.zeros(num_blocks, block_size, s.num_kv_heads, s.head_dim, dtype=self.dtype,
                                  device=self.device)
@@ -239,10 +254,20 @@ class StarKVLlamaForCausalLM:
         else:
             h, qkv = self._norm_linear(x, layer.ln1, layer.qkv_proj, few, capture is not None)
             q, k, v = (t.view(T, n, D) for t, n in zip(qkv.split([H * D, Hkv * D, Hkv * D], dim=-1), (H, Hkv, Hkv)))
-            kc, vc = self.kv_caches[li]
             ka, va = k, v  # the prefill attention's operands
             slots = md.slot_mapping[:T]
-            if self._own_rotation() and model_ops.rope_write_fits(self.rotary.cos_sin_cache, positions, q, k, v, kc, vc, slots):
+            if self.cache8 is None:
+                kc, vc = self.kv_caches[li]
+            if self.cache8 is not None:
+                if self._own_rotation() and model_ops.rope_fits(self.rotary.cos_sin_cache, positions, q, k, v):
+                    norms = (layer.q_norm, layer.k_norm, s.rms_norm_eps) if layer.q_norm is not None else None
+                    q, k, ka, va = model_ops.rope_rows(positions, q, k, v, self.rotary.cos_sin_cache, bool(md.num_prefills), norms)
+                else:
+                    q, k = self._normed(layer, q, k)
+                    q, k = self.rotary.apply(positions, q), self.rotary.apply(positions, k)
+                    ka = k
+                write_kv8(k, v, self.kv_caches[li], slots)
+            elif self._own_rotation() and model_ops.rope_write_fits(self.rotary.cos_sin_cache, positions, q, k, v, kc, vc, slots):
                 if layer.q_norm is None:
                     q, k, ka, va = model_ops.rope_write(positions, q, k, v, self.rotary.cos_sin_cache, kc, vc, slots,
                                                         capture is not None, bool(md.num_prefills))
@@ -256,7 +281,7 @@ class StarKVLlamaForCausalLM:
                 ka = k
                 write_kv_full(k, v, kc, vc, slots)
             if md.num_prefills:  # whole prompts only (prefill_step): causal attention over each prompt
-                out = prefill_attention(q, ka, va, md.prefill_seq_lens_cpu, self.scale).view(T, H * D)
+                out = prefill_attention(q, ka, va, md.prefill_seq_lens_cpu, self.scale, window=self.window).view(T, H * D)
                 if self.sparse is not None:
                     update_key_bounds(kc, self.key_bounds[li], md.block_table[:md.num_prefills], md.seq_lens,
                                       md.max_seq_len)
@@ -297,8 +322,12 @@ class StarKVLlamaForCausalLM:
     def _decode_attention(self, li: int, q: torch.Tensor, md: StarKVMetadata, span: int) -> torch.Tensor:
         """An uncompressed layer's attention of a decode step, its keys and values written."""
         T = q.shape[0]
-        kc, vc = self.kv_caches[li]
         table, lens = md.block_table[:T], md.seq_lens[:T]
+        if self.cache8 is not None:
+            return paged_decode_8(q, self.kv_caches[li], table, lens, span, self.scale, window=self.window)
+        kc, vc = self.kv_caches[li]
+        if self.window is not None:
+            return paged_decode_window(q, kc, vc, table, lens, span, self.scale, self.window)
         if self.sparse is not None:
             update_key_bounds(kc, self.key_bounds[li], table, lens, 1)
             sel = select_blocks(q, self.key_bounds[li], table, lens, span, self.block_size, self.sparse.keep,
@@ -418,8 +447,10 @@ class StarKVLlamaForCausalLM:
                 out = torch.empty(T, q.shape[1], dtype=self.dtype, device=self.device)
                 layer.impl.forward_from_hidden(q, hidden, self.kv_caches[li], md, out, in_full_graph=in_graph)
             else:
-                kc, vc = self.kv_caches[li]
-                write_kv_full(k, v, kc, vc, md.slot_mapping[:T])
+                if self.cache8 is not None:
+                    write_kv8(k, v, self.kv_caches[li], md.slot_mapping[:T])
+                else:
+                    write_kv_full(k, v, *self.kv_caches[li], md.slot_mapping[:T])
                 self._decode_attention(li, q, md, self.max_model_len if in_graph else max(md.max_seq_len, 1))
 
     @torch.no_grad()
