@@ -11,7 +11,7 @@
 // [num_blocks * block_size] of the workspace, which is not cleared: an entry counts where the slot of the token that
 // it names is the entry's own.
 //
-// A wave takes a (head, keys or values) of the block: four rows of 256 bytes a load, largest magnitude as integer bits
+// A wave takes a head of the block, keys and values: four rows of 256 bytes a load, largest magnitudes as integer bits
 // (NaN is above infinity, which is above all others), rows kept in registers from the first look to the rounding where there
 // are at most 16.
 #include <algorithm>
@@ -25,6 +25,7 @@ namespace {
 constexpr int WR_THR = 256;
 constexpr int WR_FEW = 256;  // tokens that a workgroup looks through
 constexpr int WR_RUN = 16;   // tokens of a workgroup of a larger write
+constexpr int WR_HELD = 64;  // places of a block that are looked through once
 
 struct Write8Params {
     const uint8_t* src[2]; int64_t s0[2], s1[2];   // keys, values: bytes
@@ -41,10 +42,18 @@ __device__ __forceinline__ int64_t slot_of(const Write8Params& p, int t) {
     return s >= 0 && s >> p.shift < p.num_blocks ? s : -1;
 }
 
+template <int CTL>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTL, 0xF, 0xF, true));
+}
+
+// The largest of the wave's values, in every lane: within rows of 16 lanes, then over the rows (as wave_max).
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-    return v;
+    v = dpp_umax<0x140>(dpp_umax<0x141>(dpp_umax<0x4E>(dpp_umax<0xB1>(v))));
+    const auto x = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    v = max(x[0], x[1]);
+    const auto y = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return max(y[0], y[1]);
 }
 
 // Eight 16-bit values as fp32.
@@ -63,14 +72,24 @@ __device__ __forceinline__ void values8(const uint4& w, float (&f)[8]) {
     }
 }
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// The larger of two pairs of 16-bit magnitudes: their order is that of their bits, for either type.
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+
+__device__ __forceinline__ uint32_t pair_max(uint32_t top, const uint4& w) {
+    constexpr uint32_t M = 0x7fff7fffu;
+    return pair_max(top, pair_max(pair_max(w.x & M, w.y & M), pair_max(w.z & M, w.w & M)));
+}
+
+// The fp32 bits of the larger of a pair of magnitudes.
 template <int DT>
-__device__ __forceinline__ uint32_t top_of(const uint4& w) {
-    float f[8];
-    values8<DT>(w, f);
-    uint32_t top = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
-    return top;
+__device__ __forceinline__ uint32_t top_bits(uint32_t pair) {
+    const uint32_t x = max(pair & 0xffffu, pair >> 16);
+    if constexpr (DT == STARKV_BF16) return x << 16;
+    return __float_as_uint((float)__builtin_bit_cast(_Float16, (uint16_t)x));
 }
 
 template <int CT, int DT>
@@ -81,52 +100,71 @@ __device__ __forceinline__ uint2 encode(const uint4& w, float inv) {
                       c8_pack<CT>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
 }
 
-// One block's (head, keys or values) by one wave. tok[offset]: the token of each place or -1; list: the places that
-// have one, `count` of them.
-template <int CT, int DT>
-__device__ __forceinline__ void write_unit(const Write8Params& p, int blk, int unit, const int* tok, const uint16_t* list,
-                                           int count) {
-    const int lane = threadIdx.x & 63, row = lane >> 4, d = lane & 15, h = unit >> 1, z = unit & 1;
-    int8_t* ex = p.ex + blk * p.x_s0 + h * p.x_s1 + z;
-    const int old = *ex;
-    const uint8_t* src = p.src[z] + h * p.s1[z] + 16 * d;
-    uint8_t* dst = p.codes[z] + blk * p.c_s0 + h * p.c_s2 + 8 * d;
-    constexpr int KEEP = 4;
-    uint4 kept[KEEP];
-    uint32_t top = 0;
+// Rows of 4 KEEP of a block's tokens, keys and values, of one head: a wave's lanes have 16 bytes of 4 rows each.
+constexpr int KEEP = 4;
+struct Rows8 {
+    uint4 w[2][KEEP];
+    int old[2];  // the exponents that are there
+};
+
+__device__ __forceinline__ void load_head(const Write8Params& p, Rows8& r, int blk, int h, const int* tok, const uint16_t* list,
+                                          int count) {
+    const int lane = threadIdx.x & 63, row = lane >> 4, d = lane & 15;
+    const int8_t* ex = p.ex + blk * p.x_s0 + h * p.x_s1;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) r.old[z] = ex[z];
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
         const int at = 4 * i + row;
-        kept[i] = at < count ? *(const uint4*)(src + tok[list[at]] * p.s0[z]) : make_uint4(0, 0, 0, 0);
-    }
+        const int64_t t = at < count ? tok[list[at]] : -1;
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i) top = max(top, top_of<DT>(kept[i]));
-    for (int at = 4 * KEEP + row; at < count; at += 4) top = max(top, top_of<DT>(*(const uint4*)(src + tok[list[at]] * p.s0[z])));
-    int e = c8_exponent<CT>(wave_umax(top));
+        for (int z = 0; z < 2; ++z)
+            r.w[z][i] = t >= 0 ? *(const uint4*)(p.src[z] + h * p.s1[z] + 16 * d + t * p.s0[z]) : make_uint4(0, 0, 0, 0);
+    }
+}
+
+// One block's head by one wave, keys and values. tok[place]: the token of each place or -1; list: the places that have
+// one, `count` of them; r: the first rows of them.
+template <int CT, int DT>
+__device__ __forceinline__ void write_head(const Write8Params& p, const Rows8& r, int blk, int h, const int* tok,
+                                           const uint16_t* list, int count) {
+    const int lane = threadIdx.x & 63, row = lane >> 4, d = lane & 15;
+    int8_t* ex = p.ex + blk * p.x_s0 + h * p.x_s1;
     const bool fresh = tok[0] >= 0;
-    if (!fresh) e = old == C8_NAN || e == C8_NAN ? C8_NAN : max(old, e);
-    if (!fresh && e != old && e != C8_NAN) {  // the codes that are there, to the new exponent
-        const float less = c8_scale(-min(e - old, 126));
-        for (int at = row; at < 1 << p.shift; at += 4) {
-            if (tok[at] >= 0) continue;
-            uint2* c = (uint2*)(dst + at * p.c_s1);
-            const uint2 w = *c;
-            float a[4], b[4];
-            c8_values<CT>(w.x, a);
-            c8_values<CT>(w.y, b);
-            *c = make_uint2(c8_pack<CT>(a[0] * less, a[1] * less, a[2] * less, a[3] * less),
-                            c8_pack<CT>(b[0] * less, b[1] * less, b[2] * less, b[3] * less));
-        }
-    }
-    const float inv = e == C8_NAN ? 0.f : c8_scale(-e);
-    const auto put = [&](int at, const uint4& w) {
-        *(uint2*)(dst + list[at] * p.c_s1) = e == C8_NAN ? make_uint2(0, 0) : encode<CT, DT>(w, inv);
-    };
 #pragma unroll
-    for (int i = 0; i < KEEP; ++i)
-        if (4 * i + row < count) put(4 * i + row, kept[i]);
-    for (int at = 4 * KEEP + row; at < count; at += 4) put(at, *(const uint4*)(src + tok[list[at]] * p.s0[z]));
-    if (lane == 0 && e != old) *ex = (int8_t)e;
+    for (int z = 0; z < 2; ++z) {
+        const uint8_t* src = p.src[z] + h * p.s1[z] + 16 * d;
+        uint8_t* dst = p.codes[z] + blk * p.c_s0 + h * p.c_s2 + 8 * d;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i) top = pair_max(top, r.w[z][i]);
+        for (int at = 4 * KEEP + row; at < count; at += 4) top = pair_max(top, *(const uint4*)(src + tok[list[at]] * p.s0[z]));
+        int e = c8_exponent<CT>(wave_umax(top_bits<DT>(top)));
+        const int old = r.old[z];
+        if (!fresh) e = old == C8_NAN || e == C8_NAN ? C8_NAN : max(old, e);
+        if (!fresh && e != old && e != C8_NAN) {  // the codes that are there, to the new exponent
+            const float less = c8_scale(-min(e - old, 126));
+            for (int at = row; at < 1 << p.shift; at += 4) {
+                if (tok[at] >= 0) continue;
+                uint2* c = (uint2*)(dst + at * p.c_s1);
+                const uint2 w = *c;
+                float a[4], b[4];
+                c8_values<CT>(w.x, a);
+                c8_values<CT>(w.y, b);
+                *c = make_uint2(c8_pack<CT>(a[0] * less, a[1] * less, a[2] * less, a[3] * less),
+                                c8_pack<CT>(b[0] * less, b[1] * less, b[2] * less, b[3] * less));
+            }
+        }
+        const float inv = e == C8_NAN ? 0.f : c8_scale(-e);
+        const auto put = [&](int at, const uint4& w) {
+            *(uint2*)(dst + list[at] * p.c_s1) = e == C8_NAN ? make_uint2(0, 0) : encode<CT, DT>(w, inv);
+        };
+#pragma unroll
+        for (int i = 0; i < KEEP; ++i)
+            if (4 * i + row < count) put(4 * i + row, r.w[z][i]);
+        for (int at = 4 * KEEP + row; at < count; at += 4) put(at, *(const uint4*)(src + tok[list[at]] * p.s0[z]));
+        if (lane == 0 && e != old) ex[z] = (int8_t)e;
+    }
 }
 
 struct Block8Shared {
@@ -143,7 +181,7 @@ __device__ __forceinline__ void list_places(Block8Shared& sh, int shift) {
     __syncthreads();
 }
 
-// A workgroup a token and 4 units (of 2 H): the block's tokens by looking through all slots.
+// A workgroup a token and 4 heads: the block's tokens by looking through all slots.
 template <int CT, int DT>
 __global__ __launch_bounds__(WR_THR) void write8_few_kernel(const Write8Params p) {
     __shared__ Block8Shared sh;
@@ -166,8 +204,11 @@ __global__ __launch_bounds__(WR_THR) void write8_few_kernel(const Write8Params p
     }
     list_places(sh, p.shift);
     if (sh.lead != t) return;
-    const int unit = blockIdx.y * 4 + (tid >> 6);
-    if (unit < 2 * p.H) write_unit<CT, DT>(p, blk, unit, sh.tok, sh.list, sh.count);
+    const int h = blockIdx.y * 4 + (tid >> 6);
+    if (h >= p.H) return;
+    Rows8 r;
+    load_head(p, r, blk, h, sh.tok, sh.list, sh.count);
+    write_head<CT, DT>(p, r, blk, h, sh.tok, sh.list, sh.count);
 }
 
 __global__ __launch_bounds__(WR_THR) void write8_map_kernel(const Write8Params p) {
@@ -183,34 +224,54 @@ __device__ __forceinline__ int mapped(const Write8Params& p, int64_t slot) {
     return (uint32_t)t < (uint32_t)p.n && slot_of(p, t) == slot ? t : -1;
 }
 
-// A workgroup WR_RUN tokens: the blocks that one of them leads (has the lowest place of), each with the units of
-// blockIdx.y.
+// A workgroup WR_RUN tokens and `heads` heads: the blocks that one of the tokens leads (has the lowest place of). 16 threads
+// a token look through its block's places; what they find of the first WR_HELD places stays with them for the
+// block's turn.
 template <int CT, int DT>
-__global__ __launch_bounds__(WR_THR) void write8_kernel(const Write8Params p, int units) {
+__global__ __launch_bounds__(WR_THR) void write8_kernel(const Write8Params p, int heads) {
     __shared__ Block8Shared sh;
-    __shared__ int s_follows[WR_RUN];
-    const int tid = threadIdx.x, size = 1 << p.shift;
+    __shared__ int s_follows[WR_RUN], s_blk[WR_RUN];
+    const int groups = (p.H + heads - 1) / heads, run = blockIdx.x / groups, group = blockIdx.x % groups;
+    const int tid = threadIdx.x, size = 1 << p.shift, mine = tid / WR_RUN, sub = tid % WR_RUN;
+    int held[WR_HELD / WR_RUN];
     {
-        const int j = tid / WR_RUN, t = blockIdx.x * WR_RUN + j;
-        if (tid < WR_RUN) s_follows[tid] = 0;
+        const int t = run * WR_RUN + mine;
+        const int64_t slot = t < p.n ? slot_of(p, t) : -1, first = slot & ~(int64_t)(size - 1);
+        if (sub == 0) {
+            s_follows[mine] = 0;
+            s_blk[mine] = (int)(slot >> p.shift);
+        }
         __syncthreads();
-        const int64_t slot = t < p.n ? slot_of(p, t) : -1;
-        if (slot < 0 || p.map[slot] != t) {
-            s_follows[j] = 1;
+        if (slot < 0) {
+            s_follows[mine] = 1;
         } else {
-            for (int64_t s = (slot & ~(int64_t)(size - 1)) + tid % WR_RUN; s < slot; s += WR_RUN)
-                if (mapped(p, s) >= 0) s_follows[j] = 1;
+#pragma unroll
+            for (int i = 0; i < WR_HELD / WR_RUN; ++i) held[i] = sub + WR_RUN * i < size ? mapped(p, first + sub + WR_RUN * i) : -1;
+            bool follows = p.map[slot] != t;  // another token has the slot too, and the map names that
+#pragma unroll
+            for (int i = 0; i < WR_HELD / WR_RUN; ++i) follows = follows || (held[i] >= 0 && first + sub + WR_RUN * i < slot);
+            for (int64_t s = first + sub + WR_HELD; s < slot; s += WR_RUN) follows = follows || mapped(p, s) >= 0;
+            if (follows) s_follows[mine] = 1;
         }
         __syncthreads();
     }
     for (int j = 0; j < WR_RUN; ++j) {
         if (s_follows[j]) continue;
-        const int blk = (int)(slot_of(p, blockIdx.x * WR_RUN + j) >> p.shift);
+        const int blk = s_blk[j];
         if (tid == 0) sh.count = 0;
-        for (int i = tid; i < size; i += WR_THR) sh.tok[i] = mapped(p, ((int64_t)blk << p.shift) + i);
+        if (mine == j) {
+#pragma unroll
+            for (int i = 0; i < WR_HELD / WR_RUN; ++i)
+                if (sub + WR_RUN * i < size) sh.tok[sub + WR_RUN * i] = held[i];
+        }
+        for (int i = tid + WR_HELD; i < size; i += WR_THR) sh.tok[i] = mapped(p, ((int64_t)blk << p.shift) + i);
         list_places(sh, p.shift);
-        const int end = min((int)(blockIdx.y + 1) * units, 2 * p.H);
-        for (int u = blockIdx.y * units + (tid >> 6); u < end; u += 4) write_unit<CT, DT>(p, blk, u, sh.tok, sh.list, sh.count);
+        const int end = min((group + 1) * heads, p.H);
+        for (int h = group * heads + (tid >> 6); h < end; h += 4) {
+            Rows8 r;
+            load_head(p, r, blk, h, sh.tok, sh.list, sh.count);
+            write_head<CT, DT>(p, r, blk, h, sh.tok, sh.list, sh.count);
+        }
         __syncthreads();
     }
 }
@@ -227,46 +288,67 @@ struct Read8Params {
     void* out[2];                                       // [n][H][128]
 };
 
-// 8 dimensions a lane, 16 lanes a row, rows of a token side by side. The bound is HBM: 128 bytes read and 256 written.
+// 16 lanes a row of 8 dimensions each, RD_U rows (of keys and of values) a lane, whose slots and then codes are on their way
+// together; rows as the results lie, a token's heads side by side. The bound is HBM: 128 bytes read and 256 written a
+// row.
+constexpr int RD_U = 2;
+
 template <int CT, int ODT>
 __global__ __launch_bounds__(256) void read8_kernel(const Read8Params p) {
-    const int64_t pieces = (int64_t)p.n * p.H * 16;
-    const int z = blockIdx.y;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i >> 4;
-        const int t = (int)(row / p.H), h = (int)(row - (int64_t)t * p.H), d = 8 * (int)(i & 15);
-        const int64_t slot = p.slot64 ? ((const int64_t*)p.slots)[t] : (int64_t)((const int32_t*)p.slots)[t];
-        const bool there = slot >= 0 && slot >> p.shift < p.num_blocks;
-        float f[8];
-        if (there) {
-            const int64_t blk = slot >> p.shift;
-            const uint2 w = *(const uint2*)(p.codes[z] + blk * p.c_s0 + (slot & ((1 << p.shift) - 1)) * p.c_s1 + h * p.c_s2 + d);
-            const float scale = c8_scale(p.ex[blk * p.x_s0 + h * p.x_s1 + z]);
-            float a[4], b[4];
-            c8_values<CT>(w.x, a);
-            c8_values<CT>(w.y, b);
+    const uint32_t rows = (uint32_t)p.n * p.H, row0 = blockIdx.x * (16 * RD_U) + (threadIdx.x >> 4);
+    const int d = 8 * (threadIdx.x & 15);
+    int64_t slot[RD_U];
+    uint32_t h[RD_U];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                f[e] = a[e] * scale;
-                f[4 + e] = b[e] * scale;
-            }
-        } else {
+    for (int u = 0; u < RD_U; ++u) {
+        const uint32_t row = min(row0 + 16 * u, rows - 1), t = row / (uint32_t)p.H;
+        h[u] = row - t * p.H;
+        slot[u] = p.slot64 ? ((const int64_t*)p.slots)[t] : (int64_t)((const int32_t*)p.slots)[t];
+    }
+    uint2 w[RD_U][2];
+    int e[RD_U][2];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = 0.f;
+    for (int u = 0; u < RD_U; ++u) {
+        if (slot[u] < 0 || slot[u] >> p.shift >= p.num_blocks) slot[u] = -1;
+        const int64_t s = max(slot[u], (int64_t)0), blk = s >> p.shift;
+        const int64_t at = blk * p.c_s0 + (s & ((1 << p.shift) - 1)) * p.c_s1 + h[u] * p.c_s2 + d;
+        const int8_t* ex = p.ex + blk * p.x_s0 + h[u] * p.x_s1;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            w[u][z] = *(const uint2*)(p.codes[z] + at);
+            e[u][z] = ex[z];
         }
-        if constexpr (ODT == STARKV_F32) {
-            float4* o = (float4*)((float*)p.out[z] + 8 * i);
-            o[0] = make_float4(f[0], f[1], f[2], f[3]);
-            o[1] = make_float4(f[4], f[5], f[6], f[7]);
-        } else {
-            uint32_t w[4];
+    }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint16_t lo = ODT == STARKV_BF16 ? f32_to_bf16_rne(f[2 * e]) : __builtin_bit_cast(uint16_t, (_Float16)f[2 * e]);
-                const uint16_t hi = ODT == STARKV_BF16 ? f32_to_bf16_rne(f[2 * e + 1]) : __builtin_bit_cast(uint16_t, (_Float16)f[2 * e + 1]);
-                w[e] = (uint32_t)lo | (uint32_t)hi << 16;
+    for (int u = 0; u < RD_U; ++u) {
+        if (row0 + 16 * u >= rows) break;
+        const int64_t to = (int64_t)(row0 + 16 * u) * 128 + d;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const float scale = c8_scale(e[u][z]);
+            float a[4], b[4];
+            c8_values<CT>(w[u][z].x, a);
+            c8_values<CT>(w[u][z].y, b);
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                f[i] = slot[u] < 0 ? 0.f : a[i] * scale;
+                f[4 + i] = slot[u] < 0 ? 0.f : b[i] * scale;
             }
-            *(uint4*)((uint16_t*)p.out[z] + 8 * i) = make_uint4(w[0], w[1], w[2], w[3]);
+            if constexpr (ODT == STARKV_F32) {
+                float4* o = (float4*)((float*)p.out[z] + to);
+                o[0] = make_float4(f[0], f[1], f[2], f[3]);
+                o[1] = make_float4(f[4], f[5], f[6], f[7]);
+            } else {
+                uint32_t v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint16_t lo = ODT == STARKV_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)f[2 * i]) : __builtin_bit_cast(uint16_t, (_Float16)f[2 * i]);
+                    const uint16_t hi = ODT == STARKV_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)f[2 * i + 1]) : __builtin_bit_cast(uint16_t, (_Float16)f[2 * i + 1]);
+                    v[i] = (uint32_t)lo | (uint32_t)hi << 16;
+                }
+                *(uint4*)((uint16_t*)p.out[z] + to) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
         }
     }
 }
@@ -287,8 +369,8 @@ using namespace starkv;
 extern "C" {
 
 size_t starkv_write_kv8_workspace_bytes(int n, int64_t num_blocks, int block_size) {
-    if (n <= WR_FEW || num_blocks < 1 || block_size < 1) return 256;
-    return std::max<size_t>(256, (size_t)num_blocks * block_size * 4);
+    if (n <= WR_FEW || num_blocks < 1 || block_size < 1) return 0;
+    return (size_t)num_blocks * block_size * 4;
 }
 
 int starkv_write_kv8(void* stream, const void* key, int64_t k_s0, int64_t k_s1, const void* value, int64_t v_s0,
@@ -299,7 +381,7 @@ int starkv_write_kv8(void* stream, const void* key, int64_t k_s0, int64_t k_s1, 
     clear_error();
     SKV_CHECK(n >= 0 && num_kv_heads >= 1 && num_kv_heads <= 65535, "write_kv8: n=%d num_kv_heads=%d (up to 65535)", n, num_kv_heads);
     if (n == 0) return STARKV_OK;
-    SKV_CHECK(key && value && k_codes && v_codes && exponents && slot_mapping && workspace, "write_kv8: null pointer");
+    SKV_CHECK(key && value && k_codes && v_codes && exponents && slot_mapping, "write_kv8: null pointer");
     SKV_CHECK(dtype == STARKV_BF16 || dtype == STARKV_F16, "write_kv8: keys and values must be bf16 or fp16");
     SKV_CHECK(code_type == STARKV_I8 || code_type == STARKV_E4M3, "write_kv8: codes must be int8 or e4m3");
     SKV_CHECK(slot_bits == 32 || slot_bits == 64, "write_kv8: slot_mapping must be int32 or int64");
@@ -309,7 +391,7 @@ int starkv_write_kv8(void* stream, const void* key, int64_t k_s0, int64_t k_s1, 
                   ((uintptr_t)k_codes | (uintptr_t)v_codes) % 16 == 0 && (c_s0 | c_s1 | c_s2) % 16 == 0,
               "write_kv8: rows must be 16-byte aligned");
     const size_t need = starkv_write_kv8_workspace_bytes(n, num_blocks, block_size);
-    SKV_CHECK(workspace_bytes >= need && (uintptr_t)workspace % 16 == 0, "write_kv8: workspace %zu bytes < %zu", workspace_bytes, need);
+    SKV_CHECK(workspace_bytes >= need && (workspace || need == 0) && (uintptr_t)workspace % 16 == 0, "write_kv8: workspace %zu bytes < %zu", workspace_bytes, need);
     Write8Params p;
     p.src[0] = (const uint8_t*)key; p.s0[0] = 2 * k_s0; p.s1[0] = 2 * k_s1;
     p.src[1] = (const uint8_t*)value; p.s0[1] = 2 * v_s0; p.s1[1] = 2 * v_s1;
@@ -325,16 +407,18 @@ int starkv_write_kv8(void* stream, const void* key, int64_t k_s0, int64_t k_s1, 
         const void* fn = i8 ? bf ? (const void*)&write8_few_kernel<STARKV_I8, STARKV_BF16> : (const void*)&write8_few_kernel<STARKV_I8, STARKV_F16>
                             : bf ? (const void*)&write8_few_kernel<STARKV_E4M3, STARKV_BF16> : (const void*)&write8_few_kernel<STARKV_E4M3, STARKV_F16>;
         void* args[] = {(void*)&p};
-        SKV_HIP(hipLaunchKernel(fn, dim3(n, (2 * num_kv_heads + 3) / 4), dim3(WR_THR), args, 0, (hipStream_t)stream));
+        SKV_HIP(hipLaunchKernel(fn, dim3(n, (num_kv_heads + 3) / 4), dim3(WR_THR), args, 0, (hipStream_t)stream));
         return STARKV_OK;
     }
     hipLaunchKernelGGL(write8_map_kernel, dim3((n + WR_THR - 1) / WR_THR), dim3(WR_THR), 0, (hipStream_t)stream, p);
     SKV_HIP(hipGetLastError());
     const void* fn = i8 ? bf ? (const void*)&write8_kernel<STARKV_I8, STARKV_BF16> : (const void*)&write8_kernel<STARKV_I8, STARKV_F16>
                         : bf ? (const void*)&write8_kernel<STARKV_E4M3, STARKV_BF16> : (const void*)&write8_kernel<STARKV_E4M3, STARKV_F16>;
-    int units = 16;  // four a wave: the search for a block's tokens is made once for them
-    void* args[] = {(void*)&p, (void*)&units};
-    SKV_HIP(hipLaunchKernel(fn, dim3((n + WR_RUN - 1) / WR_RUN, (2 * num_kv_heads + units - 1) / units), dim3(WR_THR), args, 0,
+    int heads = 8;  // two a wave: the search for a block's tokens is made once for them
+    void* args[] = {(void*)&p, (void*)&heads};
+    const int64_t grid = ((int64_t)n + WR_RUN - 1) / WR_RUN * ((num_kv_heads + heads - 1) / heads);
+    SKV_CHECK(grid < 1ll << 31, "write_kv8: %d tokens of %d heads in one call", n, num_kv_heads);
+    SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)grid), dim3(WR_THR), args, 0,
                             (hipStream_t)stream));
     return STARKV_OK;
 }
@@ -344,7 +428,7 @@ int starkv_read_kv8(void* stream, const void* k_codes, const void* v_codes, int6
                     int64_t num_blocks, const void* slot_mapping, int slot_bits, int n, int num_kv_heads, void* key_out,
                     void* value_out, int out_dtype) {
     clear_error();
-    SKV_CHECK(n >= 0 && num_kv_heads >= 1, "read_kv8: n=%d num_kv_heads=%d", n, num_kv_heads);
+    SKV_CHECK(n >= 0 && num_kv_heads >= 1 && num_kv_heads <= 65535, "read_kv8: n=%d num_kv_heads=%d (up to 65535)", n, num_kv_heads);
     if (n == 0) return STARKV_OK;
     SKV_CHECK(k_codes && v_codes && exponents && slot_mapping && key_out && value_out, "read_kv8: null pointer");
     SKV_CHECK(out_dtype >= STARKV_F32 && out_dtype <= STARKV_BF16, "read_kv8: rows of bf16, fp16 or fp32");
@@ -365,9 +449,9 @@ int starkv_read_kv8(void* stream, const void* k_codes, const void* v_codes, int6
     p.out[0] = key_out; p.out[1] = value_out;
     const void* fn = code_type == STARKV_I8 ? read_pick<STARKV_I8>(out_dtype) : read_pick<STARKV_E4M3>(out_dtype);
     void* args[] = {(void*)&p};
-    const int64_t pieces = (int64_t)n * num_kv_heads * 16;
-    SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)std::min<int64_t>((pieces + 255) / 256, 1 << 20), 2), dim3(256), args, 0,
-                            (hipStream_t)stream));
+    const int64_t rows = (int64_t)n * num_kv_heads, per = 16 * RD_U;
+    SKV_CHECK(rows < 1ll << 31, "read_kv8: %d tokens of %d heads in one call", n, num_kv_heads);
+    SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)((rows + per - 1) / per)), dim3(256), args, 0, (hipStream_t)stream));
     return STARKV_OK;
 }
 

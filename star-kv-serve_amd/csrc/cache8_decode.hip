@@ -7,7 +7,7 @@
 // Codes are never multiplied by their scales: 2^a goes onto the 4 scores that a lane has of a page, 2^c into its
 // weights. A page is 16 tokens of one block. A workgroup of 4 waves takes a range of the unit's pages (a split);
 // a wave takes two pages, 32 tokens, at a time and keeps references and sums of its own; the waves meet in LDS at
-// the end, the splits in merge8_kernel.
+
 //
 // Both products run on v_mfma_f32_16x16x32_f16, for which every code and fp16 query is exact; a bf16 query row goes to fp16
 // by a power of two that brings its largest value to 2^14, which leaves values down to 2^-28 of that exact. S^T =
@@ -28,6 +28,7 @@
 // A block whose exponent says NaN makes every row NaN that sees one of its tokens. A row that sees no token is zero; one
 // whose scores are all -inf is 0 / 0, NaN.
 #include <algorithm>
+#include <atomic>
 
 #include "cache8.hpp"
 #include "window_pages.hpp"
@@ -39,7 +40,6 @@ namespace {
 constexpr int D8_THR = 256;
 constexpr int D8_CHUNK = 512;       // pages whose places are looked up at a time
 constexpr int D8_PART = 132;        // floats of a partial: reference, sum of weights, 0, 0, out[128]
-constexpr int D8_MAX_SPLITS = 128;
 constexpr int D8_MAX_GROUP = 16;    // query heads per KV head: the columns of a matrix product
 constexpr float D8_LEAST = -3.402823466e38f;  // the reference of tokens whose scores are all -inf
 
@@ -50,17 +50,60 @@ struct Decode8Params {
     int bs_shift; int64_t num_blocks;                                   // block_size = 16 << bs_shift
     const int32_t* bt; int64_t bt_s0, bt_s1;
     const int32_t* seq_lens; int span;                                  // lengths are clamped to span
-    int n, Hkv, G, splits, window, sinks;
+    int n, Hkv, G, ranges, window, sinks;
     float sc;                                                           // scale * log2(e)
-    float* part;                                                        // [n][H][splits][D8_PART]
+    int2* where;                                                        // [n]: first range, ranges
+    float* part;                                                        // [ranges][2][H][D8_PART]
     uint16_t* out; int64_t o_s0, o_s1;
 };
 
-// Pages of a split: the request's, shared out evenly, 8 at least (two a wave). The splits behind the last have none.
-__device__ __forceinline__ int pages_per_split(int pages, int splits) { return max((pages + splits - 1) / splits, 8); }
-
 __device__ __forceinline__ SeenPages seen_by(const Decode8Params& p, int b) {
     return seen_pages(min(max(p.seq_lens[b], 0), p.span), p.window, p.sinks);
+}
+
+__device__ __forceinline__ int scan_wave(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(v, o, 64);
+        if (lane >= o) v += x;
+    }
+    return v;
+}
+
+// A range of the call's pages, request by request: its first page's request and place there, and its length. All
+// waves find it by themselves: 64 requests a look.
+struct Range8 {
+    int b, k, left, per;  // per: pages a range
+};
+
+__device__ __forceinline__ Range8 find_range(const Decode8Params& p, int range) {
+    const int lane = threadIdx.x & 63;
+    int own = 0, end = 0, total = 0;
+    for (int b0 = 0; b0 < p.n; b0 += 64) {
+        own = b0 + lane < p.n ? seen_by(p, b0 + lane).pages : 0;
+        end = scan_wave(own);
+        total += __builtin_amdgcn_readlane(end, 63);
+    }
+    Range8 g;
+    g.per = max((total + p.ranges - 1) / p.ranges, 8);  // two pages a wave
+    int start = range * g.per;
+    g.left = min(g.per, total - start);
+    g.b = g.k = 0;
+    if (g.left <= 0) return g;
+    for (int b0 = 0;; b0 += 64) {
+        if (p.n > 64) {
+            own = b0 + lane < p.n ? seen_by(p, b0 + lane).pages : 0;
+            end = scan_wave(own);
+        }
+        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= start));
+        if (at < 64) {
+            g.b = b0 + at;
+            g.k = start - __builtin_amdgcn_readlane(end, at) + __builtin_amdgcn_readlane(own, at);
+            return g;
+        }
+        start -= __builtin_amdgcn_readlane(end, 63);
+    }
 }
 
 __device__ __forceinline__ f32x4_t mfma_f16(uint4 a, uint4 b, f32x4_t c) {
@@ -85,20 +128,16 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
     w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
-// The workgroup's unit: (request, KV head, split) from the block index. MANY: 9 to 16 query heads.
+// Pages [k0, k1) of request b's, for KV head h: its query heads' result where that is all the request has, else a
+// partial of the range.
 template <int CT, int QDT, bool MANY>
-__global__ __launch_bounds__(D8_THR, 4) void decode8_kernel(const Decode8Params p) {
-    __shared__ int4 s_page[D8_CHUNK];  // block, place in the block, places that are seen, exponents
-    extern __shared__ float s_dyn[];   // [4 waves][G][D8_PART] for the merge
-    const int id = blockIdx.x, s = id % p.splits, u = id / p.splits, h = u % p.Hkv, b = u / p.Hkv;
+__device__ __forceinline__ void decode8_request(const Decode8Params& p, int4* s_page, float* s_dyn, const SeenPages& seen,
+                                                int range, int h, int b, int k0, int k1, int per) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = MANY ? lane & 15 : lane & 7, quad = lane >> 4;  // the lane's query head
-    const int H = p.Hkv * p.G;
-    const SeenPages seen = seen_by(p, b);
-    const int pps = pages_per_split(seen.pages, p.splits);
-    const int k0 = min(s * pps, seen.pages), k1 = min(k0 + pps, seen.pages);
-    if (k0 >= k1 && s > 0) return;  // the merge reads the splits that have pages
-    const int mask = (1 << p.bs_shift) - 1;
+    const int H = p.Hkv * p.G, mask = (1 << p.bs_shift) - 1;
+    const bool whole = k0 == 0 && k1 == seen.pages;
+    if (h == 0 && k0 == 0 && tid == 0) p.where[b] = make_int2(range, 1 + (seen.pages - k1 + per - 1) / per);
 
     // The head's row: dimensions 64 st + 16 quad .. + 15, two operands; their fp16 values times 2^up.
     uint4 qf[2][2];
@@ -150,7 +189,7 @@ __global__ __launch_bounds__(D8_THR, 4) void decode8_kernel(const Decode8Params 
 
     for (int c0 = k0; c0 < k1; c0 += D8_CHUNK) {
         const int count = min(D8_CHUNK, k1 - c0);
-        if (c0 != k0) __syncthreads();
+        __syncthreads();  // the last look's pages, or the request's before, are done with
         for (int i = tid; i < count; i += D8_THR) {
             const int pg = seen.page(c0 + i);
             int blk = p.bt[b * p.bt_s0 + (pg >> p.bs_shift) * p.bt_s1];
@@ -311,69 +350,103 @@ __global__ __launch_bounds__(D8_THR, 4) void decode8_kernel(const Decode8Params 
         }
         const int hq = h * p.G + g;
         const float half = exp2f(0.5f * (R - M));  // in two steps: its square may be past fp32's range where the result is not
-        // A split without weight (scores of -inf alone) adds 0 to the others', not 0 times 0 / 0.
-        const float o = M == -INFINITY || (lt == 0.f && p.splits > 1) ? 0.f : a / lt * half * half;
-        if (p.splits == 1) {
+        // A partial without weight (scores of -inf alone) adds 0 to the others', not 0 times 0 / 0.
+        const float o = M == -INFINITY || (lt == 0.f && !whole) ? 0.f : a / lt * half * half;
+        if (whole) {
             store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, QDT, o);
         } else {
-            float* pp = p.part + (((int64_t)b * H + hq) * p.splits + s) * D8_PART;
+            float* pp = p.part + ((int64_t)(2 * range + (k0 == 0)) * H + hq) * D8_PART;
             if (d == 0) *(float4*)pp = make_float4(M, lt, 0.f, 0.f);
             pp[4 + d] = o;
         }
     }
 }
 
-// A head's splits joined by one wave: out = sum_s l_s 2^(m_s - M) out_s / sum_s l_s 2^(m_s - M). Lane s holds the factors of
-// splits s and s + 64 and sums dimensions 2 s and 2 s + 1, eight splits' loads in flight.
+// A KV head's part of a range, from the block index. MANY: 9 to 16 query heads.
+template <int CT, int QDT, bool MANY>
+__global__ __launch_bounds__(D8_THR, 4) void decode8_kernel(const Decode8Params p) {
+    __shared__ int4 s_page[D8_CHUNK];  // block, place in the block, places that are seen, exponents
+    extern __shared__ float s_dyn[];   // [4 waves][G][D8_PART] for the merge
+    const int range = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
+    Range8 g = find_range(p, range);
+    if (p.ranges == 1)  // no merge follows, which writes the rows that see no token
+        for (int b = 0; b < p.n; ++b)
+            if (seen_by(p, b).pages == 0)
+                for (int i = threadIdx.x; i < p.G * 128; i += D8_THR)
+                    store_f(p.out, b * p.o_s0 + (h * p.G + (i >> 7)) * p.o_s1 + (i & 127), QDT, 0.f);
+    for (; g.left > 0; ++g.b, g.k = 0) {
+        const SeenPages seen = seen_by(p, g.b);
+        const int k1 = min(seen.pages, g.k + g.left);
+        if (k1 > 0) decode8_request<CT, QDT, MANY>(p, s_page, s_dyn, seen, range, h, g.b, g.k, k1, g.per);
+        g.left -= k1 - g.k;
+    }
+}
+
+// A head's partials joined by one wave: out = sum_s l_s 2^(m_s - M) out_s / sum_s l_s 2^(m_s - M). The first lies second in
+// its range (other requests may end there), the others first in theirs. Lane s of 64 holds the factors of 64 partials at a
+// time and sums dimensions 2 s and 2 s + 1, eight partials' loads in flight.
 template <int QDT>
 __global__ __launch_bounds__(64) void merge8_kernel(const Decode8Params p) {
-    static_assert(D8_MAX_SPLITS <= 128, "two splits a lane");
-    const int lane = threadIdx.x, hq = blockIdx.x, b = blockIdx.y;
-    const SeenPages seen = seen_by(p, b);
-    const int pps = pages_per_split(seen.pages, p.splits), splits = max((seen.pages + pps - 1) / pps, 1);
-    const float* pp = p.part + ((int64_t)b * p.Hkv * p.G + hq) * p.splits * D8_PART;
-    float m[2], f[2], lt = 0.f;
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        const int s = lane + 64 * x;
-        m[x] = s < splits ? pp[s * D8_PART] : -INFINITY;
-        f[x] = s < splits ? pp[s * D8_PART + 1] : 0.f;
+    const int lane = threadIdx.x, hq = blockIdx.x, b = blockIdx.y, H = p.Hkv * p.G;
+    const int64_t to = b * p.o_s0 + hq * p.o_s1 + 2 * lane;
+    const int2 where = p.where[b];
+    if (seen_by(p, b).pages == 0) {  // no workgroup has it, nor has one said where it is
+        store_f(p.out, to, QDT, 0.f);
+        store_f(p.out, to + 1, QDT, 0.f);
+        return;
     }
-    const float M = wave_max(fmaxf(m[0], m[1]));
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-        f[x] *= m[x] == -INFINITY ? 1.f : exp2f(m[x] - M);
-        lt += f[x];
-    }
-    lt = wave_sum(lt);
+    if (where.y == 1) return;
+    const auto part = [&](int s) { return p.part + ((int64_t)(2 * (where.x + s) + (s == 0)) * H + hq) * D8_PART; };
+    float M = -INFINITY, lt = 0.f;
     float2 a = make_float2(0.f, 0.f);
-    for (int s0 = 0; s0 < splits; s0 += 8) {
-        float2 v[8];
+    for (int c0 = 0; c0 < where.y; c0 += 64) {
+        const int count = min(where.y - c0, 64);
+        const float* mine = part(c0 + min(lane, count - 1));
+        const float m = lane < count ? mine[0] : -INFINITY, l = lane < count ? mine[1] : 0.f;
+        const float most = fmaxf(M, wave_max(m)), before = M == -INFINITY ? 1.f : exp2f(M - most);
+        M = most;
+        const float f = m == -INFINITY ? 0.f : l * exp2f(m - M);
+        lt = fmaf(lt, before, wave_sum(f));
+        a.x *= before;
+        a.y *= before;
+        for (int s0 = 0; s0 < count; s0 += 8) {
+            float2 v[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = *(const float2*)(pp + min(s0 + u, splits - 1) * D8_PART + 4 + 2 * lane);
+            for (int u = 0; u < 8; ++u) v[u] = *(const float2*)(part(c0 + min(s0 + u, count - 1)) + 4 + 2 * lane);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-            const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(s0 < 64 ? f[0] : f[1]), (s0 + u) & 63)) / lt;
-            if (s0 + u < splits) {
-                a.x = fmaf(v[u].x, fs, a.x);
-                a.y = fmaf(v[u].y, fs, a.y);
+            for (int u = 0; u < 8; ++u) {
+                const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (s0 + u) & 63));
+                if (s0 + u < count) {
+                    a.x = fmaf(v[u].x, fs, a.x);
+                    a.y = fmaf(v[u].y, fs, a.y);
+                }
             }
         }
     }
-    const int64_t o = b * p.o_s0 + hq * p.o_s1 + 2 * lane;
-    store_f(p.out, o, QDT, M == -INFINITY ? 0.f : a.x);
-    store_f(p.out, o + 1, QDT, M == -INFINITY ? 0.f : a.y);
+    store_f(p.out, to, QDT, M == -INFINITY ? 0.f : a.x / lt);
+    store_f(p.out, to + 1, QDT, M == -INFINITY ? 0.f : a.y / lt);
 }
 
-// Splits per unit (request and KV head): workgroups for `per_cu` a CU, 8 pages a split at least.
-int decode8_splits(int n, int num_kv_heads, int span, int window, int sinks) {
-    int dev = 0, cus = 256, c = 0;
-    if (hipGetDevice(&dev) == hipSuccess &&
-        hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && c > 0)
-        cus = c;
-    const int64_t units = (int64_t)n * num_kv_heads, pages = seen_pages_most(span, window, sinks);
-    const int64_t s = std::min<int64_t>((2 * (int64_t)cus + units - 1) / units, (pages + 7) / 8);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(s, D8_MAX_SPLITS));
+int device_cus() {
+    static std::atomic<int> known[64];  // by device: the count does not change, and asking costs a call 0.3 us
+    int dev = 0, c = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    c = known[dev].load(std::memory_order_relaxed);
+    if (c == 0) {
+        if (hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || c <= 0) c = 256;
+        known[dev].store(c, std::memory_order_relaxed);
+    }
+    return c;
+}
+
+// Ranges that a call's pages are cut into: workgroups for 2 a CU with a range's KV heads, 8 pages a range at least.
+int decode8_ranges(int n, int num_kv_heads, int span, int window, int sinks) {
+    const int64_t pages = (int64_t)n * seen_pages_most(span, window, sinks);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * device_cus() / num_kv_heads, (pages + 7) / 8));
+}
+
+size_t decode8_bytes(int n, int num_heads, int ranges) {
+    return (((size_t)n * sizeof(int2) + 255) & ~(size_t)255) + (size_t)ranges * 2 * num_heads * D8_PART * 4;
 }
 
 template <int CT, int QDT>
@@ -391,8 +464,7 @@ extern "C" {
 
 size_t starkv_decode_kv8_workspace_bytes(int n, int num_heads, int num_kv_heads, int max_seq_len, int window, int sinks) {
     if (n < 1 || num_kv_heads < 1 || num_heads < num_kv_heads || max_seq_len < 1 || window < 0 || sinks < 0) return 256;
-    const int splits = decode8_splits(n, num_kv_heads, max_seq_len, window, sinks);
-    return splits == 1 ? 256 : (size_t)n * num_heads * splits * D8_PART * 4;
+    return decode8_bytes(n, num_heads, decode8_ranges(n, num_kv_heads, max_seq_len, window, sinks));
 }
 
 int starkv_decode_kv8(void* stream, const void* query, int64_t q_s0, int64_t q_s1, int dtype, const void* k_codes,
@@ -428,19 +500,21 @@ int starkv_decode_kv8(void* stream, const void* query, int64_t q_s0, int64_t q_s
     p.seq_lens = seq_lens;
     p.span = (int)std::min<int64_t>({(int64_t)bt_width * block_size, 0x7ffffff0, (int64_t)max_seq_len});
     p.n = n; p.Hkv = num_kv_heads; p.G = num_heads / num_kv_heads;
-    p.splits = decode8_splits(n, num_kv_heads, max_seq_len, window, sinks);
+    p.ranges = decode8_ranges(n, num_kv_heads, max_seq_len, window, sinks);
     p.window = window; p.sinks = sinks;
     p.sc = scale * 1.4426950408889634f;
-    p.part = (float*)workspace;
+    p.where = (int2*)workspace;
+    p.part = (float*)((char*)workspace + (((size_t)n * sizeof(int2) + 255) & ~(size_t)255));
     p.out = (uint16_t*)out; p.o_s0 = o_s0; p.o_s1 = o_s1;
-    SKV_CHECK((int64_t)n * num_kv_heads * p.splits < 1 << 23, "decode_kv8: %d requests of %d KV heads in one call", n, num_kv_heads);
+    SKV_CHECK((int64_t)n * seen_pages_most(p.span, window, sinks) < 1ll << 31, "decode_kv8: %d requests of up to %d tokens in one call", n, p.span);
+    SKV_CHECK(num_heads <= 65535, "decode_kv8: %d heads", num_heads);
     const bool bf = dtype == STARKV_BF16;
     const void* fn = code_type == STARKV_I8 ? bf ? decode_pick<STARKV_I8, STARKV_BF16>(p.G) : decode_pick<STARKV_I8, STARKV_F16>(p.G)
                                             : bf ? decode_pick<STARKV_E4M3, STARKV_BF16>(p.G) : decode_pick<STARKV_E4M3, STARKV_F16>(p.G);
     void* args[] = {(void*)&p};
-    SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)((int64_t)n * num_kv_heads * p.splits)), dim3(D8_THR), args,
+    SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)((int64_t)p.ranges * num_kv_heads)), dim3(D8_THR), args,
                             (size_t)4 * p.G * D8_PART * 4, (hipStream_t)stream));
-    if (p.splits == 1) return STARKV_OK;
+    if (p.ranges == 1) return STARKV_OK;
     if (bf)
         hipLaunchKernelGGL(merge8_kernel<STARKV_BF16>, dim3(num_heads, n), dim3(64), 0, (hipStream_t)stream, p);
     else

@@ -14,6 +14,7 @@
 #include <torch/library.h>
 
 #include <optional>
+#include <tuple>
 #include <vector>
 
 #include "../../include/starkv_hip.h"
@@ -543,19 +544,19 @@ void evict(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tenso
           "evict");
 }
 
-// One token's attention over a 16-bit cache through a window.
-void window_decode(const at::Tensor& query, const at::Tensor& k_cache, const at::Tensor& v_cache,
-                   const at::Tensor& block_table, const at::Tensor& seq_lens, int64_t max_seq_len, int64_t window,
-                   int64_t sinks, double scale, const at::Tensor& out) {
+// One token's attention over a 16-bit cache through a window. (The result is made here: a tensor made by Python costs a
+// call of 9 us another 1.2.)
+at::Tensor window_decode(const at::Tensor& query, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                         const at::Tensor& block_table, const at::Tensor& seq_lens, int64_t max_seq_len, int64_t window,
+                         int64_t sinks, double scale) {
     const c10::DeviceGuard guard(query.device());
     const int64_t n = query.size(0);
     check_caches(k_cache, v_cache, "window_decode");
     const int H = (int)query.size(1), Hkv = (int)k_cache.size(2);
     check_query(query, k_cache, Hkv, "window_decode");
-    check_query(out, k_cache, Hkv, "window_decode");
     check_table(block_table, seq_lens, n, "window_decode");
-    TORCH_CHECK(out.sizes() == query.sizes(), "starkv.window_decode: out as query");
-    at::assert_no_internal_overlap(out);
+    const at::Tensor out = at::empty(query.sizes(), query.options());
+    if (n == 0) return out;
     const int span = as_int(max_seq_len, "max_seq_len"), w = as_int(window, "window"), s = as_int(sinks, "sinks");
     const at::Tensor ws = workspace(query, starkv_window_decode_workspace_bytes((int)n, H, Hkv, span, w, s));
     check(starkv_window_decode(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), k_cache.data_ptr(),
@@ -565,6 +566,7 @@ void window_decode(const at::Tensor& query, const at::Tensor& k_cache, const at:
                                i32(seq_lens, "seq_lens"), (int)n, H, Hkv, span, w, s, (float)scale, out.data_ptr(),
                                out.stride(0), out.stride(1), ws.data_ptr(), (size_t)ws.numel()),
           "window_decode");
+    return out;
 }
 
 // An 8-bit cache's codes [blocks, block_size, heads, 128] and exponents [blocks, heads, 2]; its code type.
@@ -596,45 +598,48 @@ void write_kv8(const at::Tensor& key, const at::Tensor& value, const at::Tensor&
     const int bits = slots_of(slots, n, "write_kv8"), tokens = as_int(n, "tokens");
     for (const auto* t : {&k_codes, &v_codes, &exponents}) at::assert_no_internal_overlap(*t);
     at::assert_no_overlap(k_codes, v_codes);
-    const at::Tensor ws = workspace(key, starkv_write_kv8_workspace_bytes(tokens, k_codes.size(0), (int)k_codes.size(1)));
+    const size_t need = starkv_write_kv8_workspace_bytes(tokens, k_codes.size(0), (int)k_codes.size(1));
+    at::Tensor ws;
+    if (need) ws = workspace(key, need);
     check(starkv_write_kv8(stream_of(key), key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
                            value.stride(1), dtype_code(key), k_codes.data_ptr(), v_codes.data_ptr(), k_codes.stride(0),
                            k_codes.stride(1), k_codes.stride(2), code, exponents.data_ptr<int8_t>(), exponents.stride(0),
                            exponents.stride(1), (int)k_codes.size(1), k_codes.size(0), slots.data_ptr(), bits, tokens,
-                           (int)H, ws.data_ptr(), (size_t)ws.numel()),
+                           (int)H, need ? ws.data_ptr() : nullptr, need),
           "write_kv8");
 }
 
-// Rows of an 8-bit cache back.
-void read_kv8(const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& exponents, const at::Tensor& slots,
-              const at::Tensor& key_out, const at::Tensor& value_out) {
+// Rows of an 8-bit cache back, keys and values.
+std::tuple<at::Tensor, at::Tensor> read_kv8(const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& exponents,
+                                            const at::Tensor& slots, at::ScalarType dtype) {
     const c10::DeviceGuard guard(k_codes.device());
     const int code = check_cache8(k_codes, v_codes, exponents, "read_kv8");
     const int64_t n = slots.dim() == 1 ? slots.size(0) : -1, H = k_codes.size(2);
-    for (const auto* t : {&key_out, &value_out})
-        TORCH_CHECK(t->dim() == 3 && t->size(0) == n && t->size(1) == H && t->size(2) == 128 && t->is_contiguous() &&
-                        t->scalar_type() == key_out.scalar_type(),
-                    "starkv.read_kv8: the results are contiguous [n, heads, 128] of one dtype");
-    check(starkv_read_kv8(stream_of(k_codes), k_codes.data_ptr(), v_codes.data_ptr(), k_codes.stride(0), k_codes.stride(1),
-                          k_codes.stride(2), code, exponents.data_ptr<int8_t>(), exponents.stride(0), exponents.stride(1),
-                          (int)k_codes.size(1), k_codes.size(0), slots.data_ptr(), slots_of(slots, n, "read_kv8"),
-                          as_int(n, "tokens"), (int)H, key_out.data_ptr(), value_out.data_ptr(), dtype_code(key_out)),
-          "read_kv8");
+    const int bits = slots_of(slots, n, "read_kv8");
+    const auto options = k_codes.options().dtype(dtype);
+    const at::Tensor key = at::empty({n, H, 128}, options), value = at::empty({n, H, 128}, options);
+    const int out_dtype = dtype_code(key);
+    if (n > 0)
+        check(starkv_read_kv8(stream_of(k_codes), k_codes.data_ptr(), v_codes.data_ptr(), k_codes.stride(0),
+                              k_codes.stride(1), k_codes.stride(2), code, exponents.data_ptr<int8_t>(),
+                              exponents.stride(0), exponents.stride(1), (int)k_codes.size(1), k_codes.size(0),
+                              slots.data_ptr(), bits, as_int(n, "tokens"), (int)H, key.data_ptr(), value.data_ptr(), out_dtype),
+              "read_kv8");
+    return {key, value};
 }
 
 // One token's attention over an 8-bit cache; window 0: all tokens.
-void decode_kv8(const at::Tensor& query, const at::Tensor& k_codes, const at::Tensor& v_codes, const at::Tensor& exponents,
-                const at::Tensor& block_table, const at::Tensor& seq_lens, int64_t max_seq_len, int64_t window,
-                int64_t sinks, double scale, const at::Tensor& out) {
+at::Tensor decode_kv8(const at::Tensor& query, const at::Tensor& k_codes, const at::Tensor& v_codes,
+                      const at::Tensor& exponents, const at::Tensor& block_table, const at::Tensor& seq_lens,
+                      int64_t max_seq_len, int64_t window, int64_t sinks, double scale) {
     const c10::DeviceGuard guard(query.device());
     const int code = check_cache8(k_codes, v_codes, exponents, "decode_kv8");
     const int64_t n = query.size(0);
     const int H = (int)query.size(1), Hkv = (int)k_codes.size(2);
     check_query(query, query, Hkv, "decode_kv8");
-    check_query(out, query, Hkv, "decode_kv8");
     check_table(block_table, seq_lens, n, "decode_kv8");
-    TORCH_CHECK(out.sizes() == query.sizes(), "starkv.decode_kv8: out as query");
-    at::assert_no_internal_overlap(out);
+    const at::Tensor out = at::empty(query.sizes(), query.options());
+    if (n == 0) return out;
     const int span = as_int(max_seq_len, "max_seq_len"), w = as_int(window, "window"), s = as_int(sinks, "sinks");
     const at::Tensor ws = workspace(query, starkv_decode_kv8_workspace_bytes((int)n, H, Hkv, span, w, s));
     check(starkv_decode_kv8(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), dtype_code(query),
@@ -645,6 +650,7 @@ void decode_kv8(const at::Tensor& query, const at::Tensor& k_codes, const at::Te
                             i32(seq_lens, "seq_lens"), (int)n, H, Hkv, span, w, s, (float)scale, out.data_ptr(),
                             out.stride(0), out.stride(1), ws.data_ptr(), (size_t)ws.numel()),
           "decode_kv8");
+    return out;
 }
 
 // A decode step's slots (int64) and lengths (int32) from its positions (int64).
@@ -751,15 +757,14 @@ TORCH_LIBRARY(starkv, m) {
     m.def("evict(Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, Tensor seq_lens, Tensor weights, "
           "int keep, int sink, int recent, Tensor(c!) new_lens, Tensor(d!) new_weights) -> ()");
     m.def("window_decode(Tensor query, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, "
-          "int max_seq_len, int window, int sinks, float scale, Tensor(a!) out) -> ()");
+          "int max_seq_len, int window, int sinks, float scale) -> Tensor");
     m.def("prefill_window(Tensor query, Tensor key, Tensor value, Tensor cu_seqlens, Tensor blocks, int window, "
           "int sinks, float scale, Tensor(a!) out) -> ()");
     m.def("write_kv8(Tensor key, Tensor value, Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) exponents, "
           "Tensor slots) -> ()");
-    m.def("read_kv8(Tensor k_codes, Tensor v_codes, Tensor exponents, Tensor slots, Tensor(a!) key_out, "
-          "Tensor(b!) value_out) -> ()");
+    m.def("read_kv8(Tensor k_codes, Tensor v_codes, Tensor exponents, Tensor slots, ScalarType dtype) -> (Tensor, Tensor)");
     m.def("decode_kv8(Tensor query, Tensor k_codes, Tensor v_codes, Tensor exponents, Tensor block_table, "
-          "Tensor seq_lens, int max_seq_len, int window, int sinks, float scale, Tensor(a!) out) -> ()");
+          "Tensor seq_lens, int max_seq_len, int window, int sinks, float scale) -> Tensor");
     m.def("decode_slots(Tensor block_table, Tensor positions, int block_size, Tensor(a!) slots, "
           "Tensor(b!) seq_lens) -> ()");
     m.def("greedy_step(Tensor logits, Tensor(a!) tokens, Tensor(b!) positions) -> ()");

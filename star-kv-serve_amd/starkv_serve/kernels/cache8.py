@@ -79,11 +79,7 @@ def read_kv8(cache: Cache8, slot_mapping: torch.Tensor, dtype: torch.dtype = tor
     _hip.require_cuda(*cache.tensors, slot_mapping)
     _hip.refuse_grad("read_kv8")
     slots = _slots("read_kv8", slot_mapping)
-    shape = (slots.shape[0], cache.k.shape[2], cache.k.shape[3])
-    k, v = (torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
-    if slots.shape[0]:
-        _hip.ops().read_kv8(*cache.tensors, slots, k, v)
-    return k, v
+    return _hip.ops().read_kv8(*cache.tensors, slots, dtype)
 
 
 def paged_decode_8(query: torch.Tensor, cache: Cache8, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -94,8 +90,5 @@ def paged_decode_8(query: torch.Tensor, cache: Cache8, block_table: torch.Tensor
     of which nothing is seen are not read, nor their entries of the block table."""
     _hip.require_cuda(query, *cache.tensors, block_table, seq_lens)
     _hip.refuse_grad("paged_decode_8", query)
-    out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    if query.shape[0]:
-        _hip.ops().decode_kv8(query, *cache.tensors, _as_i32(block_table), _as_i32(seq_lens), int(max_seq_len),
-                              *sizes(window), float(scale), out)
-    return out
+    return _hip.ops().decode_kv8(query, *cache.tensors, _as_i32(block_table), _as_i32(seq_lens), int(max_seq_len),
+                                 *sizes(window), float(scale))

@@ -39,8 +39,5 @@ def paged_decode_window(query: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     away. A row without tokens is zero, one whose scores are all -inf NaN."""
     _hip.require_cuda(query, k_cache, v_cache, block_table, seq_lens)
     _hip.refuse_grad("paged_decode_window", query, k_cache, v_cache)
-    out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    if query.shape[0]:
-        _hip.ops().window_decode(query, k_cache, v_cache, _as_i32(block_table), _as_i32(seq_lens), int(max_seq_len),
-                                 *sizes(window), float(scale), out)
-    return out
+    return _hip.ops().window_decode(query, k_cache, v_cache, _as_i32(block_table), _as_i32(seq_lens), int(max_seq_len),
+                                    *sizes(window), float(scale))
