@@ -405,7 +405,7 @@ int starkv_prefill_attention(void *stream, const void *query, int64_t q_s0, int6
 /*
  * Keys and values [T, num_kv_heads, 128] of bf16 or fp32 (one dtype, each its own element strides,
  * last dimension contiguous) as the contiguous fp16 tensors starkv_prefill_attention takes, in one
- * launch.
+ * launch. key and key_out may be null: values alone.
  */
 int starkv_prefill_to_half(void *stream, const void *key, int64_t k_s0, int64_t k_s1, void *key_out,
                            const void *value, int64_t v_s0, int64_t v_s1, void *value_out, int dtype, int num_tokens,
@@ -562,7 +562,8 @@ int starkv_evict(void *stream, void *k_cache, void *v_cache, int64_t c_s0, int64
  * starkv_window_decode: the decode over a bf16 or fp16 cache through a window; lengths are clamped to max_seq_len. At
  * most 16 query heads a KV head. A row that sees no token gives zeros, one whose scores are all -inf NaN.
  *
- * starkv_prefill_window: starkv_prefill_attention through a window.
+ * starkv_prefill_window: starkv_prefill_attention through a window. Keys are fp16, with the strides of the values, or, with
+ * bf16 queries, bf16 of any strides; values are fp16.
  *
  * An 8-bit cache: k_codes and v_codes [num_blocks, block_size, num_kv_heads, 128] of one byte (code_type; byte strides
  * c_s0, c_s1, c_s2 shared by both, multiples of 16, rows 16-byte aligned; block_size 16 * 2^s up to 1024), and exponents
@@ -591,8 +592,8 @@ int starkv_window_decode(void *stream, const void *query, int64_t q_s0, int64_t 
                          int sinks, float scale, void *out, int64_t o_s0, int64_t o_s1, void *workspace,
                          size_t workspace_bytes);
 int starkv_prefill_window(void *stream, const void *query, int64_t q_s0, int64_t q_s1, int q_dtype, const void *key,
-                          const void *value, int64_t kv_s0, int64_t kv_s1, int kv_dtype, const int32_t *cu_seqlens,
-                          const int32_t *blocks, int num_blocks, int num_heads, int num_kv_heads, int head_size,
+                          int64_t k_s0, int64_t k_s1, int k_dtype, const void *value, int64_t v_s0, int64_t v_s1,
+                          const int32_t *cu_seqlens, const int32_t *blocks, int num_blocks, int num_heads, int num_kv_heads, int head_size,
                           int window, int sinks, float scale, void *out, int64_t o_s0, int64_t o_s1, int out_dtype);
 size_t starkv_write_kv8_workspace_bytes(int n, int64_t num_blocks, int block_size);
 int starkv_write_kv8(void *stream, const void *key, int64_t k_s0, int64_t k_s1, const void *value, int64_t v_s0,

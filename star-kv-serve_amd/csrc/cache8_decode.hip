@@ -38,7 +38,6 @@ namespace starkv {
 namespace {
 
 constexpr int D8_THR = 256;
-constexpr int D8_CHUNK = 512;       // pages whose places are looked up at a time
 constexpr int D8_PART = 132;        // floats of a partial: reference, sum of weights, 0, 0, out[128]
 constexpr int D8_MAX_GROUP = 16;    // query heads per KV head: the columns of a matrix product
 constexpr float D8_LEAST = -3.402823466e38f;  // the reference of tokens whose scores are all -inf
@@ -80,10 +79,14 @@ struct Range8 {
 __device__ __forceinline__ Range8 find_range(const Decode8Params& p, int range) {
     const int lane = threadIdx.x & 63;
     int own = 0, end = 0, total = 0;
-    for (int b0 = 0; b0 < p.n; b0 += 64) {
-        own = b0 + lane < p.n ? seen_by(p, b0 + lane).pages : 0;
-        end = scan_wave(own);
-        total += __builtin_amdgcn_readlane(end, 63);
+    if (p.n == 1) {
+        own = end = total = seen_by(p, 0).pages;
+    } else {
+        for (int b0 = 0; b0 < p.n; b0 += 64) {
+            own = b0 + lane < p.n ? seen_by(p, b0 + lane).pages : 0;
+            end = scan_wave(own);
+            total += __builtin_amdgcn_readlane(end, 63);
+        }
     }
     Range8 g;
     g.per = max((total + p.ranges - 1) / p.ranges, 8);  // two pages a wave
@@ -128,28 +131,66 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
     w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
-// Pages [k0, k1) of request b's, for KV head h: its query heads' result where that is all the request has, else a
-// partial of the range.
+// What a wave's lanes know of 32 pairs of pages: pages c0, c0 + 1, c0 + 8, c0 + 9, ... of the request's. The block, the places
+// that are seen | the page's place in the block << 16, the exponents (which the rows need not wait for).
+struct Look8 {
+    int blk, ek, ev;
+    uint32_t see;
+};
+
+__device__ __forceinline__ Look8 look_up(const Decode8Params& p, const SeenPages& seen, int b, int h, int c0, int k1) {
+    const int lane = threadIdx.x & 63, mine = c0 + 8 * (lane >> 1) + (lane & 1);
+    Look8 l = {0, 0, 0, 0};
+    if (mine < k1) {
+        const int pg = seen.page(mine);
+        l.blk = p.bt[b * p.bt_s0 + (pg >> p.bs_shift) * p.bt_s1];
+        l.see = seen.mask(pg) | (uint32_t)(pg & ((1 << p.bs_shift) - 1)) << 16;
+        if (l.blk < 0 || l.blk >= p.num_blocks) l.blk = l.see = 0;  // no block of the cache: no tokens
+        const int8_t* e = p.ex + l.blk * p.x_s0 + h * p.x_s1;
+        l.ek = e[0];
+        l.ev = e[1];
+    }
+    return l;
+}
+
+// A KV head's part of a range, from the block index: request by request, the result of its query heads where the range has
+// all of a request's pages, else a partial. What lies where and the queries of the next request are on their way while
+// the waves of one meet. MANY: 9 to 16 query heads.
 template <int CT, int QDT, bool MANY>
-__device__ __forceinline__ void decode8_request(const Decode8Params& p, int4* s_page, float* s_dyn, const SeenPages& seen,
-                                                int range, int h, int b, int k0, int k1, int per) {
+__global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params p) {
+    extern __shared__ float s_dyn[];  // [4 waves][G][D8_PART] for the merge
+    const int range = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv, H = p.Hkv * p.G;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = MANY ? lane & 15 : lane & 7, quad = lane >> 4;  // the lane's query head
-    const int H = p.Hkv * p.G, mask = (1 << p.bs_shift) - 1;
-    const bool whole = k0 == 0 && k1 == seen.pages;
-    if (h == 0 && k0 == 0 && tid == 0) p.where[b] = make_int2(range, 1 + (seen.pages - k1 + per - 1) / per);
-
-    // The head's row: dimensions 64 st + 16 quad .. + 15, two operands; their fp16 values times 2^up.
-    uint4 qf[2][2];
-    float sc = p.sc;
-    {
-        uint4 w[2][2];
+    if (p.ranges == 1)  // no merge follows, which writes the rows that see no token
+        for (int b = 0; b < p.n; ++b)
+            if (seen_by(p, b).pages == 0)
+                for (int i = tid; i < p.G * 128; i += D8_THR)
+                    store_f(p.out, b * p.o_s0 + (h * p.G + (i >> 7)) * p.o_s1 + (i & 127), QDT, 0.f);
+    const Range8 g = find_range(p, range);
+    if (g.left <= 0) return;
+    const uint8_t* kh = p.kc + h * p.c_s2 + 16 * quad + (int64_t)(lane & 15) * p.c_s1;
+    const uint8_t* vh = p.vc + h * p.c_s2 + 8 * (lane & 15) + (int64_t)(4 * quad) * p.c_s1;
+    // The head's row: dimensions 64 st + 16 quad .. + 15, two operands.
+    uint4 w[2][2];
+    const auto load_q = [&](int b) {
 #pragma unroll
         for (int st = 0; st < 2; ++st)
 #pragma unroll
             for (int x = 0; x < 2; ++x)
                 w[st][x] = col < p.G ? *(const uint4*)(p.q + b * p.q_s0 + (int64_t)(h * p.G + col) * p.q_s1 + 64 * st + 16 * quad + 8 * x)
                                      : make_uint4(0, 0, 0, 0);
+    };
+    int b = g.b, k0 = g.k, left = g.left;
+    SeenPages seen = seen_by(p, b);
+    int k1 = min(seen.pages, k0 + left);
+    Look8 ahead = look_up(p, seen, b, h, k0 + 2 * wave, k1);
+    load_q(b);
+    for (;;) {
+        const bool whole = k0 == 0 && k1 == seen.pages;
+        if (h == 0 && k0 == 0 && tid == 0) p.where[b] = make_int2(range, 1 + (seen.pages - k1 + g.per - 1) / g.per);
+        uint4 qf[2][2];  // fp16 values of the queries, times 2^up
+        float sc = p.sc;
         if constexpr (QDT == STARKV_F16) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) qf[i >> 1][i & 1] = w[i >> 1][i & 1];
@@ -179,206 +220,188 @@ __device__ __forceinline__ void decode8_request(const Decode8Params& p, int4* s_
                 qf[i >> 1][i & 1] = __builtin_bit_cast(uint4, o);
             }
         }
-    }
-    const uint8_t* kh = p.kc + h * p.c_s2 + 16 * quad + (int64_t)(lane & 15) * p.c_s1;
-    const uint8_t* vh = p.vc + h * p.c_s2 + 8 * (lane & 15) + (int64_t)(4 * quad) * p.c_s1;
-    float m = -INFINITY, r = -INFINITY, l = 0.f;
-    f32x4_t acc[8];
+        float m = -INFINITY, r = -INFINITY, l = 0.f;
+        f32x4_t acc[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < 8; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-    for (int c0 = k0; c0 < k1; c0 += D8_CHUNK) {
-        const int count = min(D8_CHUNK, k1 - c0);
-        __syncthreads();  // the last look's pages, or the request's before, are done with
-        for (int i = tid; i < count; i += D8_THR) {
-            const int pg = seen.page(c0 + i);
-            int blk = p.bt[b * p.bt_s0 + (pg >> p.bs_shift) * p.bt_s1];
-            uint32_t see = seen.mask(pg);
-            int ex = 0;
-            if (blk < 0 || blk >= p.num_blocks) {
-                blk = 0;  // no block of the cache: no tokens
-                see = 0;
-            } else {
-                const int8_t* e = p.ex + blk * p.x_s0 + h * p.x_s1;
-                ex = (uint8_t)e[0] | (int)e[1] << 8;
-            }
-            s_page[i] = make_int4(blk, pg & mask, (int)see, ex);
-        }
-        __syncthreads();
-        for (int i = 2 * wave; i < count; i += 8) {
-            uint32_t see[2];
-            int at[2], place[2], ex[2];
+        // A wave takes pages k0 + 2 wave and the next, k0 + 2 wave + 8 and the next, ..., 32 such pairs' places at a time in its
+        // lanes: what lies where, which places are seen and the exponents, which the rows need not wait for.
+        for (int c0 = k0 + 2 * wave; c0 < k1; c0 += 8 * 32) {
+            const Look8 now = c0 < k0 + 8 ? ahead : look_up(p, seen, b, h, c0, k1);
+            const int pairs = min((k1 - c0 + 7) / 8, 32);
+            for (int i = 0; i < pairs; ++i) {
+                uint32_t see[2];
+                int at[2], place[2], ek[2], ev[2];
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const int4 v = s_page[min(i + x, count - 1)];
-                at[x] = __builtin_amdgcn_readfirstlane(v.x);
-                place[x] = __builtin_amdgcn_readfirstlane(v.y);
-                see[x] = i + x < count ? (uint32_t)__builtin_amdgcn_readfirstlane(v.z) : 0u;
-                ex[x] = __builtin_amdgcn_readfirstlane(v.w);
-            }
-            if ((see[0] | see[1]) == 0) continue;
-            uint4 kr[2][2];
-            uint2 vr[2][4];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                // A page of which nothing is seen reads the other one again. A page lies within its block whatever
-                // the request's length, so every row of it can be read.
-                const int y = see[x] ? x : x ^ 1;
-                const int64_t base = at[y] * p.c_s0 + (int64_t)(16 * place[y]) * p.c_s1;
-#pragma unroll
-                for (int st = 0; st < 2; ++st) kr[x][st] = *(const uint4*)(kh + base + 64 * st);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) vr[x][j] = *(const uint2*)(vh + base + j * p.c_s1);
-            }
-            float sv[2][4], up[2];  // scores; the exponents of the values
-            float mx = -INFINITY, rx = -INFINITY;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                f32x4_t d = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    const uint2 a = c8_halves<CT>(kr[x][st].x), c = c8_halves<CT>(kr[x][st].y);
-                    const uint2 e = c8_halves<CT>(kr[x][st].z), f = c8_halves<CT>(kr[x][st].w);
-                    d = mfma_f16(make_uint4(a.x, a.y, c.x, c.y), qf[st][0], d);
-                    d = mfma_f16(make_uint4(e.x, e.y, f.x, f.y), qf[st][1], d);
+                for (int x = 0; x < 2; ++x) {
+                    at[x] = __builtin_amdgcn_readlane(now.blk, 2 * i + x);
+                    const uint32_t v = (uint32_t)__builtin_amdgcn_readlane((int)now.see, 2 * i + x);
+                    place[x] = (int)(v >> 16);
+                    see[x] = v & 0xffffu;
                 }
-                const float by = sc * c8_scale((int)(int8_t)ex[x]);
-                const int ev = ex[x] >> 8;
-                up[x] = ev == C8_NAN ? __builtin_nanf("") : (float)ev;
-                if (see[x] == 0) up[x] = 0.f;
+                if ((see[0] | see[1]) == 0) continue;
+                uint4 kr[2][2];
+                uint2 vr[2][4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) sv[x][k] = d[k] * by;
-                if (see[x] != 0xffffu) {  // tokens out of sight: no score, and codes of 0 (an e4m3 code may be NaN)
+                for (int x = 0; x < 2; ++x) {
+                    // A page of which nothing is seen reads the other one again. A page lies within its block whatever
+                    // the request's length, so every row of it can be read.
+                    const int y = see[x] ? x : x ^ 1;
+                    const int64_t base = at[y] * p.c_s0 + (int64_t)(16 * place[y]) * p.c_s1;
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) kr[x][st] = *(const uint4*)(kh + base + 64 * st);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) vr[x][j] = *(const uint2*)(vh + base + j * p.c_s1);
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    ek[x] = __builtin_amdgcn_readlane(now.ek, 2 * i + x);
+                    ev[x] = __builtin_amdgcn_readlane(now.ev, 2 * i + x);
+                }
+                float sv[2][4], up[2];  // scores; the exponents of the values
+                float mx = -INFINITY, rx = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    f32x4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        const uint2 a = c8_halves<CT>(kr[x][st].x), c = c8_halves<CT>(kr[x][st].y);
+                        const uint2 e = c8_halves<CT>(kr[x][st].z), f = c8_halves<CT>(kr[x][st].w);
+                        d = mfma_f16(make_uint4(a.x, a.y, c.x, c.y), qf[st][0], d);
+                        d = mfma_f16(make_uint4(e.x, e.y, f.x, f.y), qf[st][1], d);
+                    }
+                    const float by = sc * c8_scale(ek[x]);
+                    up[x] = ev[x] == C8_NAN && see[x] != 0 ? __builtin_nanf("") : (float)ev[x];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) sv[x][k] = d[k] * by;
+                    if (see[x] != 0xffffu) {  // tokens out of sight: no score, and codes of 0 (an e4m3 code may be NaN)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const bool ok = see[x] >> (4 * quad + k) & 1u;
+                            sv[x][k] = ok ? sv[x][k] : -INFINITY;
+                            vr[x][k] = ok ? vr[x][k] : make_uint2(0, 0);
+                        }
+                    }
+                    const float px = fmaxf(fmaxf(sv[x][0], sv[x][1]), fmaxf(sv[x][2], sv[x][3]));
+                    mx = fmaxf(mx, px);
+                    rx = fmaxf(rx, px + up[x]);
+                }
+                mx = max_rows(mx);
+                rx = max_rows(rx);
+                m = fmaxf(m, D8_LEAST);
+                r = fmaxf(r, D8_LEAST);
+                if (__builtin_amdgcn_ballot_w64(mx > m + 15.f || rx > r + 15.f) != 0) {
+                    const float mn = mx > m + 15.f ? mx - 7.f : m, rn = rx > r + 15.f ? rx - 7.f : r;
+                    l *= mn == m ? 1.f : exp2f(m - mn);
+                    const float alpha = rn == r ? 1.f : exp2f(r - rn);
+                    m = mn;
+                    r = rn;
+#pragma unroll
+                    for (int i8 = 0; i8 < 8; ++i8) acc[i8] *= alpha;
+                }
+                float pe[2][4];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const float f = exp2f(up[x] + (m - r));
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const bool ok = see[x] >> (4 * quad + k) & 1u;
-                        sv[x][k] = ok ? sv[x][k] : -INFINITY;
-                        vr[x][k] = ok ? vr[x][k] : make_uint2(0, 0);
+                        const float w = ok ? exp2f(sv[x][k] - m) : 0.f;
+                        l += w;
+                        pe[x][k] = ok ? w * f : 0.f;
                     }
                 }
-                const float px = fmaxf(fmaxf(sv[x][0], sv[x][1]), fmaxf(sv[x][2], sv[x][3]));
-                mx = fmaxf(mx, px);
-                rx = fmaxf(rx, px + up[x]);
-            }
-            mx = max_rows(mx);
-            rx = max_rows(rx);
-            m = fmaxf(m, D8_LEAST);
-            r = fmaxf(r, D8_LEAST);
-            if (__builtin_amdgcn_ballot_w64(mx > m + 15.f || rx > r + 15.f) != 0) {
-                const float mn = mx > m + 15.f ? mx - 7.f : m, rn = rx > r + 15.f ? rx - 7.f : r;
-                l *= mn == m ? 1.f : exp2f(m - mn);
-                const float alpha = rn == r ? 1.f : exp2f(r - rn);
-                m = mn;
-                r = rn;
-#pragma unroll
-                for (int i8 = 0; i8 < 8; ++i8) acc[i8] *= alpha;
-            }
-            float pe[2][4];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const float f = exp2f(up[x] + (m - r));
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const bool ok = see[x] >> (4 * quad + k) & 1u;
-                    const float w = ok ? exp2f(sv[x][k] - m) : 0.f;
-                    l += w;
-                    pe[x][k] = ok ? w * f : 0.f;
-                }
-            }
-            // The weights' values: the first, and what it left; up to 8 heads the lanes of the second columns take that.
-            uint4 pw[MANY ? 2 : 1];
-            pw[0] = make_uint4(split_half(pe[0][0], pe[0][1]), split_half(pe[0][2], pe[0][3]),
-                               split_half(pe[1][0], pe[1][1]), split_half(pe[1][2], pe[1][3]));
-            const uint4 rest = make_uint4(split_half(pe[0][0], pe[0][1]), split_half(pe[0][2], pe[0][3]),
-                                          split_half(pe[1][0], pe[1][1]), split_half(pe[1][2], pe[1][3]));
-            if constexpr (MANY) {
-                pw[1] = rest;
-            } else if (lane & 8) {
-                pw[0] = rest;
-            }
-#pragma unroll
-            for (int hd = 0; hd < 2; ++hd) {
-                uint32_t w[2][4];
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) w[x][j] = hd ? vr[x][j].y : vr[x][j].x;
-                    transpose4(w[x]);
+                // The weights' values: the first, and what it left; up to 8 heads the lanes of the second columns take that.
+                uint4 pw[MANY ? 2 : 1];
+                pw[0] = make_uint4(split_half(pe[0][0], pe[0][1]), split_half(pe[0][2], pe[0][3]),
+                                   split_half(pe[1][0], pe[1][1]), split_half(pe[1][2], pe[1][3]));
+                const uint4 rest = make_uint4(split_half(pe[0][0], pe[0][1]), split_half(pe[0][2], pe[0][3]),
+                                              split_half(pe[1][0], pe[1][1]), split_half(pe[1][2], pe[1][3]));
+                if constexpr (MANY) {
+                    pw[1] = rest;
+                } else if (lane & 8) {
+                    pw[0] = rest;
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint2 a = c8_halves<CT>(w[0][i]), c = c8_halves<CT>(w[1][i]);
-                    const uint4 vt = make_uint4(a.x, a.y, c.x, c.y);
+                for (int hd = 0; hd < 2; ++hd) {
+                    uint32_t w[2][4];
 #pragma unroll
-                    for (int k = 0; k < (MANY ? 2 : 1); ++k) acc[4 * hd + i] = mfma_f16(vt, pw[k], acc[4 * hd + i]);
+                    for (int x = 0; x < 2; ++x) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w[x][j] = hd ? vr[x][j].y : vr[x][j].x;
+                        transpose4(w[x]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint2 a = c8_halves<CT>(w[0][i]), c = c8_halves<CT>(w[1][i]);
+                        const uint4 vt = make_uint4(a.x, a.y, c.x, c.y);
+#pragma unroll
+                        for (int k = 0; k < (MANY ? 2 : 1); ++k) acc[4 * hd + i] = mfma_f16(vt, pw[k], acc[4 * hd + i]);
+                    }
                 }
             }
         }
-    }
-    l = sum_rows(l);
-    if constexpr (!MANY) {  // both columns of a head: lanes 8 apart in a row of 16
-#pragma unroll
-        for (int i8 = 0; i8 < 8; ++i8)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) acc[i8][x] += dpp_f<0x128>(acc[i8][x]);  // row_ror:8
-    }
-    if (col < p.G && (MANY || !(lane & 8))) {
-        float* w = s_dyn + (wave * p.G + col) * D8_PART;
-        if (quad == 0) *(float4*)w = make_float4(m, l, r, 0.f);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {  // dimensions 32 quad + 8 x + i
-            *(float4*)(w + 4 + 32 * quad + 8 * x) = make_float4(acc[0][x], acc[1][x], acc[2][x], acc[3][x]);
-            *(float4*)(w + 8 + 32 * quad + 8 * x) = make_float4(acc[4][x], acc[5][x], acc[6][x], acc[7][x]);
+        left -= k1 - k0;
+        int next = b;
+        SeenPages then = seen;
+        if (left > 0) {
+            do then = seen_by(p, ++next);
+            while (then.pages == 0);
+            ahead = look_up(p, then, next, h, 2 * wave, min(then.pages, left));
+            load_q(next);
         }
-    }
-    __syncthreads();
-    for (int i = tid; i < p.G * 128; i += D8_THR) {
-        const int g = i >> 7, d = i & 127;
-        const float* w = s_dyn + g * D8_PART;
-        float M = -INFINITY, R = -INFINITY, lt = 0.f, a = 0.f;
+        l = sum_rows(l);
+        if constexpr (!MANY) {  // both columns of a head: lanes 8 apart in a row of 16
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            M = fmaxf(M, w[k * p.G * D8_PART]);
-            R = fmaxf(R, w[k * p.G * D8_PART + 2]);
-        }
+            for (int i8 = 0; i8 < 8; ++i8)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float* x = w + k * p.G * D8_PART;
-            // A wave without tokens has references of -inf and sums of 0.
-            lt = fmaf(x[1], x[0] == -INFINITY ? 1.f : exp2f(x[0] - M), lt);
-            a = fmaf(x[4 + d], x[2] == -INFINITY ? 1.f : exp2f(x[2] - R), a);
+                for (int x = 0; x < 4; ++x) acc[i8][x] += dpp_f<0x128>(acc[i8][x]);  // row_ror:8
         }
-        const int hq = h * p.G + g;
-        const float half = exp2f(0.5f * (R - M));  // in two steps: its square may be past fp32's range where the result is not
-        // A partial without weight (scores of -inf alone) adds 0 to the others', not 0 times 0 / 0.
-        const float o = M == -INFINITY || (lt == 0.f && !whole) ? 0.f : a / lt * half * half;
-        if (whole) {
-            store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, QDT, o);
-        } else {
-            float* pp = p.part + ((int64_t)(2 * range + (k0 == 0)) * H + hq) * D8_PART;
-            if (d == 0) *(float4*)pp = make_float4(M, lt, 0.f, 0.f);
-            pp[4 + d] = o;
+        __syncthreads();  // the request before is done with s_dyn
+        if (col < p.G && (MANY || !(lane & 8))) {
+            float* w = s_dyn + (wave * p.G + col) * D8_PART;
+            if (quad == 0) *(float4*)w = make_float4(m, l, r, 0.f);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {  // dimensions 32 quad + 8 x + i
+                *(float4*)(w + 4 + 32 * quad + 8 * x) = make_float4(acc[0][x], acc[1][x], acc[2][x], acc[3][x]);
+                *(float4*)(w + 8 + 32 * quad + 8 * x) = make_float4(acc[4][x], acc[5][x], acc[6][x], acc[7][x]);
+            }
         }
-    }
-}
-
-// A KV head's part of a range, from the block index. MANY: 9 to 16 query heads.
-template <int CT, int QDT, bool MANY>
-__global__ __launch_bounds__(D8_THR, 4) void decode8_kernel(const Decode8Params p) {
-    __shared__ int4 s_page[D8_CHUNK];  // block, place in the block, places that are seen, exponents
-    extern __shared__ float s_dyn[];   // [4 waves][G][D8_PART] for the merge
-    const int range = blockIdx.x / p.Hkv, h = blockIdx.x % p.Hkv;
-    Range8 g = find_range(p, range);
-    if (p.ranges == 1)  // no merge follows, which writes the rows that see no token
-        for (int b = 0; b < p.n; ++b)
-            if (seen_by(p, b).pages == 0)
-                for (int i = threadIdx.x; i < p.G * 128; i += D8_THR)
-                    store_f(p.out, b * p.o_s0 + (h * p.G + (i >> 7)) * p.o_s1 + (i & 127), QDT, 0.f);
-    for (; g.left > 0; ++g.b, g.k = 0) {
-        const SeenPages seen = seen_by(p, g.b);
-        const int k1 = min(seen.pages, g.k + g.left);
-        if (k1 > 0) decode8_request<CT, QDT, MANY>(p, s_page, s_dyn, seen, range, h, g.b, g.k, k1, g.per);
-        g.left -= k1 - g.k;
+        __syncthreads();
+        for (int i = tid; i < p.G * 128; i += D8_THR) {
+            const int g = i >> 7, d = i & 127;
+            const float* w = s_dyn + g * D8_PART;
+            float M = -INFINITY, R = -INFINITY, lt = 0.f, a = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                M = fmaxf(M, w[k * p.G * D8_PART]);
+                R = fmaxf(R, w[k * p.G * D8_PART + 2]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float* x = w + k * p.G * D8_PART;
+                // A wave without tokens has references of -inf and sums of 0.
+                lt = fmaf(x[1], x[0] == -INFINITY ? 1.f : exp2f(x[0] - M), lt);
+                a = fmaf(x[4 + d], x[2] == -INFINITY ? 1.f : exp2f(x[2] - R), a);
+            }
+            const int hq = h * p.G + g;
+            const float half = exp2f(0.5f * (R - M));  // in two steps: its square may be past fp32's range where the result is not
+            // A partial without weight (scores of -inf alone) adds 0 to the others', not 0 times 0 / 0.
+            const float o = M == -INFINITY || (lt == 0.f && !whole) ? 0.f : a / lt * half * half;
+            if (whole) {
+                store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, QDT, o);
+            } else {
+                float* pp = p.part + ((int64_t)(2 * range + (k0 == 0)) * H + hq) * D8_PART;
+                if (d == 0) *(float4*)pp = make_float4(M, lt, 0.f, 0.f);
+                pp[4 + d] = o;
+            }
+        }
+        if (left <= 0) break;
+        b = next;
+        seen = then;
+        k0 = 0;
+        k1 = min(seen.pages, left);
     }
 }
 
@@ -402,6 +425,9 @@ __global__ __launch_bounds__(64) void merge8_kernel(const Decode8Params p) {
     for (int c0 = 0; c0 < where.y; c0 += 64) {
         const int count = min(where.y - c0, 64);
         const float* mine = part(c0 + min(lane, count - 1));
+        float2 v[8];  // the first eight's sums are on their way with the references
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = *(const float2*)(part(c0 + min(u, count - 1)) + 4 + 2 * lane);
         const float m = lane < count ? mine[0] : -INFINITY, l = lane < count ? mine[1] : 0.f;
         const float most = fmaxf(M, wave_max(m)), before = M == -INFINITY ? 1.f : exp2f(M - most);
         M = most;
@@ -410,9 +436,10 @@ __global__ __launch_bounds__(64) void merge8_kernel(const Decode8Params p) {
         a.x *= before;
         a.y *= before;
         for (int s0 = 0; s0 < count; s0 += 8) {
-            float2 v[8];
+            if (s0 > 0) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = *(const float2*)(part(c0 + min(s0 + u, count - 1)) + 4 + 2 * lane);
+                for (int u = 0; u < 8; ++u) v[u] = *(const float2*)(part(c0 + min(s0 + u, count - 1)) + 4 + 2 * lane);
+            }
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (s0 + u) & 63));

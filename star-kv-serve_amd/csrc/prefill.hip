@@ -39,7 +39,8 @@
 // s < sinks: a workgroup takes the tiles that hold the first tokens and those from its first query's window on, and
 // tiles across an edge are masked (its later waves mask up to two whole ones). The scale goes onto
 // the fp32 scores there (one fused multiply-add in front of the exponential in place of a subtraction) and not into q, whose
-// fp16 values are then those of bf16 and fp16 queries themselves.
+// fp16 values are then those of bf16 and fp16 queries themselves; bf16 queries and keys are multiplied as they are, which
+// saves half of the conversion in front.
 #include <algorithm>
 #include <array>
 #include <type_traits>
@@ -64,7 +65,8 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 struct PrefillParams {
     const void* q; int64_t q_s0, q_s1; int q_dt;
-    const uint8_t* k; const uint8_t* v; int64_t kv_s0, kv_s1;  // bytes
+    const uint8_t* k; const uint8_t* v;                       // bytes, as their strides
+    int64_t k_s0, k_s1, v_s0, v_s1;
     const int32_t* cu;                                        // [P + 1]
     const int32_t* blocks; int nblocks;                       // [nblocks][2]: prompt, query block
     int Hq, G;
@@ -115,6 +117,13 @@ __device__ __forceinline__ half8_t pf_load_q(const PrefillParams& p, int64_t tok
     return r;
 }
 
+// 8 query dimensions of bf16 as they are, times `by` (1, -1 or 0).
+__device__ __forceinline__ bf16x8_t pf_load_q_bf16(const PrefillParams& p, int64_t tok, int hq, int d0, bool ok, float by) {
+    const uint4 w = ok && by != 0.f ? *(const uint4*)((const uint16_t*)p.q + tok * p.q_s0 + (int64_t)hq * p.q_s1 + d0) : make_uint4(0, 0, 0, 0);
+    const uint32_t flip = by < 0.f ? 0x80008000u : 0u;
+    return __builtin_bit_cast(bf16x8_t, make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip));
+}
+
 // 4 transposed 16-bit elements (see the file comment).
 __device__ __forceinline__ uint2 pf_tr(uint32_t addr) {
     typedef short s4_t __attribute__((ext_vector_type(4)));
@@ -139,7 +148,8 @@ __device__ __forceinline__ void pf_work(const PrefillParams& p, int& entry, int&
     }
 }
 
-template <int QDT, int ODT, bool WINDOW>
+// KDT: the type of the keys, fp16 or (through a window, with queries of the same) bf16.
+template <int QDT, int ODT, bool WINDOW, int KDT = STARKV_F16>
 __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) void prefill_kernel(const PrefillParams p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t s_kv[];  // K tiles 0, 1, V tiles 0, 1
     const int tid = threadIdx.x, lane = tid & 63, wave = rfl(tid >> 6);
@@ -168,29 +178,38 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
     // LDS bytes [1024 (PF_WAVES c + w), + 1024): rows 4 (PF_WAVES c + w) .. + 3; lane j writes
     // physical granule j % 16 of row (j / 16) of them, i.e. logical granule (j % 16) ^ pf_swz(row).
     const uint32_t base = lds_addr(s_kv);
-    uint32_t coff[PF_CPW];
+    uint32_t coff[PF_CPW], voff[PF_CPW];
 #pragma unroll
     for (int c = 0; c < PF_CPW; ++c) {
         const int row = (PF_WAVES * c + wave) * 4 + (lane >> 4);
-        coff[c] = (uint32_t)(row * p.kv_s0 + 16 * ((lane & 15) ^ pf_swz(row)));
+        coff[c] = (uint32_t)(row * p.k_s0 + 16 * ((lane & 15) ^ pf_swz(row)));
+        voff[c] = KDT == STARKV_F16 ? coff[c] : (uint32_t)(row * p.v_s0 + 16 * ((lane & 15) ^ pf_swz(row)));
     }
-    const int64_t kv0 = (int64_t)s * p.kv_s0 + (int64_t)hk * p.kv_s1;
+    const int64_t k0v = (int64_t)s * p.k_s0 + (int64_t)hk * p.k_s1, v0v = (int64_t)s * p.v_s0 + (int64_t)hk * p.v_s1;
     // Tile t of K (or V) into its buffer at LDS address dst.
-    auto issue = [&](const uint8_t* src, int t, uint32_t dst) {
+    auto issue = [&](bool val, int t, uint32_t dst) {
+        const int64_t s0 = KDT == STARKV_F16 || !val ? p.k_s0 : p.v_s0;  // fp16 keys have the values' strides
+        const uint8_t* src = val ? p.v + (KDT == STARKV_F16 ? k0v : v0v) : p.k + k0v;
         const int r0 = tile_of(t) * PF_KT;
         const int rows = max(0, min(PF_KT, L - r0));
-        int4v_t rs = buffer_rsrc(src + kv0 + (int64_t)r0 * p.kv_s0, (int)(rows * p.kv_s0));
+        const int64_t bytes = KDT == STARKV_F16 ? rows * s0 : rows > 0 ? (rows - 1) * s0 + 256 : 0;  // strides of any kind
+        int4v_t rs = buffer_rsrc(src + (int64_t)r0 * s0, (int)bytes);
 #pragma unroll
         for (int e = 0; e < 4; ++e) rs[e] = rfl(rs[e]);  // uniform by construction; the copies take them in SGPRs
 #pragma unroll
-        for (int c = 0; c < PF_CPW; ++c) lds_copy16(rs, dst + (uint32_t)(PF_WAVES * c + wave) * 1024u, coff[c]);
+        for (int c = 0; c < PF_CPW; ++c) lds_copy16(rs, dst + (uint32_t)(PF_WAVES * c + wave) * 1024u, val ? voff[c] : coff[c]);
     };
-    issue(p.k, 0, base);
+    issue(false, 0, base);
 
     // Q as the B operand of S^T = K Q^T: query n, dimensions 16 ks + 8 h .. + 7.
     half8_t qb[8];
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks) qb[ks] = pf_load_q<QDT>(p, (int64_t)s + qi, hq, 16 * ks + 8 * h, qi < L, sq);
+    for (int ks = 0; ks < 8; ++ks) {
+        if constexpr (KDT == STARKV_F16)
+            qb[ks] = pf_load_q<QDT>(p, (int64_t)s + qi, hq, 16 * ks + 8 * h, qi < L, sq);
+        else
+            qb[ks] = __builtin_bit_cast(half8_t, pf_load_q_bf16(p, (int64_t)s + qi, hq, 16 * ks + 8 * h, qi < L, sq));
+    }
 
     // Per-lane LDS addresses of buffer 0; the other buffer and the row blocks are immediates.
     // A of S^T: key row 32 mb + n, granule 2 ks + h (block mb = 1 is 32 rows further: the same
@@ -223,9 +242,13 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
-            for (int mb = 0; mb < 2; ++mb)
-                x[mb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(lds_ld<half8_t>(ka[ks] + (uint32_t)(B * PF_TILE + 8192 * mb)),
-                                                               qb[ks], x[mb], 0, 0, 0);
+            for (int mb = 0; mb < 2; ++mb) {
+                const half8_t k = lds_ld<half8_t>(ka[ks] + (uint32_t)(B * PF_TILE + 8192 * mb));
+                if constexpr (KDT == STARKV_F16)
+                    x[mb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[ks], x[mb], 0, 0, 0);
+                else
+                    x[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, qb[ks]), x[mb], 0, 0, 0);
+            }
     };
     // Tile t, its scores in sc, its V in buffer B; the next tile's scores (NEXT, into nx) are formed
     // beside the exponentials: matrix and vector work of one wave with no dependence between them.
@@ -317,15 +340,15 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
     auto step = [&](auto B, int t, f32x16_t* sc, f32x16_t* nx) {
         SKV_WAIT_VM_LGKM0(0);  // V tile t and K tile t + 1 have landed (this wave's copies)
         lds_barrier();         // every wave's copies; every wave done with K tile t and V tile t - 1
-        if (t + 2 < ntile) issue(p.k, t + 2, base + (uint32_t)(B * PF_TILE));
-        if (t + 1 < ntile) issue(p.v, t + 1, base + (uint32_t)((3 - B) * PF_TILE));
+        if (t + 2 < ntile) issue(false, t + 2, base + (uint32_t)(B * PF_TILE));
+        if (t + 1 < ntile) issue(true, t + 1, base + (uint32_t)((3 - B) * PF_TILE));
         if (t <= last) tile(B, t, sc, nx);
     };
     // Two workgroups share a CU (64 KB of LDS each).
     SKV_WAIT_VM_LGKM0(0);
     lds_barrier();
-    issue(p.v, 0, base + 2 * PF_TILE);
-    if (ntile > 1) issue(p.k, 1, base + PF_TILE);
+    issue(true, 0, base + 2 * PF_TILE);
+    if (ntile > 1) issue(false, 1, base + PF_TILE);
     if (last >= 0) scores(std::integral_constant<int, 0>{}, sa);
     for (int t = 0; t < ntile; t += 2) {
         step(std::integral_constant<int, 0>{}, t, sa, sb);
@@ -378,7 +401,7 @@ struct ToHalfParams {
 
 template <int DT>
 __global__ __launch_bounds__(256) void to_half_kernel(const ToHalfParams p) {
-    const int z = blockIdx.y;
+    const int z = 1 - blockIdx.y;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.pieces; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i >> 4, t = row / p.H;
         const int h = (int)(row - t * p.H);
@@ -402,6 +425,12 @@ const void* pf_pick(int odt) {
     if (odt == STARKV_F32) return (const void*)&prefill_kernel<QDT, STARKV_F32, WINDOW>;
     if (odt == STARKV_F16) return (const void*)&prefill_kernel<QDT, STARKV_F16, WINDOW>;
     return (const void*)&prefill_kernel<QDT, STARKV_BF16, WINDOW>;
+}
+
+const void* pf_pick_bf16(int odt) {
+    if (odt == STARKV_F32) return (const void*)&prefill_kernel<STARKV_BF16, STARKV_F32, true, STARKV_BF16>;
+    if (odt == STARKV_F16) return (const void*)&prefill_kernel<STARKV_BF16, STARKV_F16, true, STARKV_BF16>;
+    return (const void*)&prefill_kernel<STARKV_BF16, STARKV_BF16, true, STARKV_BF16>;
 }
 
 template <bool WINDOW>
@@ -443,8 +472,8 @@ int starkv_prefill_block_list(const int32_t* cu_seqlens, int num_prompts, int32_
 
 // window 0: every key up to the query.
 static int prefill_call(void* stream, const void* query, int64_t q_s0, int64_t q_s1, int q_dtype,
-                        const void* key, const void* value, int64_t kv_s0, int64_t kv_s1, int kv_dtype,
-                        const int32_t* cu_seqlens, const int32_t* blocks, int num_blocks, int num_heads,
+                        const void* key, int64_t k_s0, int64_t k_s1, int k_dtype, const void* value, int64_t v_s0,
+                        int64_t v_s1, const int32_t* cu_seqlens, const int32_t* blocks, int num_blocks, int num_heads,
                         int num_kv_heads, int head_size, int window, int sinks, float scale, void* out, int64_t o_s0, int64_t o_s1,
                         int out_dtype) {
     clear_error();
@@ -454,12 +483,14 @@ static int prefill_call(void* stream, const void* query, int64_t q_s0, int64_t q
     SKV_CHECK(head_size == 128, "prefill: head_size %d (128 only)", head_size);
     SKV_CHECK(num_kv_heads >= 1 && num_heads >= 1 && num_heads % num_kv_heads == 0,
               "prefill: num_heads %% num_kv_heads != 0");
-    SKV_CHECK(kv_dtype == STARKV_F16, "prefill: K and V must be fp16");
+    const bool raw = k_dtype == STARKV_BF16 && window > 0 && q_dtype == STARKV_BF16;
+    SKV_CHECK(k_dtype == STARKV_F16 || raw, "prefill: K and V must be fp16");
+    SKV_CHECK(raw || (k_s0 == v_s0 && k_s1 == v_s1), "prefill: fp16 K and V must share strides");
     SKV_CHECK(q_dtype >= STARKV_F32 && q_dtype <= STARKV_BF16 && out_dtype >= STARKV_F32 && out_dtype <= STARKV_BF16,
               "prefill: query and output dtypes must be bf16, fp16 or fp32");
-    SKV_CHECK(((uintptr_t)key % 16) == 0 && ((uintptr_t)value % 16) == 0 && kv_s0 % 8 == 0 && kv_s1 % 8 == 0,
+    SKV_CHECK(((uintptr_t)key % 16) == 0 && ((uintptr_t)value % 16) == 0 && (k_s0 | k_s1 | v_s0 | v_s1) % 8 == 0,
               "prefill: K and V rows must be 16-byte aligned");
-    SKV_CHECK(kv_s0 * 2 * 64 < ((int64_t)1 << 31), "prefill: K / V row stride too large");
+    SKV_CHECK(k_s0 * 2 * 64 < ((int64_t)1 << 31) && v_s0 * 2 * 64 < ((int64_t)1 << 31), "prefill: K / V row stride too large");
     const int qal = q_dtype == STARKV_F32 ? 4 : 8;
     SKV_CHECK(((uintptr_t)query % 16) == 0 && q_s0 % qal == 0 && q_s1 % qal == 0,
               "prefill: query rows must be 16-byte aligned");
@@ -467,13 +498,13 @@ static int prefill_call(void* stream, const void* query, int64_t q_s0, int64_t q
     PrefillParams p;
     p.q = query; p.q_s0 = q_s0; p.q_s1 = q_s1; p.q_dt = q_dtype;
     p.k = (const uint8_t*)key; p.v = (const uint8_t*)value;
-    p.kv_s0 = kv_s0 * 2; p.kv_s1 = kv_s1 * 2;
+    p.k_s0 = k_s0 * 2; p.k_s1 = k_s1 * 2; p.v_s0 = v_s0 * 2; p.v_s1 = v_s1 * 2;
     p.cu = cu_seqlens; p.blocks = blocks; p.nblocks = num_blocks;
     p.Hq = num_heads; p.G = num_heads / num_kv_heads;
     p.sc = scale * 1.4426950408889634f;
     p.out = out; p.o_s0 = o_s0; p.o_s1 = o_s1; p.out_dt = out_dtype;
     p.window = window; p.sinks = sinks;
-    const void* fn = window > 0 ? pf_pick<true>(q_dtype, out_dtype) : pf_pick<false>(q_dtype, out_dtype);
+    const void* fn = raw ? pf_pick_bf16(out_dtype) : window > 0 ? pf_pick<true>(q_dtype, out_dtype) : pf_pick<false>(q_dtype, out_dtype);
     const int lds = PF_LDS;
     static const void* raised[32];
     static int nraised = 0;
@@ -493,18 +524,18 @@ int starkv_prefill_attention(void* stream, const void* query, int64_t q_s0, int6
                              const int32_t* cu_seqlens, const int32_t* blocks, int num_blocks, int num_heads,
                              int num_kv_heads, int head_size, float scale, void* out, int64_t o_s0, int64_t o_s1,
                              int out_dtype) {
-    return prefill_call(stream, query, q_s0, q_s1, q_dtype, key, value, kv_s0, kv_s1, kv_dtype, cu_seqlens, blocks,
-                        num_blocks, num_heads, num_kv_heads, head_size, 0, 0, scale, out, o_s0, o_s1, out_dtype);
+    return prefill_call(stream, query, q_s0, q_s1, q_dtype, key, kv_s0, kv_s1, kv_dtype == STARKV_F16 ? kv_dtype : -1, value,
+                        kv_s0, kv_s1, cu_seqlens, blocks, num_blocks, num_heads, num_kv_heads, head_size, 0, 0, scale, out, o_s0, o_s1, out_dtype);
 }
 
 int starkv_prefill_window(void* stream, const void* query, int64_t q_s0, int64_t q_s1, int q_dtype, const void* key,
-                          const void* value, int64_t kv_s0, int64_t kv_s1, int kv_dtype, const int32_t* cu_seqlens,
-                          const int32_t* blocks, int num_blocks, int num_heads, int num_kv_heads, int head_size,
+                          int64_t k_s0, int64_t k_s1, int k_dtype, const void* value, int64_t v_s0, int64_t v_s1,
+                          const int32_t* cu_seqlens, const int32_t* blocks, int num_blocks, int num_heads, int num_kv_heads, int head_size,
                           int window, int sinks, float scale, void* out, int64_t o_s0, int64_t o_s1, int out_dtype) {
     clear_error();
     SKV_CHECK(window >= 1 && sinks >= 0, "prefill_window: window=%d sinks=%d", window, sinks);
-    return prefill_call(stream, query, q_s0, q_s1, q_dtype, key, value, kv_s0, kv_s1, kv_dtype, cu_seqlens, blocks,
-                        num_blocks, num_heads, num_kv_heads, head_size, window, sinks, scale, out, o_s0, o_s1, out_dtype);
+    return prefill_call(stream, query, q_s0, q_s1, q_dtype, key, k_s0, k_s1, k_dtype, value, v_s0, v_s1, cu_seqlens,
+                        blocks, num_blocks, num_heads, num_kv_heads, head_size, window, sinks, scale, out, o_s0, o_s1, out_dtype);
 }
 
 int starkv_prefill_to_half(void* stream, const void* key, int64_t k_s0, int64_t k_s1, void* key_out, const void* value,
@@ -515,7 +546,7 @@ int starkv_prefill_to_half(void* stream, const void* key, int64_t k_s0, int64_t 
     SKV_CHECK(((uintptr_t)key_out % 16) == 0 && ((uintptr_t)value_out % 16) == 0,
               "prefill_to_half: the results must be 16-byte aligned");
     if (num_tokens == 0) return STARKV_OK;
-    SKV_CHECK(key && value && key_out && value_out, "prefill_to_half: null pointer");
+    SKV_CHECK(value && value_out && !key == !key_out, "prefill_to_half: null pointer");
     ToHalfParams p;
     p.src[0] = key; p.s0[0] = k_s0; p.s1[0] = k_s1; p.dst[0] = (uint16_t*)key_out;
     p.src[1] = value; p.s0[1] = v_s0; p.s1[1] = v_s1; p.dst[1] = (uint16_t*)value_out;
@@ -523,9 +554,9 @@ int starkv_prefill_to_half(void* stream, const void* key, int64_t k_s0, int64_t 
     p.pieces = (int64_t)num_tokens * num_kv_heads * 16;
     p.wide = 1;
     const int al = dtype == STARKV_F32 ? 4 : 8;
-    for (int z = 0; z < 2; ++z)
+    for (int z = key ? 0 : 1; z < 2; ++z)
         if (((uintptr_t)p.src[z] % 16) != 0 || p.s0[z] % al != 0 || p.s1[z] % al != 0) p.wide = 0;
-    const dim3 grid((unsigned)std::min<int64_t>((p.pieces + 255) / 256, 4096), 2);
+    const dim3 grid((unsigned)std::min<int64_t>((p.pieces + 255) / 256, 4096), key ? 2 : 1);
     if (dtype == STARKV_BF16)
         hipLaunchKernelGGL(to_half_kernel<STARKV_BF16>, grid, dim3(256), 0, (hipStream_t)stream, p);
     else

@@ -86,8 +86,8 @@ SIGNATURES = {
     "starkv_window_decode_workspace_bytes": (_SZ, [_I, _I, _I, _I, _I, _I]),
     "starkv_window_decode": (_I, [_P, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _I, _I64, _P, _I64, _I64, _I, _P, _I,
                                   _I, _I, _I, _I, _I, _F, _P, _I64, _I64, _P, _SZ]),
-    "starkv_prefill_window": (_I, [_P, _P, _I64, _I64, _I, _P, _P, _I64, _I64, _I, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P,
-                                   _I64, _I64, _I]),
+    "starkv_prefill_window": (_I, [_P, _P, _I64, _I64, _I, _P, _I64, _I64, _I, _P, _I64, _I64, _P, _P, _I, _I, _I, _I, _I,
+                                   _I, _F, _P, _I64, _I64, _I]),
     "starkv_write_kv8_workspace_bytes": (_SZ, [_I, _I64, _I]),
     "starkv_write_kv8": (_I, [_P, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _P, _I64, _I64, _I64, _I, _P, _I64, _I64, _I,
                               _I64, _P, _I, _I, _I, _P, _SZ]),

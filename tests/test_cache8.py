@@ -64,7 +64,7 @@ GOOD = {
     "starkv_window_decode": dict(stream=None, q=P, q0=512, q1=128, k=P, v=P, c0=4096, c1=256, c2=128, dtype=2, bs=16, blocks=6, bt=P, t0=3,
                                  t1=1, width=3, lens=P, n=2, hq=4, heads=2, span=48, window=8, sinks=1, scale=0.1, out=P, o0=512, o1=128,
                                  ws=P, bytes=1 << 20),
-    "starkv_prefill_window": dict(stream=None, q=P, q0=512, q1=128, dtype=2, k=P, v=P, k0=256, k1=128, kv=1, cu=P, blk=P, blocks=3, hq=4, heads=2,
+    "starkv_prefill_window": dict(stream=None, q=P, q0=512, q1=128, dtype=2, k=P, k0=256, k1=128, kdt=1, v=P, v0=256, v1=128, cu=P, blk=P, blocks=3, hq=4, heads=2,
                                   D=128, window=8, sinks=1, scale=0.1, out=P, o0=512, o1=128, odt=2),
     "starkv_write_kv8": dict(stream=None, key=P, k0=256, k1=128, v=P, v0=256, v1=128, dtype=2, kc=P, vc=P, c0=4096, c1=256, c2=128, code=3, ex=P,
                              x0=4, x1=2, bs=16, blocks=6, slots=P, bits=64, n=2, heads=2, ws=P, bytes=1 << 20),
@@ -81,7 +81,8 @@ DECODE = [("n", -1, b"n="), ("n", 65536, b"n="), ("span", 0, b"max_seq_len"), ("
           ("window", -1, b"window"), ("sinks", -1, b"sinks")]
 BAD = {
     "starkv_window_decode": [*DECODE, ("window", 0, b"window"), ("c2", 4, b"16-byte"), ("k", P + 2, b"16-byte")],
-    "starkv_prefill_window": [("window", 0, b"window"), ("sinks", -1, b"sinks"), ("D", 64, b"head_size"), ("kv", 2, b"fp16"), ("q", None, b"null")],
+    "starkv_prefill_window": [("window", 0, b"window"), ("sinks", -1, b"sinks"), ("D", 64, b"head_size"), ("kdt", 0, b"fp16"), ("q", None, b"null"),
+                              ("k0", 128, b"share strides"), ("q0", 4, b"aligned"), ("o0", 2, b"aligned")],
     "starkv_write_kv8": [*CACHE8, ("n", -1, b"n="), ("heads", 0, b"heads"), ("heads", 65536, b"heads"), ("dtype", 0, b"bf16 or fp16"),
                          ("bits", 16, b"int32 or int64"), ("k1", 4, b"16-byte"), ("ws", P + 4, b"workspace"), ("bytes", 0, b"workspace")],
     "starkv_read_kv8": [*CACHE8, ("odt", 3, b"bf16, fp16 or fp32"), ("ko", P + 4, b"16-byte"), ("bits", 8, b"int32 or int64"), ("n", -1, b"n=")],
@@ -97,6 +98,8 @@ def test_c_abi_refuses(name, change):
     args["n" if "n" in args else "blocks"] = max(args.get("n", 3), 1)
     if key == "bytes" and name == "starkv_decode_kv8":
         args["span"] = 1 << 16  # several splits, which need room
+    if key == "bytes" and name == "starkv_write_kv8":
+        args["n"] = 300  # the map of slots
     if key == "bytes" and name == "starkv_window_decode":
         args.update(span=1 << 16, window=1 << 15)
     args[key] = value

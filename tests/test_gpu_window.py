@@ -226,6 +226,23 @@ def test_prompts_of_other_types_and_scales(cuda):
         prompts_close(out, q, k, v, lens, w, scale, scale)
 
 
+def test_prompts_of_any_strides(cuda):
+    """bf16 keys where they lie: broadcast over heads or tokens, rows in the middle of wider ones, unaligned ones; values past
+    fp16's range are the one thing that is not taken."""
+    g = torch.Generator().manual_seed(12)
+    L, w = 300, Window(70, 5)
+    wide = torch.randn(L, 5, 3 * D, generator=g).to(BF16).to(cuda)
+    q = torch.randn(L, 4, D, generator=g).to(BF16).to(cuda)
+    v = torch.randn(L, 2, D, generator=g).to(BF16).to(cuda)
+    for k in (wide[:, 1:3, D:2 * D], wide[:, :1, :D].expand(L, 2, D), wide[:1, :2, :D].expand(L, 2, D), wide[:, ::2, 8:8 + D][:, :2],
+              wide[:, 2:4, 4:4 + D], wide.transpose(0, 1).contiguous().transpose(0, 1)[:, :2, :D]):
+        prompts_close(prefill_attention(q, k, v, [L], SCALE, window=w), q, k, v, [L], w, k.stride())
+    one = wide[7:8, :2, :D]
+    prompts_close(prefill_attention(q[:1], one.as_strided(one.shape, (0, 3 * D, 1)), v[:1], [1], SCALE, window=w), q, one, v, [1], w)
+    k = wide[:, :2, :D] * 1e20  # keys of any size that bf16 has
+    prompts_close(prefill_attention(q, k, v, [L], SCALE * 1e-20, window=w), q, k, v, [L], w, "large", SCALE * 1e-20)
+
+
 def test_prompts_large_keys_out_of_sight(cuda):
     """Keys that a row does not see do not change it: not by a bit from row 288 on, and by roundings in rows 264 to 287, for
     which 32 rows of a wave move their references together and the rows in front of them see some of the keys."""
