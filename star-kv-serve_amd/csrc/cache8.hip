@@ -13,7 +13,8 @@
 //
 // A wave takes a head of the block, keys and values: four rows of 256 bytes a load, largest magnitudes as integer bits
 // (NaN is above infinity, which is above all others), rows kept in registers from the first look to the rounding where there
-// are at most 16.
+// are at most 16. Rows are read past the caches: the codes stay there for what reads them next (11400 tokens of 32 heads
+// written and read back 130 -> 107 us).
 #include <algorithm>
 
 #include "cache8.hpp"
@@ -119,7 +120,7 @@ __device__ __forceinline__ void load_head(const Write8Params& p, Rows8& r, int b
         const int64_t t = at < count ? tok[list[at]] : -1;
 #pragma unroll
         for (int z = 0; z < 2; ++z)
-            r.w[z][i] = t >= 0 ? *(const uint4*)(p.src[z] + h * p.s1[z] + 16 * d + t * p.s0[z]) : make_uint4(0, 0, 0, 0);
+            r.w[z][i] = t >= 0 ? load_once16(p.src[z] + h * p.s1[z] + 16 * d + t * p.s0[z]) : make_uint4(0, 0, 0, 0);
     }
 }
 
@@ -284,7 +285,8 @@ struct Read8Params {
     const int8_t* ex; int64_t x_s0, x_s1;
     int shift; int64_t num_blocks;
     const void* slots; int slot64;
-    int n, H, out_dt;
+    int n, H;
+    int once;                                           // codes past the caches
     void* out[2];                                       // [n][H][128]
 };
 
@@ -292,6 +294,10 @@ struct Read8Params {
 // together; rows as the results lie, a token's heads side by side. The bound is HBM: 128 bytes read and 256 written a
 // row.
 constexpr int RD_U = 2;
+// Calls that read more than this many bytes of codes load them past the caches, which hold the results for their reader
+// then: 73000 tokens of 8 heads (149 MB) 72 -> 57 us. Fewer are likely to be in the last level (256 MB) from the write or
+// the decode before: one session of 4096 tokens, 32 heads (34 MB) 16.7 us, 19.8 past them.
+constexpr int64_t RD_ONCE = 64 << 20;
 
 template <int CT, int ODT>
 __global__ __launch_bounds__(256) void read8_kernel(const Read8Params p) {
@@ -315,7 +321,7 @@ __global__ __launch_bounds__(256) void read8_kernel(const Read8Params p) {
         const int8_t* ex = p.ex + blk * p.x_s0 + h[u] * p.x_s1;
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-            w[u][z] = *(const uint2*)(p.codes[z] + at);
+            w[u][z] = p.once ? load_once8(p.codes[z] + at) : *(const uint2*)(p.codes[z] + at);
             e[u][z] = ex[z];
         }
     }
@@ -445,7 +451,8 @@ int starkv_read_kv8(void* stream, const void* k_codes, const void* v_codes, int6
     p.ex = exponents; p.x_s0 = x_s0; p.x_s1 = x_s1;
     p.shift = c8_block_shift(block_size); p.num_blocks = num_blocks;
     p.slots = slot_mapping; p.slot64 = slot_bits == 64;
-    p.n = n; p.H = num_kv_heads; p.out_dt = out_dtype;
+    p.n = n; p.H = num_kv_heads;
+    p.once = (int64_t)n * num_kv_heads * 256 > RD_ONCE;
     p.out[0] = key_out; p.out[1] = value_out;
     const void* fn = code_type == STARKV_I8 ? read_pick<STARKV_I8>(out_dtype) : read_pick<STARKV_E4M3>(out_dtype);
     void* args[] = {(void*)&p};
