@@ -286,7 +286,6 @@ struct Read8Params {
     int shift; int64_t num_blocks;
     const void* slots; int slot64;
     int n, H;
-    int once;                                           // codes past the caches
     void* out[2];                                       // [n][H][128]
 };
 
@@ -294,12 +293,22 @@ struct Read8Params {
 // together; rows as the results lie, a token's heads side by side. The bound is HBM: 128 bytes read and 256 written a
 // row.
 constexpr int RD_U = 2;
-// Calls that read more than this many bytes of codes load them past the caches, which hold the results for their reader
-// then: 73000 tokens of 8 heads (149 MB) 72 -> 57 us. Fewer are likely to be in the last level (256 MB) from the write or
-// the decode before: one session of 4096 tokens, 32 heads (34 MB) 16.7 us, 19.8 past them.
-constexpr int64_t RD_ONCE = 64 << 20;
+// Results of 16 bits of more than this many bytes go past the caches (256 MB in the last level), which they would not fit: 11400
+// tokens of 32 heads behind their write 105 -> 96 us, 73000 of 8 heads (300 MB) 72 -> 66. Fewer stay there for their reader
+// (4096 tokens of 32 heads, 67 MB: 16.8 us, 16.5 past them).
+constexpr int64_t RD_ONCE = 128 << 20;
 
-template <int CT, int ODT>
+template <bool ONCE>
+__device__ __forceinline__ void store_row(uint16_t* to, const uint32_t (&v)[4]) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    const u32x4 w = {v[0], v[1], v[2], v[3]};
+    if constexpr (ONCE)
+        __builtin_nontemporal_store(w, (u32x4*)to);
+    else
+        *(u32x4*)to = w;
+}
+
+template <int CT, int ODT, bool ONCE>
 __global__ __launch_bounds__(256) void read8_kernel(const Read8Params p) {
     const uint32_t rows = (uint32_t)p.n * p.H, row0 = blockIdx.x * (16 * RD_U) + (threadIdx.x >> 4);
     const int d = 8 * (threadIdx.x & 15);
@@ -321,7 +330,7 @@ __global__ __launch_bounds__(256) void read8_kernel(const Read8Params p) {
         const int8_t* ex = p.ex + blk * p.x_s0 + h[u] * p.x_s1;
 #pragma unroll
         for (int z = 0; z < 2; ++z) {
-            w[u][z] = p.once ? load_once8(p.codes[z] + at) : *(const uint2*)(p.codes[z] + at);
+            w[u][z] = *(const uint2*)(p.codes[z] + at);
             e[u][z] = ex[z];
         }
     }
@@ -353,17 +362,17 @@ __global__ __launch_bounds__(256) void read8_kernel(const Read8Params p) {
                     const uint16_t hi = ODT == STARKV_BF16 ? __builtin_bit_cast(uint16_t, (__bf16)f[2 * i + 1]) : __builtin_bit_cast(uint16_t, (_Float16)f[2 * i + 1]);
                     v[i] = (uint32_t)lo | (uint32_t)hi << 16;
                 }
-                *(uint4*)((uint16_t*)p.out[z] + to) = make_uint4(v[0], v[1], v[2], v[3]);
+                store_row<ONCE>((uint16_t*)p.out[z] + to, v);
             }
         }
     }
 }
 
 template <int CT>
-const void* read_pick(int dt) {
-    return dt == STARKV_F32 ? (const void*)&read8_kernel<CT, STARKV_F32>
-           : dt == STARKV_F16 ? (const void*)&read8_kernel<CT, STARKV_F16>
-                              : (const void*)&read8_kernel<CT, STARKV_BF16>;
+const void* read_pick(int dt, bool once) {
+    if (dt == STARKV_F32) return (const void*)&read8_kernel<CT, STARKV_F32, false>;
+    if (dt == STARKV_F16) return once ? (const void*)&read8_kernel<CT, STARKV_F16, true> : (const void*)&read8_kernel<CT, STARKV_F16, false>;
+    return once ? (const void*)&read8_kernel<CT, STARKV_BF16, true> : (const void*)&read8_kernel<CT, STARKV_BF16, false>;
 }
 
 }  // namespace
@@ -452,9 +461,9 @@ int starkv_read_kv8(void* stream, const void* k_codes, const void* v_codes, int6
     p.shift = c8_block_shift(block_size); p.num_blocks = num_blocks;
     p.slots = slot_mapping; p.slot64 = slot_bits == 64;
     p.n = n; p.H = num_kv_heads;
-    p.once = (int64_t)n * num_kv_heads * 256 > RD_ONCE;
+    const bool once = (int64_t)n * num_kv_heads * 512 > RD_ONCE;
     p.out[0] = key_out; p.out[1] = value_out;
-    const void* fn = code_type == STARKV_I8 ? read_pick<STARKV_I8>(out_dtype) : read_pick<STARKV_E4M3>(out_dtype);
+    const void* fn = code_type == STARKV_I8 ? read_pick<STARKV_I8>(out_dtype, once) : read_pick<STARKV_E4M3>(out_dtype, once);
     void* args[] = {(void*)&p};
     const int64_t rows = (int64_t)n * num_kv_heads, per = 16 * RD_U;
     SKV_CHECK(rows < 1ll << 31, "read_kv8: %d tokens of %d heads in one call", n, num_kv_heads);
