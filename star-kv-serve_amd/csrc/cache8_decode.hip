@@ -42,9 +42,9 @@ constexpr int D8_PART = 132;        // floats of a partial: reference, sum of we
 constexpr int D8_MAX_GROUP = 16;    // query heads per KV head: the columns of a matrix product
 constexpr float D8_LEAST = -3.402823466e38f;  // the reference of tokens whose scores are all -inf
 
-// Calls of more pages (a KV head's, 4 KB of codes) load them past the caches: 64 x 8192 tokens of 8 heads 204 -> 178 us, 24 x 8192
-// 90 -> 80, 8 x 8192 (134 MB) 39 -> 33. Fewer may be in the last level (256 MB) from the step before: 4 x 8192 (67 MB)
-// 21.8 us, 23.7 past it.
+// Calls of more pages (a KV head's, 4 KB of codes) load keys past the caches: 64 x 8192 tokens of 8 heads 193 -> 178 us, 24 x 8192
+// 84 -> 80, 8 x 8192 (134 MB) 37 -> 33; keys and values both past them 180, 83, 36. Fewer pages may be in the last level
+// (256 MB) from the step before: 4 x 8192 (67 MB) 21.8 us, 23.7 past it.
 constexpr int D8_ONCE = (96 << 20) / 4096;
 
 struct Decode8Params {
@@ -79,7 +79,7 @@ __device__ __forceinline__ int scan_wave(int v) {
 // waves find it by themselves: 64 requests a look.
 struct Range8 {
     int b, k, left, per;  // per: pages a range
-    bool once;            // rows go past the caches
+    bool once;            // keys go past the caches
 };
 
 __device__ __forceinline__ Range8 find_range(const Decode8Params& p, int range) {
@@ -259,14 +259,12 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
                     if (g.once) {
 #pragma unroll
                         for (int st = 0; st < 2; ++st) kr[x][st] = load_once16(kh + base + 64 * st);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) vr[x][j] = load_once8(vh + base + j * p.c_s1);
                     } else {
 #pragma unroll
                         for (int st = 0; st < 2; ++st) kr[x][st] = *(const uint4*)(kh + base + 64 * st);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) vr[x][j] = *(const uint2*)(vh + base + j * p.c_s1);
                     }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) vr[x][j] = *(const uint2*)(vh + base + j * p.c_s1);
                 }
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {

@@ -95,15 +95,10 @@ __device__ __forceinline__ void load8_f(const void* p, int64_t i, int dt, float*
     }
 }
 
-// 16 and 8 bytes that are read once: past the caches, which keep what others hold there.
+// 16 bytes that are read once: past the caches, which keep what others hold there.
 __device__ __forceinline__ uint4 load_once16(const void* at) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     return __builtin_bit_cast(uint4, __builtin_nontemporal_load((const u32x4*)at));
-}
-
-__device__ __forceinline__ uint2 load_once8(const void* at) {
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint2, __builtin_nontemporal_load((const u32x2*)at));
 }
 
 __device__ __forceinline__ int dtype_size(int dt) { return dt == STARKV_F32 ? 4 : 2; }
