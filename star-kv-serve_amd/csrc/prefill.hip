@@ -131,6 +131,18 @@ __device__ __forceinline__ uint2 pf_tr(uint32_t addr) {
     return __builtin_bit_cast(uint2, r);
 }
 
+// Of a pair of fp16 values: the finite ones (mode 0, others 0), or 1 for each that is +inf (1), -inf (2) or NaN (3).
+__device__ __forceinline__ uint32_t pf_class(uint32_t w, int mode) {
+    uint32_t res = 0;
+#pragma unroll
+    for (int x = 0; x < 32; x += 16) {
+        const uint32_t v = w >> x & 0xffffu, size = v & 0x7fffu;
+        const bool is = mode == 1 ? v == 0x7c00u : mode == 2 ? v == 0xfc00u : size > 0x7c00u;
+        res |= (mode == 0 ? size < 0x7c00u ? v : 0u : is ? 0x3c00u : 0u) << x;
+    }
+    return res;
+}
+
 // The work of one workgroup: a (prompt, query block) entry of the list and a query head. Where
 // the heads divide over the 8 XCDs (workgroups are dealt to them round-robin), an XCD takes the
 // blocks of its own heads in list order, block by block: its L2 then streams an eighth of the K
@@ -250,10 +262,8 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
                     x[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, qb[ks]), x[mb], 0, 0, 0);
             }
     };
-    // Tile t, its scores in sc, its V in buffer B; the next tile's scores (NEXT, into nx) are formed
-    // beside the exponentials: matrix and vector work of one wave with no dependence between them.
-    auto tile = [&](auto B, int t, f32x16_t* sc, f32x16_t* nx) {
-        const int k0 = tile_of(t) * PF_KT;
+    // The scores of the tile at key k0 that their query does not see.
+    auto hide = [&](int k0, f32x16_t* sc) {
         // Scores of this lane's query (already scaled through q): key k0 + 32 mb + 8 (r / 4) +
         // 4 h + r % 4. Only a tile that reaches past the wave's first query or the prompt's
         // end needs the causal / end mask.
@@ -275,6 +285,12 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
                     if (c <= lo && c >= head) sc[mb][r] = -INFINITY;
                 }
         }
+    };
+    // Tile t, its scores in sc, its V in buffer B; the next tile's scores (NEXT, into nx) are formed
+    // beside the exponentials: matrix and vector work of one wave with no dependence between them.
+    auto tile = [&](auto B, int t, f32x16_t* sc, f32x16_t* nx) {
+        const int k0 = tile_of(t) * PF_KT;
+        hide(k0, sc);
         float mx = -INFINITY;
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb)
@@ -359,8 +375,82 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
         const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
         l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
     }
+    // An infinite value or NaN of a key that its tile's rows do not all see gives NaN as 0 times it (through a window; a causal
+    // tile has the same for its later keys). Where sums are not finite though their weights are, the workgroup goes over
+    // its tiles again with the reference that it has: which results see a NaN, a -inf and a +inf, then the finite values.
+    uint64_t nan = 0, low = 0, high = 0;  // by the results' order in o
+    if constexpr (WINDOW) {
+        float odd = 0.f;
+#pragma unroll
+        for (int md = 0; md < 4; ++md)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) odd = fmaf(o[md][r], 0.f, odd);
+        const bool mine = __builtin_amdgcn_ballot_w64(odd != odd && l == l && qi < L && nq > 0) != 0;
+        uint32_t* flag = (uint32_t*)s_kv;  // a word a wave
+        __syncthreads();
+        if (lane == 0) flag[wave] = mine;
+        __syncthreads();
+        const uint4 flags = *(const uint4*)flag;
+        if (__builtin_expect((flags.x | flags.y | flags.z | flags.w) != 0, 0)) {
+            const float mr = m == -INFINITY ? 0.f : m;
+#pragma unroll 1
+            for (int mode = 3; mode >= 0; --mode) {
+#pragma unroll
+                for (int md = 0; md < 4; ++md) o[md] = (f32x16_t){};
+#pragma unroll 1
+                for (int t = 0; t < ntile; ++t) {
+                    __syncthreads();  // every wave is done with the tile before, and with the flags
+                    issue(false, t, base);
+                    issue(true, t, base + 2 * PF_TILE);
+                    SKV_WAIT_VM_LGKM0(0);
+                    __syncthreads();
+                    if (t > last) continue;
+                    scores(std::integral_constant<int, 0>{}, sa);
+                    hide(tile_of(t) * PF_KT, sa);
+                    half8_t pb[4];
+#pragma unroll
+                    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) {
+                            const float e = __builtin_amdgcn_exp2f(fmaf(sa[mb][r], ss, -mr));
+                            pb[2 * mb + (r >> 3)][r & 7] = (_Float16)(mode == 0 ? e : e > 0.f ? 1.f : 0.f);
+                        }
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                        for (int md = 0; md < 4; ++md) {
+                            const uint2 a0 = pf_tr(va[md][0] + 4096 * ks), a1 = pf_tr(va[md][1] + 4096 * ks);
+                            const uint4 av = make_uint4(pf_class(a0.x, mode), pf_class(a0.y, mode), pf_class(a1.x, mode), pf_class(a1.y, mode));
+                            o[md] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, av), pb[ks], o[md], 0, 0, 0);
+                        }
+                }
+                uint64_t seen = 0;
+#pragma unroll
+                for (int md = 0; md < 4; ++md)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) seen |= (uint64_t)(o[md][r] > 0.f) << (16 * md + r);
+                if (mode == 3) nan = seen;
+                if (mode == 2) low = seen;
+                if (mode == 1) high = seen;
+            }
+            nan |= low & high;
+        }
+    }
     if (qi < L && nq > 0) {
         const float inv = 1.f / l;
+        if constexpr (WINDOW) {
+            if (__builtin_expect((nan | low | high) != 0, 0)) {
+#pragma unroll
+                for (int md = 0; md < 4; ++md)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int at = 16 * md + r;
+                        if (low >> at & 1) o[md][r] = -INFINITY;
+                        if (high >> at & 1) o[md][r] = INFINITY;
+                        if (nan >> at & 1) o[md][r] = __builtin_nanf("");
+                    }
+            }
+        }
         const int64_t ob = ((int64_t)s + qi) * p.o_s0 + (int64_t)hq * p.o_s1;
 #pragma unroll
         for (int md = 0; md < 4; ++md)

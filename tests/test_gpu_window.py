@@ -180,7 +180,7 @@ def test_captured_steps(cuda):
 
 
 # -- prompts ----------------------------------------------------------------------------------
-def prompts_close(got, q, k, v, lens, w, what="", scale=SCALE):
+def prompts_close(got, q, k, v, lens, w, what="", scale=SCALE, fine=None):
     G, u, o = q.shape[1] // k.shape[1], torch.finfo(got.dtype).eps / 2, 0
     for L in filter(None, lens):
         t = torch.arange(L)
@@ -197,7 +197,8 @@ def prompts_close(got, q, k, v, lens, w, what="", scale=SCALE):
                    + u * out.abs() * 1.01 + (2.0 ** -25 if got.dtype == F16 else 0))
             y = got[o:o + L, h].cpu().double()
             assert y.isfinite().all(), (what, h)
-            off = ((y - out).abs() - tol).max().item()
+            off = (y - out).abs() - tol
+            off = (off if fine is None else off[fine[o:o + L, h]]).max().item()
             assert off <= 0, (what, L, h, off)
         o += L
 
@@ -241,6 +242,40 @@ def test_prompts_of_any_strides(cuda):
     prompts_close(prefill_attention(q[:1], one.as_strided(one.shape, (0, 3 * D, 1)), v[:1], [1], SCALE, window=w), q, one, v, [1], w)
     k = wide[:, :2, :D] * 1e20  # keys of any size that bf16 has
     prompts_close(prefill_attention(q, k, v, [L], SCALE * 1e-20, window=w), q, k, v, [L], w, "large", SCALE * 1e-20)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_prompts_of_infinite_values(cuda, dt):
+    """Infinite values and NaN reach the rows that see them, and no others; keys that are not finite the same."""
+    g = torch.Generator().manual_seed(13)
+    lens, w, H, G = [400, 70, 200], Window(100, 20), 2, 2
+    T = sum(lens)
+    q, k, v = (torch.randn(T, h, D, generator=g).to(dt) for h in (H * G, H, H))
+    clean = v.clone()
+    odd = [(3, 0, 7, math.inf), (40, 0, 8, math.nan), (41, 0, 9, -math.inf), (150, 0, 7, -math.inf), (399, 0, 1, math.inf), (250, 1, 100, math.inf),
+           (251, 1, 100, math.inf), (400 + 69, 0, 3, math.nan), (470 + 64, 1, 2, -math.inf), (470 + 199, 1, 127, math.nan)]
+    for t, h, d, x in odd:
+        v[t, h, d], clean[t, h, d] = x, 0.0
+    got = prefill_attention(q.to(cuda), k.to(cuda), v.to(cuda), lens, SCALE, window=w).cpu()
+    expect = torch.zeros(T, H * G, D)  # what the infinite values that a row sees sum up to
+    start = 0
+    for L in lens:
+        t = torch.arange(L)
+        sees = (t[None, :] <= t[:, None]) & ((t[:, None] - t[None, :] < w.size) | (t[None, :] < w.sinks))
+        for at, h, d, x in odd:
+            if start <= at < start + L:
+                expect[start:start + L, h * G:(h + 1) * G, d] += torch.where(sees[:, at - start], x, 0.0)[:, None]
+        start += L
+    fine = expect == 0
+    assert torch.equal(got.isnan(), expect.isnan()) and torch.equal(got[expect.isinf()].float(), expect[expect.isinf()])
+    assert 0 < int(expect.isnan().sum()) < T and got[fine].isfinite().all()
+    prompts_close(torch.where(fine, got, 0.0).to(dt), q, k, clean, lens, w, "zero", fine=fine)
+    # a NaN key: its row's sight is NaN, the others' rows are as without it
+    k[100, 0, 5] = math.nan
+    got = prefill_attention(q.to(cuda), k.to(cuda), clean.to(cuda), lens, SCALE, window=w).cpu()
+    bad = torch.zeros(T, H * G, dtype=torch.bool)
+    bad[100:200, :G] = True
+    assert torch.equal(got.isnan().all(-1), bad) and torch.equal(got.isnan().any(-1), bad)
 
 
 def test_prompts_large_keys_out_of_sight(cuda):
