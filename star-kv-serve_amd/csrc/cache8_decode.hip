@@ -5,9 +5,19 @@
 // k_t 2^a, V_t = v_t 2^c (k, v codes; a, c the exponents of t's block):
 //     s_t = scale log2(e) 2^a (q . k_t),  out = sum_t 2^(s_t - m) 2^c v_t / sum_t 2^(s_t - m).
 // Codes are never multiplied by their scales: 2^a goes onto the 4 scores that a lane has of a page, 2^c into its
-// weights. A page is 16 tokens of one block. A workgroup of 4 waves takes a range of the unit's pages (a split);
-// a wave takes two pages, 32 tokens, at a time and keeps references and sums of its own; the waves meet in LDS at
-
+// weights. A page is 16 tokens of one block.
+//
+// All pages that the call's requests see are laid end to end, request by request, and cut into as many equal ranges as fill
+// the device with a workgroup for each of a range's KV heads (two a CU): a batch's longest request is no workgroup's alone,
+// and lengths that a captured call only reads on the device need no bound. A workgroup of 4 waves goes through its
+// range's requests; a wave takes two pages, 32 tokens, at a time and keeps references and sums of its own; the waves
+// meet in LDS at a request's end. A request that a range has whole is written there, parts of others are joined by
+// merge8_kernel. (One split of every request by the longest's length: 24 requests of 1000 to 8191 tokens over 8 KV heads 76
+// us, ranges 63; 96 of them 243 and 201.)
+//
+// Memory bounds it: 256 bytes of codes a token and KV head, far above the instructions' time for any G. 64 requests of
+// 8192 tokens over 8 KV heads (1.08 GB) 178 us, 6.0 TB/s; 24 of 1000 to 8191 (237 MB) 58; one of 4096 over 32 KV heads (34 MB) 15,
+// of which 4 are the merge. The next pages' loads ahead of a pair's products gained nothing, nor did 3 or 4 workgroups a CU.
 //
 // Both products run on v_mfma_f32_16x16x32_f16, for which every code and fp16 query is exact; a bf16 query row goes to fp16
 // by a power of two that brings its largest value to 2^14, which leaves values down to 2^-28 of that exact. S^T =
@@ -22,8 +32,8 @@
 // again, take the second one, so that one product does. Two references are kept for that: m of the scores s for
 // the sum of weights, and r of s + c for the weights of the values, each 2^7 below the largest when it was set and moved
 // when that passes it by 2^15, so that neither overflows fp16 and what a value contributes keeps its bits whatever the
-// blocks' exponents are (a first token with a large weight and values of 2^-40 of the others' keeps them). Partials
-// are divided by their sum and scaled by 2^(r - m) where they are left, so values near fp32's largest stay finite.
+// blocks' exponents are (a first token with a large weight and values of 2^-40 of the others' keeps them). Partials keep both
+// references, and the result is scaled by 2^(r - m) in two steps, so values near fp32's largest stay finite.
 //
 // A block whose exponent says NaN makes every row NaN that sees one of its tokens. A row that sees no token is zero; one
 // whose scores are all -inf is 0 / 0, NaN.
@@ -38,7 +48,7 @@ namespace starkv {
 namespace {
 
 constexpr int D8_THR = 256;
-constexpr int D8_PART = 132;        // floats of a partial: reference, sum of weights, 0, 0, out[128]
+constexpr int D8_PART = 132;        // floats of a partial: m, sum of weights above it, r, 0, sums of values above r [128]
 constexpr int D8_MAX_GROUP = 16;    // query heads per KV head: the columns of a matrix product
 constexpr float D8_LEAST = -3.402823466e38f;  // the reference of tokens whose scores are all -inf
 
@@ -138,6 +148,13 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
     w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
 }
 
+// The result of sums a above reference r and l above m: a / l 2^(r - m), in two steps, of which 2^(r - m) may be past fp32's
+// range where the result is not. 0 where there were no tokens.
+__device__ __forceinline__ float weigh_out(float a, float l, float m, float r) {
+    const float half = exp2f(0.5f * (r - m));
+    return m == -INFINITY ? 0.f : a / l * half * half;
+}
+
 // What a wave's lanes know of 32 pairs of pages: pages c0, c0 + 1, c0 + 8, c0 + 9, ... of the request's. The block, the places
 // that are seen | the page's place in the block << 16, the exponents (which the rows need not wait for).
 struct Look8 {
@@ -197,7 +214,7 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
         const bool whole = k0 == 0 && k1 == seen.pages;
         if (h == 0 && k0 == 0 && tid == 0) p.where[b] = make_int2(range, 1 + (seen.pages - k1 + g.per - 1) / g.per);
         uint4 qf[2][2];  // fp16 values of the queries, times 2^up
-        float sc = p.sc;
+        int up_q = 0;
         if constexpr (QDT == STARKV_F16) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) qf[i >> 1][i & 1] = w[i >> 1][i & 1];
@@ -212,9 +229,8 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
                 }
             top = max_rows(top);
             // 2^14 <= top 2^up < 2^15; of zeros, subnormal numbers and infinities the nearest power there is.
-            const int x = (int)(__float_as_uint(top) >> 23), up = min(max(141 - x, -126), 126);
-            const float by = __uint_as_float((uint32_t)(up + 127) << 23);
-            sc *= __uint_as_float((uint32_t)(127 - up) << 23);
+            up_q = min(max(141 - (int)(__float_as_uint(top) >> 23), -126), 126);
+            const float by = __uint_as_float((uint32_t)(up_q + 127) << 23);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 half8_t o;
@@ -283,10 +299,10 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
                         d = mfma_f16(make_uint4(a.x, a.y, c.x, c.y), qf[st][0], d);
                         d = mfma_f16(make_uint4(e.x, e.y, f.x, f.y), qf[st][1], d);
                     }
-                    const float by = sc * c8_scale(ek[x]);
+                    const float sc = ek[x] == C8_NAN ? __builtin_nanf("") : p.sc;
                     up[x] = ev[x] == C8_NAN && see[x] != 0 ? __builtin_nanf("") : (float)ev[x];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) sv[x][k] = d[k] * by;
+                    for (int k = 0; k < 4; ++k) sv[x][k] = __builtin_ldexpf(d[k] * sc, ek[x] - up_q);  // whatever the two exponents are
                     if (see[x] != 0xffffu) {  // tokens out of sight: no score, and codes of 0 (an e4m3 code may be NaN)
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
@@ -315,13 +331,18 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
                 float pe[2][4];
 #pragma unroll
                 for (int x = 0; x < 2; ++x) {
-                    const float f = exp2f(up[x] + (m - r));
+                    const float e = up[x] + (m - r), f = exp2f(e);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const bool ok = see[x] >> (4 * quad + k) & 1u;
                         const float w = ok ? exp2f(sv[x][k] - m) : 0.f;
                         l += w;
                         pe[x][k] = ok ? w * f : 0.f;
+                    }
+                    // Values so much larger than others' that a weight of next to nothing counts: past fp32's range one by one.
+                    if (__builtin_amdgcn_ballot_w64(e > 60.f) != 0) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) pe[x][k] = see[x] >> (4 * quad + k) & 1u ? exp2f(sv[x][k] + (up[x] - r)) : 0.f;
                     }
                 }
                 // The weights' values: the first, and what it left; up to 8 heads the lanes of the second columns take that.
@@ -398,15 +419,12 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
                 a = fmaf(x[4 + d], x[2] == -INFINITY ? 1.f : exp2f(x[2] - R), a);
             }
             const int hq = h * p.G + g;
-            const float half = exp2f(0.5f * (R - M));  // in two steps: its square may be past fp32's range where the result is not
-            // A partial without weight (scores of -inf alone) adds 0 to the others', not 0 times 0 / 0.
-            const float o = M == -INFINITY || (lt == 0.f && !whole) ? 0.f : a / lt * half * half;
             if (whole) {
-                store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, QDT, o);
+                store_f(p.out, b * p.o_s0 + hq * p.o_s1 + d, QDT, weigh_out(a, lt, M, R));
             } else {
                 float* pp = p.part + ((int64_t)(2 * range + (k0 == 0)) * H + hq) * D8_PART;
-                if (d == 0) *(float4*)pp = make_float4(M, lt, 0.f, 0.f);
-                pp[4 + d] = o;
+                if (d == 0) *(float4*)pp = make_float4(M, lt, R, 0.f);
+                pp[4 + d] = a;
             }
         }
         if (left <= 0) break;
@@ -417,9 +435,9 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
     }
 }
 
-// A head's partials joined by one wave: out = sum_s l_s 2^(m_s - M) out_s / sum_s l_s 2^(m_s - M). The first lies second in
-// its range (other requests may end there), the others first in theirs. Lane s of 64 holds the factors of 64 partials at a
-// time and sums dimensions 2 s and 2 s + 1, eight partials' loads in flight.
+// A head's partials joined by one wave: sums of weights above the largest m, of values above the largest r. The first lies
+// second in its range (other requests may end there), the others first in theirs. Lane s of 64 holds the factors of 64
+// partials at a time and sums dimensions 2 s and 2 s + 1, eight partials' loads in flight.
 template <int QDT>
 __global__ __launch_bounds__(64) void merge8_kernel(const Decode8Params p) {
     const int lane = threadIdx.x, hq = blockIdx.x, b = blockIdx.y, H = p.Hkv * p.G;
@@ -432,21 +450,24 @@ __global__ __launch_bounds__(64) void merge8_kernel(const Decode8Params p) {
     }
     if (where.y == 1) return;
     const auto part = [&](int s) { return p.part + ((int64_t)(2 * (where.x + s) + (s == 0)) * H + hq) * D8_PART; };
-    float M = -INFINITY, lt = 0.f;
+    float M = -INFINITY, R = -INFINITY, lt = 0.f;
     float2 a = make_float2(0.f, 0.f);
     for (int c0 = 0; c0 < where.y; c0 += 64) {
         const int count = min(where.y - c0, 64);
-        const float* mine = part(c0 + min(lane, count - 1));
         float2 v[8];  // the first eight's sums are on their way with the references
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[u] = *(const float2*)(part(c0 + min(u, count - 1)) + 4 + 2 * lane);
-        const float m = lane < count ? mine[0] : -INFINITY, l = lane < count ? mine[1] : 0.f;
-        const float most = fmaxf(M, wave_max(m)), before = M == -INFINITY ? 1.f : exp2f(M - most);
-        M = most;
-        const float f = m == -INFINITY ? 0.f : l * exp2f(m - M);
-        lt = fmaf(lt, before, wave_sum(f));
+        const float4 mine = *(const float4*)part(c0 + min(lane, count - 1));
+        const float m = lane < count ? mine.x : -INFINITY, r = lane < count ? mine.z : -INFINITY;
+        const float M1 = fmaxf(M, wave_max(m)), R1 = fmaxf(R, wave_max(r));
+        // A partial without tokens has references of -inf and sums of 0.
+        const float fl = m == -INFINITY ? 0.f : mine.y * exp2f(m - M1), fa = r == -INFINITY ? 0.f : exp2f(r - R1);
+        const float before = R == -INFINITY ? 0.f : exp2f(R - R1);
+        lt = fmaf(lt, M == -INFINITY ? 0.f : exp2f(M - M1), wave_sum(fl));
         a.x *= before;
         a.y *= before;
+        M = M1;
+        R = R1;
         for (int s0 = 0; s0 < count; s0 += 8) {
             if (s0 > 0) {
 #pragma unroll
@@ -454,7 +475,7 @@ __global__ __launch_bounds__(64) void merge8_kernel(const Decode8Params p) {
             }
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
-                const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), (s0 + u) & 63));
+                const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(fa), (s0 + u) & 63));
                 if (s0 + u < count) {
                     a.x = fmaf(v[u].x, fs, a.x);
                     a.y = fmaf(v[u].y, fs, a.y);
@@ -462,8 +483,8 @@ __global__ __launch_bounds__(64) void merge8_kernel(const Decode8Params p) {
             }
         }
     }
-    store_f(p.out, to, QDT, M == -INFINITY ? 0.f : a.x / lt);
-    store_f(p.out, to + 1, QDT, M == -INFINITY ? 0.f : a.y / lt);
+    store_f(p.out, to, QDT, weigh_out(a.x, lt, M, R));
+    store_f(p.out, to + 1, QDT, weigh_out(a.y, lt, M, R));
 }
 
 int device_cus() {

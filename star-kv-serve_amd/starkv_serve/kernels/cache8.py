@@ -36,6 +36,8 @@ class Cache8:
         as one run."""
         if dtype not in CODE_TYPES:
             raise ValueError(f"8-bit caches hold torch.int8 or torch.float8_e4m3fn, not {dtype}")
+        if block_size not in (16, 32, 64, 128, 256, 512, 1024):
+            raise ValueError(f"blocks of {block_size} tokens: 16 times a power of two, at most 1024")
         k, v = (torch.zeros(num_blocks, num_kv_heads, block_size, head_dim, dtype=torch.int8, device=device).view(dtype)
                 .transpose(1, 2) for _ in range(2))
         return cls(k, v, torch.full((num_blocks, num_kv_heads, 2), LEAST_EXPONENT, dtype=torch.int8, device=device))

@@ -20,6 +20,9 @@ def test_a_new_cache_holds_zeros():
     for dtype in (torch.uint8, torch.float16, torch.float8_e5m2):
         with pytest.raises(ValueError, match="int8"):
             Cache8.zeros(5, 32, 3, dtype, "cpu")
+    for size in (8, 24, 2048, 0):
+        with pytest.raises(ValueError, match="blocks of"):
+            Cache8.zeros(5, size, 3, I8, "cpu")
 
 
 def test_windows():

@@ -310,6 +310,61 @@ def test_decode_through_a_window(cuda, size, sinks):
         close(paged_decode_8(q, c, bt, sl, max(lens), SCALE, window=w), q, c, bt, lens, w, what=(code, dt))
 
 
+@pytest.mark.parametrize("n,H,G,most", [(65, 1, 2, 40), (200, 2, 1, 300), (131, 40, 1, 33), (300, 1, 16, 17)])
+def test_decode_of_many_requests(cuda, n, H, G, most):
+    """More requests than a wave looks at, none among them with tokens or all; ranges that hold many and that cut some."""
+    g = torch.Generator().manual_seed(n)
+    lens = torch.randint(0, most + 1, (n,), generator=g)
+    lens[torch.rand(n, generator=g) < 0.3] = 0
+    lens[:3], lens[-2:] = 0, 0
+    lens[n // 2] = 40 * most
+    lens = lens.tolist()
+    c, bt, sl = session(lens, H, 16, I8, cuda, g)
+    q = torch.randn(n, H * G, D, generator=g).to(BF16).to(cuda)
+    got = paged_decode_8(q, c, bt, sl, max(lens), SCALE)
+    close(got, q, c, bt, lens, None)
+    assert torch.equal(got, paged_decode_8(q, c, bt, sl, 1 << 20, SCALE))
+    # any order of requests: each one's result is its own (ranges cut others, so sums may be joined elsewhere)
+    back = torch.randperm(n, generator=g)
+    close(paged_decode_8(q[back.to(cuda)], c, bt[back.to(cuda)], sl[back.to(cuda)], max(lens), SCALE), q[back.to(cuda)], c, bt[back.to(cuda)],
+          [lens[i] for i in back], None)
+    assert (paged_decode_8(q, c, bt, sl * 0, 1 << 20, SCALE) == 0).all()
+
+
+def test_decode_of_more_heads_than_workgroups(cuda):
+    """One range for all pages: no partials, and rows without tokens written with the others."""
+    g = torch.Generator().manual_seed(20)
+    lens, H = [30, 0, 5], 600
+    c, bt, sl = session(lens, H, 16, F8, cuda, g)
+    q = torch.randn(3, H, D, generator=g).to(F16).to(cuda)
+    close(paged_decode_8(q, c, bt, sl, 64, SCALE), q, c, bt, lens, None)
+
+
+def test_calls_on_two_streams(cuda):
+    """Writes, reads and decodes of two caches at once, each on a stream of its own."""
+    g = torch.Generator().manual_seed(21)
+    H, n, steps = 4, 400, 20
+    jobs = []
+    for code in (I8, F8):
+        c = some_cache(64, 16, H, code, cuda, g)
+        jobs.append(dict(c=c, plain=Plain8(c), k=rows(n, H, BF16, cuda, g), slots=torch.randperm(64 * 16, generator=g)[:n].to(cuda),
+                         q=torch.randn(3, 8, D, generator=g).to(BF16).to(cuda), bt=torch.randperm(64, generator=g)[:60].view(3, 20).int().to(cuda),
+                         sl=torch.tensor([320, 17, 200], device=cuda).int(), stream=torch.cuda.Stream(), got=[]))
+    torch.cuda.synchronize()
+    for _ in range(steps):
+        for j in jobs:
+            with torch.cuda.stream(j["stream"]):
+                write_kv8(*j["k"], j["c"], j["slots"])
+                j["got"].append((paged_decode_8(j["q"], j["c"], j["bt"], j["sl"], 320, SCALE), read_kv8(j["c"], j["slots"])[0]))
+    torch.cuda.synchronize()
+    for j in jobs:
+        j["plain"].write(*j["k"], j["slots"].cpu())
+        assert j["plain"].same(j["c"])
+        first, back = j["got"][0]
+        close(first, j["q"], j["c"], j["bt"], [320, 17, 200], None)
+        assert all(torch.equal(first, x) and torch.equal(back, y) for x, y in j["got"])
+
+
 def test_decode_cuts_lengths_and_leaves_bad_blocks_out(cuda):
     g = torch.Generator().manual_seed(5)
     c, bt, sl = session([200, 300], 2, 16, I8, cuda, g)
@@ -342,6 +397,55 @@ def test_decode_of_unlike_exponents(cuda):
                 c.k[int(bt[b, 0]), :, 0] = (k0.round() if code == I8 else k0).to(code).to(cuda)
                 c.exponents[int(bt[b, 0]), :, 0] = -3
             close(paged_decode_8(q, c, bt, sl, 300, SCALE), q, c, bt, lens, None, what=(code, e_first, e_rest))
+
+
+def test_decode_where_next_to_no_weight_counts(cuda):
+    """A block whose weights are 2^-100 to 2^-400 of the others' and whose values are as much larger, and one whose are not; keys
+    and queries at opposite ends of their type."""
+    g = torch.Generator().manual_seed(22)
+    for code in (I8, F8):
+        for e_first, e_rest, key in ((-100, 100, 0), (-126, 110, -1), (-60, 60, -1), (110, -126, 0), (0, 100, 0)):
+            lens = [40, 300]
+            c, bt, sl = session(lens, 1, 16, code, cuda, g)
+            q = torch.randn(2, 1, D, generator=g).to(BF16).to(cuda)
+            c.exponents[..., 1] = torch.where(c.exponents[..., 1] == -128, -128, e_rest)
+            for b in range(2):
+                first = int(bt[b, 0])
+                c.exponents[first, :, 1] = e_first
+                along = q[b, 0].float() / q[b, 0].float().abs().max() * 100
+                c.k[first, :, 0] = (along.round() if code == I8 else along).to(code)
+                c.exponents[first, :, 0] = key
+            close(paged_decode_8(q, c, bt, sl, 300, SCALE), q, c, bt, lens, None, what=(code, e_first, e_rest, key))
+        c, bt, sl = session([200, 50], 2, 16, code, cuda, g)
+        for power in (-112, -120, 112, 120):  # scores of an ordinary size all the same
+            q = (torch.randn(2, 4, D, generator=g) * 2.0 ** power).to(BF16).to(cuda)
+            c.exponents[..., 0] = torch.where(c.exponents[..., 0] == -128, -128, max(-7 - power, -126) if power > 0 else -7 - power)
+            close(paged_decode_8(q, c, bt, sl, 200, SCALE), q, c, bt, [200, 50], None, what=(code, power))
+
+
+def test_decode_of_partials_of_unlike_weights(cuda):
+    """Parts of one request, joined from many workgroups, whose weights and whose values differ by 2^150 the other way round: each
+    part gives about half of the result."""
+    g = torch.Generator().manual_seed(23)
+    for code in (I8, F8):
+        L = 4096
+        c, bt, sl = session([L], 1, 16, code, cuda, g)
+        q = torch.zeros(1, 2, D)
+        q[..., 0], q[0, 1, 1] = 1.0, 0.5
+        q = q.to(F16).to(cuda)
+        half = bt[0, :L // 16].long().view(2, -1)
+        c.k.view(I8)[half.flatten()] = 0
+        score = 104 / SCALE  # natural units: 2^150 between the halves
+        e = torch.tensor(100.0, dtype=torch.float64).to(code)
+        for b in half[0].tolist():
+            c.k[b, :, 0, 0] = e.to(cuda)
+        c.exponents[half.flatten(), :, 0] = 0
+        c.exponents[half[0], :, 1], c.exponents[half[1], :, 1] = -80, 70
+        scale = score * SCALE / 100.0
+        got = paged_decode_8(q, c, bt, sl, L, scale)
+        close(got, q, c, bt, [L], None, scale, what=code)
+        both = [Plain8(c).rows(1, (h.cpu()[:, None] * 16 + torch.arange(16)).flatten())[:, 0].sum(0) for h in half]
+        assert both[0].abs().max() * math.exp(104) > 0.01 * both[1].abs().max() and both[1].abs().max() > 0.01 * both[0].abs().max() * math.exp(104)
 
 
 def test_decode_of_large_and_small_queries(cuda):
@@ -546,7 +650,7 @@ def test_refusals(cuda):
     with pytest.raises(RuntimeError, match="codes of"):
         read_kv8(Cache8(c.k.view(torch.uint8), c.v.view(torch.uint8), c.exponents), slots)
     with pytest.raises(RuntimeError, match="block_size"):
-        read_kv8(Cache8.zeros(1, 2048, 1, I8, cuda), slots)
+        read_kv8(Cache8(*(torch.zeros(1, 2048, 1, D, dtype=I8, device=cuda) for _ in range(2)), torch.zeros(1, 1, 2, dtype=I8, device=cuda)), slots)
     with pytest.raises(RuntimeError, match="dtype"):
         read_kv8(c, slots, torch.float64)
     with pytest.raises(RuntimeError, match="query heads"):
