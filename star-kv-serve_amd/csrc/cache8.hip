@@ -6,15 +6,25 @@
 // that are there are rounded to it. All tokens of a block have to be known together: one workgroup does a whole
 // block, the one of the block's token that leads (its other tokens' workgroups end).
 //
-// Up to WR_FEW tokens (a decode step) each workgroup finds its block's tokens by looking through all slots (2 KB that
-// every workgroup reads from L2): one launch. More (prompts) write each token's index to its slot of a map first,
+// Up to WR_FEW tokens (a decode step) each workgroup finds its block's tokens by looking through all slots, which every
+// workgroup reads from L2: one launch. More (prompts) write each token's index to its slot of a map first,
 // [num_blocks * block_size] of the workspace, which is not cleared: an entry counts where the slot of the token that
-// it names is the entry's own.
+// it names is the entry's own. Measured, one against the other: a step of 512 requests of 8 heads, each in a block of its own,
+// 4.1 against 24 us, of 1024 4.9 against 30 (of 32 heads 10 against 31), of 2048 9.7 against 30; a prompt of 512 tokens of 8
+// heads 6.6 against 10.7, of 1024 9.6 against 10.9 (of 32 heads 20 against 13), of 2048 12.7 against 11.5 (28 against 16).
+// The map's workgroups do up to WR_RUN blocks one after the other, which is what a step of many requests pays there.
+//
+// A workgroup of the first kind has 4 heads, a wave each, up to WR_WIDE tokens times heads, and 16 above: 4 heads take a
+// prompt of 64 tokens of 32 heads from 12.6 to 6.1 us, 16 a step of 1024 tokens of 32 heads from 20 to 9.3.
 //
 // A wave takes a head of the block, keys and values: four rows of 256 bytes a load, largest magnitudes as integer bits
 // (NaN is above infinity, which is above all others), rows kept in registers from the first look to the rounding where there
-// are at most 16. Rows are read past the caches: the codes stay there for what reads them next (11400 tokens of 32 heads
-// written and read back 130 -> 107 us).
+// are at most 16. A block with one token (a step's) is write_single's. Rows are read past the caches: the codes stay there for
+// what reads them next (11400 tokens of 32 heads written and read back 130 -> 107 us).
+//
+// Bound by memory, and for small calls by latency: a step of 64 tokens of 8 heads takes 3.8 us, of which a launch in a graph
+// is 2; codes that the step has to round again add 6. Four prompts of 11400 tokens of 32 heads, 187 MB in and 93 out: 59 us,
+// 4.8 TB/s; the copy of 2 GiB runs at 4.9.
 #include <algorithm>
 
 #include "cache8.hpp"
@@ -24,7 +34,8 @@ namespace starkv {
 namespace {
 
 constexpr int WR_THR = 256;
-constexpr int WR_FEW = 256;  // tokens that a workgroup looks through
+constexpr int WR_FEW = 1024;   // tokens that a workgroup looks through
+constexpr int WR_WIDE = 4096;  // up to so many tokens times heads a workgroup of few tokens has 4 heads, else 16
 constexpr int WR_RUN = 16;   // tokens of a workgroup of a larger write
 constexpr int WR_HELD = 64;  // places of a block that are looked through once
 
@@ -48,9 +59,13 @@ __device__ __forceinline__ uint32_t dpp_umax(uint32_t v) {
     return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTL, 0xF, 0xF, true));
 }
 
-// The largest of the wave's values, in every lane: within rows of 16 lanes, then over the rows (as wave_max).
+// The largest of the values of a row of 16 lanes, and of the wave's, in every lane (as row16_max and wave_max).
+__device__ __forceinline__ uint32_t row_umax(uint32_t v) {
+    return dpp_umax<0x140>(dpp_umax<0x141>(dpp_umax<0x4E>(dpp_umax<0xB1>(v))));
+}
+
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
-    v = dpp_umax<0x140>(dpp_umax<0x141>(dpp_umax<0x4E>(dpp_umax<0xB1>(v))));
+    v = row_umax(v);
     const auto x = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     v = max(x[0], x[1]);
     const auto y = __builtin_amdgcn_permlane16_swap(v, v, false, false);
@@ -101,6 +116,34 @@ __device__ __forceinline__ uint2 encode(const uint4& w, float inv) {
                       c8_pack<CT>(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
 }
 
+// The exponent of a block's head after a write whose own is e.
+__device__ __forceinline__ int joined(int old, int e, bool fresh) {
+    return fresh ? e : old == C8_NAN || e == C8_NAN ? C8_NAN : max(old, e);
+}
+
+// The codes of places first, first + STEP, ... that have no token now (tok < 0) to an exponent that is `by` more, eight of a
+// place to a lane: the loads of DEEP places go out before the first is rounded.
+template <int CT, int STEP, int DEEP, class Tok>
+__device__ __forceinline__ void lessen(uint8_t* dst, int64_t stride, int first, int size, Tok tok, int by) {
+    const float less = c8_scale(-min(by, 126));
+    for (int at = first; at < size; at += DEEP * STEP) {
+        uint2 w[DEEP];
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i)
+            if (at + STEP * i < size) w[i] = *(const uint2*)(dst + (at + STEP * i) * stride);
+#pragma unroll
+        for (int i = 0; i < DEEP; ++i) {
+            if (at + STEP * i >= size || tok(at + STEP * i) >= 0) continue;
+            float a[4], b[4];
+            c8_values<CT>(w[i].x, a);
+            c8_values<CT>(w[i].y, b);
+            *(uint2*)(dst + (at + STEP * i) * stride) =
+                make_uint2(c8_pack<CT>(a[0] * less, a[1] * less, a[2] * less, a[3] * less),
+                           c8_pack<CT>(b[0] * less, b[1] * less, b[2] * less, b[3] * less));
+        }
+    }
+}
+
 // Rows of 4 KEEP of a block's tokens, keys and values, of one head: a wave's lanes have 16 bytes of 4 rows each.
 constexpr int KEEP = 4;
 struct Rows8 {
@@ -126,7 +169,7 @@ __device__ __forceinline__ void load_head(const Write8Params& p, Rows8& r, int b
 
 // One block's head by one wave, keys and values. tok[place]: the token of each place or -1; list: the places that have
 // one, `count` of them; r: the first rows of them.
-template <int CT, int DT>
+template <int CT, int DT, int DEEP>
 __device__ __forceinline__ void write_head(const Write8Params& p, const Rows8& r, int blk, int h, const int* tok,
                                            const uint16_t* list, int count) {
     const int lane = threadIdx.x & 63, row = lane >> 4, d = lane & 15;
@@ -140,22 +183,9 @@ __device__ __forceinline__ void write_head(const Write8Params& p, const Rows8& r
 #pragma unroll
         for (int i = 0; i < KEEP; ++i) top = pair_max(top, r.w[z][i]);
         for (int at = 4 * KEEP + row; at < count; at += 4) top = pair_max(top, *(const uint4*)(src + tok[list[at]] * p.s0[z]));
-        int e = c8_exponent<CT>(wave_umax(top_bits<DT>(top)));
-        const int old = r.old[z];
-        if (!fresh) e = old == C8_NAN || e == C8_NAN ? C8_NAN : max(old, e);
-        if (!fresh && e != old && e != C8_NAN) {  // the codes that are there, to the new exponent
-            const float less = c8_scale(-min(e - old, 126));
-            for (int at = row; at < 1 << p.shift; at += 4) {
-                if (tok[at] >= 0) continue;
-                uint2* c = (uint2*)(dst + at * p.c_s1);
-                const uint2 w = *c;
-                float a[4], b[4];
-                c8_values<CT>(w.x, a);
-                c8_values<CT>(w.y, b);
-                *c = make_uint2(c8_pack<CT>(a[0] * less, a[1] * less, a[2] * less, a[3] * less),
-                                c8_pack<CT>(b[0] * less, b[1] * less, b[2] * less, b[3] * less));
-            }
-        }
+        const int old = r.old[z], e = joined(old, c8_exponent<CT>(wave_umax(top_bits<DT>(top))), fresh);
+        if (!fresh && e != old && e != C8_NAN)  // the codes that are there, to the new exponent
+            lessen<CT, 4, DEEP>(dst, p.c_s1, row, 1 << p.shift, [&](int at) { return tok[at]; }, e - old);
         const float inv = e == C8_NAN ? 0.f : c8_scale(-e);
         const auto put = [&](int at, const uint4& w) {
             *(uint2*)(dst + list[at] * p.c_s1) = e == C8_NAN ? make_uint2(0, 0) : encode<CT, DT>(w, inv);
@@ -182,14 +212,70 @@ __device__ __forceinline__ void list_places(Block8Shared& sh, int shift) {
     __syncthreads();
 }
 
-// A workgroup a token and 4 heads: the block's tokens by looking through all slots.
+// Up to four heads of a block with one token by a wave: a step writes one token of a block. 16 lanes take the token's row of
+// a head, so that the heads' latencies pass together; codes that have to be rounded again are the whole wave's, four places
+// at a time, one head after the other.
+template <int CT, int DT, int DEEP>
+__device__ __forceinline__ void write_single(const Write8Params& p, int blk, int h0, int h1, int t, int place) {
+    const int lane = threadIdx.x & 63, row = lane >> 4, d = lane & 15, h = h0 + WR_THR / 64 * row;
+    const bool on = h < h1;
+    int8_t* ex = p.ex + blk * p.x_s0 + h * p.x_s1;
+    uint4 w[2] = {};
+    int old[2] = {};
+    if (on) {
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            w[z] = load_once16(p.src[z] + h * p.s1[z] + 16 * d + (int64_t)t * p.s0[z]);
+            old[z] = ex[z];
+        }
+    }
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+        uint8_t* dst = p.codes[z] + blk * p.c_s0 + 8 * d;
+        const int e = joined(old[z], c8_exponent<CT>(row_umax(top_bits<DT>(pair_max(0, w[z])))), place == 0);
+        for (uint64_t grown = __ballot(on && d == 0 && place != 0 && e != old[z] && e != C8_NAN); grown; grown &= grown - 1) {
+            const int g = __builtin_ctzll(grown), by = __builtin_amdgcn_readlane(e - old[z], g);
+            lessen<CT, 4, DEEP>(dst + (h0 + WR_THR / 64 * (g >> 4)) * p.c_s2, p.c_s1, row, 1 << p.shift,
+                                [&](int at) { return at == place ? t : -1; }, by);
+        }
+        if (!on) continue;
+        *(uint2*)(dst + h * p.c_s2 + place * p.c_s1) = e == C8_NAN ? make_uint2(0, 0) : encode<CT, DT>(w[z], c8_scale(-e));
+        if (d == 0 && e != old[z]) ex[z] = (int8_t)e;
+    }
+}
+
+// Heads [h0, h1) of a block by a workgroup.
+template <int CT, int DT, int DEEP>
+__device__ __forceinline__ void write_heads(const Write8Params& p, const Block8Shared& sh, int blk, int h0, int h1) {
+    const int wave = threadIdx.x >> 6;
+    if (sh.count == 1) {
+        const int place = sh.list[0];
+        for (int h = h0 + wave; h < h1; h += WR_THR / 16) write_single<CT, DT, DEEP>(p, blk, h, h1, sh.tok[place], place);
+        return;
+    }
+    for (int h = h0 + wave; h < h1; h += WR_THR / 64) {
+        Rows8 r;
+        load_head(p, r, blk, h, sh.tok, sh.list, sh.count);
+        write_head<CT, DT, DEEP>(p, r, blk, h, sh.tok, sh.list, sh.count);
+    }
+}
+
+// A workgroup a token and `heads` heads: the block's tokens by looking through all slots.
 template <int CT, int DT>
-__global__ __launch_bounds__(WR_THR) void write8_few_kernel(const Write8Params p) {
+__global__ __launch_bounds__(WR_THR) void write8_few_kernel(const Write8Params p, int heads) {
     __shared__ Block8Shared sh;
-    const int t = blockIdx.x, tid = threadIdx.x;
+    // Consecutive workgroups run on different dies, and of a prompt in order one token of 16 2^s leads its block: within each
+    // 8 tokens the order turns by one from block to block, whatever s, else one die would do all of the work.
+    const int b = blockIdx.x, tid = threadIdx.x;
+    const int t = (b & ~7) | ((b + (b >> 4) + (b >> 7) + (b >> 10)) & 7);
+    if (t >= p.n) return;
     const int64_t slot = slot_of(p, t);
     if (slot < 0) return;
     const int blk = (int)(slot >> p.shift), size = 1 << p.shift;
+    if (t > 0) {  // behind another of its block: that or one before it leads
+        const int64_t before = slot_of(p, t - 1);
+        if (before >= 0 && before >> p.shift == blk) return;
+    }
     for (int i = tid; i < size; i += WR_THR) sh.tok[i] = -1;
     if (tid == 0) {
         sh.count = 0;
@@ -205,11 +291,7 @@ __global__ __launch_bounds__(WR_THR) void write8_few_kernel(const Write8Params p
     }
     list_places(sh, p.shift);
     if (sh.lead != t) return;
-    const int h = blockIdx.y * 4 + (tid >> 6);
-    if (h >= p.H) return;
-    Rows8 r;
-    load_head(p, r, blk, h, sh.tok, sh.list, sh.count);
-    write_head<CT, DT>(p, r, blk, h, sh.tok, sh.list, sh.count);
+    write_heads<CT, DT, 4>(p, sh, blk, blockIdx.y * heads, min((int)(blockIdx.y + 1) * heads, p.H));
 }
 
 __global__ __launch_bounds__(WR_THR) void write8_map_kernel(const Write8Params p) {
@@ -267,12 +349,7 @@ __global__ __launch_bounds__(WR_THR) void write8_kernel(const Write8Params p, in
         }
         for (int i = tid + WR_HELD; i < size; i += WR_THR) sh.tok[i] = mapped(p, ((int64_t)blk << p.shift) + i);
         list_places(sh, p.shift);
-        const int end = min((group + 1) * heads, p.H);
-        for (int h = group * heads + (tid >> 6); h < end; h += 4) {
-            Rows8 r;
-            load_head(p, r, blk, h, sh.tok, sh.list, sh.count);
-            write_head<CT, DT>(p, r, blk, h, sh.tok, sh.list, sh.count);
-        }
+        write_heads<CT, DT, 1>(p, sh, blk, group * heads, min((group + 1) * heads, p.H));
         __syncthreads();
     }
 }
@@ -421,8 +498,9 @@ int starkv_write_kv8(void* stream, const void* key, int64_t k_s0, int64_t k_s1, 
     if (n <= WR_FEW) {
         const void* fn = i8 ? bf ? (const void*)&write8_few_kernel<STARKV_I8, STARKV_BF16> : (const void*)&write8_few_kernel<STARKV_I8, STARKV_F16>
                             : bf ? (const void*)&write8_few_kernel<STARKV_E4M3, STARKV_BF16> : (const void*)&write8_few_kernel<STARKV_E4M3, STARKV_F16>;
-        void* args[] = {(void*)&p};
-        SKV_HIP(hipLaunchKernel(fn, dim3(n, (num_kv_heads + 3) / 4), dim3(WR_THR), args, 0, (hipStream_t)stream));
+        int heads = (int64_t)n * num_kv_heads <= WR_WIDE ? 4 : 16;
+        void* args[] = {(void*)&p, (void*)&heads};
+        SKV_HIP(hipLaunchKernel(fn, dim3((n + 7) / 8 * 8, (num_kv_heads + heads - 1) / heads), dim3(WR_THR), args, 0, (hipStream_t)stream));
         return STARKV_OK;
     }
     hipLaunchKernelGGL(write8_map_kernel, dim3((n + WR_THR - 1) / WR_THR), dim3(WR_THR), 0, (hipStream_t)stream, p);

@@ -81,7 +81,11 @@ def test_write_few(cuda, code, dt, bs, H, n, layout, bits):
 @pytest.mark.parametrize("dt,bs,H,lens,order,layout", [(BF16, 16, 4, [257], "runs", "heads"), (F16, 32, 3, [300, 1, 45, 16], "runs", "tokens"),
                                                        (BF16, 64, 2, [200, 333], "shuffled", "pairs"),
                                                        (F16, 16, 1, [17, 400], "reversed", "heads"), (BF16, 1024, 1, [1500], "runs", "heads"),
-                                                       (BF16, 16, 40, [261], "shuffled", "heads")])
+                                                       (BF16, 16, 40, [261], "shuffled", "heads"),
+                                                       (BF16, 16, 4, [1025], "runs", "heads"), (F16, 32, 3, [1100, 1, 45, 16], "runs", "tokens"),
+                                                       (BF16, 64, 2, [600, 777], "shuffled", "pairs"), (F16, 16, 1, [17, 1400], "reversed", "heads"),
+                                                       (BF16, 1024, 1, [2500], "shuffled", "heads"), (BF16, 16, 40, [1061], "shuffled", "heads"),
+                                                       (F16, 128, 5, [1024], "runs", "heads"), (BF16, 16, 17, [1003, 20], "runs", "heads")])
 def test_write_prompts(cuda, code, dt, bs, H, lens, order, layout):
     """Whole prompts and continued ones, in any order of tokens."""
     g = torch.Generator().manual_seed(sum(lens))
@@ -109,7 +113,26 @@ def test_write_prompts(cuda, code, dt, bs, H, lens, order, layout):
     assert want.same(c)
 
 
-@pytest.mark.parametrize("n", [3, 300])
+@pytest.mark.parametrize("code", [I8, F8])
+@pytest.mark.parametrize("dt,bs,H,n,layout", [(BF16, 16, 8, 700, "heads"), (F16, 64, 3, 1024, "pairs"), (BF16, 16, 19, 1030, "tokens"), (F16, 32, 1, 2050, "heads")])
+def test_write_many_steps(cuda, code, dt, bs, H, n, layout):
+    """A token each for many requests, twice: some blocks begin, some exponents grow."""
+    g = torch.Generator().manual_seed(n)
+    nb = n + 7
+    c = some_cache(nb, bs, H, code, cuda, g, layout)
+    want = Plain8(c)
+    blocks = torch.randperm(nb, generator=g)[:n]
+    for _ in range(2):
+        k, v = rows(n, H, dt, cuda, g)
+        k.mul_(torch.exp2(torch.randint(-6, 7, (n, 1, 1), generator=g).float()).to(dt).to(cuda))
+        slots = blocks * bs + torch.randint(0, bs, (n,), generator=g)
+        slots[torch.rand(n, generator=g) < 0.05] = -1
+        write_kv8(k, v, c, slots.to(cuda))
+        want.write(k, v, slots)
+        assert want.same(c)
+
+
+@pytest.mark.parametrize("n", [3, 300, 1100])
 @pytest.mark.parametrize("code,top", [(I8, 127), (F8, 448)])
 def test_write_exponents(cuda, code, top, n):
     """Values at the borders of an exponent, zeros, the types' smallest and largest values, and halves between codes."""
@@ -121,24 +144,25 @@ def test_write_exponents(cuda, code, top, n):
         edge = [0.0, -0.0, tiny, -tiny, float(top), top * 2.0 ** -9, top * 1.0078125, -top * 4.0, 2.0 ** -3, 255.0, 1.75, big, -big, 0.5, 1.5,
                 2.5, 2.0 ** -100 if dt == BF16 else 2.0 ** -14]
         H = len(edge)
-        c = some_cache(24, bs, H, code, cuda, g)
+        nb = max(24, n // bs + 9)
+        c = some_cache(nb, bs, H, code, cuda, g)
         c.exponents[5:9] = -126
         want = Plain8(c)
         k = (torch.randint(-4, 5, (n, H, D), generator=g).double() / 4 * torch.tensor(edge, dtype=torch.float64)[None, :, None]).to(dt)
         k[0, :, 0] = torch.tensor(edge).to(dt)
         v = k.flip(1).contiguous()
-        slots = torch.randperm(24 * bs, generator=g)[:n]
+        slots = torch.randperm(nb * bs, generator=g)[:n]
         write_kv8(k.to(cuda), v.to(cuda), c, slots.to(cuda))
         want.write(k, v, slots)
         assert want.same(c)
 
 
-@pytest.mark.parametrize("n", [6, 290])
+@pytest.mark.parametrize("n", [6, 290, 1111])
 @pytest.mark.parametrize("code", [I8, F8])
 def test_write_not_finite(cuda, code, n):
     """Infinities and NaN make the head's block NaN, other heads and blocks not; a new first token ends that."""
     g = torch.Generator().manual_seed(n)
-    bs, H, nb = 16, 3, 24
+    bs, H, nb = 16, 3, max(24, n // 16 + 6)
     c = some_cache(nb, bs, H, code, cuda, g)
     want = Plain8(c)
     k, v = rows(n, H, BF16, cuda, g)
@@ -156,14 +180,15 @@ def test_write_not_finite(cuda, code, n):
     assert want.same(c) and int((c.exponents == -128).sum()) == 1
 
 
-@pytest.mark.parametrize("n", [5, 400])
+@pytest.mark.parametrize("n", [5, 400, 1200])
 def test_write_same_slot_twice(cuda, n):
     """Two tokens with one slot: one of them is there, and the block's other rows are right."""
     g = torch.Generator().manual_seed(n)
-    c = some_cache(32, 16, 2, I8, cuda, g)
+    nb = max(32, n // 16 + 8)
+    c = some_cache(nb, 16, 2, I8, cuda, g)
     one, other = Plain8(c), Plain8(c)
     k, v = rows(n, 2, BF16, cuda, g)
-    slots = torch.randperm(32 * 16, generator=g)[:n]
+    slots = torch.randperm(nb * 16, generator=g)[:n]
     slots[3] = slots[0]
     write_kv8(k, v, c, slots.to(cuda))
     keep = torch.ones(n, dtype=torch.bool)
@@ -340,14 +365,15 @@ def test_decode_of_more_heads_than_workgroups(cuda):
     close(paged_decode_8(q, c, bt, sl, 64, SCALE), q, c, bt, lens, None)
 
 
-def test_calls_on_two_streams(cuda):
+@pytest.mark.parametrize("n", [400, 1100])
+def test_calls_on_two_streams(cuda, n):
     """Writes, reads and decodes of two caches at once, each on a stream of its own."""
     g = torch.Generator().manual_seed(21)
-    H, n, steps = 4, 400, 20
+    H, nb, steps = 4, max(64, n // 16 + 5), 20
     jobs = []
     for code in (I8, F8):
-        c = some_cache(64, 16, H, code, cuda, g)
-        jobs.append(dict(c=c, plain=Plain8(c), k=rows(n, H, BF16, cuda, g), slots=torch.randperm(64 * 16, generator=g)[:n].to(cuda),
+        c = some_cache(nb, 16, H, code, cuda, g)
+        jobs.append(dict(c=c, plain=Plain8(c), k=rows(n, H, BF16, cuda, g), slots=torch.randperm(nb * 16, generator=g)[:n].to(cuda),
                          q=torch.randn(3, 8, D, generator=g).to(BF16).to(cuda), bt=torch.randperm(64, generator=g)[:60].view(3, 20).int().to(cuda),
                          sl=torch.tensor([320, 17, 200], device=cuda).int(), stream=torch.cuda.Stream(), got=[]))
     torch.cuda.synchronize()
@@ -570,11 +596,12 @@ def test_captured_steps(cuda):
         pos.add_(1)
 
 
-def test_captured_prompt_writes(cuda):
+@pytest.mark.parametrize("n", [500, 1500])
+def test_captured_prompt_writes(cuda, n):
     """A captured write of a prompt's size replays over other slots."""
     g = torch.Generator().manual_seed(17)
-    c = some_cache(64, 16, 2, I8, cuda, g)
-    n = 500
+    nb = max(64, n // 16 + 9)
+    c = some_cache(nb, 16, 2, I8, cuda, g)
     k, v = rows(n, 2, F16, cuda, g, strided=False)
     slots = torch.arange(n, device=cuda)
     plain = Plain8(c)
@@ -582,7 +609,7 @@ def test_captured_prompt_writes(cuda):
     with torch.cuda.graph(graph):
         write_kv8(k, v, c, slots)
     for i in range(4):
-        slots.copy_(torch.randperm(64 * 16, generator=g)[:n])
+        slots.copy_(torch.randperm(nb * 16, generator=g)[:n])
         k.copy_(torch.randn(k.shape, generator=g) * 2.0 ** i)
         graph.replay()
         plain.write(k, v, slots)
