@@ -66,7 +66,7 @@ def write_kv8(key: torch.Tensor, value: torch.Tensor, cache: Cache8, slot_mappin
     Per block, head, and of the two: a call that writes the block's first token begins the block anew, with the least
     exponent (at least -126) at which its own largest value has a code, and leaves the block's other rows as they
     are. Any other call keeps the exponent, or raises it to what its values need and rounds the codes that are there
-    to it. Values that are infinite or NaN give the block's head the exponent -128: all its values are NaN until it begins
+    to it; an exponent never falls until its block begins anew. Values that are infinite or NaN give the block's head the exponent -128: all its values are NaN until it begins
     anew. Results do not depend on the order of slots, nor on how requests share a call."""
     _hip.require_cuda(key, value, *cache.tensors, slot_mapping)
     _hip.refuse_grad("write_kv8", key, value)
