@@ -566,7 +566,8 @@ int starkv_decode_kv8(void* stream, const void* query, int64_t q_s0, int64_t q_s
     p.where = (int2*)workspace;
     p.part = (float*)((char*)workspace + (((size_t)n * sizeof(int2) + 255) & ~(size_t)255));
     p.out = (uint16_t*)out; p.o_s0 = o_s0; p.o_s1 = o_s1;
-    SKV_CHECK((int64_t)n * seen_pages_most(p.span, window, sinks) < 1ll << 31, "decode_kv8: %d requests of up to %d tokens in one call", n, p.span);
+    SKV_CHECK((int64_t)n * seen_pages_most(p.span, window, sinks) < 1ll << 30,  // a range's first page stays in 32 bits
+              "decode_kv8: %d requests of up to %d tokens in one call", n, p.span);
     SKV_CHECK(num_heads <= 65535, "decode_kv8: %d heads", num_heads);
     const bool bf = dtype == STARKV_BF16;
     const void* fn = code_type == STARKV_I8 ? bf ? decode_pick<STARKV_I8, STARKV_BF16>(p.G) : decode_pick<STARKV_I8, STARKV_F16>(p.G)

@@ -102,7 +102,7 @@ def test_c_abi_refuses(name, change):
     if key == "bytes" and name == "starkv_decode_kv8":
         args["span"] = 1 << 16  # several splits, which need room
     if key == "bytes" and name == "starkv_write_kv8":
-        args["n"] = 300  # the map of slots
+        args["n"] = 1300  # the map of slots
     if key == "bytes" and name == "starkv_window_decode":
         args.update(span=1 << 16, window=1 << 15)
     args[key] = value
@@ -112,8 +112,8 @@ def test_c_abi_refuses(name, change):
 
 def test_workspaces():
     L = _hip.lib()
-    assert L.starkv_write_kv8_workspace_bytes(256, 1000, 16) == 0
-    assert L.starkv_write_kv8_workspace_bytes(257, 1000, 16) == 64000
+    assert L.starkv_write_kv8_workspace_bytes(1024, 1000, 16) == 0
+    assert L.starkv_write_kv8_workspace_bytes(1025, 1000, 16) == 64000
     assert L.starkv_write_kv8_workspace_bytes(10 ** 6, 2 ** 27, 16) == 2 ** 33
     one = L.starkv_decode_kv8_workspace_bytes(1, 32, 32, 1 << 20, 0, 0)
     assert one > L.starkv_decode_kv8_workspace_bytes(1, 32, 32, 1 << 20, 64, 4)
