@@ -8,8 +8,8 @@
 // weights. A page is 16 tokens of one block.
 //
 // All pages that the call's requests see are laid end to end, request by request, and cut into as many equal ranges as fill
-// the device with a workgroup for each of a range's KV heads (two a CU): a batch's longest request is no workgroup's alone,
-// and lengths that a captured call only reads on the device need no bound. A workgroup of 4 waves goes through its
+// the device with a workgroup for each of a range's KV heads (two a CU; short requests whole): a batch's longest request is
+// no workgroup's alone, and lengths that a captured call only reads on the device need no bound. A workgroup of 4 waves goes through its
 // range's requests; a wave takes two pages, 32 tokens, at a time and keeps references and sums of its own; the waves
 // meet in LDS at a request's end. A request that a range has whole is written there, parts of others are joined by
 // merge8_kernel. (One split of every request by the longest's length: 24 requests of 1000 to 8191 tokens over 8 KV heads 76
@@ -57,6 +57,17 @@ constexpr float D8_LEAST = -3.402823466e38f;  // the reference of tokens whose s
 // (256 MB) from the step before: 4 x 8192 (67 MB) 21.8 us, 23.7 past it.
 constexpr int D8_ONCE = (96 << 20) / 4096;
 
+// A short request costs a range its latencies (look-up, rows, the waves' meeting: about 4 us) more than its pages, so
+// one of up to half as much again as a range's pages, 16 at most, is the whole of the range's that has its first page: 64 requests
+// of 20 to 60 tokens over 8 KV heads 20.9 -> 14.6 us, of 100 to 200 23.1 -> 19.2 (up to 8 pages 24.1); always up to 16 pages, 8
+// requests of 200 to 900 took 15.8 and not 13.9.
+constexpr int D8_WHOLE = 16;
+
+// Where a call's requests have no more than 16 pages each on average, it is cut into up to four times as many ranges, one
+// a request: 200 requests of 20 to 60 tokens over 8 KV heads 32.3 -> 27.5 us, 256 of 100 to 200 44.9 -> 42.1. Longer ones gain
+// nothing (256 of 300 to 700: 83.8 and 84.1) and would be cut more often.
+constexpr int D8_MORE = 4;
+
 struct Decode8Params {
     const uint16_t* q; int64_t q_s0, q_s1;                              // elements
     const uint8_t* kc; const uint8_t* vc; int64_t c_s0, c_s1, c_s2;     // bytes
@@ -64,7 +75,7 @@ struct Decode8Params {
     int bs_shift; int64_t num_blocks;                                   // block_size = 16 << bs_shift
     const int32_t* bt; int64_t bt_s0, bt_s1;
     const int32_t* seq_lens; int span;                                  // lengths are clamped to span
-    int n, Hkv, G, ranges, window, sinks;
+    int n, Hkv, G, ranges, base, window, sinks;                         // base: the ranges of long requests
     float sc;                                                           // scale * log2(e)
     int2* where;                                                        // [n]: first range, ranges
     float* part;                                                        // [ranges][2][H][D8_PART]
@@ -86,44 +97,61 @@ __device__ __forceinline__ int scan_wave(int v) {
 }
 
 // A range of the call's pages, request by request: its first page's request and place there, and its length. All
-// waves find it by themselves: 64 requests a look.
+// waves find it by themselves: a lane counts the pages of n / 64 requests, then of one in the lane's that has the first.
 struct Range8 {
-    int b, k, left, per;  // per: pages a range
+    int b, k, left, per, whole;  // per: pages a range; whole: up to which one range takes all of a request
     bool once;            // keys go past the caches
 };
 
 __device__ __forceinline__ Range8 find_range(const Decode8Params& p, int range) {
-    const int lane = threadIdx.x & 63;
-    int own = 0, end = 0, total = 0;
+    const int lane = threadIdx.x & 63, some = (p.n + 63) >> 6;
+    int own = 0, end;
     if (p.n == 1) {
-        own = end = total = seen_by(p, 0).pages;
+        own = end = seen_by(p, 0).pages;
     } else {
-        for (int b0 = 0; b0 < p.n; b0 += 64) {
-            own = b0 + lane < p.n ? seen_by(p, b0 + lane).pages : 0;
-            end = scan_wave(own);
-            total += __builtin_amdgcn_readlane(end, 63);
-        }
+        for (int b = lane * some; b < min((lane + 1) * some, p.n); ++b) own += seen_by(p, b).pages;
+        end = scan_wave(own);
     }
+    const int total = __builtin_amdgcn_readlane(end, 63);
     Range8 g;
-    g.per = max((total + p.ranges - 1) / p.ranges, 8);  // two pages a wave
+    const int ranges = total <= 16 * p.n ? p.ranges : min(p.base, p.ranges);
+    // At least two pages a wave of a long request; of short ones about one request (6 requests of one token over 8 KV heads
+    // in one range took 28 us, in six 8.4).
+    g.per = max((total + ranges - 1) / ranges, max(min(total / p.n, 8), 1));
+    g.whole = min(g.per + (g.per + 1) / 2, D8_WHOLE);
     g.once = (int64_t)total * p.Hkv > D8_ONCE;
     int start = range * g.per;
     g.left = min(g.per, total - start);
     g.b = g.k = 0;
     if (g.left <= 0) return g;
-    for (int b0 = 0;; b0 += 64) {
-        if (p.n > 64) {
-            own = b0 + lane < p.n ? seen_by(p, b0 + lane).pages : 0;
+    int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= start));
+    if (some > 1) {
+        start -= __builtin_amdgcn_readlane(end, at) - __builtin_amdgcn_readlane(own, at);
+        const int b1 = min((at + 1) * some, p.n);
+        for (g.b = at * some;; g.b += 64) {
+            own = g.b + lane < b1 ? seen_by(p, g.b + lane).pages : 0;
             end = scan_wave(own);
+            at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= start));
+            if (at < 64) break;
+            start -= __builtin_amdgcn_readlane(end, 63);
         }
-        const int at = __builtin_popcountll(__builtin_amdgcn_ballot_w64(end <= start));
-        if (at < 64) {
-            g.b = b0 + at;
-            g.k = start - __builtin_amdgcn_readlane(end, at) + __builtin_amdgcn_readlane(own, at);
-            return g;
-        }
-        start -= __builtin_amdgcn_readlane(end, 63);
     }
+    g.b += at;
+    const int pages = __builtin_amdgcn_readlane(own, at);
+    g.k = start - __builtin_amdgcn_readlane(end, at) + pages;
+    if (g.k > 0 && pages <= g.whole) {  // the range before has it
+        g.left -= pages - g.k;
+        g.k = 0;
+        if (g.left > 0)
+            do ++g.b;
+            while (seen_by(p, g.b).pages == 0);
+    }
+    return g;
+}
+
+// The end of what a range with `left` pages to its end takes of a request from page k on.
+__device__ __forceinline__ int taken(const Range8& g, const SeenPages& seen, int k, int left) {
+    return seen.pages <= g.whole ? seen.pages : min(seen.pages, k + left);
 }
 
 __device__ __forceinline__ f32x4_t mfma_f16(uint4 a, uint4 b, f32x4_t c) {
@@ -207,7 +235,7 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
     };
     int b = g.b, k0 = g.k, left = g.left;
     SeenPages seen = seen_by(p, b);
-    int k1 = min(seen.pages, k0 + left);
+    int k1 = taken(g, seen, k0, left);
     Look8 ahead = look_up(p, seen, b, h, k0 + 2 * wave, k1);
     load_q(b);
     for (;;) {
@@ -381,7 +409,7 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
         if (left > 0) {
             do then = seen_by(p, ++next);
             while (then.pages == 0);
-            ahead = look_up(p, then, next, h, 2 * wave, min(then.pages, left));
+            ahead = look_up(p, then, next, h, 2 * wave, taken(g, then, 0, left));
             load_q(next);
         }
         l = sum_rows(l);
@@ -431,7 +459,7 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
         b = next;
         seen = then;
         k0 = 0;
-        k1 = min(seen.pages, left);
+        k1 = taken(g, seen, 0, left);
     }
 }
 
@@ -499,10 +527,14 @@ int device_cus() {
     return c;
 }
 
-// Ranges that a call's pages are cut into: workgroups for 2 a CU with a range's KV heads, 8 pages a range at least.
+int decode8_base(int num_kv_heads) { return std::max(1, 2 * device_cus() / num_kv_heads); }
+
+// Ranges that a call's pages are cut into, at most: workgroups for 2 a CU with a range's KV heads, more for many requests.
 int decode8_ranges(int n, int num_kv_heads, int span, int window, int sinks) {
     const int64_t pages = (int64_t)n * seen_pages_most(span, window, sinks);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(2 * device_cus() / num_kv_heads, (pages + 7) / 8));
+    if (n == 1) return (int)std::min<int64_t>(decode8_base(num_kv_heads), pages <= D8_WHOLE ? 1 : (pages + 7) / 8);
+    const int base = decode8_base(num_kv_heads);
+    return (int)std::min<int64_t>(std::max(base, std::min(n, D8_MORE * base)), pages);
 }
 
 size_t decode8_bytes(int n, int num_heads, int ranges) {
@@ -560,6 +592,7 @@ int starkv_decode_kv8(void* stream, const void* query, int64_t q_s0, int64_t q_s
     p.seq_lens = seq_lens;
     p.span = (int)std::min<int64_t>({(int64_t)bt_width * block_size, 0x7ffffff0, (int64_t)max_seq_len});
     p.n = n; p.Hkv = num_kv_heads; p.G = num_heads / num_kv_heads;
+    p.base = decode8_base(num_kv_heads);
     p.ranges = decode8_ranges(n, num_kv_heads, max_seq_len, window, sinks);
     p.window = window; p.sinks = sinks;
     p.sc = scale * 1.4426950408889634f;

@@ -335,7 +335,8 @@ def test_decode_through_a_window(cuda, size, sinks):
         close(paged_decode_8(q, c, bt, sl, max(lens), SCALE, window=w), q, c, bt, lens, w, what=(code, dt))
 
 
-@pytest.mark.parametrize("n,H,G,most", [(65, 1, 2, 40), (200, 2, 1, 300), (131, 40, 1, 33), (300, 1, 16, 17)])
+@pytest.mark.parametrize("n,H,G,most", [(65, 1, 2, 40), (200, 2, 1, 300), (131, 40, 1, 33), (300, 1, 16, 17), (24, 5, 1, 3), (200, 8, 2, 60),
+                                        (64, 32, 1, 100), (300, 2, 4, 170), (4200, 1, 1, 20)])
 def test_decode_of_many_requests(cuda, n, H, G, most):
     """More requests than a wave looks at, none among them with tokens or all; ranges that hold many and that cut some."""
     g = torch.Generator().manual_seed(n)
