@@ -17,7 +17,7 @@
 //
 // Memory bounds it: 256 bytes of codes a token and KV head, far above the instructions' time for any G. 64 requests of
 // 8192 tokens over 8 KV heads (1.08 GB) 178 us, 6.0 TB/s; 24 of 1000 to 8191 (237 MB) 58; one of 4096 over 32 KV heads (34 MB) 15,
-// of which 4 are the merge. The next pages' loads ahead of a pair's products gained nothing, nor did 3 or 4 workgroups a CU.
+// of which 4 are the merge's launch. The next pages' loads ahead of a pair's products gained nothing, nor did 3 or 4 workgroups a CU.
 //
 // Both products run on v_mfma_f32_16x16x32_f16, for which every code and fp16 query is exact; a bf16 query row goes to fp16
 // by a power of two that brings its largest value to 2^14, which leaves values down to 2^-28 of that exact. S^T =
@@ -463,25 +463,31 @@ __global__ __launch_bounds__(D8_THR, 3) void decode8_kernel(const Decode8Params 
     }
 }
 
-// A head's partials joined by one wave: sums of weights above the largest m, of values above the largest r. The first lies
-// second in its range (other requests may end there), the others first in theirs. Lane s of 64 holds the factors of 64
-// partials at a time and sums dimensions 2 s and 2 s + 1, eight partials' loads in flight.
-template <int QDT>
-__global__ __launch_bounds__(64) void merge8_kernel(const Decode8Params p) {
-    const int lane = threadIdx.x, hq = blockIdx.x, b = blockIdx.y, H = p.Hkv * p.G;
+// A head's partials joined by WAVES waves: sums of weights above the largest m, of values above the largest r. The first lies
+// second in its range (other requests may end there), the others first in theirs. A wave takes a run of them; its lane s of
+// 64 holds the factors of 64 partials at a time and sums dimensions 2 s and 2 s + 1, eight partials' loads in flight.
+template <int QDT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void merge8_kernel(const Decode8Params p) {
+    __shared__ float4 s_ref[WAVES];
+    __shared__ float2 s_sum[WAVES][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int hq = blockIdx.x, b = blockIdx.y, H = p.Hkv * p.G;
     const int64_t to = b * p.o_s0 + hq * p.o_s1 + 2 * lane;
     const int2 where = p.where[b];
     if (seen_by(p, b).pages == 0) {  // no workgroup has it, nor has one said where it is
-        store_f(p.out, to, QDT, 0.f);
-        store_f(p.out, to + 1, QDT, 0.f);
+        if (wave == 0) {
+            store_f(p.out, to, QDT, 0.f);
+            store_f(p.out, to + 1, QDT, 0.f);
+        }
         return;
     }
     if (where.y == 1) return;
     const auto part = [&](int s) { return p.part + ((int64_t)(2 * (where.x + s) + (s == 0)) * H + hq) * D8_PART; };
+    const int run = (where.y + WAVES - 1) / WAVES, end = min((wave + 1) * run, where.y);
     float M = -INFINITY, R = -INFINITY, lt = 0.f;
     float2 a = make_float2(0.f, 0.f);
-    for (int c0 = 0; c0 < where.y; c0 += 64) {
-        const int count = min(where.y - c0, 64);
+    for (int c0 = wave * run; c0 < end; c0 += 64) {
+        const int count = min(end - c0, 64);
         float2 v[8];  // the first eight's sums are on their way with the references
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[u] = *(const float2*)(part(c0 + min(u, count - 1)) + 4 + 2 * lane);
@@ -509,6 +515,28 @@ __global__ __launch_bounds__(64) void merge8_kernel(const Decode8Params p) {
                     a.y = fmaf(v[u].y, fs, a.y);
                 }
             }
+        }
+    }
+    if constexpr (WAVES > 1) {
+        if (lane == 0) s_ref[wave] = make_float4(M, lt, R, 0.f);
+        s_sum[wave][lane] = a;
+        __syncthreads();
+        if (wave > 0) return;
+        float4 x[WAVES];
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) {
+            x[k] = s_ref[k];
+            M = fmaxf(M, x[k].x);
+            R = fmaxf(R, x[k].z);
+        }
+        lt = a.x = a.y = 0.f;
+#pragma unroll
+        for (int k = 0; k < WAVES; ++k) {
+            const float f = x[k].z == -INFINITY ? 0.f : exp2f(x[k].z - R);
+            const float2 v = s_sum[k][lane];
+            lt = fmaf(x[k].y, x[k].x == -INFINITY ? 0.f : exp2f(x[k].x - M), lt);
+            a.x = fmaf(v.x, f, a.x);
+            a.y = fmaf(v.y, f, a.y);
         }
     }
     store_f(p.out, to, QDT, weigh_out(a.x, lt, M, R));
@@ -544,6 +572,11 @@ size_t decode8_bytes(int n, int num_heads, int ranges) {
 template <int CT, int QDT>
 const void* decode_pick(int G) {
     return G <= 8 ? (const void*)&decode8_kernel<CT, QDT, false> : (const void*)&decode8_kernel<CT, QDT, true>;
+}
+
+template <int QDT>
+const void* merge_pick(int waves) {
+    return waves == 1 ? (const void*)&merge8_kernel<QDT, 1> : waves == 4 ? (const void*)&merge8_kernel<QDT, 4> : (const void*)&merge8_kernel<QDT, 16>;
 }
 
 }  // namespace
@@ -609,11 +642,11 @@ int starkv_decode_kv8(void* stream, const void* query, int64_t q_s0, int64_t q_s
     SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)((int64_t)p.ranges * num_kv_heads)), dim3(D8_THR), args,
                             (size_t)4 * p.G * D8_PART * 4, (hipStream_t)stream));
     if (p.ranges == 1) return STARKV_OK;
-    if (bf)
-        hipLaunchKernelGGL(merge8_kernel<STARKV_BF16>, dim3(num_heads, n), dim3(64), 0, (hipStream_t)stream, p);
-    else
-        hipLaunchKernelGGL(merge8_kernel<STARKV_F16>, dim3(num_heads, n), dim3(64), 0, (hipStream_t)stream, p);
-    SKV_HIP(hipGetLastError());
+    // One wave joins eight partials in the time of one; more by several: one request of 8192 tokens over 8 KV heads (64) 17.6 us by
+    // one wave, 14.4 by 4, 15.1 by 16; of 65536 over one (512) 58.7, 24.6, 18.1; of 1000 over 8 (8) 9.7 by one, 10.3 by 4.
+    const int waves = p.ranges < 16 * n ? 1 : p.ranges < 128 * n ? 4 : 16;
+    SKV_HIP(hipLaunchKernel(bf ? merge_pick<STARKV_BF16>(waves) : merge_pick<STARKV_F16>(waves), dim3(num_heads, n), dim3(64 * waves),
+                            args, 0, (hipStream_t)stream));
     return STARKV_OK;
 }
 

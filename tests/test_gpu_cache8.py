@@ -357,6 +357,20 @@ def test_decode_of_many_requests(cuda, n, H, G, most):
     assert (paged_decode_8(q, c, bt, sl * 0, 1 << 20, SCALE) == 0).all()
 
 
+@pytest.mark.parametrize("G", [2, 9])
+@pytest.mark.parametrize("L", [1, 100, 257, 700, 2500, 20000])
+def test_decode_of_one_request(cuda, L, G):
+    """Few and many parts of one request, joined by as many waves as its longest length asks for."""
+    g = torch.Generator().manual_seed(L)
+    c, bt, sl = session([L], 1, 16, F8, cuda, g)
+    q = torch.randn(1, G, D, generator=g).to(F16).to(cuda)
+    for span in (L, 1 << 20):
+        close(paged_decode_8(q, c, bt, sl, span, SCALE), q, c, bt, [L], None)
+    two = paged_decode_8(q.repeat(2, 1, 1), c, bt.repeat(2, 1), torch.cat([sl * 0, sl]), 1 << 20, SCALE)
+    assert (two[0] == 0).all()
+    close(two[1:], q, c, bt, [L], None)
+
+
 def test_decode_of_more_heads_than_workgroups(cuda):
     """One range for all pages: no partials, and rows without tokens written with the others."""
     g = torch.Generator().manual_seed(20)
