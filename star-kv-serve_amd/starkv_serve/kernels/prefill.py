@@ -13,31 +13,39 @@ from starkv_serve import _hip
 from starkv_serve.kernels.window import Window, sizes
 
 
-def block_list(query_lens: List[int]) -> List[int]:
-    """The kernel's workgroup rows, (prompt, query block) pairs flattened, from the
-    library's host helper starkv_prefill_block_list (the query block size is the
-    kernel's): the blocks with the most keys first."""
+def _tables(query_lens: List[int]) -> tuple:
+    """The prompts' first tokens and their ends, then the workgroup rows, as int32 in one buffer; how many of the latter."""
     cu = [0]
     for L in query_lens:
         if L < 0:
             raise ValueError(f"negative prompt length {L}")
         cu.append(cu[-1] + int(L))
-    lib = _hip.lib()
-    cu_c = (ctypes.c_int32 * len(cu))(*cu)
-    n = lib.starkv_prefill_block_list(cu_c, len(query_lens), None, 0)
-    buf = (ctypes.c_int32 * (2 * max(n, 1)))()
-    if n < 0 or lib.starkv_prefill_block_list(cu_c, len(query_lens), buf, n) != n:
+    lib, P = _hip.lib(), len(cu)
+    cu_c = (ctypes.c_int32 * P)(*cu)
+    n = lib.starkv_prefill_block_list(cu_c, P - 1, None, 0)
+    buf = (ctypes.c_int32 * (P + 2 * max(n, 1)))()
+    rows = (ctypes.c_int32 * (2 * max(n, 1))).from_buffer(buf, 4 * P)
+    if n < 0 or lib.starkv_prefill_block_list(cu_c, P - 1, rows, n) != n:
         raise RuntimeError("starkv_prefill_block_list failed")
-    return list(buf)[:2 * n]
+    ctypes.memmove(buf, cu_c, 4 * P)
+    return buf, n
+
+
+def block_list(query_lens: List[int]) -> List[int]:
+    """The kernel's workgroup rows, (prompt, query block) pairs flattened, from the
+    library's host helper starkv_prefill_block_list (the query block size is the
+    kernel's): the blocks with the most keys first."""
+    buf, n = _tables(query_lens)
+    P = len(query_lens) + 1
+    return buf[P:P + 2 * n]
 
 
 def prompt_tables(query_lens: List[int], device) -> tuple:
     """(cu_seqlens [P + 1], blocks [num_blocks, 2]) int32 on `device`, in one upload."""
-    cu = [0]
-    for L in query_lens:
-        cu.append(cu[-1] + int(L))
-    meta = torch.tensor(cu + block_list(query_lens), dtype=torch.int32).to(device, non_blocking=True)
-    return meta[:len(cu)], meta[len(cu):].view(-1, 2)
+    buf, n = _tables(query_lens)
+    P = len(query_lens) + 1
+    meta = torch.frombuffer(buf, dtype=torch.int32).to(device, non_blocking=True)
+    return meta[:P], meta.as_strided((n, 2), (2, 1), P)
 
 
 def prefill_lift(k_codes: torch.Tensor, v_codes: torch.Tensor, cu_seqlens: torch.Tensor, k_up: torch.Tensor,
