@@ -209,7 +209,7 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
         const uint8_t* src = val ? p.v + (KDT == STARKV_F16 ? k0v : v0v) : p.k + k0v;
         const int r0 = tile_of(t) * PF_KT;
         const int rows = max(0, min(PF_KT, L - r0));
-        const int64_t bytes = KDT == STARKV_F16 ? rows * s0 : rows > 0 ? (rows - 1) * s0 + 256 : 0;  // strides of any kind
+        const int64_t bytes = !WINDOW ? rows * s0 : rows > 0 ? (rows - 1) * s0 + 256 : 0;  // strides of any kind
         int4v_t rs = buffer_rsrc(src + (int64_t)r0 * s0, (int)bytes);
 #pragma unroll
         for (int e = 0; e < 4; ++e) rs[e] = rfl(rs[e]);  // uniform by construction; the copies take them in SGPRs

@@ -89,18 +89,21 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_l
     if T == 0:
         return out
     _hip.require_cuda(q, k, v, out)
-    # Through a window bf16 keys are read as they are; values are fp16, as the weights that multiply them.
-    raw = (window is not None and q.dtype == k.dtype == v.dtype == torch.bfloat16 and k.stride(-1) == v.stride(-1) == 1
-           and k.stride(0) % 8 == k.stride(1) % 8 == k.data_ptr() % 16 == 0 and k.stride(0) < 1 << 23)
-    if raw:
+    # Through a window keys of bf16, and keys and values of fp16, are read as they are; values are fp16, as the weights that
+    # multiply them.
+    as_is = (window is not None and q.dtype == k.dtype == v.dtype and k.stride(-1) == v.stride(-1) == 1
+             and k.stride(0) % 8 == k.stride(1) % 8 == k.data_ptr() % 16 == 0 and k.stride(0) < 1 << 23)
+    if as_is and k.dtype == torch.float16 and k.stride() == v.stride() and v.data_ptr() % 16 == 0:
+        pass
+    elif as_is and k.dtype == torch.bfloat16:
         v16 = torch.empty(v.shape, dtype=torch.float16, device=v.device)
         _hip.ops().prefill_to_half(None, v, None, v16)
         v = v16
-    elif k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.stride(-1) == v.stride(-1) == 1:
-        kv = torch.empty((2, *k.shape), dtype=torch.float16, device=k.device)
-        _hip.ops().prefill_to_half(k, v, kv[0], kv[1])
-        k, v = kv[0], kv[1]
-    if not raw:
+    else:
+        if k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.stride(-1) == v.stride(-1) == 1:
+            kv = torch.empty((2, *k.shape), dtype=torch.float16, device=k.device)
+            _hip.ops().prefill_to_half(k, v, kv[0], kv[1])
+            k, v = kv[0], kv[1]
         k, v = k.to(torch.float16), v.to(torch.float16)
         k, v = k.contiguous(), v.contiguous()
     q = q if q.stride(-1) == 1 else q.contiguous()

@@ -244,6 +244,22 @@ def test_prompts_of_any_strides(cuda):
     prompts_close(prefill_attention(q, k, v, [L], SCALE * 1e-20, window=w), q, k, v, [L], w, "large", SCALE * 1e-20)
 
 
+def test_prompts_of_any_fp16_strides(cuda):
+    """fp16 keys and values where they lie, with strides of one kind or two, broadcast, unaligned, of one token."""
+    g = torch.Generator().manual_seed(14)
+    L, w = 300, Window(70, 5)
+    wide = torch.randn(L, 6, 3 * D, generator=g).to(F16).to(cuda)
+    q = torch.randn(L, 4, D, generator=g).to(F16).to(cuda)
+    by_head = wide.transpose(0, 1).contiguous().transpose(0, 1)
+    for k, v in ((wide[:, 1:3, D:2 * D], wide[:, 3:5, :D]), (wide[:, :1, :D].expand(L, 2, D), wide[:, 5:, D:2 * D].expand(L, 2, D)),
+                 (wide[:1, :2, :D].expand(L, 2, D), wide[4:5, :2, :D].expand(L, 2, D)), (wide[:, ::3, 8:8 + D], wide[:, 1::3, 16:16 + D]),
+                 (wide[:, 2:4, 4:4 + D], wide[:, :2, 4:4 + D]), (wide[:, :2, :D], wide[:, 2:4, 2:2 + D]), (by_head[:, :2, :D], by_head[:, 4:, D:2 * D]),
+                 (by_head[:, :2, :D], wide[:, :2, :D])):
+        prompts_close(prefill_attention(q, k, v, [L - 20, 20], SCALE, window=w), q, k, v, [L - 20, 20], w, (k.stride(), v.stride()))
+    k1, v1 = (t.as_strided((1, 2, D), (8, 3 * D, 1)) for t in (wide[7:8, :2, :D], wide[9:10, :2, :D]))
+    prompts_close(prefill_attention(q[:1], k1, v1, [1], SCALE, window=w), q[:1], k1, v1, [1], w)
+
+
 @pytest.mark.parametrize("dt", [BF16, F16])
 def test_prompts_of_infinite_values(cuda, dt):
     """Infinite values and NaN reach the rows that see them, and no others; keys that are not finite the same."""
