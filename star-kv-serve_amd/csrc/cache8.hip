@@ -14,12 +14,15 @@
 // heads 6.6 against 10.7, of 1024 9.6 against 10.9 (of 32 heads 20 against 13), of 2048 12.7 against 11.5 (28 against 16).
 // The map's workgroups do up to WR_RUN blocks one after the other, which is what a step of many requests pays there.
 //
-// A workgroup of the first kind has 4 heads, a wave each, up to WR_WIDE tokens times heads, and 16 above: 4 heads take a
-// prompt of 64 tokens of 32 heads from 12.6 to 6.1 us, 16 a step of 1024 tokens of 32 heads from 20 to 9.3.
+// A workgroup of the first kind has 4 heads, a wave each, and up to 16 where there would be more than WR_WIDE workgroups: 4 heads
+// take a prompt of 64 tokens of 32 heads from 12.6 to 6.1 us, 16 a step of 1024 tokens of 32 heads from 20 to 9.3. In blocks
+// of 32 it begins with 2 heads, in larger ones with one, up to WR_WIDE_LARGE workgroups: 300 tokens of 32 heads in blocks of 64 66 ->
+// 24 us, a step of 300 7.8 -> 11.
 //
 // A wave takes a head of the block, keys and values: four rows of 256 bytes a load, largest magnitudes as integer bits
 // (NaN is above infinity, which is above all others), rows kept in registers from the first look to the rounding where there
-// are at most 16. A block with one token (a step's) is write_single's. Rows are read past the caches: the codes stay there for
+// are at most 16; of more, 2 or 4 waves share a head and meet in LDS (11400 tokens of 32 heads in blocks of 64 191 -> 82 us, of
+// 1024 999 -> 163). A block with one token (a step's) is write_single's. Rows are read past the caches: the codes stay there for
 // what reads them next (11400 tokens of 32 heads written and read back 130 -> 107 us).
 //
 // Bound by memory, and for small calls by latency: a step of 64 tokens of 8 heads takes 3.8 us, of which a launch in a graph
@@ -35,7 +38,8 @@ namespace {
 
 constexpr int WR_THR = 256;
 constexpr int WR_FEW = 1024;   // tokens that a workgroup looks through
-constexpr int WR_WIDE = 4096;  // up to so many tokens times heads a workgroup of few tokens has 4 heads, else 16
+constexpr int WR_WIDE = 1024;  // workgroups of few tokens: more heads each rather than more, in blocks of 16;
+constexpr int WR_WIDE_LARGE = 4096;  // in larger ones
 constexpr int WR_RUN = 16;   // tokens of a workgroup of a larger write
 constexpr int WR_HELD = 64;  // places of a block that are looked through once
 
@@ -121,23 +125,23 @@ __device__ __forceinline__ int joined(int old, int e, bool fresh) {
     return fresh ? e : old == C8_NAN || e == C8_NAN ? C8_NAN : max(old, e);
 }
 
-// The codes of places first, first + STEP, ... that have no token now (tok < 0) to an exponent that is `by` more, eight of a
+// The codes of places first, first + step, ... that have no token now (tok < 0) to an exponent that is `by` more, eight of a
 // place to a lane: the loads of DEEP places go out before the first is rounded.
-template <int CT, int STEP, int DEEP, class Tok>
-__device__ __forceinline__ void lessen(uint8_t* dst, int64_t stride, int first, int size, Tok tok, int by) {
+template <int CT, int DEEP, class Tok>
+__device__ __forceinline__ void lessen(uint8_t* dst, int64_t stride, int first, int step, int size, Tok tok, int by) {
     const float less = c8_scale(-min(by, 126));
-    for (int at = first; at < size; at += DEEP * STEP) {
+    for (int at = first; at < size; at += DEEP * step) {
         uint2 w[DEEP];
 #pragma unroll
         for (int i = 0; i < DEEP; ++i)
-            if (at + STEP * i < size) w[i] = *(const uint2*)(dst + (at + STEP * i) * stride);
+            if (at + step * i < size) w[i] = *(const uint2*)(dst + (at + step * i) * stride);
 #pragma unroll
         for (int i = 0; i < DEEP; ++i) {
-            if (at + STEP * i >= size || tok(at + STEP * i) >= 0) continue;
+            if (at + step * i >= size || tok(at + step * i) >= 0) continue;
             float a[4], b[4];
             c8_values<CT>(w[i].x, a);
             c8_values<CT>(w[i].y, b);
-            *(uint2*)(dst + (at + STEP * i) * stride) =
+            *(uint2*)(dst + (at + step * i) * stride) =
                 make_uint2(c8_pack<CT>(a[0] * less, a[1] * less, a[2] * less, a[3] * less),
                            c8_pack<CT>(b[0] * less, b[1] * less, b[2] * less, b[3] * less));
         }
@@ -177,15 +181,13 @@ __device__ __forceinline__ void write_head(const Write8Params& p, const Rows8& r
     const bool fresh = tok[0] >= 0;
 #pragma unroll
     for (int z = 0; z < 2; ++z) {
-        const uint8_t* src = p.src[z] + h * p.s1[z] + 16 * d;
         uint8_t* dst = p.codes[z] + blk * p.c_s0 + h * p.c_s2 + 8 * d;
         uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < KEEP; ++i) top = pair_max(top, r.w[z][i]);
-        for (int at = 4 * KEEP + row; at < count; at += 4) top = pair_max(top, *(const uint4*)(src + tok[list[at]] * p.s0[z]));
         const int old = r.old[z], e = joined(old, c8_exponent<CT>(wave_umax(top_bits<DT>(top))), fresh);
         if (!fresh && e != old && e != C8_NAN)  // the codes that are there, to the new exponent
-            lessen<CT, 4, DEEP>(dst, p.c_s1, row, 1 << p.shift, [&](int at) { return tok[at]; }, e - old);
+            lessen<CT, DEEP>(dst, p.c_s1, row, 4, 1 << p.shift, [&](int at) { return tok[at]; }, e - old);
         const float inv = e == C8_NAN ? 0.f : c8_scale(-e);
         const auto put = [&](int at, const uint4& w) {
             *(uint2*)(dst + list[at] * p.c_s1) = e == C8_NAN ? make_uint2(0, 0) : encode<CT, DT>(w, inv);
@@ -193,7 +195,6 @@ __device__ __forceinline__ void write_head(const Write8Params& p, const Rows8& r
 #pragma unroll
         for (int i = 0; i < KEEP; ++i)
             if (4 * i + row < count) put(4 * i + row, r.w[z][i]);
-        for (int at = 4 * KEEP + row; at < count; at += 4) put(at, *(const uint4*)(src + tok[list[at]] * p.s0[z]));
         if (lane == 0 && e != old) ex[z] = (int8_t)e;
     }
 }
@@ -202,6 +203,7 @@ struct Block8Shared {
     int tok[C8_MAX_BLOCK];        // the token of each place, -1
     uint16_t list[C8_MAX_BLOCK];  // the places that have one
     int count, lead;
+    uint32_t top[2][2][WR_THR / 64];  // by turn, keys or values, wave
 };
 
 // The places with tokens, from tok; the workgroup's threads meet on both sides.
@@ -235,7 +237,7 @@ __device__ __forceinline__ void write_single(const Write8Params& p, int blk, int
         const int e = joined(old[z], c8_exponent<CT>(row_umax(top_bits<DT>(pair_max(0, w[z])))), place == 0);
         for (uint64_t grown = __ballot(on && d == 0 && place != 0 && e != old[z] && e != C8_NAN); grown; grown &= grown - 1) {
             const int g = __builtin_ctzll(grown), by = __builtin_amdgcn_readlane(e - old[z], g);
-            lessen<CT, 4, DEEP>(dst + (h0 + WR_THR / 64 * (g >> 4)) * p.c_s2, p.c_s1, row, 1 << p.shift,
+            lessen<CT, DEEP>(dst + (h0 + WR_THR / 64 * (g >> 4)) * p.c_s2, p.c_s1, row, 4, 1 << p.shift,
                                 [&](int at) { return at == place ? t : -1; }, by);
         }
         if (!on) continue;
@@ -244,13 +246,83 @@ __device__ __forceinline__ void write_single(const Write8Params& p, int blk, int
     }
 }
 
-// Heads [h0, h1) of a block by a workgroup.
+// Heads of a block of more than 4 KEEP tokens by teams of 2 or 4 waves (`team` of them), 4 KEEP rows a wave at a time: the first
+// ones stay in registers from the first look to the rounding, others are read twice. The largest magnitudes meet in LDS, one
+// barrier a head.
 template <int CT, int DT, int DEEP>
-__device__ __forceinline__ void write_heads(const Write8Params& p, const Block8Shared& sh, int blk, int h0, int h1) {
+__device__ __forceinline__ void write_together(const Write8Params& p, Block8Shared& sh, int blk, int h0, int h1, int team) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane >> 4, d = lane & 15;
+    const int member = wave & (team - 1), teams = WR_THR / 64 / team, count = sh.count, stride = 4 * KEEP * team;
+    const bool fresh = sh.tok[0] >= 0;
+    for (int i = 0; h0 + i * teams < h1; ++i) {
+        const int h = h0 + i * teams + wave / team;
+        const bool on = h < h1;
+        int8_t* ex = p.ex + blk * p.x_s0 + h * p.x_s1;
+        uint4 w[2][KEEP];
+        int old[2] = {0, 0};
+        // Rows of places first + 4 i + row of the list.
+        const auto load = [&](int z, int first) {
+#pragma unroll
+            for (int k = 0; k < KEEP; ++k) {
+                const int at = first + 4 * k + row;
+                w[z][k] = on && at < count ? load_once16(p.src[z] + h * p.s1[z] + 16 * d + (int64_t)sh.tok[sh.list[at]] * p.s0[z])
+                                           : make_uint4(0, 0, 0, 0);
+            }
+        };
+        const int own = 4 * KEEP * member;
+        uint32_t top[2] = {0, 0};
+        for (int first = own + (count - 1 - own) / stride * stride; first >= own; first -= stride) {  // its first rows last
+#pragma unroll
+            for (int z = 0; z < 2; ++z) load(z, first);
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+#pragma unroll
+                for (int k = 0; k < KEEP; ++k) top[z] = pair_max(top[z], w[z][k]);
+        }
+        if (on) {
+#pragma unroll
+            for (int z = 0; z < 2; ++z) old[z] = ex[z];
+        }
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            const uint32_t t = wave_umax(top_bits<DT>(top[z]));
+            if (lane == 0) sh.top[i & 1][z][wave] = t;
+        }
+        __syncthreads();
+        if (!on) continue;
+#pragma unroll
+        for (int z = 0; z < 2; ++z) {
+            uint32_t t = 0;
+            for (int k = 0; k < team; ++k) t = max(t, sh.top[i & 1][z][wave - member + k]);
+            uint8_t* dst = p.codes[z] + blk * p.c_s0 + h * p.c_s2 + 8 * d;
+            const int e = joined(old[z], c8_exponent<CT>(t), fresh);
+            if (!fresh && e != old[z] && e != C8_NAN)
+                lessen<CT, DEEP>(dst, p.c_s1, 4 * member + row, 4 * team, 1 << p.shift, [&](int at) { return sh.tok[at]; }, e - old[z]);
+            const float inv = e == C8_NAN ? 0.f : c8_scale(-e);
+            for (int first = own; first < count; first += stride) {
+                if (first > own) load(z, first);
+#pragma unroll
+                for (int k = 0; k < KEEP; ++k) {
+                    const int at = first + 4 * k + row;
+                    if (at < count) *(uint2*)(dst + sh.list[at] * p.c_s1) = e == C8_NAN ? make_uint2(0, 0) : encode<CT, DT>(w[z][k], inv);
+                }
+            }
+            if (member == 0 && lane == 0 && e != old[z]) ex[z] = (int8_t)e;
+        }
+    }
+}
+
+// Heads [h0, h1) of a block by a workgroup.
+template <int CT, int DT, int DEEP, bool LARGE>
+__device__ __forceinline__ void write_heads(const Write8Params& p, Block8Shared& sh, int blk, int h0, int h1) {
     const int wave = threadIdx.x >> 6;
     if (sh.count == 1) {
         const int place = sh.list[0];
         for (int h = h0 + wave; h < h1; h += WR_THR / 16) write_single<CT, DT, DEEP>(p, blk, h, h1, sh.tok[place], place);
+        return;
+    }
+    if (LARGE && sh.count > 4 * KEEP) {
+        write_together<CT, DT, DEEP>(p, sh, blk, h0, h1, sh.count > 8 * KEEP ? 4 : 2);
         return;
     }
     for (int h = h0 + wave; h < h1; h += WR_THR / 64) {
@@ -291,7 +363,7 @@ __global__ __launch_bounds__(WR_THR) void write8_few_kernel(const Write8Params p
     }
     list_places(sh, p.shift);
     if (sh.lead != t) return;
-    write_heads<CT, DT, 4>(p, sh, blk, blockIdx.y * heads, min((int)(blockIdx.y + 1) * heads, p.H));
+    write_heads<CT, DT, 4, true>(p, sh, blk, blockIdx.y * heads, min((int)(blockIdx.y + 1) * heads, p.H));
 }
 
 __global__ __launch_bounds__(WR_THR) void write8_map_kernel(const Write8Params p) {
@@ -307,50 +379,71 @@ __device__ __forceinline__ int mapped(const Write8Params& p, int64_t slot) {
     return (uint32_t)t < (uint32_t)p.n && slot_of(p, t) == slot ? t : -1;
 }
 
-// A workgroup WR_RUN tokens and `heads` heads: the blocks that one of the tokens leads (has the lowest place of). 16 threads
-// a token look through its block's places; what they find of the first WR_HELD places stays with them for the
-// block's turn.
-template <int CT, int DT>
-__global__ __launch_bounds__(WR_THR) void write8_kernel(const Write8Params p, int heads) {
+// Whether token t has a slot and the one before it has no lower place of the same block.
+__device__ __forceinline__ bool may_lead(const Write8Params& p, int t) {
+    const int64_t slot = t < p.n ? slot_of(p, t) : -1, before = t > 0 && t < p.n ? slot_of(p, t - 1) : -1;
+    return slot >= 0 && !(before < slot && before >= (slot >> p.shift << p.shift));
+}
+
+// A workgroup `runs` times WR_RUN tokens (WR_THR at most) and `heads` heads: the blocks that one of the tokens leads (has the
+// lowest place of). 16 threads a token that may lead look through its block's places; what they find of the first
+// WR_HELD places stays with them for the block's turn. LARGE: blocks of more than 16 tokens (one run of blocks of 16 with the
+// others' registers would leave room for a quarter fewer waves).
+template <int CT, int DT, bool LARGE>
+__global__ __launch_bounds__(WR_THR) void write8_kernel(const Write8Params p, int runs, int heads) {
     __shared__ Block8Shared sh;
-    __shared__ int s_follows[WR_RUN], s_blk[WR_RUN];
-    const int groups = (p.H + heads - 1) / heads, run = blockIdx.x / groups, group = blockIdx.x % groups;
+    __shared__ int s_follows[WR_RUN], s_blk[WR_RUN], s_any[WR_THR / WR_RUN];
+    const int groups = (p.H + heads - 1) / heads, first_t = blockIdx.x / groups * runs * WR_RUN, group = blockIdx.x % groups;
     const int tid = threadIdx.x, size = 1 << p.shift, mine = tid / WR_RUN, sub = tid % WR_RUN;
-    int held[WR_HELD / WR_RUN];
-    {
-        const int t = run * WR_RUN + mine;
-        const int64_t slot = t < p.n ? slot_of(p, t) : -1, first = slot & ~(int64_t)(size - 1);
-        if (sub == 0) {
-            s_follows[mine] = 0;
-            s_blk[mine] = (int)(slot >> p.shift);
-        }
-        __syncthreads();
-        if (slot < 0) {
-            s_follows[mine] = 1;
-        } else {
-#pragma unroll
-            for (int i = 0; i < WR_HELD / WR_RUN; ++i) held[i] = sub + WR_RUN * i < size ? mapped(p, first + sub + WR_RUN * i) : -1;
-            bool follows = p.map[slot] != t;  // another token has the slot too, and the map names that
-#pragma unroll
-            for (int i = 0; i < WR_HELD / WR_RUN; ++i) follows = follows || (held[i] >= 0 && first + sub + WR_RUN * i < slot);
-            for (int64_t s = first + sub + WR_HELD; s < slot; s += WR_RUN) follows = follows || mapped(p, s) >= 0;
-            if (follows) s_follows[mine] = 1;
-        }
-        __syncthreads();
+    if (LARGE && runs > 1) {  // of several runs most have none that may lead
+        const uint64_t may = __ballot(tid < runs * WR_RUN && may_lead(p, first_t + tid));
+        if (sub == 0) s_any[mine] = (may >> (tid & 48) & 0xffff) != 0;
+    } else if (tid == 0) {
+        s_any[0] = 1;
     }
-    for (int j = 0; j < WR_RUN; ++j) {
-        if (s_follows[j]) continue;
-        const int blk = s_blk[j];
-        if (tid == 0) sh.count = 0;
-        if (mine == j) {
-#pragma unroll
-            for (int i = 0; i < WR_HELD / WR_RUN; ++i)
-                if (sub + WR_RUN * i < size) sh.tok[sub + WR_RUN * i] = held[i];
-        }
-        for (int i = tid + WR_HELD; i < size; i += WR_THR) sh.tok[i] = mapped(p, ((int64_t)blk << p.shift) + i);
-        list_places(sh, p.shift);
-        write_heads<CT, DT, 1>(p, sh, blk, group * heads, min((group + 1) * heads, p.H));
+    for (int r = 0; r < runs; ++r) {
         __syncthreads();
+        if (!s_any[r]) continue;
+        int held[WR_HELD / WR_RUN];
+        {
+            const int t = first_t + r * WR_RUN + mine;
+            const int64_t slot = t < p.n ? slot_of(p, t) : -1, first = slot & ~(int64_t)(size - 1);
+            bool follows = !may_lead(p, t);
+            if (sub == 0) {
+                s_follows[mine] = follows;
+                s_blk[mine] = (int)(slot >> p.shift);
+            }
+            __syncthreads();
+            if (!follows) {
+#pragma unroll
+                for (int i = 0; i < WR_HELD / WR_RUN; ++i) held[i] = sub + WR_RUN * i < size ? mapped(p, first + sub + WR_RUN * i) : -1;
+                follows = p.map[slot] != t;  // another token has the slot too, and the map names that
+#pragma unroll
+                for (int i = 0; i < WR_HELD / WR_RUN; ++i) follows = follows || (held[i] >= 0 && first + sub + WR_RUN * i < slot);
+                // In larger blocks the nearest lower places first: a prompt's token has its neighbour there.
+                if (size > WR_HELD)
+                    for (int64_t s = slot - 1 - sub; s >= first + WR_HELD; s -= WR_RUN) {
+                        follows = follows || mapped(p, s) >= 0;
+                        if (__ballot(follows) >> (tid & 48) & 0xffff) break;
+                    }
+                if (follows) s_follows[mine] = 1;
+            }
+            __syncthreads();
+        }
+        for (int j = 0; j < WR_RUN; ++j) {
+            if (s_follows[j]) continue;
+            const int blk = s_blk[j];
+            if (tid == 0) sh.count = 0;
+            if (mine == j) {
+#pragma unroll
+                for (int i = 0; i < WR_HELD / WR_RUN; ++i)
+                    if (sub + WR_RUN * i < size) sh.tok[sub + WR_RUN * i] = held[i];
+            }
+            for (int i = tid + WR_HELD; i < size; i += WR_THR) sh.tok[i] = mapped(p, ((int64_t)blk << p.shift) + i);
+            list_places(sh, p.shift);
+            write_heads<CT, DT, 1, LARGE>(p, sh, blk, group * heads, min((group + 1) * heads, p.H));
+            __syncthreads();
+        }
     }
 }
 
@@ -445,6 +538,11 @@ __global__ __launch_bounds__(256) void read8_kernel(const Read8Params p) {
     }
 }
 
+template <int CT, bool LARGE>
+const void* write_pick(bool bf) {
+    return bf ? (const void*)&write8_kernel<CT, STARKV_BF16, LARGE> : (const void*)&write8_kernel<CT, STARKV_F16, LARGE>;
+}
+
 template <int CT>
 const void* read_pick(int dt, bool once) {
     if (dt == STARKV_F32) return (const void*)&read8_kernel<CT, STARKV_F32, false>;
@@ -498,18 +596,22 @@ int starkv_write_kv8(void* stream, const void* key, int64_t k_s0, int64_t k_s1, 
     if (n <= WR_FEW) {
         const void* fn = i8 ? bf ? (const void*)&write8_few_kernel<STARKV_I8, STARKV_BF16> : (const void*)&write8_few_kernel<STARKV_I8, STARKV_F16>
                             : bf ? (const void*)&write8_few_kernel<STARKV_E4M3, STARKV_BF16> : (const void*)&write8_few_kernel<STARKV_E4M3, STARKV_F16>;
-        int heads = (int64_t)n * num_kv_heads <= WR_WIDE ? 4 : 16;
+        int heads = 4 >> std::min(p.shift - 4, 2);
+        while (heads < 16 && (int64_t)n * ((num_kv_heads + heads - 1) / heads) > (p.shift > 4 ? WR_WIDE_LARGE : WR_WIDE)) heads *= 2;
         void* args[] = {(void*)&p, (void*)&heads};
         SKV_HIP(hipLaunchKernel(fn, dim3((n + 7) / 8 * 8, (num_kv_heads + heads - 1) / heads), dim3(WR_THR), args, 0, (hipStream_t)stream));
         return STARKV_OK;
     }
     hipLaunchKernelGGL(write8_map_kernel, dim3((n + WR_THR - 1) / WR_THR), dim3(WR_THR), 0, (hipStream_t)stream, p);
     SKV_HIP(hipGetLastError());
-    const void* fn = i8 ? bf ? (const void*)&write8_kernel<STARKV_I8, STARKV_BF16> : (const void*)&write8_kernel<STARKV_I8, STARKV_F16>
-                        : bf ? (const void*)&write8_kernel<STARKV_E4M3, STARKV_BF16> : (const void*)&write8_kernel<STARKV_E4M3, STARKV_F16>;
-    int heads = 8;  // two a wave: the search for a block's tokens is made once for them
-    void* args[] = {(void*)&p, (void*)&heads};
-    const int64_t grid = ((int64_t)n + WR_RUN - 1) / WR_RUN * ((num_kv_heads + heads - 1) / heads);
+    const void* fn = p.shift > 4 ? i8 ? write_pick<STARKV_I8, true>(bf) : write_pick<STARKV_E4M3, true>(bf)
+                                 : i8 ? write_pick<STARKV_I8, false>(bf) : write_pick<STARKV_E4M3, false>(bf);
+    // Of blocks of 16 two heads a wave: the search for a block's tokens is made once for them. Of larger ones as many rows. More
+    // tokens than a step has requests are prompts', of which a block's first token leads: a block's tokens to a workgroup then
+    // (11400 tokens of 32 heads in blocks of 64: 120 us where three workgroups of four found nothing to do, 82).
+    int heads = std::max(8 >> (p.shift - 4), 1), runs = n > 2 * WR_FEW ? std::min(1 << (p.shift - 4), WR_THR / WR_RUN) : 1;
+    void* args[] = {(void*)&p, (void*)&runs, (void*)&heads};
+    const int64_t grid = ((int64_t)n + runs * WR_RUN - 1) / (runs * WR_RUN) * ((num_kv_heads + heads - 1) / heads);
     SKV_CHECK(grid < 1ll << 31, "write_kv8: %d tokens of %d heads in one call", n, num_kv_heads);
     SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)grid), dim3(WR_THR), args, 0,
                             (hipStream_t)stream));

@@ -85,7 +85,10 @@ def test_write_few(cuda, code, dt, bs, H, n, layout, bits):
                                                        (BF16, 16, 4, [1025], "runs", "heads"), (F16, 32, 3, [1100, 1, 45, 16], "runs", "tokens"),
                                                        (BF16, 64, 2, [600, 777], "shuffled", "pairs"), (F16, 16, 1, [17, 1400], "reversed", "heads"),
                                                        (BF16, 1024, 1, [2500], "shuffled", "heads"), (BF16, 16, 40, [1061], "shuffled", "heads"),
-                                                       (F16, 128, 5, [1024], "runs", "heads"), (BF16, 16, 17, [1003, 20], "runs", "heads")])
+                                                       (F16, 128, 5, [1024], "runs", "heads"), (BF16, 16, 17, [1003, 20], "runs", "heads"),
+                                                       (BF16, 32, 9, [40, 18, 33], "runs", "heads"), (F16, 64, 3, [50, 29, 77], "runs", "heads"),
+                                                       (BF16, 32, 7, [1040, 30], "shuffled", "pairs"), (F16, 64, 5, [65, 1100], "reversed", "tokens"),
+                                                       (BF16, 256, 3, [100, 500], "runs", "heads"), (F16, 512, 2, [1200, 90], "shuffled", "heads")])
 def test_write_prompts(cuda, code, dt, bs, H, lens, order, layout):
     """Whole prompts and continued ones, in any order of tokens."""
     g = torch.Generator().manual_seed(sum(lens))
@@ -130,6 +133,27 @@ def test_write_many_steps(cuda, code, dt, bs, H, n, layout):
         write_kv8(k, v, c, slots.to(cuda))
         want.write(k, v, slots)
         assert want.same(c)
+
+
+@pytest.mark.parametrize("code", [I8, F8])
+@pytest.mark.parametrize("bs,n", [(32, 20), (64, 40), (128, 90), (1024, 700), (64, 1060), (512, 1400)])
+def test_write_into_half_full_blocks(cuda, code, bs, n):
+    """Chunks of a prompt behind others of the same blocks, larger and smaller ones, so that codes that are there are rounded
+    again by several waves; an infinite value in the last."""
+    g = torch.Generator().manual_seed(n)
+    H, nb = 6, -(-4 * n // bs) + 2
+    c = some_cache(nb, bs, H, code, cuda, g)
+    want = Plain8(c)
+    for i, scale in enumerate((1.0, 2.0 ** 5, 2.0 ** -9, 2.0 ** 7)):
+        k, v = rows(n, H, BF16, cuda, g)
+        k.mul_(scale)
+        v.mul_(2.0 ** i)
+        if i == 3:
+            v[n // 2, 4, 3] = math.inf
+        slots = bs + i * n + torch.arange(n)
+        write_kv8(k, v, c, slots.to(cuda))
+        want.write(k, v, slots)
+        assert want.same(c), i
 
 
 @pytest.mark.parametrize("n", [3, 300, 1100])
