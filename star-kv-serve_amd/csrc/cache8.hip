@@ -607,11 +607,16 @@ int starkv_write_kv8(void* stream, const void* key, int64_t k_s0, int64_t k_s1, 
     const void* fn = p.shift > 4 ? i8 ? write_pick<STARKV_I8, true>(bf) : write_pick<STARKV_E4M3, true>(bf)
                                  : i8 ? write_pick<STARKV_I8, false>(bf) : write_pick<STARKV_E4M3, false>(bf);
     // Of blocks of 16 two heads a wave: the search for a block's tokens is made once for them. Of larger ones as many rows. More
-    // tokens than a step has requests are prompts', of which a block's first token leads: a block's tokens to a workgroup then
-    // (11400 tokens of 32 heads in blocks of 64: 120 us where three workgroups of four found nothing to do, 82).
-    int heads = std::max(8 >> (p.shift - 4), 1), runs = n > 2 * WR_FEW ? std::min(1 << (p.shift - 4), WR_THR / WR_RUN) : 1;
+    // tokens than a step has requests are prompts', of which a block's first token leads: up to a block's tokens to a workgroup
+    // then, while there are 512 workgroups (in blocks of 64, where one workgroup of four finds something to do: 4 prompts of 2900
+    // tokens of 32 heads 144 -> 82 us, 17 of 255 of 8 heads 34 -> 21 with two runs, 29 with four).
+    int heads = std::max(8 >> (p.shift - 4), 1), runs = 1;
+    const int64_t groups = (num_kv_heads + heads - 1) / heads;
+    const auto grid_of = [&](int r) { return ((int64_t)n + r * WR_RUN - 1) / (r * WR_RUN) * groups; };
+    if (n > 2 * WR_FEW)
+        while (runs < 1 << (p.shift - 4) && runs < WR_THR / WR_RUN && grid_of(2 * runs) >= 512) runs *= 2;
     void* args[] = {(void*)&p, (void*)&runs, (void*)&heads};
-    const int64_t grid = ((int64_t)n + runs * WR_RUN - 1) / (runs * WR_RUN) * ((num_kv_heads + heads - 1) / heads);
+    const int64_t grid = grid_of(runs);
     SKV_CHECK(grid < 1ll << 31, "write_kv8: %d tokens of %d heads in one call", n, num_kv_heads);
     SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)grid), dim3(WR_THR), args, 0,
                             (hipStream_t)stream));

@@ -88,7 +88,9 @@ def test_write_few(cuda, code, dt, bs, H, n, layout, bits):
                                                        (F16, 128, 5, [1024], "runs", "heads"), (BF16, 16, 17, [1003, 20], "runs", "heads"),
                                                        (BF16, 32, 9, [40, 18, 33], "runs", "heads"), (F16, 64, 3, [50, 29, 77], "runs", "heads"),
                                                        (BF16, 32, 7, [1040, 30], "shuffled", "pairs"), (F16, 64, 5, [65, 1100], "reversed", "tokens"),
-                                                       (BF16, 256, 3, [100, 500], "runs", "heads"), (F16, 512, 2, [1200, 90], "shuffled", "heads")])
+                                                       (BF16, 256, 3, [100, 500], "runs", "heads"), (F16, 512, 2, [1200, 90], "shuffled", "heads"),
+                                                       (BF16, 64, 40, [2100, 30], "runs", "heads"), (F16, 64, 17, [300, 1800, 90], "shuffled", "heads"),
+                                                       (BF16, 32, 33, [2070], "reversed", "pairs"), (F16, 256, 20, [1000, 45, 1100], "runs", "tokens")])
 def test_write_prompts(cuda, code, dt, bs, H, lens, order, layout):
     """Whole prompts and continued ones, in any order of tokens."""
     g = torch.Generator().manual_seed(sum(lens))
