@@ -395,20 +395,21 @@ __global__ __launch_bounds__(WR_THR) void write8_kernel(const Write8Params p, in
     __shared__ int s_follows[WR_RUN], s_blk[WR_RUN], s_any[WR_THR / WR_RUN];
     const int groups = (p.H + heads - 1) / heads, first_t = blockIdx.x / groups * runs * WR_RUN, group = blockIdx.x % groups;
     const int tid = threadIdx.x, size = 1 << p.shift, mine = tid / WR_RUN, sub = tid % WR_RUN;
-    if (LARGE && runs > 1) {  // of several runs most have none that may lead
+    if (!LARGE) runs = 1;
+    if (runs > 1) {  // of several runs most have none that may lead
         const uint64_t may = __ballot(tid < runs * WR_RUN && may_lead(p, first_t + tid));
         if (sub == 0) s_any[mine] = (may >> (tid & 48) & 0xffff) != 0;
-    } else if (tid == 0) {
-        s_any[0] = 1;
     }
     for (int r = 0; r < runs; ++r) {
-        __syncthreads();
-        if (!s_any[r]) continue;
+        if (runs > 1) {
+            __syncthreads();
+            if (!s_any[r]) continue;
+        }
         int held[WR_HELD / WR_RUN];
         {
             const int t = first_t + r * WR_RUN + mine;
             const int64_t slot = t < p.n ? slot_of(p, t) : -1, first = slot & ~(int64_t)(size - 1);
-            bool follows = !may_lead(p, t);
+            bool follows = LARGE ? !may_lead(p, t) : slot < 0;  // of 16 places the look costs less than the question
             if (sub == 0) {
                 s_follows[mine] = follows;
                 s_blk[mine] = (int)(slot >> p.shift);
