@@ -239,19 +239,53 @@ void prefill(const at::Tensor& query, const at::Tensor& key, const at::Tensor& v
           "prefill");
 }
 
-// The same through a window.
-void prefill_window(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, const at::Tensor& cu_seqlens,
-                    const at::Tensor& blocks, int64_t window, int64_t sinks, double scale, const at::Tensor& out) {
+// The same through a window. Without cu_seqlens and blocks they are made of query_lens here, and values of bf16 become fp16
+// here (for a prompt of a few tokens, which waits for the host: fp16 18.8 -> 14.3 us, bf16 25 -> 17).
+void prefill_window(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, const std::optional<at::Tensor>& cu_seqlens,
+                    const std::optional<at::Tensor>& blocks, at::IntArrayRef query_lens, int64_t window, int64_t sinks, double scale,
+                    const at::Tensor& out) {
     const c10::DeviceGuard guard(query.device());
-    TORCH_CHECK(blocks.dim() == 2 && blocks.size(1) == 2, "starkv.prefill_window: blocks must be [num_blocks, 2]");
-    TORCH_CHECK(value.scalar_type() == at::kHalf && key.dim() == 3 && key.sizes() == value.sizes() && key.stride(2) == 1 &&
-                    value.stride(2) == 1 && query.dim() == 3 && query.stride(2) == 1 && out.stride(2) == 1,
-                "starkv.prefill_window: keys and fp16 values [T, heads, 128]");
+    TORCH_CHECK(key.dim() == 3 && key.sizes() == value.sizes() && key.size(2) == 128 && key.stride(2) == 1 && value.stride(2) == 1 &&
+                    query.dim() == 3 && query.size(0) == key.size(0) && query.stride(2) == 1 && out.sizes() == query.sizes() &&
+                    out.stride(2) == 1 && (value.scalar_type() == at::kHalf || (value.scalar_type() == at::kBFloat16 && key.scalar_type() == at::kBFloat16)),
+                "starkv.prefill_window: queries [T, heads, 128], keys and fp16 values (or bf16 ones of both) [T, heads, 128]");
     for (const int64_t v : {window, sinks}) TORCH_CHECK(v >= 0 && v <= INT32_MAX, "starkv.prefill_window: window ", window, ", sinks ", sinks);
+    TORCH_CHECK(cu_seqlens.has_value() == blocks.has_value(), "starkv.prefill_window: cu_seqlens and blocks, or neither");
+    at::Tensor meta;
+    const int32_t *cu, *rows;
+    int n;
+    if (blocks) {
+        TORCH_CHECK(blocks->dim() == 2 && blocks->size(1) == 2, "starkv.prefill_window: blocks must be [num_blocks, 2]");
+        cu = i32(*cu_seqlens, "cu_seqlens");
+        rows = i32(*blocks, "blocks");
+        n = (int)blocks->size(0);
+    } else {
+        std::vector<int32_t> first(1, 0);
+        int64_t end = 0;
+        for (const int64_t L : query_lens) {
+            TORCH_CHECK(L >= 0 && (end += L) <= query.size(0) && end <= INT32_MAX, "starkv.prefill_window: prompts of more tokens than there are");
+            first.push_back((int32_t)end);
+        }
+        const int prompts = (int)query_lens.size();
+        n = starkv_prefill_block_list(first.data(), prompts, nullptr, 0);
+        TORCH_CHECK(n >= 0, "starkv.prefill_window: prompt lengths");
+        const at::Tensor host = at::empty({prompts + 1 + 2 * (int64_t)n}, at::kInt);
+        std::copy(first.begin(), first.end(), host.data_ptr<int32_t>());
+        starkv_prefill_block_list(first.data(), prompts, host.data_ptr<int32_t>() + prompts + 1, n);
+        meta = host.to(query.device(), at::kInt, /*non_blocking=*/true);
+        cu = meta.data_ptr<int32_t>();
+        rows = cu + prompts + 1;
+    }
+    at::Tensor v = value;
+    if (value.scalar_type() == at::kBFloat16) {
+        v = at::empty(value.sizes(), value.options().dtype(at::kHalf));
+        check(starkv_prefill_to_half(stream_of(value), nullptr, 0, 0, nullptr, value.data_ptr(), value.stride(0), value.stride(1), v.data_ptr(),
+                                     dtype_code(value), (int)value.size(0), (int)value.size(1)),
+              "prefill_to_half");
+    }
     check(starkv_prefill_window(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), dtype_code(query),
-                                key.data_ptr(), key.stride(0), key.stride(1), dtype_code(key), value.data_ptr(),
-                                value.stride(0), value.stride(1), i32(cu_seqlens, "cu_seqlens"), i32(blocks, "blocks"),
-                                (int)blocks.size(0), (int)query.size(1), (int)key.size(1), (int)query.size(2), (int)window, (int)sinks,
+                                key.data_ptr(), key.stride(0), key.stride(1), dtype_code(key), v.data_ptr(), v.stride(0), v.stride(1), cu, rows,
+                                n, (int)query.size(1), (int)key.size(1), (int)query.size(2), (int)window, (int)sinks,
                                 (float)scale, out.data_ptr(), out.stride(0), out.stride(1), dtype_code(out)),
           "prefill_window");
 }
@@ -761,8 +795,8 @@ TORCH_LIBRARY(starkv, m) {
           "int keep, int sink, int recent, Tensor(c!) new_lens, Tensor(d!) new_weights) -> ()");
     m.def("window_decode(Tensor query, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, "
           "int max_seq_len, int window, int sinks, float scale) -> Tensor");
-    m.def("prefill_window(Tensor query, Tensor key, Tensor value, Tensor cu_seqlens, Tensor blocks, int window, "
-          "int sinks, float scale, Tensor(a!) out) -> ()");
+    m.def("prefill_window(Tensor query, Tensor key, Tensor value, Tensor? cu_seqlens, Tensor? blocks, int[] query_lens, "
+          "int window, int sinks, float scale, Tensor(a!) out) -> ()");
     m.def("write_kv8(Tensor key, Tensor value, Tensor(a!) k_codes, Tensor(b!) v_codes, Tensor(c!) exponents, "
           "Tensor slots) -> ()");
     m.def("read_kv8(Tensor k_codes, Tensor v_codes, Tensor exponents, Tensor slots, ScalarType dtype) -> (Tensor, Tensor)");

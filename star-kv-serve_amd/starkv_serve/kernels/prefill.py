@@ -89,17 +89,12 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_l
     if T == 0:
         return out
     _hip.require_cuda(q, k, v, out)
-    # Through a window keys of bf16, and keys and values of fp16, are read as they are; values are fp16, as the weights that
-    # multiply them.
+    # Through a window keys of bf16, and keys and values of fp16, are read as they are; values of bf16 become fp16, as the
+    # weights that multiply them.
     as_is = (window is not None and q.dtype == k.dtype == v.dtype and k.stride(-1) == v.stride(-1) == 1
-             and k.stride(0) % 8 == k.stride(1) % 8 == k.data_ptr() % 16 == 0 and k.stride(0) < 1 << 23)
-    if as_is and k.dtype == torch.float16 and k.stride() == v.stride() and v.data_ptr() % 16 == 0:
-        pass
-    elif as_is and k.dtype == torch.bfloat16:
-        v16 = torch.empty(v.shape, dtype=torch.float16, device=v.device)
-        _hip.ops().prefill_to_half(None, v, None, v16)
-        v = v16
-    else:
+             and k.stride(0) % 8 == k.stride(1) % 8 == k.data_ptr() % 16 == 0 and k.stride(0) < 1 << 23
+             and (k.dtype == torch.bfloat16 or (k.dtype == torch.float16 and k.stride() == v.stride() and v.data_ptr() % 16 == 0)))
+    if not as_is:
         if k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.stride(-1) == v.stride(-1) == 1:
             kv = torch.empty((2, *k.shape), dtype=torch.float16, device=k.device)
             _hip.ops().prefill_to_half(k, v, kv[0], kv[1])
@@ -107,9 +102,12 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_l
         k, v = k.to(torch.float16), v.to(torch.float16)
         k, v = k.contiguous(), v.contiguous()
     q = q if q.stride(-1) == 1 else q.contiguous()
+    if window is not None:
+        if tables is None and min(query_lens) < 0:
+            raise ValueError(f"negative prompt length {min(query_lens)}")
+        cu_d, blk_d = (None, None) if tables is None else tables
+        _hip.ops().prefill_window(q, k, v, cu_d, blk_d, list(map(int, query_lens)) if tables is None else [], *sizes(window), float(scale), out)
+        return out
     cu_d, blk_d = prompt_tables(query_lens, q.device) if tables is None else tables
-    if window is None:
-        _hip.ops().prefill(q, k, v, cu_d, blk_d, float(scale), out)
-    else:
-        _hip.ops().prefill_window(q, k, v, cu_d, blk_d, *sizes(window), float(scale), out)
+    _hip.ops().prefill(q, k, v, cu_d, blk_d, float(scale), out)
     return out
