@@ -249,8 +249,12 @@ def output_for(out, shape, dtype, device) -> torch.Tensor:
 
 def require_cuda(*ts: torch.Tensor) -> None:
     at = ts[0].get_device()  # -1 on the CPU
-    if at >= 0 and all(t.get_device() == at and t.is_cuda for t in ts):
-        return
+    if at >= 0 and ts[0].is_cuda:  # plain loops: every call of a step comes through here
+        for t in ts:
+            if t.get_device() != at or not t.is_cuda:
+                break
+        else:
+            return
     dev = ts[0].device
     for t in ts:
         if t.device.type != "cuda":
@@ -263,7 +267,9 @@ def require_cuda(*ts: torch.Tensor) -> None:
 def refuse_grad(what: str, *ts: torch.Tensor) -> None:
     """Serving operators without a backward, a forward-mode derivative or a batching rule: a result that looks
     differentiable (or mapped) and is not would be silent."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
-        raise NotImplementedError(f"{what} has no gradient; call it under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t.requires_grad:
+                raise NotImplementedError(f"{what} has no gradient; call it under torch.no_grad()")
     if forward_ad._current_level >= 0 or torch._C._functorch.peek_interpreter_stack() is not None:
         raise NotImplementedError(f"{what} has no forward-mode derivative and does not run under torch.func transforms")
