@@ -38,7 +38,6 @@
 // A block whose exponent says NaN makes every row NaN that sees one of its tokens. A row that sees no token is zero; one
 // whose scores are all -inf is 0 / 0, NaN.
 #include <algorithm>
-#include <atomic>
 
 #include "cache8.hpp"
 #include "window_pages.hpp"
@@ -567,18 +566,6 @@ __global__ __launch_bounds__(64 * WAVES) void merge8_kernel(const Decode8Params 
     }
     store_f(p.out, to, QDT, weigh_out(a.x, lt, M, R));
     store_f(p.out, to + 1, QDT, weigh_out(a.y, lt, M, R));
-}
-
-int device_cus() {
-    static std::atomic<int> known[64];  // by device: the count does not change, and asking costs a call 0.3 us
-    int dev = 0, c = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-    c = known[dev].load(std::memory_order_relaxed);
-    if (c == 0) {
-        if (hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || c <= 0) c = 256;
-        known[dev].store(c, std::memory_order_relaxed);
-    }
-    return c;
 }
 
 int decode8_base(int num_kv_heads) { return std::max(1, 2 * device_cus() / num_kv_heads); }

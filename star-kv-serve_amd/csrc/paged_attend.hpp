@@ -406,11 +406,7 @@ __device__ __forceinline__ void attend_merge_head(const AttendParams& p, int b, 
 // Splits per unit (request and KV head) of at most `pages` pages: workgroups for `per_cu` a CU, `least` pages a
 // split at least.
 inline int attend_splits(int64_t units, int pages, int per_cu, int least) {
-    int dev = 0, cus = 256, c = 0;
-    if (hipGetDevice(&dev) == hipSuccess &&
-        hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && c > 0)
-        cus = c;
-    const int64_t s = std::min<int64_t>((per_cu * (int64_t)cus + units - 1) / units, (pages + least - 1) / least);
+    const int64_t s = std::min<int64_t>((per_cu * (int64_t)device_cus() + units - 1) / units, (pages + least - 1) / least);
     return (int)std::max<int64_t>(1, std::min<int64_t>(s, AT_MAX_SPLITS));
 }
 

@@ -11,6 +11,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 namespace starkv {
 
@@ -44,6 +45,19 @@ inline int seen_pages_most(int span, int window, int sinks) {
     const int all = (int)(((int64_t)span + 15) / 16);
     if (window <= 0) return all;
     return (int)std::min<int64_t>(all, ((int64_t)std::min(sinks, span) + 15) / 16 + ((int64_t)window + 14) / 16 + 1);
+}
+
+// The current device's compute units (256 where it does not say).
+inline int device_cus() {
+    static std::atomic<int> known[64];  // by device: the count does not change, and asking costs a call 0.3 us
+    int dev = 0, c = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    c = known[dev].load(std::memory_order_relaxed);
+    if (c == 0) {
+        if (hipDeviceGetAttribute(&c, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || c <= 0) c = 256;
+        known[dev].store(c, std::memory_order_relaxed);
+    }
+    return c;
 }
 
 }  // namespace starkv
