@@ -260,6 +260,10 @@ void prefill_window(const at::Tensor& query, const at::Tensor& key, const at::Te
         rows = i32(*blocks, "blocks");
         n = (int)blocks->size(0);
     } else {
+        // A graph would read the prompts' tables from this call's host memory again at each replay.
+        hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+        TORCH_CHECK(hipStreamIsCapturing((hipStream_t)stream_of(query), &capturing) == hipSuccess && capturing == hipStreamCaptureStatusNone,
+                    "starkv.prefill_window: in a capture the prompts' tables are those of prompt_tables(), made before it: tables=");
         std::vector<int32_t> first(1, 0);
         int64_t end = 0;
         for (const int64_t L : query_lens) {

@@ -41,7 +41,10 @@ def block_list(query_lens: List[int]) -> List[int]:
 
 
 def prompt_tables(query_lens: List[int], device) -> tuple:
-    """(cu_seqlens [P + 1], blocks [num_blocks, 2]) int32 on `device`, in one upload."""
+    """(cu_seqlens [P + 1], blocks [num_blocks, 2]) int32 on `device`, in one upload. Made before a capture: a graph would
+    read them from this call's host memory again at each replay."""
+    if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("in a capture the prompts' tables are those of prompt_tables(), made before it: tables=")
     buf, n = _tables(query_lens)
     P = len(query_lens) + 1
     meta = torch.frombuffer(buf, dtype=torch.int32).to(device, non_blocking=True)
@@ -77,7 +80,7 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_l
 
     q [T, H_q, 128] (bf16, fp16 or fp32); k, v [T, H_kv, 128] (converted to fp16 once
     here when they are not); query_lens: the prompts' token counts (host ints, summing to
-    T); tables: their ``prompt_tables``, when the caller has them. Returns ``out``
+    T); tables: their ``prompt_tables``, when the caller has them (in a capture it must). Returns ``out``
     [T, H_q, 128] (new, in q's dtype, when not given)."""
     T, Hq, D = q.shape
     assert D == 128 and k.shape == v.shape and k.shape[0] == T and k.shape[2] == D and Hq % k.shape[1] == 0
