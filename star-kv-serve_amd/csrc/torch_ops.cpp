@@ -439,9 +439,9 @@ void check_table(const at::Tensor& block_table, const at::Tensor& seq_lens, int6
 }
 
 void check_query(const at::Tensor& query, const at::Tensor& like, int64_t heads, const char* what) {
-    TORCH_CHECK(query.dim() == 3 && query.size(2) == 128 && query.stride(2) == 1 && query.size(1) % heads == 0 &&
+    TORCH_CHECK(heads >= 1 && query.dim() == 3 && query.size(2) == 128 && query.stride(2) == 1 && query.size(1) % heads == 0 &&
                     query.scalar_type() == like.scalar_type(),
-                "starkv.", what, ": query [n, heads, 128] of the cache's dtype");
+                "starkv.", what, ": query [n, heads, 128] of the cache's dtype, over ", heads, " KV heads");
 }
 
 int as_int(int64_t v, const char* name) {
