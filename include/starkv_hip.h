@@ -405,7 +405,7 @@ int starkv_prefill_attention(void *stream, const void *query, int64_t q_s0, int6
 /*
  * Keys and values [T, num_kv_heads, 128] of bf16 or fp32 (one dtype, each its own element strides,
  * last dimension contiguous) as the contiguous fp16 tensors starkv_prefill_attention takes, in one
- * launch. key and key_out may be null: values alone.
+ * launch.
  */
 int starkv_prefill_to_half(void *stream, const void *key, int64_t k_s0, int64_t k_s1, void *key_out,
                            const void *value, int64_t v_s0, int64_t v_s1, void *value_out, int dtype, int num_tokens,
@@ -565,6 +565,11 @@ int starkv_evict(void *stream, void *k_cache, void *v_cache, int64_t c_s0, int64
  * starkv_prefill_window: starkv_prefill_attention through a window. Keys are fp16, with the strides of the values, or, with
  * bf16 queries, bf16 of any strides; values are fp16.
  *
+ * starkv_prefill_window_bf16: the same for queries, keys and values [num_tokens, num_kv_heads, 128] of bf16, each of any strides
+ * (the values' rows at any element), over bf16's whole range: values become fp16 in the workspace, and where fp16 does not hold
+ * them (past its range, or all values of a workgroup's tokens below 2^-10) are multiplied as bf16. A value below 2^-17 among
+ * larger ones is off by up to 2^-25.
+ *
  * An 8-bit cache: k_codes and v_codes [num_blocks, block_size, num_kv_heads, 128] of one byte (code_type; byte strides
  * c_s0, c_s1, c_s2 shared by both, multiples of 16, rows 16-byte aligned; block_size 16 * 2^s up to 1024), and exponents
  * [num_blocks, num_kv_heads, 2] int8 (strides x_s0, x_s1; last dimension contiguous): a key is code * 2^exponents[..][0], a
@@ -595,6 +600,12 @@ int starkv_prefill_window(void *stream, const void *query, int64_t q_s0, int64_t
                           int64_t k_s0, int64_t k_s1, int k_dtype, const void *value, int64_t v_s0, int64_t v_s1,
                           const int32_t *cu_seqlens, const int32_t *blocks, int num_blocks, int num_heads, int num_kv_heads, int head_size,
                           int window, int sinks, float scale, void *out, int64_t o_s0, int64_t o_s1, int out_dtype);
+size_t starkv_prefill_window_bf16_workspace_bytes(int num_tokens, int num_kv_heads);
+int starkv_prefill_window_bf16(void *stream, const void *query, int64_t q_s0, int64_t q_s1, const void *key, int64_t k_s0,
+                               int64_t k_s1, const void *value, int64_t v_s0, int64_t v_s1, const int32_t *cu_seqlens,
+                               const int32_t *blocks, int num_blocks, int num_tokens, int num_heads, int num_kv_heads, int head_size,
+                               int window, int sinks, float scale, void *out, int64_t o_s0, int64_t o_s1, int out_dtype,
+                               void *workspace, size_t workspace_bytes);
 size_t starkv_write_kv8_workspace_bytes(int n, int64_t num_blocks, int block_size);
 int starkv_write_kv8(void *stream, const void *key, int64_t k_s0, int64_t k_s1, const void *value, int64_t v_s0,
                      int64_t v_s1, int dtype, void *k_codes, void *v_codes, int64_t c_s0, int64_t c_s1, int64_t c_s2,

@@ -242,7 +242,7 @@ using namespace starkv;
 
 extern "C" {
 
-int starkv_abi_version(void) { return 9; }
+int starkv_abi_version(void) { return 10; }
 
 const char* starkv_last_error(void) { return g_err; }
 

@@ -40,7 +40,9 @@
 // tiles across an edge are masked (its later waves mask up to two whole ones). The scale goes onto
 // the fp32 scores there (one fused multiply-add in front of the exponential in place of a subtraction) and not into q, whose
 // fp16 values are then those of bf16 and fp16 queries themselves; bf16 queries and keys are multiplied as they are, which
-// saves half of the conversion in front. Values past fp16's range become infinite in that conversion.
+// saves half of the conversion in front. bf16 values' fp16 rows (starkv_prefill_window_bf16) are what tiles have where fp16 holds
+// them: 8 bits are exact in it from 2^-17 to 65504, and a product of fp16 weights has 11 bits of those, one of bf16 weights 8. The
+// values themselves are multiplied in a second pass where it does not.
 //
 // Two prompts of 9300 tokens together, 32 heads, window 1024: 211 us, 153 GFLOP of pairs that are seen (725 TFLOP/s; 870 with the masked
 // halves of edge tiles), the conversion in front 27; one of 2047 tokens with window 512: 34 and 4. The matrix unit is busy 42 %
@@ -65,6 +67,7 @@ constexpr int PF_TILE = PF_KT * 256;      // bytes of K (or V) per tile: 64 rows
 constexpr int PF_LDS = 4 * PF_TILE;       // two K and two V tiles: the next lands while one is used
 constexpr int PF_CPW = 16 / PF_WAVES;     // 1 KB copies per wave per K (or V) tile
 constexpr float PF_LAZY = 8.f;            // log2 headroom of the reference max
+constexpr int PF_FINE = 127 - 10;         // exponent field of 2^-10: bf16 values that are all less are multiplied as bf16
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
@@ -78,6 +81,9 @@ struct PrefillParams {
     float sc;                                                 // scale * log2(e)
     void* out; int64_t o_s0, o_s1; int out_dt;                // elements
     int window, sinks;
+    // RAW: the bf16 values as they are, and the exponent fields of their rows' largest, [Hkv][tops_s]. v has their fp16 rows.
+    const uint16_t* raw; int64_t r_s0, r_s1; int raw_wide;    // elements; rows 16-byte aligned
+    const uint8_t* tops; int64_t tops_s;
 };
 
 // A row's granules (16 bytes, 16 a row) lie XOR-swizzled by its low 4 bits, their two halves
@@ -136,16 +142,27 @@ __device__ __forceinline__ uint2 pf_tr(uint32_t addr) {
     return __builtin_bit_cast(uint2, r);
 }
 
-// Of a pair of fp16 values: the finite ones (mode 0, others 0), or 1 for each that is +inf (1), -inf (2) or NaN (3).
+// Of a pair of fp16 or bf16 values: the finite ones (mode 0, others 0), or 1 for each that is +inf (1), -inf (2) or NaN (3).
+template <int DT>
 __device__ __forceinline__ uint32_t pf_class(uint32_t w, int mode) {
+    constexpr uint32_t inf = DT == STARKV_BF16 ? 0x7f80u : 0x7c00u, one = DT == STARKV_BF16 ? 0x3f80u : 0x3c00u;
     uint32_t res = 0;
 #pragma unroll
     for (int x = 0; x < 32; x += 16) {
         const uint32_t v = w >> x & 0xffffu, size = v & 0x7fffu;
-        const bool is = mode == 1 ? v == 0x7c00u : mode == 2 ? v == 0xfc00u : size > 0x7c00u;
-        res |= (mode == 0 ? size < 0x7c00u ? v : 0u : is ? 0x3c00u : 0u) << x;
+        const bool is = mode == 1 ? v == inf : mode == 2 ? v == (inf | 0x8000u) : size > inf;
+        res |= (mode == 0 ? size < inf ? v : 0u : is ? one : 0u) << x;
     }
     return res;
+}
+
+// 8 bf16 values from element i on of rows that need not be aligned.
+__device__ __forceinline__ uint4 pf_load_raw(const PrefillParams& p, int64_t i) {
+    if (p.raw_wide) return *(const uint4*)(p.raw + i);
+    uint32_t w[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] = (uint32_t)p.raw[i + 2 * k] | (uint32_t)p.raw[i + 2 * k + 1] << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // The work of one workgroup: a (prompt, query block) entry of the list and a query head. Where
@@ -165,8 +182,9 @@ __device__ __forceinline__ void pf_work(const PrefillParams& p, int& entry, int&
     }
 }
 
-// KDT: the type of the keys, fp16 or (through a window, with queries of the same) bf16.
-template <int QDT, int ODT, bool WINDOW, int KDT = STARKV_F16>
+// KDT: the type of the keys, fp16 or (through a window, with queries of the same) bf16. RAW: of the values too, whose fp16 rows
+// the tiles have.
+template <int QDT, int ODT, bool WINDOW, int KDT = STARKV_F16, bool RAW = false>
 __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) void prefill_kernel(const PrefillParams p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t s_kv[];  // K tiles 0, 1, V tiles 0, 1
     const int tid = threadIdx.x, lane = tid & 63, wave = rfl(tid >> 6);
@@ -217,6 +235,22 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
         for (int c = 0; c < PF_CPW; ++c) lds_copy16(rs, dst + (uint32_t)(PF_WAVES * c + wave) * 1024u, val ? voff[c] : coff[c]);
     };
     issue(false, 0, base);
+
+    // The values of the workgroup's tokens: whether one reaches 2^-10, and whether there are others than 0 (a thread's part). A
+    // byte a token, 8 of them a load, which nothing waits for until the tiles are done.
+    uint64_t large = 0, some = 0;
+    if constexpr (RAW) {
+        const int head = s + min(first * PF_KT, kend), from = s + second * PF_KT, end = s + kend;  // [s, head) and [from, end)
+        const int words = head > s ? ((head + 7) >> 3) - (s >> 3) : 0, all = words + ((end + 7) >> 3) - (from >> 3);
+        for (int i = tid; i < all; i += PF_THR) {
+            const int lo = i < words ? s : from, hi = i < words ? head : end, at = i < words ? (s >> 3) + i : (from >> 3) + i - words;
+            uint64_t w = *(const uint64_t*)(p.tops + (int64_t)hk * p.tops_s + 8 * at);
+            if (8 * at < lo) w &= ~0ull << 8 * (lo - 8 * at);
+            if (8 * at + 8 > hi) w &= ~0ull >> 8 * (8 * at + 8 - hi);
+            some |= w;
+            large |= ((w & 0x7f7f7f7f7f7f7f7full) + 0x0101010101010101ull * (128 - PF_FINE)) | w;
+        }
+    }
 
     // Q as the B operand of S^T = K Q^T: query n, dimensions 16 ks + 8 h .. + 7.
     half8_t qb[8];
@@ -383,7 +417,13 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
     // An infinite value or NaN of a key that its tile's rows do not all see gives NaN as 0 times it (through a window; a causal
     // tile has the same for its later keys). Where sums are not finite though their weights are, the workgroup goes over
     // its tiles again with the reference that it has: which results see a NaN, a -inf and a +inf, then the finite values.
+    // bf16 values are those of the caller there, and their weights p / l in two bf16 values, 16 bits: finite values past fp16's
+    // range have become infinite in its rows, and where all values of the workgroup's tokens are below 2^-10 (those below 2^-17
+    // lose bits in fp16, up to 2^-25) it goes over them too, for the finite values alone. Others' results are so off by no more
+    // than 2^-15 of the largest value among its tokens. One prompt of 2047 tokens, 32 heads over 8, window 512: 44 us, 261 with values
+    // of 2^-20, 600 with values of 2^20, 454 where one value is past fp16's range.
     uint64_t nan = 0, low = 0, high = 0;  // by the results' order in o
+    float inv = 1.f / l;
     if constexpr (WINDOW) {
         float odd = 0.f;
 #pragma unroll
@@ -393,40 +433,64 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
         const bool mine = __builtin_amdgcn_ballot_w64(odd != odd && l == l && qi < L && nq > 0) != 0;
         uint32_t* flag = (uint32_t*)s_kv;  // a word a wave
         __syncthreads();
-        if (lane == 0) flag[wave] = mine;
+        uint32_t size = 0;
+        if (RAW) size = __builtin_amdgcn_ballot_w64((large & 0x8080808080808080ull) != 0) != 0 ? 2 : __builtin_amdgcn_ballot_w64(some != 0) != 0 ? 4 : 0;
+        if (lane == 0) flag[wave] = (uint32_t)mine | size;
         __syncthreads();
         const uint4 flags = *(const uint4*)flag;
-        if (__builtin_expect((flags.x | flags.y | flags.z | flags.w) != 0, 0)) {
+        const uint32_t any = rfl(flags.x | flags.y | flags.z | flags.w);
+        if (__builtin_expect((any & 1) != 0 || (any & 6) == 4, 0)) {
             const float mr = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
-            for (int mode = 3; mode >= 0; --mode) {
+            for (int mode = any & 1 ? 3 : 0; mode >= (RAW ? -1 : 0); --mode) {
+                if (mode >= 0)  // -1 adds what the weights' first values left
 #pragma unroll
-                for (int md = 0; md < 4; ++md) o[md] = (f32x16_t){};
+                    for (int md = 0; md < 4; ++md) o[md] = (f32x16_t){};
+                const int kind = max(mode, 0);
 #pragma unroll 1
                 for (int t = 0; t < ntile; ++t) {
                     __syncthreads();  // every wave is done with the tile before, and with the flags
                     issue(false, t, base);
-                    issue(true, t, base + 2 * PF_TILE);
+                    if constexpr (RAW) {
+                        const int r0 = tile_of(t) * PF_KT;
+#pragma unroll
+                        for (int c = 0; c < PF_CPW; ++c) {
+                            const int row = PF_KT / PF_CPW * c + (tid >> 4), g = tid & 15;
+                            const uint4 w = r0 + row < L ? pf_load_raw(p, (s + r0 + row) * p.r_s0 + hk * p.r_s1 + 8 * g) : make_uint4(0, 0, 0, 0);
+                            *(uint4*)(s_kv + 2 * PF_TILE + pf_addr(row, g)) = w;
+                        }
+                    } else {
+                        issue(true, t, base + 2 * PF_TILE);
+                    }
                     SKV_WAIT_VM_LGKM0(0);
                     __syncthreads();
                     if (t > last) continue;
                     scores(std::integral_constant<int, 0>{}, sa);
                     hide(tile_of(t) * PF_KT, sa);
-                    half8_t pb[4];
+                    typedef std::conditional_t<RAW, bf16x8_t, half8_t> weights_t;
+                    typedef std::conditional_t<RAW, __bf16, _Float16> weight_t;
+                    weights_t pb[4];
 #pragma unroll
                     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
                         for (int r = 0; r < 16; ++r) {
                             const float e = __builtin_amdgcn_exp2f(fmaf(sa[mb][r], ss, -mr));
-                            pb[2 * mb + (r >> 3)][r & 7] = (_Float16)(mode == 0 ? e : e > 0.f ? 1.f : 0.f);
+                            float w = mode <= 0 ? RAW ? e * inv : e : e > 0.f ? 1.f : 0.f;
+                            if (RAW && mode < 0) w -= (float)(weight_t)w;
+                            pb[2 * mb + (r >> 3)][r & 7] = (weight_t)w;
                         }
 #pragma unroll
                     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
                         for (int md = 0; md < 4; ++md) {
+                            constexpr int VDT = RAW ? STARKV_BF16 : STARKV_F16;
                             const uint2 a0 = pf_tr(va[md][0] + 4096 * ks), a1 = pf_tr(va[md][1] + 4096 * ks);
-                            const uint4 av = make_uint4(pf_class(a0.x, mode), pf_class(a0.y, mode), pf_class(a1.x, mode), pf_class(a1.y, mode));
-                            o[md] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, av), pb[ks], o[md], 0, 0, 0);
+                            const weights_t av = __builtin_bit_cast(weights_t, make_uint4(pf_class<VDT>(a0.x, kind), pf_class<VDT>(a0.y, kind),
+                                                                                          pf_class<VDT>(a1.x, kind), pf_class<VDT>(a1.y, kind)));
+                            if constexpr (RAW)
+                                o[md] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(av, pb[ks], o[md], 0, 0, 0);
+                            else
+                                o[md] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, pb[ks], o[md], 0, 0, 0);
                         }
                 }
                 uint64_t seen = 0;
@@ -439,10 +503,10 @@ __global__ __launch_bounds__(PF_THR) __attribute__((amdgpu_waves_per_eu(2))) voi
                 if (mode == 1) high = seen;
             }
             nan |= low & high;
+            if (RAW) inv = 1.f;
         }
     }
     if (qi < L && nq > 0) {
-        const float inv = 1.f / l;
         if constexpr (WINDOW) {
             if (__builtin_expect((nan | low | high) != 0, 0)) {
 #pragma unroll
@@ -496,7 +560,7 @@ struct ToHalfParams {
 
 template <int DT>
 __global__ __launch_bounds__(256) void to_half_kernel(const ToHalfParams p) {
-    const int z = 1 - blockIdx.y;
+    const int z = blockIdx.y;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.pieces; i += (int64_t)gridDim.x * 256) {
         const int64_t row = i >> 4, t = row / p.H;
         const int h = (int)(row - t * p.H);
@@ -515,6 +579,31 @@ __global__ __launch_bounds__(256) void to_half_kernel(const ToHalfParams p) {
     }
 }
 
+// Values of bf16 alone, and the exponent field of each row's largest, [H][tops_s] (a NaN says nothing). 16 lanes have a row.
+__global__ __launch_bounds__(256) void values_to_half_kernel(const ToHalfParams p, uint8_t* tops, int64_t tops_s) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.pieces; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i >> 4, t = row / p.H;
+        const int h = (int)(row - t * p.H);
+        const int64_t at = t * p.s0[1] + h * p.s1[1] + 8 * (i & 15);
+        float x[8], top = 0.f;
+        if (p.wide) {
+            load8_f(p.src[1], at, STARKV_BF16, x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = load_f(p.src[1], at + e, STARKV_BF16);
+        }
+        half8_t o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            o[e] = (_Float16)x[e];
+            top = fmaxf(top, fabsf(x[e]));
+        }
+        *(half8_t*)(p.dst[1] + 8 * i) = o;
+        top = row16_max(top);
+        if ((i & 15) == 0) tops[h * tops_s + t] = (uint8_t)(__float_as_uint(top) >> 23);
+    }
+}
+
 template <int QDT, bool WINDOW>
 const void* pf_pick(int odt) {
     if (odt == STARKV_F32) return (const void*)&prefill_kernel<QDT, STARKV_F32, WINDOW>;
@@ -522,10 +611,11 @@ const void* pf_pick(int odt) {
     return (const void*)&prefill_kernel<QDT, STARKV_BF16, WINDOW>;
 }
 
+template <bool RAW>
 const void* pf_pick_bf16(int odt) {
-    if (odt == STARKV_F32) return (const void*)&prefill_kernel<STARKV_BF16, STARKV_F32, true, STARKV_BF16>;
-    if (odt == STARKV_F16) return (const void*)&prefill_kernel<STARKV_BF16, STARKV_F16, true, STARKV_BF16>;
-    return (const void*)&prefill_kernel<STARKV_BF16, STARKV_BF16, true, STARKV_BF16>;
+    if (odt == STARKV_F32) return (const void*)&prefill_kernel<STARKV_BF16, STARKV_F32, true, STARKV_BF16, RAW>;
+    if (odt == STARKV_F16) return (const void*)&prefill_kernel<STARKV_BF16, STARKV_F16, true, STARKV_BF16, RAW>;
+    return (const void*)&prefill_kernel<STARKV_BF16, STARKV_BF16, true, STARKV_BF16, RAW>;
 }
 
 template <bool WINDOW>
@@ -565,12 +655,23 @@ int starkv_prefill_block_list(const int32_t* cu_seqlens, int num_prompts, int32_
     return (int)all.size();
 }
 
+// A head's row of the largest values' exponent fields: a byte a token, in words of 8.
+static int64_t pf_tops(int64_t tokens) { return (tokens + 7) / 8 * 8; }
+
+// bf16 values whose fp16 rows are made at prefill_call's `value`, and their rows' largest at tops.
+struct RawValues {
+    const void* rows = nullptr;
+    int64_t s0 = 0, s1 = 0;
+    uint8_t* tops = nullptr;
+    int tokens = 0;
+};
+
 // window 0: every key up to the query.
 static int prefill_call(void* stream, const void* query, int64_t q_s0, int64_t q_s1, int q_dtype,
                         const void* key, int64_t k_s0, int64_t k_s1, int k_dtype, const void* value, int64_t v_s0,
                         int64_t v_s1, const int32_t* cu_seqlens, const int32_t* blocks, int num_blocks, int num_heads,
                         int num_kv_heads, int head_size, int window, int sinks, float scale, void* out, int64_t o_s0, int64_t o_s1,
-                        int out_dtype) {
+                        int out_dtype, const RawValues& values = {}) {
     clear_error();
     SKV_CHECK(num_blocks >= 0, "prefill: num_blocks=%d", num_blocks);
     if (num_blocks == 0) return STARKV_OK;
@@ -599,7 +700,10 @@ static int prefill_call(void* stream, const void* query, int64_t q_s0, int64_t q
     p.sc = scale * 1.4426950408889634f;
     p.out = out; p.o_s0 = o_s0; p.o_s1 = o_s1; p.out_dt = out_dtype;
     p.window = window; p.sinks = sinks;
-    const void* fn = raw ? pf_pick_bf16(out_dtype) : window > 0 ? pf_pick<true>(q_dtype, out_dtype) : pf_pick<false>(q_dtype, out_dtype);
+    p.raw = (const uint16_t*)values.rows; p.r_s0 = values.s0; p.r_s1 = values.s1;
+    p.raw_wide = ((uintptr_t)values.rows % 16) == 0 && (values.s0 | values.s1) % 8 == 0;
+    p.tops = values.tops; p.tops_s = pf_tops(values.tokens);
+    const void* fn = values.rows ? pf_pick_bf16<true>(out_dtype) : raw ? pf_pick_bf16<false>(out_dtype) : window > 0 ? pf_pick<true>(q_dtype, out_dtype) : pf_pick<false>(q_dtype, out_dtype);
     const int lds = PF_LDS;
     static const void* raised[32];
     static int nraised = 0;
@@ -608,6 +712,16 @@ static int prefill_call(void* stream, const void* query, int64_t q_s0, int64_t q
     if (!seen) {
         SKV_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
         if (nraised < 32) raised[nraised++] = fn;
+    }
+    if (values.rows) {
+        ToHalfParams c = {};
+        c.src[1] = values.rows; c.s0[1] = values.s0; c.s1[1] = values.s1; c.dst[1] = (uint16_t*)value;
+        c.H = num_kv_heads;
+        c.pieces = (int64_t)values.tokens * num_kv_heads * 16;
+        c.wide = p.raw_wide;
+        hipLaunchKernelGGL(values_to_half_kernel, dim3((unsigned)std::min<int64_t>((c.pieces + 255) / 256, 4096)), dim3(256), 0, (hipStream_t)stream,
+                           c, values.tops, p.tops_s);
+        SKV_HIP(hipGetLastError());
     }
     void* args[] = {(void*)&p};
     SKV_HIP(hipLaunchKernel(fn, dim3((unsigned)(num_blocks * num_heads)), dim3(PF_THR), args, (size_t)lds, (hipStream_t)stream));
@@ -633,6 +747,29 @@ int starkv_prefill_window(void* stream, const void* query, int64_t q_s0, int64_t
                         blocks, num_blocks, num_heads, num_kv_heads, head_size, window, sinks, scale, out, o_s0, o_s1, out_dtype);
 }
 
+size_t starkv_prefill_window_bf16_workspace_bytes(int num_tokens, int num_kv_heads) {
+    if (num_tokens < 1 || num_kv_heads < 1) return 256;
+    return (size_t)num_kv_heads * ((size_t)num_tokens * 256 + pf_tops(num_tokens));
+}
+
+int starkv_prefill_window_bf16(void* stream, const void* query, int64_t q_s0, int64_t q_s1, const void* key, int64_t k_s0,
+                               int64_t k_s1, const void* value, int64_t v_s0, int64_t v_s1, const int32_t* cu_seqlens,
+                               const int32_t* blocks, int num_blocks, int num_tokens, int num_heads, int num_kv_heads, int head_size,
+                               int window, int sinks, float scale, void* out, int64_t o_s0, int64_t o_s1, int out_dtype,
+                               void* workspace, size_t workspace_bytes) {
+    clear_error();
+    SKV_CHECK(window >= 1 && sinks >= 0, "prefill_window_bf16: window=%d sinks=%d", window, sinks);
+    SKV_CHECK(num_tokens >= 0 && num_kv_heads >= 1, "prefill_window_bf16: num_tokens=%d num_kv_heads=%d", num_tokens, num_kv_heads);
+    if (num_tokens == 0) return STARKV_OK;
+    const size_t need = starkv_prefill_window_bf16_workspace_bytes(num_tokens, num_kv_heads);
+    SKV_CHECK(value && workspace && (uintptr_t)workspace % 16 == 0 && (uintptr_t)value % 2 == 0, "prefill_window_bf16: null or odd pointer");
+    SKV_CHECK(workspace_bytes >= need, "prefill_window_bf16: workspace %zu bytes < %zu", workspace_bytes, need);
+    const int64_t row = (int64_t)num_kv_heads * 128;
+    return prefill_call(stream, query, q_s0, q_s1, STARKV_BF16, key, k_s0, k_s1, STARKV_BF16, workspace, row, 128, cu_seqlens, blocks,
+                        num_blocks, num_heads, num_kv_heads, head_size, window, sinks, scale, out, o_s0, o_s1, out_dtype,
+                        RawValues{value, v_s0, v_s1, (uint8_t*)workspace + num_tokens * row * 2, num_tokens});
+}
+
 int starkv_prefill_to_half(void* stream, const void* key, int64_t k_s0, int64_t k_s1, void* key_out, const void* value,
                            int64_t v_s0, int64_t v_s1, void* value_out, int dtype, int num_tokens, int num_kv_heads) {
     clear_error();
@@ -641,7 +778,7 @@ int starkv_prefill_to_half(void* stream, const void* key, int64_t k_s0, int64_t 
     SKV_CHECK(((uintptr_t)key_out % 16) == 0 && ((uintptr_t)value_out % 16) == 0,
               "prefill_to_half: the results must be 16-byte aligned");
     if (num_tokens == 0) return STARKV_OK;
-    SKV_CHECK(value && value_out && !key == !key_out, "prefill_to_half: null pointer");
+    SKV_CHECK(key && value && key_out && value_out, "prefill_to_half: null pointer");
     ToHalfParams p;
     p.src[0] = key; p.s0[0] = k_s0; p.s1[0] = k_s1; p.dst[0] = (uint16_t*)key_out;
     p.src[1] = value; p.s0[1] = v_s0; p.s1[1] = v_s1; p.dst[1] = (uint16_t*)value_out;
@@ -649,9 +786,9 @@ int starkv_prefill_to_half(void* stream, const void* key, int64_t k_s0, int64_t 
     p.pieces = (int64_t)num_tokens * num_kv_heads * 16;
     p.wide = 1;
     const int al = dtype == STARKV_F32 ? 4 : 8;
-    for (int z = key ? 0 : 1; z < 2; ++z)
+    for (int z = 0; z < 2; ++z)
         if (((uintptr_t)p.src[z] % 16) != 0 || p.s0[z] % al != 0 || p.s1[z] % al != 0) p.wide = 0;
-    const dim3 grid((unsigned)std::min<int64_t>((p.pieces + 255) / 256, 4096), key ? 2 : 1);
+    const dim3 grid((unsigned)std::min<int64_t>((p.pieces + 255) / 256, 4096), 2);
     if (dtype == STARKV_BF16)
         hipLaunchKernelGGL(to_half_kernel<STARKV_BF16>, grid, dim3(256), 0, (hipStream_t)stream, p);
     else

@@ -239,8 +239,8 @@ void prefill(const at::Tensor& query, const at::Tensor& key, const at::Tensor& v
           "prefill");
 }
 
-// The same through a window. Without cu_seqlens and blocks they are made of query_lens here, and values of bf16 become fp16
-// here (for a prompt of a few tokens, which waits for the host: fp16 18.8 -> 14.3 us, bf16 25 -> 17).
+// The same through a window; keys and values of bf16 by the entry for them. Without cu_seqlens and blocks they are made of
+// query_lens here (a prompt of a few tokens waits for the host: fp16 18.8 -> 14.3 us, bf16 25 -> 17).
 void prefill_window(const at::Tensor& query, const at::Tensor& key, const at::Tensor& value, const std::optional<at::Tensor>& cu_seqlens,
                     const std::optional<at::Tensor>& blocks, at::IntArrayRef query_lens, int64_t window, int64_t sinks, double scale,
                     const at::Tensor& out) {
@@ -280,17 +280,21 @@ void prefill_window(const at::Tensor& query, const at::Tensor& key, const at::Te
         cu = meta.data_ptr<int32_t>();
         rows = cu + prompts + 1;
     }
-    at::Tensor v = value;
     if (value.scalar_type() == at::kBFloat16) {
-        v = at::empty(value.sizes(), value.options().dtype(at::kHalf));
-        check(starkv_prefill_to_half(stream_of(value), nullptr, 0, 0, nullptr, value.data_ptr(), value.stride(0), value.stride(1), v.data_ptr(),
-                                     dtype_code(value), (int)value.size(0), (int)value.size(1)),
-              "prefill_to_half");
+        TORCH_CHECK(query.scalar_type() == at::kBFloat16, "starkv.prefill_window: bf16 keys and values go with bf16 queries");
+        const int tokens = (int)query.size(0), kv = (int)key.size(1);
+        const at::Tensor ws = workspace(query, starkv_prefill_window_bf16_workspace_bytes(tokens, kv));
+        check(starkv_prefill_window_bf16(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), key.data_ptr(), key.stride(0),
+                                         key.stride(1), value.data_ptr(), value.stride(0), value.stride(1), cu, rows, n, tokens,
+                                         (int)query.size(1), kv, (int)query.size(2), (int)window, (int)sinks, (float)scale,
+                                         out.data_ptr(), out.stride(0), out.stride(1), dtype_code(out), ws.data_ptr(), (size_t)ws.numel()),
+              "prefill_window");
+        return;
     }
     check(starkv_prefill_window(stream_of(query), query.data_ptr(), query.stride(0), query.stride(1), dtype_code(query),
-                                key.data_ptr(), key.stride(0), key.stride(1), dtype_code(key), v.data_ptr(), v.stride(0), v.stride(1), cu, rows,
-                                n, (int)query.size(1), (int)key.size(1), (int)query.size(2), (int)window, (int)sinks,
-                                (float)scale, out.data_ptr(), out.stride(0), out.stride(1), dtype_code(out)),
+                                key.data_ptr(), key.stride(0), key.stride(1), dtype_code(key), value.data_ptr(), value.stride(0),
+                                value.stride(1), cu, rows, n, (int)query.size(1), (int)key.size(1), (int)query.size(2), (int)window,
+                                (int)sinks, (float)scale, out.data_ptr(), out.stride(0), out.stride(1), dtype_code(out)),
           "prefill_window");
 }
 

@@ -20,7 +20,7 @@ from torch.autograd import forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libstarkv_hip.so")
 OPS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libstarkv_torch.so")
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 F32, F16, BF16 = 0, 1, 2
 CACHE_Q3_2 = 16  # cache kind of the 3.2-bit QuantRow cache
@@ -88,6 +88,9 @@ SIGNATURES = {
                                   _I, _I, _I, _I, _I, _F, _P, _I64, _I64, _P, _SZ]),
     "starkv_prefill_window": (_I, [_P, _P, _I64, _I64, _I, _P, _I64, _I64, _I, _P, _I64, _I64, _P, _P, _I, _I, _I, _I, _I,
                                    _I, _F, _P, _I64, _I64, _I]),
+    "starkv_prefill_window_bf16_workspace_bytes": (_SZ, [_I, _I]),
+    "starkv_prefill_window_bf16": (_I, [_P, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F,
+                                        _P, _I64, _I64, _I, _P, _SZ]),
     "starkv_write_kv8_workspace_bytes": (_SZ, [_I, _I64, _I]),
     "starkv_write_kv8": (_I, [_P, _P, _I64, _I64, _P, _I64, _I64, _I, _P, _P, _I64, _I64, _I64, _I, _P, _I64, _I64, _I,
                               _I64, _P, _I, _I, _I, _P, _SZ]),

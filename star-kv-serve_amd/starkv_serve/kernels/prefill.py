@@ -78,10 +78,11 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_l
     """Causal attention of each prompt to itself, through `window` where there is one (which has no gradient: calls that want
     one raise).
 
-    q [T, H_q, 128] (bf16, fp16 or fp32); k, v [T, H_kv, 128] (converted to fp16 once
-    here when they are not); query_lens: the prompts' token counts (host ints, summing to
-    T); tables: their ``prompt_tables``, when the caller has them (in a capture it must). Returns ``out``
-    [T, H_q, 128] (new, in q's dtype, when not given)."""
+    q [T, H_q, 128] (bf16, fp16 or fp32; to fp16 in the kernel); k, v [T, H_kv, 128] (converted to fp16 once here when they
+    are not: values past its range become infinite, those below 2^-14 lose bits). Through a window bf16 q, k and v go as they
+    are, over bf16's whole range: a value below 2^-17 among larger ones (2^-10 or more) is off by 2^-25 at most. query_lens: the
+    prompts' token counts (host ints, summing to T); tables: their ``prompt_tables``, when the caller has them (in a capture
+    it must). Returns ``out`` [T, H_q, 128] (new, in q's dtype, when not given)."""
     T, Hq, D = q.shape
     assert D == 128 and k.shape == v.shape and k.shape[0] == T and k.shape[2] == D and Hq % k.shape[1] == 0
     assert sum(query_lens) == T
@@ -92,12 +93,14 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, query_l
     if T == 0:
         return out
     _hip.require_cuda(q, k, v, out)
-    # Through a window keys of bf16, and keys and values of fp16, are read as they are; values of bf16 become fp16, as the
-    # weights that multiply them.
-    as_is = (window is not None and q.dtype == k.dtype == v.dtype and k.stride(-1) == v.stride(-1) == 1
-             and k.stride(0) % 8 == k.stride(1) % 8 == k.data_ptr() % 16 == 0 and k.stride(0) < 1 << 23
-             and (k.dtype == torch.bfloat16 or (k.dtype == torch.float16 and k.stride() == v.stride() and v.data_ptr() % 16 == 0)))
-    if not as_is:
+    # Through a window rows of one type go as they are: bf16 over its whole range (keys 16-byte aligned), fp16 where keys and
+    # values share their strides. All others become fp16.
+    rows = window is not None and q.dtype == k.dtype == v.dtype
+    aligned = rows and k.stride(-1) == v.stride(-1) == 1 and k.stride(0) % 8 == k.stride(1) % 8 == k.data_ptr() % 16 == 0 and k.stride(0) < 1 << 23
+    if rows and k.dtype == torch.bfloat16:
+        if not aligned:
+            k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
+    elif not (aligned and k.dtype == torch.float16 and k.stride() == v.stride() and v.data_ptr() % 16 == 0):
         if k.dtype == v.dtype and k.dtype in (torch.bfloat16, torch.float32) and k.stride(-1) == v.stride(-1) == 1:
             kv = torch.empty((2, *k.shape), dtype=torch.float16, device=k.device)
             _hip.ops().prefill_to_half(k, v, kv[0], kv[1])
