@@ -298,20 +298,19 @@ void prefill_window(const at::Tensor& query, const at::Tensor& key, const at::Te
           "prefill_window");
 }
 
-// K and V [T, H, 128] of one dtype (bf16 or fp32) as contiguous fp16, or V alone.
-void prefill_to_half(const std::optional<at::Tensor>& key, const at::Tensor& value, const std::optional<at::Tensor>& key_out,
+// K and V [T, H, 128] of one dtype (bf16 or fp32) as contiguous fp16.
+void prefill_to_half(const at::Tensor& key, const at::Tensor& value, const at::Tensor& key_out,
                      const at::Tensor& value_out) {
-    const c10::DeviceGuard guard(value.device());
-    TORCH_CHECK(value.dim() == 3 && value.size(2) == 128 && value.stride(2) == 1 && key.has_value() == key_out.has_value() &&
-                    (!key || (key->scalar_type() == value.scalar_type() && key->sizes() == value.sizes() && key->stride(2) == 1)),
+    const c10::DeviceGuard guard(key.device());
+    TORCH_CHECK(key.scalar_type() == value.scalar_type() && key.sizes() == value.sizes() && key.dim() == 3 &&
+                    key.size(2) == 128 && key.stride(2) == 1 && value.stride(2) == 1,
                 "starkv.prefill_to_half: K and V [T, heads, 128] of one dtype");
-    for (const auto* o : {key_out ? &*key_out : &value_out, &value_out})
-        TORCH_CHECK(o->is_contiguous() && o->scalar_type() == at::kHalf && o->sizes() == value.sizes(),
+    for (const auto* o : {&key_out, &value_out})
+        TORCH_CHECK(o->is_contiguous() && o->scalar_type() == at::kHalf && o->sizes() == key.sizes(),
                     "starkv.prefill_to_half: the results are contiguous fp16 of the same shape");
-    check(starkv_prefill_to_half(stream_of(value), key ? key->data_ptr() : nullptr, key ? key->stride(0) : 0,
-                                 key ? key->stride(1) : 0, key ? key_out->data_ptr() : nullptr, value.data_ptr(),
-                                 value.stride(0), value.stride(1), value_out.data_ptr(), dtype_code(value),
-                                 (int)value.size(0), (int)value.size(1)),
+    check(starkv_prefill_to_half(stream_of(key), key.data_ptr(), key.stride(0), key.stride(1), key_out.data_ptr(),
+                                 value.data_ptr(), value.stride(0), value.stride(1), value_out.data_ptr(),
+                                 dtype_code(key), (int)key.size(0), (int)key.size(1)),
           "prefill_to_half");
 }
 
@@ -816,7 +815,7 @@ TORCH_LIBRARY(starkv, m) {
     m.def("silu_mul(Tensor gate_up, Tensor(a!) out) -> ()");
     m.def("few_linear(Tensor x, Tensor w, Tensor? norm_weight, float eps, Tensor(a!)? h_out, int mode, "
           "Tensor? residual, Tensor(b!) out) -> ()");
-    m.def("prefill_to_half(Tensor? key, Tensor value, Tensor(a!)? key_out, Tensor(b!) value_out) -> ()");
+    m.def("prefill_to_half(Tensor key, Tensor value, Tensor(a!) key_out, Tensor(b!) value_out) -> ()");
     m.def("prefill_lift(Tensor k_codes, Tensor v_codes, Tensor cu_seqlens, Tensor k_up, Tensor k_offsets, "
           "Tensor k_widths, Tensor cos_sin, Tensor(a!) key, Tensor(b!)? v_out) -> ()");
 }

@@ -37,3 +37,11 @@ def test_bf16_prompts_refuse(key, value, message):
 
 def test_no_tokens():
     assert _hip.lib().starkv_prefill_window_bf16(*dict(GOOD, tokens=0, blocks=0, bytes=0).values()) == 0
+
+
+def test_conversion_takes_keys_and_values():
+    """The operator that makes fp16 rows has both."""
+    schema = str(_hip.ops().prefill_to_half.default._schema)
+    assert schema == "starkv::prefill_to_half(Tensor key, Tensor value, Tensor(a!) key_out, Tensor(b!) value_out) -> ()"
+    L = _hip.lib()
+    assert L.starkv_prefill_to_half(None, None, 0, 0, None, P, 256, 128, P, 2, 4, 2) != 0 and b"null" in L.starkv_last_error()
