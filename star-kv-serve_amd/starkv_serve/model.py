@@ -254,14 +254,17 @@ class StarKVLlamaForCausalLM:
         else:
             h, qkv = self._norm_linear(x, layer.ln1, layer.qkv_proj, few, capture is not None)
             q, k, v = (t.view(T, n, D) for t, n in zip(qkv.split([H * D, Hkv * D, Hkv * D], dim=-1), (H, Hkv, Hkv)))
-            ka, va = k, v  # the prefill attention's operands
+            ka, va = k, v  # the prefill attention's operands: the rotation's fp16 rows, or through a window those of bf16 (a wider range)
+            half = bool(md.num_prefills) and (self.window is None or self.dtype != torch.bfloat16)
+            keep_k = capture is not None or bool(md.num_prefills) and not half
             slots = md.slot_mapping[:T]
             if self.cache8 is None:
                 kc, vc = self.kv_caches[li]
             if self.cache8 is not None:
                 if self._own_rotation() and model_ops.rope_fits(self.rotary.cos_sin_cache, positions, q, k, v):
                     norms = (layer.q_norm, layer.k_norm, s.rms_norm_eps) if layer.q_norm is not None else None
-                    q, k, ka, va = model_ops.rope_rows(positions, q, k, v, self.rotary.cos_sin_cache, bool(md.num_prefills), norms)
+                    q, k, k16, v16 = model_ops.rope_rows(positions, q, k, v, self.rotary.cos_sin_cache, half, norms)
+                    ka, va = (k16, v16) if half else (k, v)
                 else:
                     q, k = self._normed(layer, q, k)
                     q, k = self.rotary.apply(positions, q), self.rotary.apply(positions, k)
@@ -269,12 +272,12 @@ class StarKVLlamaForCausalLM:
                 write_kv8(k, v, self.kv_caches[li], slots)
             elif self._own_rotation() and model_ops.rope_write_fits(self.rotary.cos_sin_cache, positions, q, k, v, kc, vc, slots):
                 if layer.q_norm is None:
-                    q, k, ka, va = model_ops.rope_write(positions, q, k, v, self.rotary.cos_sin_cache, kc, vc, slots,
-                                                        capture is not None, bool(md.num_prefills))
+                    q, k, k16, v16 = model_ops.rope_write(positions, q, k, v, self.rotary.cos_sin_cache, kc, vc, slots,
+                                                          keep_k, half)
                 else:
-                    q, k, ka, va = model_ops.norm_rope_write(positions, q, k, v, self.rotary.cos_sin_cache, layer.q_norm,
-                                                             layer.k_norm, s.rms_norm_eps, kc, vc, slots,
-                                                             capture is not None, bool(md.num_prefills))
+                    q, k, k16, v16 = model_ops.norm_rope_write(positions, q, k, v, self.rotary.cos_sin_cache, layer.q_norm,
+                                                               layer.k_norm, s.rms_norm_eps, kc, vc, slots, keep_k, half)
+                ka, va = (k16, v16) if half else (k, v)
             else:
                 q, k = self._normed(layer, q, k)
                 q, k = self.rotary.apply(positions, q), self.rotary.apply(positions, k)

@@ -11,6 +11,7 @@ import math
 import pytest
 import torch
 
+import test_gpu_cache8_model as CM
 from cache8_plain import D, E, SCALE
 from starkv_serve.kernels.prefill import prefill_attention, prompt_tables
 from starkv_serve.kernels.window import Window
@@ -192,3 +193,29 @@ def test_captured_values_of_any_size(cuda):
         assert torch.equal(got, prefill_attention(q, k, v, LENS, SCALE, window=w))
         whole_range_close(got, q, k, v, LENS, w, size)
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("cache8", [None, torch.int8])
+@pytest.mark.parametrize("qk_norm", [False, True])
+def test_model_prompts_have_bf16_range(cuda, cache8, qk_norm):
+    """Keys of 2^20 with queries as much smaller and values of 2^20: neither fits fp16, and steps take them too."""
+    w = Window(40, 4)
+    model, bt = CM.build(cuda, BF16, qk_norm, cache8=cache8, window=w)
+    for layer in model.layers:
+        rows = layer.qkv_proj.view(-1, D, layer.qkv_proj.shape[1])  # 8 heads of queries, 2 of keys, 2 of values
+        if qk_norm:
+            layer.q_norm.mul_(2.0 ** -20)
+            layer.k_norm.mul_(2.0 ** 20)
+        else:
+            rows[:8].mul_(2.0 ** -20)
+            rows[8:10].mul_(2.0 ** 20)
+        rows[10:].mul_(2.0 ** 20)
+    capture = []
+    tokens, _ = CM.prefill(model, bt, capture)
+    for c in capture:
+        assert c["k"].abs().max() > 65504 and c["v"].abs().max() > 65504
+        CM.W.prompts_close(c["out"], c["q"], c["k"], c["v"], CM.PROMPTS, w, c["layer"])
+    bare, _ = CM.prefill(model, bt)  # without a capture the same
+    assert torch.equal(bare, tokens)
+    positions = torch.tensor(CM.PROMPTS, device=cuda)
+    assert model.decode_step(tokens, positions, CM.M.decode_metadata(bt, positions, 16, CM.SPAN)).isfinite().all()
