@@ -44,6 +44,7 @@
 
 #include "decode_common.hpp"
 #include "kv_gemm.hpp"
+#include "lds_limit.hpp"
 
 namespace starkv {
 // ---------------------------------------------------------------------------
@@ -886,12 +887,9 @@ struct CommonArgs {
 template <typename WT, int CB>
 static int launch_merge_cb(dim3 grid, size_t lds, hipStream_t stream, const DecodeParams& p, const WsLayout& wl,
                            const CommonArgs& a) {
-    static size_t lds_allowed = 65536;  // per function: raised as larger v_rank need it (at most 132 KB)
-    if (lds > lds_allowed) {
-        SKV_HIP(hipFuncSetAttribute((const void*)merge_kernel<WT, CB>, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                    (int)lds));
-        lds_allowed = lds;
-    }
+    static LdsLimits limits;  // raised as larger v_rank need it (at most 132 KB)
+    if (lds > 65536)
+        if (const int rc = limits.allow((const void*)merge_kernel<WT, CB>, (int)lds)) return rc;
     hipLaunchKernelGGL((merge_kernel<WT, CB>), grid, dim3(MERGE_THR), lds, stream, (const uint8_t*)p.ws, wl.plan, wl.m,
                        wl.l, wl.acc, a.n, a.Hq, a.v_rank, (const WT*)a.vup, a.vu_s0, a.vu_s1, a.out, a.o_s0, a.o_s1,
                        a.out_dt);

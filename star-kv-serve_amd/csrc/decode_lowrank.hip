@@ -32,6 +32,7 @@
 // split-K partials, and decode_wide.hip's pass runs P @ V from those logits.
 
 #include "decode_pages.hpp"
+#include "lds_limit.hpp"
 
 namespace starkv {
 
@@ -583,14 +584,8 @@ int launch_lowrank(const DecodeParams& p, int fmt, int nb, int grid, hipStream_t
     SKV_CHECK(mtv > 0, "decode: no spill-free kernel for %d rank tiles and %d V blocks", p.TT, nb);
     const void* fn = fmt == FMT_BF16 ? pick<FMT_BF16>(nbuf, nld, mtv, nb) : pick<FMT_F16>(nbuf, nld, mtv, nb);
     SKV_CHECK(fn != nullptr, "decode: no kernel for %d rank tiles and %d V blocks", p.TT, nb);
-    static const void* raised[256];  // kernels whose dynamic-LDS limit was raised (host-side bookkeeping)
-    static int nraised = 0;
-    bool seen = false;
-    for (int i = 0; i < nraised; ++i) seen = seen || raised[i] == fn;
-    if (!seen) {
-        SKV_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, LR_MAX_DYN_LDS));
-        if (nraised < 256) raised[nraised++] = fn;
-    }
+    static LdsLimits limits;
+    if (const int rc = limits.allow(fn, LR_MAX_DYN_LDS)) return rc;
     void* args[] = {(void*)&p};
     SKV_HIP(hipLaunchKernel(fn, dim3(grid), dim3(NTHR), args, (size_t)p.lds_bytes, stream));
     return STARKV_OK;

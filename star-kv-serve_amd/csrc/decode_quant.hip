@@ -45,6 +45,7 @@
 #include <type_traits>
 
 #include "decode_pages.hpp"
+#include "lds_limit.hpp"
 
 namespace starkv {
 
@@ -742,14 +743,8 @@ int launch_quant(const DecodeParams& p, int nb, int grid, hipStream_t stream) {
     SKV_CHECK(mtv > 0, "decode: no spill-free kernel for %d rank tiles and %d V blocks", p.TT, nb);
     const void* fn = nld <= 3 ? q_pick_mtv<3>(mtv, nb) : q_pick_mtv<6>(mtv, nb);
     SKV_CHECK(fn != nullptr, "decode: no kernel for %d rank tiles and %d V blocks", p.TT, nb);
-    static const void* raised[256];  // kernels whose dynamic-LDS limit was raised (host-side bookkeeping)
-    static int nraised = 0;
-    bool seen = false;
-    for (int i = 0; i < nraised; ++i) seen = seen || raised[i] == fn;
-    if (!seen) {
-        SKV_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, Q_MAX_DYN_LDS));
-        if (nraised < 256) raised[nraised++] = fn;
-    }
+    static LdsLimits limits;
+    if (const int rc = limits.allow(fn, Q_MAX_DYN_LDS)) return rc;
     void* args[] = {(void*)&p};
     SKV_HIP(hipLaunchKernel(fn, dim3(grid), dim3(NTHR), args, (size_t)p.lds_bytes, stream));
     return STARKV_OK;

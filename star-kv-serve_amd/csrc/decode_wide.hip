@@ -43,6 +43,7 @@
 #include <algorithm>
 
 #include "decode_pages.hpp"
+#include "lds_limit.hpp"
 
 namespace starkv {
 
@@ -917,13 +918,8 @@ const void* pv_pick_r(int mb, int r, int nld, int pg) {
 }
 
 int raise_lds(const void* fn, int bytes) {
-    static const void* raised[64];
-    static int nraised = 0;
-    for (int i = 0; i < nraised; ++i)
-        if (raised[i] == fn) return STARKV_OK;
-    SKV_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    if (nraised < 64) raised[nraised++] = fn;
-    return STARKV_OK;
+    static LdsLimits limits;
+    return limits.allow(fn, bytes);
 }
 
 // Dynamic LDS of lift_kernel<DT, req, thr, dq>: the rows o [req][ld], then (over them)

@@ -54,6 +54,7 @@
 #include <vector>
 
 #include "decode_pages.hpp"
+#include "lds_limit.hpp"
 
 namespace starkv {
 
@@ -705,14 +706,8 @@ static int prefill_call(void* stream, const void* query, int64_t q_s0, int64_t q
     p.tops = values.tops; p.tops_s = pf_tops(values.tokens);
     const void* fn = values.rows ? pf_pick_bf16<true>(out_dtype) : raw ? pf_pick_bf16<false>(out_dtype) : window > 0 ? pf_pick<true>(q_dtype, out_dtype) : pf_pick<false>(q_dtype, out_dtype);
     const int lds = PF_LDS;
-    static const void* raised[32];
-    static int nraised = 0;
-    bool seen = false;
-    for (int i = 0; i < nraised; ++i) seen = seen || raised[i] == fn;
-    if (!seen) {
-        SKV_HIP(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
-        if (nraised < 32) raised[nraised++] = fn;
-    }
+    static LdsLimits limits;
+    if (const int rc = limits.allow(fn, lds)) return rc;
     if (values.rows) {
         ToHalfParams c = {};
         c.src[1] = values.rows; c.s0[1] = values.s0; c.s1[1] = values.s1; c.dst[1] = (uint16_t*)value;

@@ -7,6 +7,7 @@ value of the workgroup's tokens (128 queries' and what they see) is 2^-10 at lea
 fp16 are off by 2^-11, and by 2^-25 below its range, times the values that it holds; in two bf16 values by 2^-17.
 """
 import math
+import threading
 
 import pytest
 import torch
@@ -219,3 +220,41 @@ def test_model_prompts_have_bf16_range(cuda, cache8, qk_norm):
     assert torch.equal(bare, tokens)
     positions = torch.tensor(CM.PROMPTS, device=cuda)
     assert model.decode_step(tokens, positions, CM.M.decode_metadata(bt, positions, 16, CM.SPAN)).isfinite().all()
+
+
+def test_prompts_from_several_threads(cuda):
+    """Each thread on a stream of its own, kernels of unlike types between each other; every call in each of them."""
+    g = torch.Generator().manual_seed(8)
+    calls = []
+    for dt in (BF16, F16, F32):
+        for odt in (BF16, F16, F32):
+            for window in (Window(90, 5), None):
+                q, k, v = prompts(dt, 2, 2, cuda, g) if dt != F32 else (t.float() for t in prompts(F16, 2, 2, cuda, g))
+                calls.append((q, k, v, odt, window))
+    def run(q, k, v, odt, window):
+        return prefill_attention(q, k, v, LENS, SCALE, out=torch.empty(q.shape, dtype=odt, device=cuda), window=window)
+    got, errors, start = {}, [], threading.Barrier(6)
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            start.wait()
+            with torch.cuda.stream(stream):
+                for r in range(4):
+                    for j in range(len(calls)):
+                        at = (j + 3 * i) % len(calls)
+                        got[i, at] = run(*calls[at])
+            stream.synchronize()
+        except Exception as e:  # of a thread: told to the test
+            errors.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    want = [run(*c) for c in calls]
+    for (i, at), x in got.items():
+        assert torch.equal(x, want[at]), (i, at)
