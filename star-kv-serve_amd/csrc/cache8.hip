@@ -12,7 +12,8 @@
 // it names is the entry's own. Measured, one against the other: a step of 512 requests of 8 heads, each in a block of its own,
 // 4.1 against 24 us, of 1024 4.9 against 30 (of 32 heads 10 against 31), of 2048 9.7 against 30; a prompt of 512 tokens of 8
 // heads 6.6 against 10.7, of 1024 9.6 against 10.9 (of 32 heads 20 against 13), of 2048 12.7 against 11.5 (28 against 16).
-// The map's workgroups do up to WR_RUN blocks one after the other, which is what a step of many requests pays there.
+// The map's workgroups do up to WR_RUN blocks one after the other, which is what a step of many requests pays there. The host
+// does not see which of the two a call is, so the limit is the steps': prompts of 700 to 1024 tokens of 32 heads pay up to 7 us.
 //
 // A workgroup of the first kind has 4 heads, a wave each, and up to 16 where there would be more than WR_WIDE workgroups: 4 heads
 // take a prompt of 64 tokens of 32 heads from 12.6 to 6.1 us, 16 a step of 1024 tokens of 32 heads from 20 to 9.3. In blocks
@@ -23,11 +24,11 @@
 // (NaN is above infinity, which is above all others), rows kept in registers from the first look to the rounding where there
 // are at most 16; of more, 2 or 4 waves share a head and meet in LDS (11400 tokens of 32 heads in blocks of 64 191 -> 82 us, of
 // 1024 999 -> 163). A block with one token (a step's) is write_single's. Rows are read past the caches: the codes stay there for
-// what reads them next (11400 tokens of 32 heads written and read back 130 -> 107 us).
+// what reads them next (11400 tokens of 32 heads written and read back 130 -> 105 us).
 //
 // Bound by memory, and for small calls by latency: a step of 64 tokens of 8 heads takes 3.8 us, of which a launch in a graph
-// is 2; codes that the step has to round again add 6. Four prompts of 11400 tokens of 32 heads, 187 MB in and 93 out: 59 us,
-// 4.8 TB/s; the copy of 2 GiB runs at 4.9.
+// is 2 (4.3 under the profiler); codes that the step has to round again add 2.4. Four prompts of 11407 tokens of 32 heads, 187 MB in and
+// 93 out: 56 us, 5.0 TB/s; the copy of 2 GiB runs at 4.9.
 #include <algorithm>
 
 #include "cache8.hpp"
@@ -465,7 +466,7 @@ struct Read8Params {
 // row.
 constexpr int RD_U = 2;
 // Results of 16 bits of more than this many bytes go past the caches (256 MB in the last level), which they would not fit: 11400
-// tokens of 32 heads behind their write 105 -> 96 us, 73000 of 8 heads (300 MB) 72 -> 66. Fewer stay there for their reader
+// tokens of 32 heads behind their write 105 -> 96 us, 60515 of 8 heads (248 MB) 72 -> 66. Fewer stay there for their reader
 // (4096 tokens of 32 heads, 67 MB: 16.8 us, 16.5 past them).
 constexpr int64_t RD_ONCE = 128 << 20;
 

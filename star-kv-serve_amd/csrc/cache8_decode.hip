@@ -31,8 +31,9 @@
 // that left, 22 bits; up to 8 query heads the lanes of the other 8 columns, whose scores are the same heads'
 // again, take the second one, so that one product does. Two references are kept for that: m of the scores s for
 // the sum of weights, and r of s + c for the weights of the values, each 2^7 below the largest when it was set and moved
-// when that passes it by 2^15, so that neither overflows fp16 and what a value contributes keeps its bits whatever the
-// blocks' exponents are (a first token with a large weight and values of 2^-40 of the others' keeps them). Partials keep both
+// when that passes it by 2^15, so that neither overflows fp16 and what a value contributes keeps its bits, down to 2^-31 of the
+// largest contribution to its head, whatever the blocks' exponents are (a first token with a large weight and values of 2^-40
+// of the others' keeps them). Partials keep both
 // references, and the result is scaled by 2^(r - m) in two steps, so values near fp32's largest stay finite.
 //
 // A block whose exponent says NaN makes every row NaN that sees one of its tokens. A row that sees no token is zero; one

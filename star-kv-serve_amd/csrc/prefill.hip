@@ -44,8 +44,8 @@
 // them: 8 bits are exact in it from 2^-17 to 65504, and a product of fp16 weights has 11 bits of those, one of bf16 weights 8. The
 // values themselves are multiplied in a second pass where it does not.
 //
-// Two prompts of 9300 tokens together, 32 heads, window 1024: 211 us, 153 GFLOP of pairs that are seen (725 TFLOP/s; 870 with the masked
-// halves of edge tiles), the conversion in front 27; one of 2047 tokens with window 512: 34 and 4. The matrix unit is busy 42 %
+// Two prompts of 10044 tokens together, 32 heads, window 1024: 220 us, 153 GFLOP of pairs that are seen (700 TFLOP/s; 840 with the masked
+// halves of edge tiles), the conversion in front 30; one of 2047 tokens with window 512: 35 and 4. The matrix unit is busy 42 %
 // of the time and the vector unit 45 %: with about 18 tiles a workgroup, its start (Q, the first copies) and end weigh more
 // than among a long causal prompt's. The first tokens' tiles in a loop of their own, without the mask, spilled registers.
 #include <algorithm>
